@@ -75,7 +75,21 @@ _SIGNATURES = {
     "dsa_sparse_attn_uses_mask": ([_I, _I64, _I, _I, _I], _I),
     "dsa_sparse_attn_mask_noalloc": ([_P, _I64, _P, _P, _P, _P, _I, _I64, _I64, _I, _I, _I, _F,
                                       _P, _P], _I),
+    "dsa_kv4_append": ([_P, _P, _P, _I, _P, _P, _P, _I64, _I, _P], _I),
+    "dsa_kv4_rows": ([_P, _P, _I64, _I, _P, _P, _P], _I),
+    "dsa_kv4_indexer_scores": ([_P, _P, _P, _P, _I64, _I, _I64, _P, _P], _I),
+    "dsa_kv4_attention_workspace_bytes": ([_P, _I64, _I, _I, _I64, _I], _I64),
+    "dsa_kv4_attention": ([_P, _P, _I, _P, _P, _I64, _I, _I64, _I, _F, _P, _P, _I64, _P], _I),
+    "dsa_kv4_evict": ([_P, _I64, _I64, _P, _P, _P], _I),
 }
+
+
+class Kv4Cache(ctypes.Structure):
+    """dsa_kv4_cache: the buffers and sizes of a 4-bit cache."""
+
+    _fields_ = [(n, _P) for n in ("codes", "scales", "k_idx", "length", "seen", "lost", "position",
+                                  "weight")] \
+        + [("B", _I64), ("S", _I64)] + [(n, _I) for n in ("HKV", "DK", "DV", "DI", "idx_dtype")]
 
 
 _CPU_SIGNATURES = {

@@ -10,6 +10,7 @@
 
 #include "../../include/dsa_amd.h"
 #include "dsa_launch.h"
+#include "kv4.h"
 
 namespace {
 
@@ -29,6 +30,7 @@ int hip_status(hipError_t e, const char* what) {
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
 bool pow2(int64_t v) { return v > 0 && (v & (v - 1)) == 0; }
 bool dtype_ok(int d) { return d == DSA_F32 || d == DSA_BF16 || d == DSA_F16; }
 
@@ -96,6 +98,70 @@ int check_tile_attn(int dtype, int64_t B, int64_t T, int HQ, int DQ, int DV, con
   if (!aligned16(Q) || !aligned16(K) || !aligned16(V) || !aligned16(out))
     return fail(DSA_EINVAL, "%s: Q/K/V/out must be 16-byte aligned", who);
   if (B * T * HQ * static_cast<int64_t>(DQ) > (int64_t{1} << 40)) return fail(DSA_EINVAL, "%s: Q too large", who);
+  return DSA_OK;
+}
+
+// The 4-bit cache: sizes and pointers of the struct; `codes`, `index`: which
+// parts the call needs.
+int check_kv4(const dsa_kv4_cache* c, bool codes, bool index, const char* who) {
+  if (!c) return fail(DSA_EINVAL, "%s: null cache", who);
+  if (c->B < 0 || c->S < 1) return fail(DSA_EINVAL, "%s: B=%lld must be >= 0 and S=%lld >= 1", who, (long long)c->B, (long long)c->S);
+  if (c->B > 65535 || c->S > kMaxElems) return fail(DSA_EINVAL, "%s: B=%lld above 65535 or S=%lld above 2^31", who, (long long)c->B, (long long)c->S);
+  if (c->HKV < 0 || c->DK < 0 || c->DV < 0 || c->DI < 0) return fail(DSA_EINVAL, "%s: negative head size", who);
+  if (codes) {
+    if (c->HKV < 1 || c->HKV > 1024) return fail(DSA_EINVAL, "%s: HKV=%d outside [1,1024]", who, c->HKV);
+    if (c->DK < 32 || c->DV < 32 || c->DK % 32 || c->DV % 32 || c->DK > 1024 || c->DV > 1024)
+      return fail(DSA_EUNSUPPORTED, "%s: DK=%d DV=%d must be multiples of 32 up to 1024", who, c->DK, c->DV);
+    if (c->S * c->HKV * ((c->DK + c->DV) / 2) >= (int64_t{1} << 31))
+      return fail(DSA_EINVAL, "%s: one sequence's codes, S*HKV*(DK+DV)/2 = %lld bytes, must be < 2^31", who, (long long)(c->S * c->HKV * ((c->DK + c->DV) / 2)));
+  }
+  if (c->k_idx || index) {
+    if (!dtype_ok(c->idx_dtype)) return fail(DSA_EINVAL, "%s: unknown index key dtype %d", who, c->idx_dtype);
+    if (!dsa::indexer_supported(c->idx_dtype, c->DI))
+      return fail(DSA_EUNSUPPORTED, "%s: DI=%d unsupported for dtype %d (fp32: 16..256, 16-bit: 32..256, powers of two)", who, c->DI, c->idx_dtype);
+  }
+  if (c->B == 0) return DSA_OK;
+  if (!c->length) return fail(DSA_EINVAL, "%s: null length", who);
+  if (codes && (!c->codes || !c->scales || !c->seen || !c->lost || !c->position || !c->weight))
+    return fail(DSA_EINVAL, "%s: null cache buffer", who);
+  if (index && !c->k_idx) return fail(DSA_EINVAL, "%s: the cache holds no index keys", who);
+  if (!aligned16(c->codes) || !aligned16(c->k_idx)) return fail(DSA_EINVAL, "%s: codes and k_idx must be 16-byte aligned", who);
+  if (!aligned4(c->scales) || !aligned4(c->length) || !aligned4(c->seen) || !aligned4(c->lost) ||
+      !aligned4(c->position) || !aligned4(c->weight))
+    return fail(DSA_EINVAL, "%s: cache buffers must be 4-byte aligned", who);
+  return DSA_OK;
+}
+
+dsa::Kv4 kv4_of(const dsa_kv4_cache* c) {
+  dsa::Kv4 k;
+  k.codes = c->codes;
+  k.scales = c->scales;
+  k.k_idx = c->k_idx;
+  k.length = c->length;
+  k.seen = c->seen;
+  k.lost = c->lost;
+  k.position = c->position;
+  k.weight = c->weight;
+  k.B = c->B;
+  k.S = c->S;
+  k.HKV = c->HKV;
+  k.DK = c->DK;
+  k.DV = c->DV;
+  k.DI = c->k_idx ? c->DI : 0;
+  k.idx_bytes = c->idx_dtype == DSA_F32 ? 4 : 2;
+  return k;
+}
+
+// The queries of an attention over the cache.
+int check_kv4_attention(const dsa_kv4_cache* c, int64_t Tq, int HQ, bool listed, int64_t n, const char* who) {
+  int rc = check_kv4(c, true, false, who);
+  if (rc != DSA_OK) return rc;
+  if (Tq < 0 || n < 0 || n > kMaxElems) return fail(DSA_EINVAL, "%s: Tq=%lld n=%lld", who, (long long)Tq, (long long)n);
+  if (HQ < 1 || HQ > 1024 || HQ % c->HKV) return fail(DSA_EINVAL, "%s: HQ=%d must be a multiple of HKV=%d, at most 1024", who, HQ, c->HKV);
+  if (!listed && n > c->S) return fail(DSA_EINVAL, "%s: n=%lld > S=%lld", who, (long long)n, (long long)c->S);
+  if (Tq > kMaxElems || c->B * Tq * HQ > kMaxElems) return fail(DSA_EINVAL, "%s: B*Tq*HQ must be < 2^31", who);
+  if (!dsa::kv4_attn_supported(c->DK, c->DV))
+    return fail(DSA_EUNSUPPORTED, "%s: no kernel for DK=%d DV=%d (equal ones of 32, 64, 96, 128, 192, 256, or 192 with 128)", who, c->DK, c->DV);
   return DSA_OK;
 }
 
@@ -466,6 +532,96 @@ int dsa_fused_forward(const void* q_idx, const void* k_idx, const void* w_idx, c
   if (e == hipErrorNotSupported)
     return fail(DSA_EUNSUPPORTED, "fused: no fused instance for dtype %d DI=%d HQ=%d DQ=%d DV=%d", dtype, DI, HQ, DQ, DV);
   return hip_status(e, "dsa_fused_forward");
+}
+
+int dsa_kv4_append(const dsa_kv4_cache* cache, const void* K, const void* V, int dtype,
+                   const void* k_idx, const float* weight, const int32_t* count, int64_t T,
+                   int restart, void* stream) {
+  int rc = check_kv4(cache, true, false, "kv4_append");
+  if (rc != DSA_OK) return rc;
+  if (!dtype_ok(dtype)) return fail(DSA_EINVAL, "kv4_append: unknown dtype %d", dtype);
+  if (T < 0 || T > kMaxElems) return fail(DSA_EINVAL, "kv4_append: T=%lld", (long long)T);
+  if ((k_idx != nullptr) != (cache->k_idx != nullptr) && cache->B * T != 0)
+    return fail(DSA_EINVAL, "kv4_append: index keys go with a cache that holds them");
+  // with T = 0 there is nothing to do but a restart's counters
+  if (cache->B == 0 || (T == 0 && !restart)) return DSA_OK;
+  if (T > 0 && (!K || !V)) return fail(DSA_EINVAL, "kv4_append: null pointer");
+  if (!aligned16(K) || !aligned16(V) || !aligned16(k_idx)) return fail(DSA_EINVAL, "kv4_append: K, V and k_idx must be 16-byte aligned");
+  if (!aligned4(weight) || !aligned4(count)) return fail(DSA_EINVAL, "kv4_append: weight and count must be 4-byte aligned");
+  return hip_status(dsa::launch_kv4_append(kv4_of(cache), K, V, dtype, k_idx, weight, count, T, restart != 0,
+                                           static_cast<hipStream_t>(stream)),
+                    "dsa_kv4_append");
+}
+
+int dsa_kv4_rows(const dsa_kv4_cache* cache, const int32_t* slots, int64_t N, int dtype, void* K,
+                 void* V, void* stream) {
+  int rc = check_kv4(cache, true, false, "kv4_rows");
+  if (rc != DSA_OK) return rc;
+  if (!dtype_ok(dtype)) return fail(DSA_EINVAL, "kv4_rows: unknown dtype %d", dtype);
+  if (N < 0 || N > kMaxElems) return fail(DSA_EINVAL, "kv4_rows: N=%lld", (long long)N);
+  if (cache->B * N == 0) return DSA_OK;
+  if (!K || !V) return fail(DSA_EINVAL, "kv4_rows: null pointer");
+  if (!aligned16(K) || !aligned16(V) || !aligned4(slots)) return fail(DSA_EINVAL, "kv4_rows: K and V must be 16-byte aligned, slots 4-byte");
+  return hip_status(dsa::launch_kv4_rows(kv4_of(cache), slots, N, dtype, K, V, static_cast<hipStream_t>(stream)),
+                    "dsa_kv4_rows");
+}
+
+int dsa_kv4_indexer_scores(const dsa_kv4_cache* cache, const void* q_idx, const void* w_idx,
+                           const int32_t* count, int64_t Tq, int HI, int64_t span, float* scores,
+                           void* stream) {
+  int rc = check_kv4(cache, false, true, "kv4_indexer");
+  if (rc != DSA_OK) return rc;
+  if (HI < 1 || HI > 256) return fail(DSA_EINVAL, "kv4_indexer: HI=%d outside [1,256]", HI);
+  if (Tq < 0 || Tq > kMaxElems) return fail(DSA_EINVAL, "kv4_indexer: Tq=%lld", (long long)Tq);
+  if (span < 0 || span > cache->S) return fail(DSA_EINVAL, "kv4_indexer: span=%lld outside [0, S=%lld]", (long long)span, (long long)cache->S);
+  if (cache->B * Tq * span == 0) return DSA_OK;
+  if (cache->B * Tq > kMaxElems || cache->B * Tq * span >= (int64_t{1} << 40)) return fail(DSA_EINVAL, "kv4_indexer: scores too large");
+  if (!q_idx || !w_idx || !scores) return fail(DSA_EINVAL, "kv4_indexer: null pointer");
+  if (!aligned16(q_idx) || !aligned4(scores) || !aligned4(count)) return fail(DSA_EINVAL, "kv4_indexer: q_idx must be 16-byte aligned, scores and count 4-byte");
+  return hip_status(dsa::launch_kv4_indexer(kv4_of(cache), q_idx, w_idx, cache->idx_dtype, count, Tq, HI, span,
+                                            scores, static_cast<hipStream_t>(stream)),
+                    "dsa_kv4_indexer_scores");
+}
+
+int64_t dsa_kv4_attention_workspace_bytes(const dsa_kv4_cache* cache, int64_t Tq, int HQ, int listed,
+                                          int64_t n, int accumulate) {
+  if (check_kv4_attention(cache, Tq, HQ, listed != 0, n, "kv4_attention_workspace_bytes") != DSA_OK) return 0;
+  return dsa::kv4_attn_workspace(kv4_of(cache), Tq, HQ, n, accumulate != 0);
+}
+
+int dsa_kv4_attention(const dsa_kv4_cache* cache, const void* Q, int dtype, const int32_t* slots,
+                      const int32_t* count, int64_t Tq, int HQ, int64_t n, int accumulate,
+                      float scale, float* out, void* workspace, int64_t workspace_bytes,
+                      void* stream) {
+  int rc = check_kv4_attention(cache, Tq, HQ, slots != nullptr, n, "kv4_attention");
+  if (rc != DSA_OK) return rc;
+  if (!dtype_ok(dtype)) return fail(DSA_EINVAL, "kv4_attention: unknown dtype %d", dtype);
+  if (!std::isfinite(scale)) return fail(DSA_EINVAL, "kv4_attention: scale must be finite");
+  if (workspace_bytes < 0) return fail(DSA_EINVAL, "kv4_attention: negative workspace size");
+  if (cache->B * Tq == 0) return DSA_OK;
+  if (!Q || !out) return fail(DSA_EINVAL, "kv4_attention: null pointer");
+  if (!aligned16(Q) || !aligned16(out)) return fail(DSA_EINVAL, "kv4_attention: Q and out must be 16-byte aligned");
+  if (!aligned4(slots) || !aligned4(count)) return fail(DSA_EINVAL, "kv4_attention: slots and count must be 4-byte aligned");
+  const dsa::Kv4 c = kv4_of(cache);
+  const int64_t need = dsa::kv4_attn_workspace(c, Tq, HQ, n, accumulate != 0);
+  if (need > 0 && (!workspace || !aligned16(workspace) || workspace_bytes < need))
+    return fail(DSA_EINVAL, "kv4_attention: needs a 16-byte aligned workspace of %lld bytes (got %lld)", (long long)need, (long long)workspace_bytes);
+  return hip_status(dsa::launch_kv4_attn(c, Q, dtype, slots, count, Tq, HQ, n, accumulate != 0, scale, out,
+                                         workspace, static_cast<hipStream_t>(stream)),
+                    "dsa_kv4_attention");
+}
+
+int dsa_kv4_evict(const dsa_kv4_cache* cache, int64_t keep, int64_t recent, int32_t* src,
+                  int32_t* dst, void* stream) {
+  int rc = check_kv4(cache, true, false, "kv4_evict");
+  if (rc != DSA_OK) return rc;
+  if (keep < 0 || recent < 0 || recent > keep)
+    return fail(DSA_EINVAL, "kv4_evict: keep=%lld recent=%lld must be 0 <= recent <= keep", (long long)keep, (long long)recent);
+  if (cache->B == 0 || keep >= cache->S) return DSA_OK;
+  if (keep > 0 && (!src || !dst)) return fail(DSA_EINVAL, "kv4_evict: null pointer");
+  if (!aligned4(src) || !aligned4(dst)) return fail(DSA_EINVAL, "kv4_evict: src and dst must be 4-byte aligned");
+  return hip_status(dsa::launch_kv4_evict(kv4_of(cache), keep, recent, src, dst, static_cast<hipStream_t>(stream)),
+                    "dsa_kv4_evict");
 }
 
 }  // extern "C"

@@ -1,0 +1,323 @@
+"""DSA decode over a cache held in 4 bits: what follows the prompt.
+
+The forwards of dsa_attention take whole sequences.  Here a sequence's keys and
+values stay on the GPU between calls, in OCP MXFP4 (e2m1 codes, one power-of-two
+scale per 32 elements: 4.25 bits a value), and each new token is appended,
+attends, and the slots that drew the least attention make room:
+
+    kv4_append           tokens into the cache (and index keys beside them)
+    kv4_indexer_scores   lightning indexer of the new tokens against the cached index keys
+    kv4_attention        attention over the whole cache, or over the slots that the
+                         select chose (topk_threshold.topk_indices of the scores);
+                         accumulates each slot's attention weight
+    kv4_evict            down to a budget, by that weight, the newest tokens kept
+    kv4_rows             slots back as values
+    dsa_decode           a DSA step of all of them
+
+Every function enqueues gfx950 kernels of libdsa_amd.so on torch's current
+stream of the cache's device and returns without synchronising; none moves
+anything to the host.  All can be captured into HIP graphs (replays advance the
+cache, whose counters live on the GPU).  Like the forwards they have no backward.
+The reference has no counterpart: it has no cache and no single-token form.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+
+import torch
+
+import _dsa_lib as L
+from topk_threshold import topk_indices
+
+
+class KV4Cache:
+    """The buffers of B sequences' caches of S slots (include/dsa_amd.h,
+    dsa_kv4_cache), all contiguous on one GPU and written in place:
+
+      codes uint8 [B, S, HKV, (DK+DV)/2]   scales uint8 [B, S, HKV, (DK+DV)/32]
+      k_idx [B, S, DI] fp32, bf16 or fp16 (None: no index keys)
+      length, seen, lost int32 [B]   position int32 [B, S]   weight fp32 [B, S]
+
+    length: slots in use; seen: tokens appended so far; lost: tokens that found
+    no free slot (check() raises where there are any); weight: attention weight
+    accumulated by kv4_attention.  Made from buffers in use, what is not given
+    starts as after an append of `length` tokens.  A cache of index keys alone
+    (codes None) serves kv4_indexer_scores."""
+
+    def __init__(self, codes: torch.Tensor | None, scales: torch.Tensor | None,
+                 length: torch.Tensor, k_idx: torch.Tensor | None = None,
+                 position: torch.Tensor | None = None, weight: torch.Tensor | None = None,
+                 seen: torch.Tensor | None = None, lost: torch.Tensor | None = None,
+                 DK: int | None = None):
+        first = codes if codes is not None else k_idx
+        assert first is not None, "a cache needs codes or index keys"
+        L.require_gpu(first)
+        assert first.dim() == (4 if codes is not None else 3), "codes [B,S,HKV,(DK+DV)/2], k_idx [B,S,DI]"
+        B, S = first.shape[:2]
+        device = first.device
+        HKV = DV = DI = 0
+        if codes is not None:
+            HKV, row = codes.shape[2], codes.shape[3]
+            DK = row if DK is None else int(DK)
+            DV = 2 * row - DK
+            assert DK > 0 and DV > 0 and DK % 32 == 0 and DV % 32 == 0, \
+                f"DK={DK} DV={DV} must be multiples of 32"
+            assert scales is not None, "codes go with scales"
+            if position is None:
+                position = torch.arange(S, device=device, dtype=torch.int32).repeat(B, 1)
+            if weight is None:
+                weight = torch.zeros(B, S, device=device)
+            if seen is None:
+                seen = length.clone()
+            if lost is None:
+                lost = torch.zeros(B, device=device, dtype=torch.int32)
+            self._is("codes", codes, (B, S, HKV, row), torch.uint8, device)
+            self._is("scales", scales, (B, S, HKV, row // 16), torch.uint8, device)
+            self._is("position", position, (B, S), torch.int32, device)
+            self._is("weight", weight, (B, S), torch.float32, device)
+            self._is("seen", seen, (B,), torch.int32, device)
+            self._is("lost", lost, (B,), torch.int32, device)
+        self._is("length", length, (B,), torch.int32, device)
+        idx_dtype = torch.float32
+        if k_idx is not None:
+            DI, idx_dtype = k_idx.shape[2], k_idx.dtype
+            assert idx_dtype in (torch.float32, torch.bfloat16, torch.float16), \
+                f"index keys: fp32, bf16 or fp16 (got {idx_dtype})"
+            self._is("k_idx", k_idx, (B, S, DI), idx_dtype, device)
+        self.codes, self.scales, self.k_idx = codes, scales, k_idx
+        self.length, self.seen, self.lost = length, seen, lost
+        self.position, self.weight = position, weight
+        self.B, self.S, self.HKV, self.DK, self.DV, self.DI = B, S, HKV, DK or 0, DV, DI
+        self.device, self.idx_dtype = device, idx_dtype
+
+        def at(x):
+            return x.data_ptr() if x is not None else None
+
+        self._c = L.Kv4Cache(at(codes), at(scales), at(k_idx), at(length), at(seen), at(lost),
+                             at(position), at(weight), B, S, HKV, self.DK, DV, DI,
+                             L.dtype_code(idx_dtype))
+        self._ref = ctypes.addressof(self._c)
+
+    @staticmethod
+    def _is(name, x, shape, dtype, device):
+        assert x.device == device and x.dtype == dtype and tuple(x.shape) == shape \
+            and x.is_contiguous() and (x.data_ptr() % 16 == 0 or not x.numel()), \
+            f"{name}: contiguous 16-byte aligned {dtype} {shape} on {device} " \
+            f"(got {x.dtype} {tuple(x.shape)} on {x.device})"
+
+    @classmethod
+    def empty(cls, B: int, S: int, HKV: int, DK: int, DV: int, DI: int = 0,
+              idx_dtype: torch.dtype = torch.bfloat16, device="cuda") -> "KV4Cache":
+        """A cache with nothing in it (DI = 0: without index keys)."""
+        assert DK > 0 and DV > 0 and DK % 32 == 0 and DV % 32 == 0, \
+            f"DK={DK} DV={DV} must be multiples of 32"
+        dev = torch.device(device)
+        if dev.type == "cuda" and dev.index is None:
+            dev = torch.device("cuda", torch.cuda.current_device())
+        return cls(torch.zeros(B, S, HKV, (DK + DV) // 2, device=dev, dtype=torch.uint8),
+                   torch.zeros(B, S, HKV, (DK + DV) // 32, device=dev, dtype=torch.uint8),
+                   torch.zeros(B, device=dev, dtype=torch.int32),
+                   torch.zeros(B, S, DI, device=dev, dtype=idx_dtype) if DI else None, DK=DK)
+
+    def check(self) -> None:
+        """RuntimeError if a token found no free slot (waits for the GPU)."""
+        if self.lost is not None and int(self.lost.max()) > 0:
+            raise RuntimeError(f"KV4Cache: {int(self.lost.sum())} tokens found no free slot "
+                               f"(S={self.S}): evict before appending")
+
+
+def _stored(cache: KV4Cache) -> None:
+    assert cache.codes is not None, "this cache holds index keys only"
+
+
+def _ints(x: torch.Tensor | None, shape, name: str, cache: KV4Cache):
+    """An optional int32 tensor and its pointer; contiguous copies where it is not."""
+    if x is None:
+        return None, None
+    assert x.dtype == torch.int32 and tuple(x.shape) == shape and x.device == cache.device, \
+        f"{name}: int32 {shape} on {cache.device} (got {x.dtype} {tuple(x.shape)} on {x.device})"
+    x = x.contiguous()
+    return x, x.data_ptr()
+
+
+def _on(cache: KV4Cache, *xs: torch.Tensor) -> None:
+    for x in xs:
+        assert x.device == cache.device, f"inputs must be on the cache's GPU {cache.device} (got {x.device})"
+
+
+def _span(cache: KV4Cache, span: int | None) -> int:
+    n = cache.S if span is None else int(span)
+    assert 0 <= n <= cache.S, f"span={n} outside [0, S={cache.S}]"
+    return n
+
+
+def kv4_append(cache: KV4Cache, K: torch.Tensor, V: torch.Tensor, k_idx: torch.Tensor | None = None,
+               *, count: torch.Tensor | None = None, weight: torch.Tensor | None = None,
+               restart: bool = False) -> None:
+    """Quantise T new tokens a sequence into the cache's next slots.
+
+    K [B,T,HKV,DK], V [B,T,HKV,DV] (fp32, bf16 or fp16), k_idx [B,T,DI] where the
+    cache holds index keys.  count int32 [B]: how many of the T are tokens (a
+    padded batch; default all).  weight fp32 [B,T]: the new slots' first weights,
+    e.g. what a prompt's own attention gave them (default 0).  restart: the
+    sequences begin anew, at slot 0 and position 0 (a new batch of prompts).
+    Tokens past slot S - 1 are not stored but counted in cache.lost."""
+    _stored(cache)
+    B, T = K.shape[:2]
+    assert K.shape == (cache.B, T, cache.HKV, cache.DK), \
+        f"K shape {tuple(K.shape)} != {(cache.B, T, cache.HKV, cache.DK)}"
+    assert V.shape == (cache.B, T, cache.HKV, cache.DV), \
+        f"V shape {tuple(V.shape)} != {(cache.B, T, cache.HKV, cache.DV)}"
+    _on(cache, K, V)
+    assert (k_idx is None) == (cache.k_idx is None), "index keys go with a cache that holds them"
+    dt = L.common_dtype(K, V)
+    K, V = L.prep(K, dt), L.prep(V, dt)
+    if k_idx is not None:
+        assert k_idx.shape == (B, T, cache.DI), f"k_idx shape {tuple(k_idx.shape)} != {(B, T, cache.DI)}"
+        _on(cache, k_idx)
+        k_idx = L.prep(k_idx, cache.idx_dtype)
+    if weight is not None:
+        assert weight.shape == (B, T), f"weight shape {tuple(weight.shape)} != {(B, T)}"
+        _on(cache, weight)
+        weight = L.prep(weight, torch.float32)
+    count, count_ptr = _ints(count, (B,), "count", cache)
+    with L.on_device(cache.device):
+        L.check(L.lib().dsa_kv4_append(
+            cache._ref, K.data_ptr(), V.data_ptr(), L.dtype_code(dt),
+            k_idx.data_ptr() if k_idx is not None else None,
+            weight.data_ptr() if weight is not None else None, count_ptr, T, 1 if restart else 0,
+            L.stream_ptr(cache.device)), "kv4_append")
+
+
+def kv4_rows(cache: KV4Cache, slots: torch.Tensor | None = None, *, span: int | None = None,
+             dtype: torch.dtype = torch.float32):
+    """The values that slots stand for: (K [B,N,HKV,DK], V [B,N,HKV,DV]).
+
+    slots int32 [B,N], or the first `span` slots (default all).  Slots that hold
+    nothing give zeros.  Exact in fp32 and bf16."""
+    _stored(cache)
+    N = slots.shape[1] if slots is not None else _span(cache, span)
+    assert slots is None or span is None, "slots or span, not both"
+    slots, slots_ptr = _ints(slots, (cache.B, N), "slots", cache)
+    code = L.dtype_code(dtype)
+    K = torch.empty(cache.B, N, cache.HKV, cache.DK, device=cache.device, dtype=dtype)
+    V = torch.empty(cache.B, N, cache.HKV, cache.DV, device=cache.device, dtype=dtype)
+    with L.on_device(cache.device):
+        L.check(L.lib().dsa_kv4_rows(cache._ref, slots_ptr, N, code, K.data_ptr(), V.data_ptr(),
+                                     L.stream_ptr(cache.device)), "kv4_rows")
+    return K, V
+
+
+def kv4_indexer_scores(cache: KV4Cache, q_idx: torch.Tensor, w_idx: torch.Tensor, *,
+                       span: int | None = None, count: torch.Tensor | None = None) -> torch.Tensor:
+    """Lightning indexer of the last Tq appended tokens against the cached index
+    keys: [B,Tq,span] fp32, -inf where a token does not see the slot (its own and
+    the earlier slots it sees, the later tokens' it does not).
+
+    q_idx [B,Tq,HI,DI], w_idx [B,Tq,HI].  span: only the first span slots (default
+    all S).  count int32 [B]: how many of the Tq are tokens, as kv4_append's; the
+    others' rows are -inf."""
+    assert cache.k_idx is not None, "this cache holds no index keys"
+    B, Tq, HI, DI = q_idx.shape
+    assert (B, DI) == (cache.B, cache.DI), f"q_idx shape {tuple(q_idx.shape)}: B={cache.B}, DI={cache.DI}"
+    assert w_idx.shape == (B, Tq, HI), f"w_idx shape {tuple(w_idx.shape)} != {(B, Tq, HI)}"
+    _on(cache, q_idx, w_idx)
+    n = _span(cache, span)
+    q_idx, w_idx = L.prep(q_idx, cache.idx_dtype), L.prep(w_idx, cache.idx_dtype)
+    count, count_ptr = _ints(count, (B,), "count", cache)
+    scores = torch.empty(B, Tq, n, device=cache.device, dtype=torch.float32)
+    with L.on_device(cache.device):
+        L.check(L.lib().dsa_kv4_indexer_scores(
+            cache._ref, q_idx.data_ptr(), w_idx.data_ptr(), count_ptr, Tq, HI, n, scores.data_ptr(),
+            L.stream_ptr(cache.device)), "kv4_indexer_scores")
+    return scores
+
+
+def kv4_attention(cache: KV4Cache, Q: torch.Tensor, *, slots: torch.Tensor | None = None,
+                  span: int | None = None, count: torch.Tensor | None = None,
+                  accumulate: bool = False, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of the last Tq appended tokens over the cache: O [B,Tq,HQ,DV] fp32.
+
+    Q [B,Tq,HQ,DK] (fp32, bf16 or fp16), HQ a multiple of HKV (query head h reads
+    K/V head h // (HQ/HKV)); scale 1/sqrt(DK).  Over all slots that a token sees
+    (its own and the earlier ones) among the first `span`, or only those listed
+    in slots int32 [B,Tq,k] (topk_indices of kv4_indexer_scores); entries that it
+    does not see count for nothing.  A token that sees nothing gets NaN.
+    count int32 [B]: how many of the Tq are tokens; the others see nothing.
+    accumulate: add each slot's probabilities, over tokens and heads, to
+    cache.weight (what kv4_evict goes by)."""
+    _stored(cache)
+    B, Tq, HQ, DK = Q.shape
+    assert (B, DK) == (cache.B, cache.DK), f"Q shape {tuple(Q.shape)}: B={cache.B}, DK={cache.DK}"
+    _on(cache, Q)
+    n = _span(cache, span)
+    if slots is not None:
+        assert slots.dim() == 3, "slots: int32 [B, Tq, k]"
+        assert span is None, "slots or span, not both"
+        n = slots.shape[2]
+        slots, slots_ptr = _ints(slots, (B, Tq, n), "slots", cache)
+    else:
+        slots_ptr = None
+    count, count_ptr = _ints(count, (B,), "count", cache)
+    dt = L.common_dtype(Q)
+    Q = L.prep(Q, dt)
+    if out is None:
+        out = torch.empty(B, Tq, HQ, cache.DV, device=cache.device, dtype=torch.float32)
+    else:
+        L.check_out(out, B * Tq * HQ * cache.DV, cache.device)
+    acc = 1 if accumulate else 0
+    with L.on_device(cache.device):
+        nws = L.lib().dsa_kv4_attention_workspace_bytes(cache._ref, Tq, HQ, 0 if slots is None else 1,
+                                                        n, acc)
+        ws = torch.empty(max(nws, 16), device=cache.device, dtype=torch.uint8)
+        L.check(L.lib().dsa_kv4_attention(
+            cache._ref, Q.data_ptr(), L.dtype_code(dt), slots_ptr, count_ptr, Tq, HQ, n, acc,
+            1.0 / math.sqrt(DK), out.data_ptr(), ws.data_ptr(), nws, L.stream_ptr(cache.device)),
+            "kv4_attention")
+    return out
+
+
+def kv4_evict(cache: KV4Cache, keep: int, recent: int = 0) -> torch.Tensor:
+    """Evict every sequence that has more than `keep` slots down to them: the
+    `recent` newest tokens stay, then those of the largest accumulated weight
+    (among equals the lowest slot).
+
+    Kept slots at or past `keep` move into the freed ones.  Returns them as int32
+    [2,B,M], M = min(keep, S - keep): the slots they came from and went to, in
+    order, -1 past the last (for buffers of the caller's that go by slot)."""
+    _stored(cache)
+    keep, recent = int(keep), int(recent)
+    moved = torch.empty(2, cache.B, max(0, min(keep, cache.S - keep)), device=cache.device,
+                        dtype=torch.int32)
+    with L.on_device(cache.device):
+        L.check(L.lib().dsa_kv4_evict(cache._ref, keep, recent, moved[0].data_ptr(),
+                                      moved[1].data_ptr(), L.stream_ptr(cache.device)), "kv4_evict")
+    return moved
+
+
+def dsa_decode(cache: KV4Cache, q_idx, k_idx, w_idx, Q, K, V, top_k: int, *,
+               span: int | None = None, count: torch.Tensor | None = None,
+               keep: int | None = None, recent: int = 0) -> torch.Tensor:
+    """A DSA step of Tq new tokens a sequence: append them, score the cached index
+    keys, select the top_k slots of each token, attend to those, and (with `keep`)
+    accumulate their weights and evict down to `keep` slots.  O [B,Tq,HQ,DV] fp32.
+
+    q_idx [B,Tq,HI,DI]  k_idx [B,Tq,DI]  w_idx [B,Tq,HI]  Q [B,Tq,HQ,DK]
+    K [B,Tq,HKV,DK]  V [B,Tq,HKV,DV].  Exactly top_k slots a token (the lowest
+    slot wins ties), all it sees where it sees fewer.  span: no sequence has more
+    slots than that in use (default S); where top_k >= span all of them are
+    attended to and nothing is scored.  The cache needs room for the Tq tokens:
+    keep + Tq <= S in steady state."""
+    assert top_k >= 1, "top_k must be >= 1"
+    n = _span(cache, span)
+    kv4_append(cache, K, V, k_idx, count=count)
+    slots = None
+    if top_k < n:
+        scores = kv4_indexer_scores(cache, q_idx, w_idx, span=n, count=count)
+        _, slots = topk_indices(scores, int(top_k))
+    out = kv4_attention(cache, Q, slots=slots, span=None if slots is not None else n, count=count,
+                        accumulate=keep is not None)
+    if keep is not None:
+        kv4_evict(cache, keep, recent)
+    return out

@@ -423,6 +423,121 @@ int dsa_fused_forward(const void* q_idx, const void* k_idx, const void* w_idx,
 /* Largest T dsa_fused_forward accepts (2048). */
 int64_t dsa_fused_max_T(void);
 
+/*
+ * ---- Decode over a cache held in 4 bits -------------------------------------
+ *
+ * The keys and values of B sequences, S slots each, in OCP MXFP4: e2m1 codes
+ * (0, 1/2, 1, 3/2, 2, 3, 4, 6 with a sign; the even element of a pair in the
+ * low nibble) and one E8M0 scale byte, 2^(byte-127), per 32 elements of a head's
+ * row.  A slot holds one token; the slots in use are 0 .. length-1, in no
+ * particular order of positions once something was evicted.  The buffers are
+ * device memory of the caller's, dense row-major, in this struct on the host,
+ * which is read before the call returns.  A call that writes the cache and any
+ * other call on it need the order of one stream or an event between them; calls
+ * that only read it may overlap.  Values of length outside [0, S] count as the
+ * nearer end.
+ * No reference counterpart: it has no cache and no single-token form.
+ * Constraints: B <= 65535; 1 <= S < 2^31; 1 <= HKV <= 1024; DK, DV multiples of 32, at most
+ *   1024; one sequence's codes below 2 GiB; DI = 0 (no index keys: k_idx null) or
+ *   16 (fp32 only), 32, 64, 128 or 256; codes and k_idx 16-byte aligned, the
+ *   others 4-byte.
+ */
+typedef struct dsa_kv4_cache {
+  uint8_t* codes;    /* [B, S, HKV, (DK+DV)/2]: K, then V, of each head; null: index keys only */
+  uint8_t* scales;   /* [B, S, HKV, (DK+DV)/32], in the same order                             */
+  void* k_idx;       /* [B, S, DI] index keys of idx_dtype (fp32, bf16 or fp16), or null       */
+  int32_t* length;   /* [B] slots in use                                                       */
+  int32_t* seen;     /* [B] tokens appended so far: the position of the next one               */
+  int32_t* lost;     /* [B] tokens that found no free slot                                     */
+  int32_t* position; /* [B, S] each slot's token's position                                    */
+  float* weight;     /* [B, S] attention weight accumulated on each slot                       */
+  int64_t B, S;
+  int HKV, DK, DV, DI, idx_dtype;
+} dsa_kv4_cache;
+
+/*
+ * Append: token i of sequence b goes into slot length[b] + i, for i < count[b]
+ * (count null: T).  With restart != 0 the sequences begin anew, at slot 0 and
+ * position 0.  Then length, seen and lost are brought up to date; tokens past
+ * slot S - 1 are counted in lost and not stored.  Slots behind the last token
+ * keep what they hold.
+ *   A block of 32 elements gets the least scale 2^e with max|x| < 7 * 2^e (so no
+ * element is off by more than half of the widest step, 2^e), 2^-125 <= 2^e <=
+ * 2^125; its elements x / 2^e round to the nearest e2m1, ties to even, beyond 6
+ * to 6.  A block with an Inf or NaN in it becomes NaN.
+ *   K [B,T,HKV,DK], V [B,T,HKV,DV] of dtype (fp32, bf16, fp16); k_idx [B,T,DI] of
+ *   the cache's idx_dtype, null exactly where the cache holds none; weight [B,T]
+ *   fp32, the new slots' first weights (null: 0).  16-byte aligned (weight and
+ *   count 4).
+ */
+int dsa_kv4_append(const dsa_kv4_cache* cache, const void* K, const void* V, int dtype,
+                   const void* k_idx, const float* weight, const int32_t* count, int64_t T,
+                   int restart, void* stream);
+
+/*
+ * The values that N slots of each sequence stand for, K [B,N,HKV,DK] and
+ * V [B,N,HKV,DV] of dtype (exact in fp32 and bf16; fp16 rounds, to Inf past its
+ * range): slots [B,N], or 0 .. N-1 where null.  Slots outside [0, length) give
+ * zeros.  K and V 16-byte aligned.
+ */
+int dsa_kv4_rows(const dsa_kv4_cache* cache, const int32_t* slots, int64_t N, int dtype, void* K,
+                 void* V, void* stream);
+
+/*
+ * Indexer scores of each sequence's last Tq tokens against the cached index keys:
+ *   scores[b,t,s] = sum_j w[b,t,j] * ReLU(<q[b,t,j,:], k_idx[b,s,:]>)
+ * where query t sees slot s, s < length[b] - n + t + 1, else -inf; n = count[b]
+ * (null: Tq) of the Tq queries are tokens, those from n on see nothing.
+ * scores [B,Tq,span] fp32: the first span slots.  fp32 sums.
+ *   q_idx [B,Tq,HI,DI] (16-byte aligned), w_idx [B,Tq,HI], of the cache's
+ *   idx_dtype; 1 <= HI <= 256; span <= S; B*Tq*span < 2^40.
+ * Replaces: nothing (the reference's indexer, lightning_indexer.py:54-125, is
+ *   the square [B,T,T]).
+ */
+int dsa_kv4_indexer_scores(const dsa_kv4_cache* cache, const void* q_idx, const void* w_idx,
+                           const int32_t* count, int64_t Tq, int HI, int64_t span, float* scores,
+                           void* stream);
+
+/*
+ * Attention of each sequence's last Tq tokens over the cache:
+ *   O[b,t,h,:] = sum_s p[b,t,h,s] V[b,s,h/G,:],
+ *   p[b,t,h,:] = softmax_s(<Q[b,t,h], K[b,s,h/G]> * scale),  G = HQ / HKV,
+ * over the slots that query t sees (as above) among the first n, or (slots not
+ * null) over those of them that slots[b,t,0..n) lists: entries outside what the
+ * query sees count for nothing, one listed twice counts twice.  A query that
+ * sees no slot gets O = NaN, as dsa_sparse_attn_threshold's empty rows do.
+ *   accumulate != 0: weight[b,s] += sum over t and h of p[b,t,h,s], with the same
+ * result in every run.
+ *   fp32 logits, softmax and sums; a probability enters the sum over V as two
+ * bf16 pieces (16 bits).
+ *   Q [B,Tq,HQ,DK] of dtype (fp32, bf16, fp16), out [B,Tq,HQ,DV] fp32, 16-byte
+ *   aligned; HQ a multiple of HKV, at most 1024; n < 2^31; without slots n <= S;
+ *   B*Tq*HQ < 2^31; DK = DV in {32, 64, 96, 128, 192, 256} or DK 192 with DV 128
+ *   (else DSA_EUNSUPPORTED).
+ *   workspace: device memory of dsa_kv4_attention_workspace_bytes, 16-byte
+ *   aligned, used by no other work until the launches complete, contents on entry
+ *   free (a smaller one is refused).  Needs the device (its compute-unit count).
+ */
+int64_t dsa_kv4_attention_workspace_bytes(const dsa_kv4_cache* cache, int64_t Tq, int HQ, int listed,
+                                          int64_t n, int accumulate);
+int dsa_kv4_attention(const dsa_kv4_cache* cache, const void* Q, int dtype, const int32_t* slots,
+                      const int32_t* count, int64_t Tq, int HQ, int64_t n, int accumulate,
+                      float scale, float* out, void* workspace, int64_t workspace_bytes,
+                      void* stream);
+
+/*
+ * Evict down to `keep` slots every sequence that has more.  The slots of the
+ * `recent` newest positions (position >= seen - recent) stay before all others,
+ * then those of the largest weight (NaN above +inf; among equals the lowest slot
+ * stays).  Kept slots at or past `keep` move into the freed ones below it, the
+ * i-th into the i-th, both ascending: codes, scales, index key, position and
+ * weight.  length becomes keep; slots from keep on keep what they hold.
+ *   src, dst [B, M], M = min(keep, S - keep): where the i-th moved slot came from
+ * and went, -1 past the last.  0 <= recent <= keep; keep >= S does nothing.
+ */
+int dsa_kv4_evict(const dsa_kv4_cache* cache, int64_t keep, int64_t recent, int32_t* src,
+                  int32_t* dst, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
