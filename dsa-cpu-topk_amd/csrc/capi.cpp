@@ -159,7 +159,9 @@ int check_kv4_attention(const dsa_kv4_cache* c, int64_t Tq, int HQ, bool listed,
   if (Tq < 0 || n < 0 || n > kMaxElems) return fail(DSA_EINVAL, "%s: Tq=%lld n=%lld", who, (long long)Tq, (long long)n);
   if (HQ < 1 || HQ > 1024 || HQ % c->HKV) return fail(DSA_EINVAL, "%s: HQ=%d must be a multiple of HKV=%d, at most 1024", who, HQ, c->HKV);
   if (!listed && n > c->S) return fail(DSA_EINVAL, "%s: n=%lld > S=%lld", who, (long long)n, (long long)c->S);
-  if (Tq > kMaxElems || c->B * Tq * HQ > kMaxElems) return fail(DSA_EINVAL, "%s: B*Tq*HQ must be < 2^31", who);
+  // a launch holds 2^32 threads
+  if (Tq > kMaxElems || c->B * Tq * HQ >= (int64_t{1} << 23) || c->B * n >= (int64_t{1} << 31))
+    return fail(DSA_EINVAL, "%s: B*Tq*HQ must be < 2^23 and B*n < 2^31", who);
   if (!dsa::kv4_attn_supported(c->DK, c->DV))
     return fail(DSA_EUNSUPPORTED, "%s: no kernel for DK=%d DV=%d (equal ones of 32, 64, 96, 128, 192, 256, or 192 with 128)", who, c->DK, c->DV);
   return DSA_OK;
@@ -540,7 +542,7 @@ int dsa_kv4_append(const dsa_kv4_cache* cache, const void* K, const void* V, int
   int rc = check_kv4(cache, true, false, "kv4_append");
   if (rc != DSA_OK) return rc;
   if (!dtype_ok(dtype)) return fail(DSA_EINVAL, "kv4_append: unknown dtype %d", dtype);
-  if (T < 0 || T > kMaxElems) return fail(DSA_EINVAL, "kv4_append: T=%lld", (long long)T);
+  if (T < 0 || T >= (int64_t{1} << 25)) return fail(DSA_EINVAL, "kv4_append: T=%lld outside [0, 2^25)", (long long)T);
   if ((k_idx != nullptr) != (cache->k_idx != nullptr) && cache->B * T != 0)
     return fail(DSA_EINVAL, "kv4_append: index keys go with a cache that holds them");
   // with T = 0 there is nothing to do but a restart's counters
@@ -558,7 +560,7 @@ int dsa_kv4_rows(const dsa_kv4_cache* cache, const int32_t* slots, int64_t N, in
   int rc = check_kv4(cache, true, false, "kv4_rows");
   if (rc != DSA_OK) return rc;
   if (!dtype_ok(dtype)) return fail(DSA_EINVAL, "kv4_rows: unknown dtype %d", dtype);
-  if (N < 0 || N > kMaxElems) return fail(DSA_EINVAL, "kv4_rows: N=%lld", (long long)N);
+  if (N < 0 || N >= (int64_t{1} << 25)) return fail(DSA_EINVAL, "kv4_rows: N=%lld outside [0, 2^25)", (long long)N);
   if (cache->B * N == 0) return DSA_OK;
   if (!K || !V) return fail(DSA_EINVAL, "kv4_rows: null pointer");
   if (!aligned16(K) || !aligned16(V) || !aligned4(slots)) return fail(DSA_EINVAL, "kv4_rows: K and V must be 16-byte aligned, slots 4-byte");

@@ -41,7 +41,7 @@ __device__ __forceinline__ int32_t kv4_visible(const int32_t* length, const int3
 }
 
 // An E8M0 byte as the fp32 scale the conversions take: 255 becomes +inf, for
-// which they give NaN (checked over the values here).
+// which they give NaN.
 __device__ __forceinline__ float e8m0(uint32_t byte) { return __uint_as_float(byte << 23); }
 
 // The scale byte of a block whose largest magnitude has these bits: the least

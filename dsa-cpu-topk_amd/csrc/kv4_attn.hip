@@ -1,111 +1,521 @@
 // kv4_attn.hip -- attention of new tokens over the 4-bit decode cache (gfx950):
 //   p = softmax over the visible (or listed) slots of <Q, K> * scale
 //   O = sum p V,   weight[b, slot] += sum over queries and heads of p
+//
+// One pass over the cache with a running maximum and sum.  A wave takes 32 slots
+// at a time of one K/V head and up to 16 query heads of its group, on
+// v_mfma_f32_16x16x32_bf16:
+//
+//   S^T[slot, head] = K Q^T    A: a lane holds 8-element runs of one slot's K row,
+//                              converted from e2m1 with their scale by one
+//                              instruction a pair (exact in bf16);
+//   O^T[d, head]  += V^T P^T   A: a lane holds W/16 columns of 8 slots (W = 128, 64
+//                              or 32 columns at a time), pairs of slots put
+//                              together by v_perm.
+//
+// The sum over a matrix instruction's 32 terms may take them in any order, as long
+// as both operands agree.  So a lane's K run is what one wide load brings, and the
+// slots of P are those whose logits the lane already has (rows 4g .. 4g+3 of S^T's
+// two tiles, g = lane / 16): nothing is transposed and nothing goes through LDS
+// until the block's four waves join their sums.
+//
+// fp32 operands enter as bf16 pieces: Q as one (bf16), two (fp16) or three (fp32),
+// p as three, which hold its 24 bits.  For up to 5 heads of a group the three
+// pieces of p stand side by side in the 16 columns (Q is repeated there, so each
+// lane has the p whose piece it takes) and one instruction takes them all.
+//
+// Long caches are split: a block takes one chunk of a query's slots and leaves
+// its sums, relative to its own maximum, for the second launch to join.  That
+// launch also adds the probabilities onto the slots' weights, from the logits that
+// the first one stored.
+#include "dsa_launch.h"
 #include "kv4.h"
+#include "tile_common.h"
 
 namespace dsa {
 namespace {
 
-constexpr int kNT = 256;
+constexpr int kWaves = kNT / kWave;
+constexpr int kTile = 32;                  // slots a wave takes at once
+constexpr int kStep = kTile * kWaves;      // slots a block takes at once
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kSlack = 8.0f;             // how far a logit may pass the running maximum, in powers of 2
 
-__device__ __forceinline__ int32_t slot_of(const int32_t* slots, int64_t row, int64_t n, int64_t j) {
-  return slots ? slots[row * n + j] : static_cast<int32_t>(j);
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+
+// A row of D elements in pieces of 128, 64 and 32 columns.
+__host__ __device__ constexpr int seg_count(int D) { return D / 128 + (D % 128) / 64 + (D % 64) / 32; }
+__host__ __device__ constexpr int seg_width(int D, int s) {
+  return s < D / 128 ? 128 : s == D / 128 && D % 128 >= 64 ? 64 : 32;
+}
+__host__ __device__ constexpr int seg_at(int D, int s) {
+  int at = 0;
+  for (int i = 0; i < s; ++i) at += seg_width(D, i);
+  return at;
 }
 
-// Logits of one query head: a thread a slot.
-template <typename Tag>
-__global__ __launch_bounds__(kNT) void logits_kernel(Kv4 c, const typename Tag::raw* __restrict__ Q,
-                                                     const int32_t* __restrict__ slots,
-                                                     const int32_t* __restrict__ count, int Tq, int HQ,
-                                                     int64_t n, float scale, float* __restrict__ logits) {
-  __shared__ float q[256];
-  const int64_t bt = blockIdx.z, b = bt / Tq, j = static_cast<int64_t>(blockIdx.x) * kNT + threadIdx.x;
-  const int h = blockIdx.y, hk = h / (HQ / c.HKV);
-  if (static_cast<int>(threadIdx.x) < c.DK) q[threadIdx.x] = to_f32(Tag{}, Q[(bt * HQ + h) * c.DK + threadIdx.x]);
-  __syncthreads();
-  if (j >= n) return;
-  const int32_t seen = kv4_visible(c.length, count, b, c.S, static_cast<int>(bt % Tq), Tq);
-  const int32_t s = slot_of(slots, bt, n, j);
-  if (s < 0 || s >= seen) return;
-  const int64_t slot = b * c.S + s;
-  const int u0 = hk * (c.DK + c.DV) / 8;
-  const uint32_t* w = reinterpret_cast<const uint32_t*>(c.codes) + slot * c.words() + u0;
-  const uint8_t* e = c.scales + slot * c.scale_bytes() + u0 / 4;
-  float dot = 0.0f;
-  for (int u = 0; u < c.DK / 8; ++u) {
-    float x[8];
-    e2m1_unpack8(w[u], e8m0(e[u / 4]), x);
+struct AttnArgs {
+  Kv4 c;
+  const void* Q;
+  const int32_t* slots;  // or null
+  const int32_t* count;  // or null
+  int Tq, HQ, G, row_tiles;
+  int64_t n, stride;  // slots a query; floats between rows of logits
+  int splits, chunk;  // a chunk is a multiple of kStep slots
+  float scale;
+  float* out;
+  float* part;    // [B*Tq*HQ][splits][DV] sums, where splits > 1
+  float2* ml;     // [B*Tq*HQ][splits] maximum (in powers of 2) and sum of exponentials
+  float* logits;  // [B*Tq*HQ][stride], in powers of 2, or null
+};
+
+__device__ __forceinline__ uint32_t load_u8(__amdgpu_buffer_rsrc_t r, uint32_t off) {
+  return __builtin_amdgcn_raw_buffer_load_b8(r, static_cast<int>(off), 0, 0);
+}
+template <int BYTES>
+__device__ __forceinline__ uint32_t load_small(__amdgpu_buffer_rsrc_t r, uint32_t off) {
+  if constexpr (BYTES == 4) return __float_as_uint(buffer_load_f32(r, static_cast<int>(off), 0, 0));
+  else if constexpr (BYTES == 2) return __builtin_amdgcn_raw_buffer_load_b16(r, static_cast<int>(off), 0, 0);
+  else return load_u8(r, off);
+}
+
+// What a wave holds of its 32 slots.
+template <int DK, int DV>
+struct Frag {
+  uint32_t k[2][DK / 32];
+  uint32_t ks[2][seg_count(DK)];
+  uint32_t v[8][seg_count(DV)];
+  uint32_t vs[8][seg_count(DV)];
+  uint32_t ok;  // bit i: the lane's i-th slot (4g + i of the first tile, then of the second) counts
+};
+
+constexpr uint32_t kNowhere = 0x80000000u;  // past any sequence's codes: such loads give zeros
+
+template <int DK, int DV>
+__device__ __forceinline__ void load_frag(Frag<DK, DV>& f, __amdgpu_buffer_rsrc_t rc,
+                                          __amdgpu_buffer_rsrc_t rs, const uint32_t (&krow)[2],
+                                          const uint32_t (&vrow)[8], int hk) {
+  const int lane = threadIdx.x & 63, g = lane >> 4, col = lane & 15;
+  const uint32_t head = hk * (DK + DV) / 2, heads = hk * (DK + DV) / 32;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) dot += q[u * 8 + i] * x[i];
+  for (int t = 0; t < 2; ++t) {
+    int w = 0;
+#pragma unroll
+    for (int s = 0; s < seg_count(DK); ++s) {
+      const int W = seg_width(DK, s), at = seg_at(DK, s);
+      const uint32_t off = krow[t] + head + at / 2 + g * (W / 8);
+      if (W == 128) {
+        const dsa_f32x4 x = buffer_load_f32x4(rc, static_cast<int>(off), 0, 0);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f.k[t][w + i] = __float_as_uint(x[i]);
+      } else if (W == 64) {
+        const dsa_f32x2 x = buffer_load_f32x2(rc, static_cast<int>(off), 0, 0);
+        f.k[t][w] = __float_as_uint(x[0]);
+        f.k[t][w + 1] = __float_as_uint(x[1]);
+      } else {
+        f.k[t][w] = load_small<4>(rc, off);
+      }
+      w += W / 32;
+      f.ks[t][s] = load_u8(rs, krow[t] / 16 + heads + (at + g * (W / 4)) / 32);
+    }
   }
-  logits[(bt * HQ + h) * n + j] = dot * scale;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+#pragma unroll
+    for (int s = 0; s < seg_count(DV); ++s) {
+      const int W = seg_width(DV, s), at = seg_at(DV, s);
+      const uint32_t off = vrow[i] + head + DK / 2 + at / 2 + col * (W / 32);
+      f.v[i][s] = W == 128 ? load_small<4>(rc, off) : W == 64 ? load_small<2>(rc, off) : load_small<1>(rc, off);
+      f.vs[i][s] = load_u8(rs, vrow[i] / 16 + heads + DK / 32 + (at + col * (W / 16)) / 32);
+    }
+  }
 }
 
-// Softmax and the sum over V of one query head; its probabilities replace the logits.
-__global__ __launch_bounds__(kNT) void rows_kernel(Kv4 c, const int32_t* __restrict__ slots,
-                                                   const int32_t* __restrict__ count, int Tq, int HQ,
-                                                   int64_t n, float* __restrict__ logits,
-                                                   float* __restrict__ out) {
-  __shared__ float red[kNT / kWave];
-  const int64_t bt = blockIdx.y, b = bt / Tq;
-  const int h = blockIdx.x, hk = h / (HQ / c.HKV);
-  const int32_t seen = kv4_visible(c.length, count, b, c.S, static_cast<int>(bt % Tq), Tq);
-  float* row = logits + (bt * HQ + h) * n;
-  auto ok = [&](int64_t j) {
-    const int32_t s = slot_of(slots, bt, n, j);
-    return s >= 0 && s < seen;
+template <int SEL>
+__device__ __forceinline__ uint32_t cvt2(uint32_t w, float scale) {
+  return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, SEL));
+}
+__device__ __forceinline__ float hi16(float x) { return __uint_as_float(__float_as_uint(x) & 0xffff0000u); }
+__device__ __forceinline__ uint32_t pack_hi(float lo, float hi) {  // the upper halves
+  return __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302u);
+}
+__device__ __forceinline__ f32x4 mfma(const u32x4& a, const u32x4& b, f32x4 c) {
+  return Mfma16x16x32<BF16>::run(a, b, c);
+}
+
+// 8 consecutive elements of a query row as NP pieces of bf16.
+template <typename Tag, int NP>
+__device__ __forceinline__ void load_q8(const typename Tag::raw* p, u32x4 (&q)[NP]) {
+  float x[8];
+  load_cvt<Tag, 8>(p, x);
+#pragma unroll
+  for (int i = 0; i < NP; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      q[i][j] = pack_hi(x[2 * j], x[2 * j + 1]);
+      x[2 * j] -= hi16(x[2 * j]);
+      x[2 * j + 1] -= hi16(x[2 * j + 1]);
+    }
+}
+
+template <typename Tag, int NP, int DK, int DV, bool SIDE, bool LISTED>
+__global__ __launch_bounds__(kNT) void attn_kernel(AttnArgs a) {
+  constexpr int NW = DK / 32, NO = DV / 16, LD = DV + 4;
+  __shared__ float sum_o[kWaves][16][LD];
+  __shared__ float sum_m[kWaves][16], sum_l[kWaves][16];
+
+  // Blocks go round-robin over the 8 XCDs; the blocks of one chunk (its heads)
+  // read the same rows, so they go to one XCD, one after another.
+  const int per = a.c.HKV * a.row_tiles;
+  const int64_t i = blockIdx.x / 8, chunk_id = i / per * 8 + blockIdx.x % 8;
+  if (chunk_id >= a.c.B * a.Tq * a.splits) return;
+  const int member = static_cast<int>(i % per), hk = member / a.row_tiles, rt = member % a.row_tiles;
+  const int64_t bt = chunk_id / a.splits, b = bt / a.Tq;
+  const int split = static_cast<int>(chunk_id % a.splits);
+  const int32_t seen = kv4_visible(a.c.length, a.count, b, a.c.S, static_cast<int>(bt % a.Tq), a.Tq);
+
+  const int wave = threadIdx.x / kWave, lane = threadIdx.x & 63, g = lane >> 4, col = lane & 15;
+  // the lane's query head, and (SIDE) which piece of p it takes
+  const int row = SIDE ? col % a.G : rt * 16 + col;
+  const int piece = SIDE ? col / a.G : 0;
+  const bool used = SIDE ? piece < 3 : row < a.G;
+  const int64_t bh = bt * a.HQ + hk * a.G;  // the group's first head
+
+  const int32_t limit = LISTED ? seen : static_cast<int32_t>(min(static_cast<int64_t>(seen), a.n));
+  const int64_t j_end = LISTED ? a.n : limit;
+  const int64_t c0 = static_cast<int64_t>(split) * a.chunk, c1 = min(c0 + a.chunk, j_end);
+  if (c0 >= c1 || limit == 0) {  // nothing here: no sum, and no sums to read
+    const int rows = min(16, a.G - rt * 16);
+    if (a.splits > 1) {
+      if (static_cast<int>(threadIdx.x) < rows)
+        a.ml[(bh + rt * 16 + threadIdx.x) * a.splits + split] = make_float2(-INFINITY, 0.0f);
+    } else {
+      for (int e = threadIdx.x; e < rows * DV; e += kNT)
+        a.out[(bh + rt * 16) * DV + e] = __builtin_nanf("");
+      if (static_cast<int>(threadIdx.x) < rows)
+        a.ml[bh + rt * 16 + threadIdx.x] = make_float2(-INFINITY, 0.0f);
+    }
+    return;
+  }
+
+  // the query row, in the order of the K runs
+  u32x4 q[NW][NP];
+  {
+    const typename Tag::raw* src = static_cast<const typename Tag::raw*>(a.Q) + (bh + row) * DK;
+    int w = 0;
+#pragma unroll
+    for (int s = 0; s < seg_count(DK); ++s) {
+      const int W = seg_width(DK, s);
+#pragma unroll
+      for (int j = 0; j < W / 32; ++j, ++w) {
+        if (used) load_q8<Tag, NP>(src + seg_at(DK, s) + g * (W / 4) + 8 * j, q[w]);
+        else
+#pragma unroll
+          for (int p = 0; p < NP; ++p) q[w][p] = u32x4{0, 0, 0, 0};
+      }
+    }
+  }
+  const uint32_t mask1 = piece >= 1 ? 0xffff0000u : 0u, mask2 = piece >= 2 ? 0xffff0000u : 0u;
+
+  const uint32_t cb = a.c.words() * 4;  // bytes of a slot's codes; of its scales: cb / 16
+  const uint8_t* codes = a.c.codes + b * a.c.S * cb;
+  const uint8_t* scales = a.c.scales + b * a.c.S * (cb / 16);
+  // rows end at the last slot that counts: loads past it give zeros
+  auto rsrc = [](const uint8_t* base, int64_t bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(base), 0, static_cast<int>(bytes), 0x00020000);
   };
-  float m = -INFINITY;
-  for (int64_t j = threadIdx.x; j < n; j += kNT)
-    if (ok(j)) m = fmaxf(m, row[j]);
-  m = wave_max(m);
-  if (threadIdx.x % kWave == 0) red[threadIdx.x / kWave] = m;
-  __syncthreads();
-  m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-  if (m == -INFINITY) m = 0.0f;
-  __syncthreads();
-  float l = 0.0f;
-  for (int64_t j = threadIdx.x; j < n; j += kNT)
-    if (ok(j)) l += expf(row[j] - m);
-  l = wave_sum(l);
-  if (threadIdx.x % kWave == 0) red[threadIdx.x / kWave] = l;
-  __syncthreads();
-  l = red[0] + red[1] + red[2] + red[3];
-  for (int64_t j = threadIdx.x; j < n; j += kNT)
-    if (ok(j)) row[j] = expf(row[j] - m) / l;
-  __syncthreads();
-  const int d = threadIdx.x;
-  if (d >= c.DV) return;
-  const int u = hk * (c.DK + c.DV) / 8 + (c.DK + d) / 8;
-  float o = 0.0f;
-  for (int64_t j = 0; j < n; ++j) {
-    const int32_t s = slot_of(slots, bt, n, j);
-    if (s < 0 || s >= seen) continue;
-    const int64_t slot = b * c.S + s;
-    float x[8];
-    e2m1_unpack8(reinterpret_cast<const uint32_t*>(c.codes)[slot * c.words() + u],
-                 e8m0(c.scales[slot * c.scale_bytes() + u / 4]), x);
-    float v = x[0];
+  const __amdgpu_buffer_rsrc_t all_codes = rsrc(codes, static_cast<int64_t>(limit) * cb);
+  const __amdgpu_buffer_rsrc_t all_scales = rsrc(scales, static_cast<int64_t>(limit) * (cb / 16));
+  const int32_t* list = LISTED ? a.slots + bt * a.n : nullptr;
+
+  auto load = [&](Frag<DK, DV>& f, int64_t j0) {
+    uint32_t krow[2], vrow[8];
+    f.ok = 0;
+    if constexpr (LISTED) {
+      auto at = [&](int64_t j) -> uint32_t {
+        const uint32_t s = j < c1 ? static_cast<uint32_t>(list[j]) : ~0u;
+        return s < static_cast<uint32_t>(limit) ? s * cb : kNowhere;
+      };
 #pragma unroll
-    for (int i = 1; i < 8; ++i) v = (d & 7) == i ? x[i] : v;
-    o += row[j] * v;
+      for (int t = 0; t < 2; ++t) krow[t] = at(j0 + 16 * t + col);
+#pragma unroll
+      for (int r = 0; r < 8; ++r) {
+        vrow[r] = at(j0 + (r >> 2) * 16 + 4 * g + (r & 3));
+        f.ok |= (vrow[r] != kNowhere ? 1u : 0u) << r;
+      }
+      load_frag<DK, DV>(f, all_codes, all_scales, krow, vrow, hk);
+    } else {
+#pragma unroll
+      for (int t = 0; t < 2; ++t) krow[t] = (16 * t + col) * cb;
+#pragma unroll
+      for (int r = 0; r < 8; ++r) vrow[r] = ((r >> 2) * 16 + 4 * g + (r & 3)) * cb;
+      const int64_t rest = max(static_cast<int64_t>(0), limit - j0);
+      load_frag<DK, DV>(f, rsrc(codes + j0 * cb, rest * cb), rsrc(scales + j0 * (cb / 16), rest * (cb / 16)), krow, vrow, hk);
+#pragma unroll
+      for (int r = 0; r < 8; ++r) f.ok |= ((r >> 2) * 16 + 4 * g + (r & 3) < rest ? 1u : 0u) << r;
+    }
+  };
+
+  f32x4 o[NO];
+#pragma unroll
+  for (int i2 = 0; i2 < NO; ++i2) o[i2] = f32x4{0, 0, 0, 0};
+  float m = -INFINITY, l = 0.0f;
+  const float to2 = a.scale * kLog2e;
+
+  auto compute = [&](const Frag<DK, DV>& f, int64_t j0) {
+    f32x4 s[2] = {f32x4{0, 0, 0, 0}, f32x4{0, 0, 0, 0}};
+    {
+      int w = 0;
+#pragma unroll
+      for (int sg = 0; sg < seg_count(DK); ++sg)
+#pragma unroll
+        for (int j = 0; j < seg_width(DK, sg) / 32; ++j, ++w)
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            const float e = e8m0(f.ks[t][sg]);
+            const uint32_t x = f.k[t][w];
+            const u32x4 k = {cvt2<0>(x, e), cvt2<1>(x, e), cvt2<2>(x, e), cvt2<3>(x, e)};
+#pragma unroll
+            for (int p = 0; p < NP; ++p) s[t] = mfma(k, q[w][p], s[t]);
+          }
+    }
+    float p[8];
+#pragma unroll
+    for (int r = 0; r < 8; ++r) p[r] = s[r >> 2][r & 3] * to2;
+    if (__builtin_amdgcn_ballot_w64(f.ok != 0xffu)) {
+#pragma unroll
+      for (int r = 0; r < 8; ++r) p[r] = (f.ok >> r) & 1u ? p[r] : -INFINITY;
+    }
+    if (a.logits && (SIDE ? piece == 0 : used)) {
+      float* to = a.logits + (bh + row) * a.stride + j0 + 4 * g;
+      *reinterpret_cast<float4*>(to) = make_float4(p[0], p[1], p[2], p[3]);
+      *reinterpret_cast<float4*>(to + 16) = make_float4(p[4], p[5], p[6], p[7]);
+    }
+    // The maximum moves only when a logit passes it by kSlack: exponentials up to
+    // 2^8 do no harm in fp32, and most tiles then leave the sums as they are.
+    float top = fmaxf(fmaxf(fmaxf(p[0], p[1]), fmaxf(p[2], p[3])), fmaxf(fmaxf(p[4], p[5]), fmaxf(p[6], p[7])));
+    if (__builtin_amdgcn_ballot_w64(top > m + kSlack)) {
+      const float next = fmaxf(m, max_xor32(max_xor16(top)));
+      const float old = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - next);
+      m = next;
+      l *= old;
+#pragma unroll
+      for (int i2 = 0; i2 < NO; ++i2) o[i2] *= old;
+    }
+    const float ref = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+      p[r] = __builtin_amdgcn_exp2f(p[r] - ref);
+      l += p[r];
+    }
+    constexpr int NX = SIDE ? 1 : 3;
+    u32x4 x[NX];
+    if constexpr (SIDE) {
+#pragma unroll
+      for (int r = 0; r < 8; ++r) {
+        p[r] -= __uint_as_float(__float_as_uint(p[r]) & mask1);
+        p[r] -= __uint_as_float(__float_as_uint(p[r]) & mask2);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[0][j] = pack_hi(p[2 * j], p[2 * j + 1]);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 3; ++k) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[k][j] = pack_hi(p[2 * j], p[2 * j + 1]);
+#pragma unroll
+        for (int r = 0; r < 8; ++r) p[r] -= hi16(p[r]);
+      }
+    }
+    int out = 0;
+#pragma unroll
+    for (int sg = 0; sg < seg_count(DV); ++sg) {
+      constexpr int kPairs = 4;
+#pragma unroll
+      for (int pr = 0; pr < kPairs; ++pr) {
+        if (pr >= seg_width(DV, sg) / 32) break;
+        uint32_t y[8];
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+          const float e = e8m0(f.vs[r][sg]);
+          y[r] = pr == 0 ? cvt2<0>(f.v[r][sg], e) : pr == 1 ? cvt2<1>(f.v[r][sg], e)
+                 : pr == 2 ? cvt2<2>(f.v[r][sg], e) : cvt2<3>(f.v[r][sg], e);
+        }
+        u32x4 lo, hi;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          lo[j] = __builtin_amdgcn_perm(y[2 * j + 1], y[2 * j], 0x05040100u);
+          hi[j] = __builtin_amdgcn_perm(y[2 * j + 1], y[2 * j], 0x07060302u);
+        }
+#pragma unroll
+        for (int k = 0; k < NX; ++k) {
+          o[out] = mfma(lo, x[k], o[out]);
+          o[out + 1] = mfma(hi, x[k], o[out + 1]);
+        }
+        out += 2;
+      }
+    }
+  };
+
+  int64_t j = c0 + wave * kTile;
+  if (j < c1) {
+    Frag<DK, DV> f0, f1;
+    load(f0, j);
+    for (; j < c1; j += 2 * kStep) {
+      const bool more = j + kStep < c1;
+      if (more) load(f1, j + kStep);
+      compute(f0, j);
+      if (!more) break;
+      if (j + 2 * kStep < c1) load(f0, j + 2 * kStep);
+      compute(f1, j + kStep);
+    }
   }
-  out[(bt * HQ + h) * c.DV + d] = l == 0.0f ? __builtin_nanf("") : o;
+
+  // Join the waves (and the pieces of p).
+  l = sum_xor32(sum_xor16(l));
+  if (g == 0) {
+    sum_m[wave][col] = m;
+    sum_l[wave][col] = l;
+  }
+  {
+    int out = 0;
+#pragma unroll
+    for (int sg = 0; sg < seg_count(DV); ++sg) {
+      const int W = seg_width(DV, sg), at = seg_at(DV, sg);
+#pragma unroll
+      for (int i2 = 0; i2 < W / 16; ++i2, ++out)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) sum_o[wave][col][at + (4 * g + r) * (W / 16) + i2] = o[out][r];
+    }
+  }
+  __syncthreads();
+  const int rows = SIDE ? a.G : min(16, a.G - rt * 16);
+  for (int e = threadIdx.x; e < rows * DV; e += kNT) {
+    const int rw = e / DV, d = e % DV;
+    float top = sum_m[0][rw];
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) top = fmaxf(top, sum_m[w][rw]);
+    const float ref = top == -INFINITY ? 0.0f : top;
+    float total = 0.0f, x = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      const float f = __builtin_amdgcn_exp2f(sum_m[w][rw] - ref);
+      total += f * sum_l[w][rw];
+      float y = sum_o[w][rw][d];
+      if constexpr (SIDE) y = sum_o[w][rw + 2 * a.G][d] + sum_o[w][rw + a.G][d] + y;
+      x += f * y;
+    }
+    const int64_t h = bh + rt * 16 + rw;
+    if (a.splits > 1) a.part[(h * a.splits + split) * DV + d] = x;
+    else a.out[h * DV + d] = x / total;  // 0 / 0 where no logit is above -inf
+    if (d == 0) a.ml[h * a.splits + split] = make_float2(top, total);
+  }
 }
 
-// weight += the probabilities of query t's heads.  Queries come in launches of
-// their own, so that no two of them add to one slot at once; a slot that one
-// query lists twice takes the same addend twice, in whatever order.
-__global__ __launch_bounds__(kNT) void weight_kernel(Kv4 c, const int32_t* __restrict__ slots,
-                                                     const int32_t* __restrict__ count, int t, int Tq,
-                                                     int HQ, int64_t n, const float* __restrict__ p) {
-  const int64_t b = blockIdx.y, bt = b * Tq + t, j = static_cast<int64_t>(blockIdx.x) * kNT + threadIdx.x;
-  if (j >= n) return;
-  const int32_t s = slot_of(slots, bt, n, j);
-  if (s < 0 || s >= kv4_visible(c.length, count, b, c.S, t, Tq)) return;
+// One query head's maximum and 1 / sum over its splits.
+__device__ __forceinline__ float2 join_ml(const float2* ml, int splits) {
+  float top = -INFINITY;
+  for (int s = 0; s < splits; ++s) top = fmaxf(top, ml[s].x);
+  const float ref = top == -INFINITY ? 0.0f : top;
+  float total = 0.0f;
+  for (int s = 0; s < splits; ++s) total += __builtin_amdgcn_exp2f(ml[s].x - ref) * ml[s].y;
+  return make_float2(ref, 1.0f / total);
+}
+
+// The first `joins` blocks join the splits of a query head each (joins = 0: there
+// is one split, or they are joined already); the others add query t's
+// probabilities onto the weights of kNT slots of a sequence.  t < 0: of all
+// queries, a slot having one thread.  Else one query's, listed ones: two queries
+// never add to one slot at the same time, and a slot that one query lists twice
+// takes the same addend twice, so that the sums have one order.
+__global__ __launch_bounds__(kNT) void finish_kernel(AttnArgs a, int DV, int64_t joins, int t, int64_t per_b) {
+  __shared__ float2 head[1024];
+  if (blockIdx.x < joins) {
+    const int64_t h = blockIdx.x;
+    const float2* ml = a.ml + h * a.splits;
+    const float2 all = join_ml(ml, a.splits);
+    for (int d = threadIdx.x; d < DV; d += kNT) {
+      float x = 0.0f;
+      for (int s = 0; s < a.splits; ++s)
+        if (ml[s].y != 0.0f)  // a chunk without a sum has left none
+          x += __builtin_amdgcn_exp2f(ml[s].x - all.x) * a.part[(h * a.splits + s) * DV + d];
+      a.out[h * DV + d] = x * all.y;
+    }
+    return;
+  }
+  const int64_t blk = blockIdx.x - joins, b = blk / per_b, j = blk % per_b * kNT + threadIdx.x;
+  float* weight = a.c.weight + b * a.c.S;
   float sum = 0.0f;
-  for (int h = 0; h < HQ; ++h) sum += p[(bt * HQ + h) * n + j];
-  atomicAdd(c.weight + b * c.S + s, sum);
+  int32_t slot = -1;
+  for (int tt = t < 0 ? 0 : t; tt < (t < 0 ? a.Tq : t + 1); ++tt) {
+    const int64_t bt = b * a.Tq + tt;
+    const int32_t seen = kv4_visible(a.c.length, a.count, b, a.c.S, tt, a.Tq);
+    __syncthreads();
+    for (int h = threadIdx.x; h < a.HQ; h += kNT) head[h] = join_ml(a.ml + (bt * a.HQ + h) * a.splits, a.splits);
+    __syncthreads();
+    const int32_t s = j >= a.n ? -1 : a.slots ? a.slots[bt * a.n + j] : static_cast<int32_t>(j);
+    if (s < 0 || s >= seen) continue;
+    slot = s;
+    for (int h = 0; h < a.HQ; ++h)
+      sum += __builtin_amdgcn_exp2f(a.logits[(bt * a.HQ + h) * a.stride + j] - head[h].x) * head[h].y;
+  }
+  if (slot < 0) return;
+  if (a.slots) atomicAdd(weight + slot, sum);
+  else weight[slot] += sum;
+}
+
+struct Plan {
+  int splits, chunk, row_tiles;
+  bool side;
+  int64_t ml, part, logits, total, stride;  // byte offsets; floats a row
+};
+
+Plan plan_of(const Kv4& c, int64_t Tq, int HQ, int64_t n, bool accumulate) {
+  Plan p;
+  const int G = HQ / c.HKV;
+  p.side = G <= 5;
+  p.row_tiles = p.side ? 1 : (G + 15) / 16;
+  const int64_t blocks = c.B * Tq * c.HKV * p.row_tiles;
+  const int64_t steps = n > 0 ? (n + kStep - 1) / kStep : 1;
+  const int cus = device_cus() > 0 ? device_cus() : 256;
+  int64_t splits = blocks > 0 ? (4 * cus + blocks - 1) / blocks : 1;
+  splits = splits < 1 ? 1 : splits > steps ? steps : splits;
+  p.chunk = static_cast<int>((steps + splits - 1) / splits) * kStep;
+  p.splits = static_cast<int>((steps * kStep + p.chunk - 1) / p.chunk);
+  auto up = [](int64_t v) { return (v + 255) / 256 * 256; };
+  const int64_t heads = c.B * Tq * HQ;
+  p.stride = steps * kStep;
+  p.ml = 0;
+  p.part = up(heads * p.splits * 8);
+  p.logits = p.part + (p.splits > 1 ? up(heads * p.splits * c.DV * 4) : 0);
+  p.total = p.logits + (accumulate ? up(heads * p.stride * 4) : 0);
+  return p;
+}
+
+template <typename Tag, int NP, int DK, int DV>
+hipError_t launch_dims(const AttnArgs& a, bool side, int64_t blocks, hipStream_t stream) {
+  const uint32_t grid = static_cast<uint32_t>(blocks);
+  if (a.slots) {
+    if (side) attn_kernel<Tag, NP, DK, DV, true, true><<<grid, kNT, 0, stream>>>(a);
+    else attn_kernel<Tag, NP, DK, DV, false, true><<<grid, kNT, 0, stream>>>(a);
+  } else {
+    if (side) attn_kernel<Tag, NP, DK, DV, true, false><<<grid, kNT, 0, stream>>>(a);
+    else attn_kernel<Tag, NP, DK, DV, false, false><<<grid, kNT, 0, stream>>>(a);
+  }
+  return hipGetLastError();
+}
+
+template <typename Tag, int NP>
+hipError_t launch_type(const AttnArgs& a, bool side, int64_t blocks, hipStream_t stream) {
+  if (a.c.DK != a.c.DV) return launch_dims<Tag, NP, 192, 128>(a, side, blocks, stream);
+  switch (a.c.DK) {
+    case 32: return launch_dims<Tag, NP, 32, 32>(a, side, blocks, stream);
+    case 64: return launch_dims<Tag, NP, 64, 64>(a, side, blocks, stream);
+    case 96: return launch_dims<Tag, NP, 96, 96>(a, side, blocks, stream);
+    case 128: return launch_dims<Tag, NP, 128, 128>(a, side, blocks, stream);
+    case 192: return launch_dims<Tag, NP, 192, 192>(a, side, blocks, stream);
+    default: return launch_dims<Tag, NP, 256, 256>(a, side, blocks, stream);
+  }
 }
 
 }  // namespace
@@ -115,26 +525,46 @@ bool kv4_attn_supported(int DK, int DV) {
   return DK == DV && (DK == 32 || DK == 64 || DK == 96 || DK == 128 || DK == 192 || DK == 256);
 }
 
-int64_t kv4_attn_workspace(const Kv4& c, int64_t Tq, int HQ, int64_t n, bool) { return c.B * Tq * HQ * n * 4; }
+int64_t kv4_attn_workspace(const Kv4& c, int64_t Tq, int HQ, int64_t n, bool accumulate) {
+  return plan_of(c, Tq, HQ, n, accumulate).total;
+}
 
 hipError_t launch_kv4_attn(const Kv4& c, const void* Q, int dtype, const int32_t* slots,
                            const int32_t* count, int64_t Tq, int HQ, int64_t n, bool accumulate,
                            float scale, float* out, void* ws, hipStream_t stream) {
-  const int tq = static_cast<int>(Tq);
-  float* logits = static_cast<float*>(ws);
-  const dim3 g1(static_cast<uint32_t>((n + kNT - 1) / kNT), HQ, static_cast<uint32_t>(c.B * Tq));
-  if (n > 0) {
-    if (dtype == 0)
-      logits_kernel<F32><<<g1, kNT, 0, stream>>>(c, static_cast<const float*>(Q), slots, count, tq, HQ, n, scale, logits);
-    else if (dtype == 1)
-      logits_kernel<BF16><<<g1, kNT, 0, stream>>>(c, static_cast<const uint16_t*>(Q), slots, count, tq, HQ, n, scale, logits);
-    else
-      logits_kernel<F16><<<g1, kNT, 0, stream>>>(c, static_cast<const uint16_t*>(Q), slots, count, tq, HQ, n, scale, logits);
+  const Plan p = plan_of(c, Tq, HQ, n, accumulate);
+  char* base = static_cast<char*>(ws);
+  AttnArgs a;
+  a.c = c;
+  a.Q = Q;
+  a.slots = slots;
+  a.count = count;
+  a.Tq = static_cast<int>(Tq);
+  a.HQ = HQ;
+  a.G = HQ / c.HKV;
+  a.row_tiles = p.row_tiles;
+  a.n = n;
+  a.stride = p.stride;
+  a.splits = p.splits;
+  a.chunk = p.chunk;
+  a.scale = scale;
+  a.out = out;
+  a.ml = reinterpret_cast<float2*>(base + p.ml);
+  a.part = reinterpret_cast<float*>(base + p.part);
+  a.logits = accumulate ? reinterpret_cast<float*>(base + p.logits) : nullptr;
+  const int64_t chunks = (c.B * Tq * p.splits + 7) / 8 * 8;
+  const int64_t blocks = chunks * c.HKV * p.row_tiles;
+  hipError_t e = dtype == 0   ? launch_type<F32, 3>(a, p.side, blocks, stream)
+                 : dtype == 1 ? launch_type<BF16, 1>(a, p.side, blocks, stream)
+                              : launch_type<F16, 2>(a, p.side, blocks, stream);
+  if (e != hipSuccess) return e;
+  int64_t joins = p.splits > 1 ? c.B * Tq * HQ : 0;
+  const int64_t per_b = accumulate ? (n + kNT - 1) / kNT : 0;
+  for (int t = slots ? 0 : -1; t < (slots && accumulate ? a.Tq : slots ? 1 : 0); ++t) {
+    if (joins + per_b * c.B > 0)
+      finish_kernel<<<static_cast<uint32_t>(joins + per_b * c.B), kNT, 0, stream>>>(a, c.DV, joins, t, per_b);
+    joins = 0;
   }
-  rows_kernel<<<dim3(HQ, static_cast<uint32_t>(c.B * Tq)), kNT, 0, stream>>>(c, slots, count, tq, HQ, n, logits, out);
-  if (accumulate && n > 0)
-    for (int t = 0; t < tq; ++t)
-      weight_kernel<<<dim3(static_cast<uint32_t>((n + kNT - 1) / kNT), static_cast<uint32_t>(c.B)), kNT, 0, stream>>>(c, slots, count, t, tq, HQ, n, logits);
   return hipGetLastError();
 }
 

@@ -468,7 +468,7 @@ typedef struct dsa_kv4_cache {
  *   K [B,T,HKV,DK], V [B,T,HKV,DV] of dtype (fp32, bf16, fp16); k_idx [B,T,DI] of
  *   the cache's idx_dtype, null exactly where the cache holds none; weight [B,T]
  *   fp32, the new slots' first weights (null: 0).  16-byte aligned (weight and
- *   count 4).
+ *   count 4).  T < 2^25.
  */
 int dsa_kv4_append(const dsa_kv4_cache* cache, const void* K, const void* V, int dtype,
                    const void* k_idx, const float* weight, const int32_t* count, int64_t T,
@@ -478,7 +478,7 @@ int dsa_kv4_append(const dsa_kv4_cache* cache, const void* K, const void* V, int
  * The values that N slots of each sequence stand for, K [B,N,HKV,DK] and
  * V [B,N,HKV,DV] of dtype (exact in fp32 and bf16; fp16 rounds, to Inf past its
  * range): slots [B,N], or 0 .. N-1 where null.  Slots outside [0, length) give
- * zeros.  K and V 16-byte aligned.
+ * zeros.  K and V 16-byte aligned; N < 2^25.
  */
 int dsa_kv4_rows(const dsa_kv4_cache* cache, const int32_t* slots, int64_t N, int dtype, void* K,
                  void* V, void* stream);
@@ -508,11 +508,11 @@ int dsa_kv4_indexer_scores(const dsa_kv4_cache* cache, const void* q_idx, const 
  * sees no slot gets O = NaN, as dsa_sparse_attn_threshold's empty rows do.
  *   accumulate != 0: weight[b,s] += sum over t and h of p[b,t,h,s], with the same
  * result in every run.
- *   fp32 logits, softmax and sums; a probability enters the sum over V as two
- * bf16 pieces (16 bits).
+ *   fp32 logits, softmax and sums; fp32 operands enter the matrix instructions
+ * whole, as bf16 pieces.
  *   Q [B,Tq,HQ,DK] of dtype (fp32, bf16, fp16), out [B,Tq,HQ,DV] fp32, 16-byte
- *   aligned; HQ a multiple of HKV, at most 1024; n < 2^31; without slots n <= S;
- *   B*Tq*HQ < 2^31; DK = DV in {32, 64, 96, 128, 192, 256} or DK 192 with DV 128
+ *   aligned; HQ a multiple of HKV, at most 1024; without slots n <= S;
+ *   B*Tq*HQ < 2^23; B*n < 2^31; DK = DV in {32, 64, 96, 128, 192, 256} or DK 192 with DV 128
  *   (else DSA_EUNSUPPORTED).
  *   workspace: device memory of dsa_kv4_attention_workspace_bytes, 16-byte
  *   aligned, used by no other work until the launches complete, contents on entry
