@@ -577,7 +577,7 @@ int dsa_kv4_indexer_scores(const dsa_kv4_cache* cache, const void* q_idx, const 
   if (Tq < 0 || Tq > kMaxElems) return fail(DSA_EINVAL, "kv4_indexer: Tq=%lld", (long long)Tq);
   if (span < 0 || span > cache->S) return fail(DSA_EINVAL, "kv4_indexer: span=%lld outside [0, S=%lld]", (long long)span, (long long)cache->S);
   if (cache->B * Tq * span == 0) return DSA_OK;
-  if (cache->B * Tq > kMaxElems || cache->B * Tq * span >= (int64_t{1} << 40)) return fail(DSA_EINVAL, "kv4_indexer: scores too large");
+  if (cache->B * Tq >= (int64_t{1} << 23)) return fail(DSA_EINVAL, "kv4_indexer: B*Tq=%lld must be < 2^23", (long long)(cache->B * Tq));
   if (!q_idx || !w_idx || !scores) return fail(DSA_EINVAL, "kv4_indexer: null pointer");
   if (!aligned16(q_idx) || !aligned4(scores) || !aligned4(count)) return fail(DSA_EINVAL, "kv4_indexer: q_idx must be 16-byte aligned, scores and count 4-byte");
   return hip_status(dsa::launch_kv4_indexer(kv4_of(cache), q_idx, w_idx, cache->idx_dtype, count, Tq, HI, span,

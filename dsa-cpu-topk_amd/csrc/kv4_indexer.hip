@@ -1,51 +1,208 @@
 // kv4_indexer.hip -- lightning indexer of new tokens against the cached index
 // keys (gfx950):
 //   I[b,t,s] = sum_j w[b,t,j] * ReLU(<q[b,t,j,:], k[b,s,:]>)  for visible s, else -inf
+//
+// The index keys are the bulk of the bytes (DI of them a slot, for 4 bytes of
+// score a token) and are read once: a wave takes 16 * KB slots into registers
+// as B operands, a lane a quarter of one slot's row, and walks the heads, 16 at a
+// time, as A operands.  A block serves up to kTokens of a sequence's tokens, whose
+// q rows (in the order in which lanes read them) and weights lie in LDS.  A lane's
+// four results are four heads of one slot: ReLU, weight and sum stay in the lane,
+// and one sum over the four lane groups ends a slot.
+//
+// fp32 takes the fp32 matrix instruction (its 157 TFLOP/s are about what 64 heads
+// of 128 need at the memory's rate, fewer heads need less).
+#include "dsa_launch.h"
 #include "kv4.h"
+#include "tile_common.h"
 
 namespace dsa {
 namespace {
 
-constexpr int kNT = 256;
+constexpr int kWaves = kNT / kWave;
+constexpr int kTokens = 4;              // of one block
+constexpr int kMaxLds = 64 * 1024;      // of q and weights; wider q rows are read through L2
 
-// One thread a slot, the query row in LDS head by head.
+struct IndexArgs {
+  Kv4 c;
+  const void* q;
+  const void* w;
+  const int32_t* count;
+  int Tq, per, groups;  // tokens a block, groups of them a sequence
+  int HI, chunks;
+  int64_t span, chunk;  // slots scored, and of one block
+  float* scores;
+};
+
 template <typename Tag>
-__global__ __launch_bounds__(kNT) void indexer_kernel(Kv4 c, const typename Tag::raw* __restrict__ q,
-                                                      const typename Tag::raw* __restrict__ w,
-                                                      const int32_t* __restrict__ count, int Tq, int HI,
-                                                      int64_t span, float* __restrict__ scores) {
-  __shared__ float qs[256];
-  const int64_t bt = blockIdx.y, b = bt / Tq;
-  const int64_t s = static_cast<int64_t>(blockIdx.x) * kNT + threadIdx.x;
-  const int32_t seen = kv4_visible(c.length, count, b, c.S, static_cast<int>(bt % Tq), Tq);
-  const bool ok = s < seen && s < span;
-  const typename Tag::raw* k = static_cast<const typename Tag::raw*>(c.k_idx) + (b * c.S + (ok ? s : 0)) * c.DI;
-  float total = 0.0f;
-  for (int j = 0; j < HI; ++j) {
-    __syncthreads();
-    if (static_cast<int>(threadIdx.x) < c.DI) qs[threadIdx.x] = to_f32(Tag{}, q[(bt * HI + j) * c.DI + threadIdx.x]);
-    __syncthreads();
-    float dot = 0.0f;
-    if (ok)
-      for (int d = 0; d < c.DI; ++d) dot += qs[d] * to_f32(Tag{}, k[d]);
-    total += to_f32(Tag{}, w[bt * HI + j]) * relu_f32(dot);
+__device__ __forceinline__ f32x4 mfma16(const u32x4& a, const u32x4& b, f32x4 acc) {
+  if constexpr (Tag::kBytes == 4) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      acc = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a[i]), __uint_as_float(b[i]), acc, 0, 0, 0);
+    return acc;
+  } else {
+    return Mfma16x16x32<Tag>::run(a, b, acc);
   }
-  if (s < span) scores[bt * span + s] = ok ? total : -INFINITY;
+}
+
+template <typename Tag, int DI, int KB, bool IN_LDS>
+__global__ __launch_bounds__(kNT) void indexer_kernel(IndexArgs a) {
+  using raw = typename Tag::raw;
+  constexpr int ROW = DI * Tag::kBytes, NC = ROW / 64;  // bytes of a row, 16-byte pieces of a lane's quarter
+  extern __shared__ u32x4 lds[];
+  const int nht = (a.HI + 15) / 16;
+  const int64_t bg = blockIdx.x / a.chunks, b = bg / a.groups;
+  const int t0 = static_cast<int>(bg % a.groups) * a.per, nt = min(a.per, a.Tq - t0);
+  const int64_t c0 = blockIdx.x % a.chunks * a.chunk;
+  const int64_t c1 = min(c0 + a.chunk, a.span);
+  const int wave = threadIdx.x / kWave, lane = threadIdx.x & 63, g = lane >> 4, r16 = lane & 15;
+  int32_t limit = 0;
+  for (int t = 0; t < nt; ++t) limit = max(limit, kv4_visible(a.c.length, a.count, b, a.c.S, t0 + t, a.Tq));
+  const int64_t bt0 = b * a.Tq + t0;
+  if (c0 >= limit) {
+    for (int t = 0; t < nt; ++t)
+      for (int64_t s = c0 + threadIdx.x; s < c1; s += kNT) a.scores[(bt0 + t) * a.span + s] = -INFINITY;
+    return;
+  }
+
+  const char* keys = static_cast<const char*>(a.c.k_idx) + b * a.c.S * ROW;
+  auto load = [&](u32x4 (&k)[KB][NC], int64_t s0) {  // rows past the last visible one give zeros
+    const __amdgpu_buffer_rsrc_t r = rows_rsrc(keys, s0, limit, ROW);
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+        k[kb][c] = __builtin_bit_cast(u32x4, buffer_load_f32x4(r, (16 * kb + r16) * ROW + g * (ROW / 4) + c * 16, 0, 0));
+  };
+  u32x4 k0[KB][NC], k1[KB][NC];
+  constexpr int64_t kStep = 16 * KB * kWaves;
+  int64_t s = c0 + wave * 16 * KB;
+  const int64_t end = min(c1, static_cast<int64_t>(limit));
+  if (s < end) load(k0, s);
+
+  const char* q = static_cast<const char*>(a.q) + bt0 * a.HI * ROW;
+  const raw* w = static_cast<const raw*>(a.w) + bt0 * a.HI;
+  float* weights = reinterpret_cast<float*>(lds + (IN_LDS ? nt * nht * NC * 64 : 0));
+  auto piece = [&](int t, int ht, int c) {  // the lane's A operand
+    const int h = 16 * ht + r16;
+    u32x4 x = {0, 0, 0, 0};
+    if (h < a.HI) x = *reinterpret_cast<const u32x4*>(q + (static_cast<int64_t>(t) * a.HI + h) * ROW + g * (ROW / 4) + c * 16);
+    return x;
+  };
+  if constexpr (IN_LDS) {
+    for (int i = wave; i < nt * nht * NC; i += kWaves)
+      lds[i * 64 + lane] = piece(i / (nht * NC), i / NC % nht, i % NC);
+  }
+  for (int i = threadIdx.x; i < nt * nht * 16; i += kNT) {
+    const int t = i / (nht * 16), h = i % (nht * 16);
+    weights[i] = h < a.HI ? to_f32(Tag{}, w[t * a.HI + h]) : 0.0f;
+  }
+  __syncthreads();
+
+  auto compute = [&](const u32x4 (&k)[KB][NC], int64_t s0) {
+    for (int t = 0; t < nt; ++t) {
+      float sum[KB];
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) sum[kb] = 0.0f;
+      for (int ht = 0; ht < nht; ++ht) {
+        f32x4 acc[KB];
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) acc[kb] = f32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+          const u32x4 x = IN_LDS ? lds[((t * nht + ht) * NC + c) * 64 + lane] : piece(t, ht, c);
+#pragma unroll
+          for (int kb = 0; kb < KB; ++kb) acc[kb] = mfma16<Tag>(x, k[kb][c], acc[kb]);
+        }
+        const float4 wv = *reinterpret_cast<const float4*>(weights + (t * nht + ht) * 16 + 4 * g);
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) {
+          // the IEEE maximum: a NaN stays one
+          sum[kb] = fmaf(wv.x, __builtin_elementwise_maximum(acc[kb][0], 0.0f), sum[kb]);
+          sum[kb] = fmaf(wv.y, __builtin_elementwise_maximum(acc[kb][1], 0.0f), sum[kb]);
+          sum[kb] = fmaf(wv.z, __builtin_elementwise_maximum(acc[kb][2], 0.0f), sum[kb]);
+          sum[kb] = fmaf(wv.w, __builtin_elementwise_maximum(acc[kb][3], 0.0f), sum[kb]);
+        }
+      }
+      float mine = 0.0f;  // lane group g stores the slots of tile g
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) {
+        const float x = sum_xor32(sum_xor16(sum[kb]));
+        mine = g == kb ? x : mine;
+      }
+      const int64_t at = s0 + 16 * g + r16;
+      const int32_t seen = kv4_visible(a.c.length, a.count, b, a.c.S, t0 + t, a.Tq);
+      if (g < KB && at < c1) a.scores[(bt0 + t) * a.span + at] = at < seen ? mine : -INFINITY;
+    }
+  };
+  for (; s < end; s += 2 * kStep) {
+    if (s + kStep < end) load(k1, s + kStep);
+    compute(k0, s);
+    if (s + kStep >= end) break;
+    if (s + 2 * kStep < end) load(k0, s + 2 * kStep);
+    compute(k1, s + kStep);
+  }
+  // what the waves' whole tiles did not reach
+  const int64_t done = c0 + (end - c0 + 16 * KB - 1) / (16 * KB) * (16 * KB);
+  for (int t = 0; t < nt; ++t)
+    for (int64_t at = done + threadIdx.x; at < c1; at += kNT) a.scores[(bt0 + t) * a.span + at] = -INFINITY;
+}
+
+template <typename Tag, int DI>
+hipError_t launch_di(IndexArgs a, hipStream_t stream) {
+  constexpr int ROW = DI * Tag::kBytes;
+  // 32 registers of keys a stage, at most the 4 tiles that 4 lane groups store
+  constexpr int KB = ROW <= 128 ? 4 : ROW <= 256 ? 2 : 1;
+  const int nht = (a.HI + 15) / 16;
+  const int row_lds = nht * 16 * (ROW + 4);  // of one token
+  a.per = a.Tq < kTokens ? a.Tq : kTokens;
+  while (a.per > 1 && a.per * row_lds > kMaxLds) --a.per;
+  a.groups = (a.Tq + a.per - 1) / a.per;
+  const bool in_lds = a.per * row_lds <= kMaxLds;
+  const int step = 16 * KB * kWaves;
+  const int64_t rows = a.c.B * a.groups, steps = (a.span + step - 1) / step;
+  const int cus = device_cus() > 0 ? device_cus() : 256;
+  int64_t chunks = (4 * cus + rows - 1) / rows;
+  chunks = chunks < 1 ? 1 : chunks > steps ? steps : chunks;
+  const int64_t per_chunk = (steps + chunks - 1) / chunks;
+  a.chunk = per_chunk * step;
+  a.chunks = static_cast<int>((steps + per_chunk - 1) / per_chunk);
+  const uint32_t grid = static_cast<uint32_t>(rows * a.chunks);
+  if (in_lds)
+    indexer_kernel<Tag, DI, KB, true><<<grid, kNT, a.per * row_lds, stream>>>(a);
+  else
+    indexer_kernel<Tag, DI, KB, false><<<grid, kNT, nht * 64, stream>>>(a);
+  return hipGetLastError();
+}
+
+template <typename Tag>
+hipError_t launch_tag(const IndexArgs& a, hipStream_t stream) {
+  switch (a.c.DI) {
+    case 16:
+      if constexpr (Tag::kBytes == 4) return launch_di<Tag, 16>(a, stream);
+      return hipErrorNotSupported;
+    case 32: return launch_di<Tag, 32>(a, stream);
+    case 64: return launch_di<Tag, 64>(a, stream);
+    case 128: return launch_di<Tag, 128>(a, stream);
+    default: return launch_di<Tag, 256>(a, stream);
+  }
 }
 
 }  // namespace
 
 hipError_t launch_kv4_indexer(const Kv4& c, const void* q, const void* w, int dtype, const int32_t* count,
                               int64_t Tq, int HI, int64_t span, float* scores, hipStream_t stream) {
-  const dim3 grid(static_cast<uint32_t>((span + kNT - 1) / kNT), static_cast<uint32_t>(c.B * Tq));
-  const int tq = static_cast<int>(Tq);
-  if (dtype == 0)
-    indexer_kernel<F32><<<grid, kNT, 0, stream>>>(c, static_cast<const float*>(q), static_cast<const float*>(w), count, tq, HI, span, scores);
-  else if (dtype == 1)
-    indexer_kernel<BF16><<<grid, kNT, 0, stream>>>(c, static_cast<const uint16_t*>(q), static_cast<const uint16_t*>(w), count, tq, HI, span, scores);
-  else
-    indexer_kernel<F16><<<grid, kNT, 0, stream>>>(c, static_cast<const uint16_t*>(q), static_cast<const uint16_t*>(w), count, tq, HI, span, scores);
-  return hipGetLastError();
+  IndexArgs a;
+  a.c = c;
+  a.q = q;
+  a.w = w;
+  a.count = count;
+  a.Tq = static_cast<int>(Tq);
+  a.HI = HI;
+  a.span = span;
+  a.scores = scores;
+  return dtype == 0 ? launch_tag<F32>(a, stream) : dtype == 1 ? launch_tag<BF16>(a, stream) : launch_tag<F16>(a, stream);
 }
 
 }  // namespace dsa

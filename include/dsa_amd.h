@@ -490,7 +490,7 @@ int dsa_kv4_rows(const dsa_kv4_cache* cache, const int32_t* slots, int64_t N, in
  * (null: Tq) of the Tq queries are tokens, those from n on see nothing.
  * scores [B,Tq,span] fp32: the first span slots.  fp32 sums.
  *   q_idx [B,Tq,HI,DI] (16-byte aligned), w_idx [B,Tq,HI], of the cache's
- *   idx_dtype; 1 <= HI <= 256; span <= S; B*Tq*span < 2^40.
+ *   idx_dtype; 1 <= HI <= 256; span <= S; B*Tq < 2^23.
  * Replaces: nothing (the reference's indexer, lightning_indexer.py:54-125, is
  *   the square [B,T,T]).
  */
