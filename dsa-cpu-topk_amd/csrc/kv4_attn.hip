@@ -69,66 +69,123 @@ struct AttnArgs {
   float* logits;  // [B*Tq*HQ][stride], in powers of 2, or null
 };
 
-__device__ __forceinline__ uint32_t load_u8(__amdgpu_buffer_rsrc_t r, uint32_t off) {
-  return __builtin_amdgcn_raw_buffer_load_b8(r, static_cast<int>(off), 0, 0);
-}
 template <int BYTES>
 __device__ __forceinline__ uint32_t load_small(__amdgpu_buffer_rsrc_t r, uint32_t off) {
   if constexpr (BYTES == 4) return __float_as_uint(buffer_load_f32(r, static_cast<int>(off), 0, 0));
   else if constexpr (BYTES == 2) return __builtin_amdgcn_raw_buffer_load_b16(r, static_cast<int>(off), 0, 0);
-  else return load_u8(r, off);
+  else return __builtin_amdgcn_raw_buffer_load_b8(r, static_cast<int>(off), 0, 0);
+}
+// W / 8 bytes: a quarter of W codes.
+template <int W>
+__device__ __forceinline__ void load_codes(__amdgpu_buffer_rsrc_t r, uint32_t off, uint32_t* to) {
+  if constexpr (W == 128) {
+    const dsa_f32x4 x = buffer_load_f32x4(r, static_cast<int>(off), 0, 0);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) to[i] = __float_as_uint(x[i]);
+  } else if constexpr (W == 64) {
+    const dsa_f32x2 x = buffer_load_f32x2(r, static_cast<int>(off), 0, 0);
+    to[0] = __float_as_uint(x[0]);
+    to[1] = __float_as_uint(x[1]);
+  } else {
+    to[0] = load_small<4>(r, off);
+  }
 }
 
-// What a wave holds of its 32 slots.
+// The sizes of a wave's 32 slots, in registers and in LDS.
+template <int DK, int DV>
+struct Shape {
+  static constexpr int kScales = (DK > DV ? DK : DV) / 32;  // bytes a lane loads
+  // their alignment: a half (K's or V's scales) starts at a multiple of it
+  static constexpr int kUnit = DK % 128 == 0 && DV % 128 == 0 ? 4 : DK % 64 == 0 && DV % 64 == 0 ? 2 : 1;
+  static constexpr int kLoads = (kScales + kUnit - 1) / kUnit;
+  static constexpr int kVBytes = 2 * 16 * DV / 2;
+  static constexpr int kBytes = kVBytes + (DK + DV);  // a multiple of 16
+};
+
+// What a wave has loaded of its 32 slots, two tiles of 16.
 template <int DK, int DV>
 struct Frag {
-  uint32_t k[2][DK / 32];
-  uint32_t ks[2][seg_count(DK)];
-  uint32_t v[8][seg_count(DV)];
-  uint32_t vs[8][seg_count(DV)];
-  uint32_t ok;  // bit i: the lane's i-th slot (4g + i of the first tile, then of the second) counts
+  uint32_t k[2][DK / 32];  // a quarter of the row of slot lane % 16
+  uint32_t v[2][DV / 32];  // a quarter of the row of slot 4 * (lane / 4 % 4) + lane / 16
+  uint32_t s[Shape<DK, DV>::kLoads];  // K's (even lanes) or V's scales of slot lane / 2 of the 32
+  uint32_t ok;  // bit i: slot i counts
 };
 
 constexpr uint32_t kNowhere = 0x80000000u;  // past any sequence's codes: such loads give zeros
 
+// krow, vrow, srow: byte offsets of the slots' codes (of their scales: 1/16 of it).
 template <int DK, int DV>
 __device__ __forceinline__ void load_frag(Frag<DK, DV>& f, __amdgpu_buffer_rsrc_t rc,
                                           __amdgpu_buffer_rsrc_t rs, const uint32_t (&krow)[2],
-                                          const uint32_t (&vrow)[8], int hk) {
-  const int lane = threadIdx.x & 63, g = lane >> 4, col = lane & 15;
-  const uint32_t head = hk * (DK + DV) / 2, heads = hk * (DK + DV) / 32;
+                                          const uint32_t (&vrow)[2], uint32_t srow, int hk) {
+  using S = Shape<DK, DV>;
+  const int lane = threadIdx.x & 63;
+  const uint32_t head = hk * (DK + DV) / 2;
 #pragma unroll
   for (int t = 0; t < 2; ++t) {
-    int w = 0;
 #pragma unroll
     for (int s = 0; s < seg_count(DK); ++s) {
-      const int W = seg_width(DK, s), at = seg_at(DK, s);
-      const uint32_t off = krow[t] + head + at / 2 + g * (W / 8);
-      if (W == 128) {
-        const dsa_f32x4 x = buffer_load_f32x4(rc, static_cast<int>(off), 0, 0);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) f.k[t][w + i] = __float_as_uint(x[i]);
-      } else if (W == 64) {
-        const dsa_f32x2 x = buffer_load_f32x2(rc, static_cast<int>(off), 0, 0);
-        f.k[t][w] = __float_as_uint(x[0]);
-        f.k[t][w + 1] = __float_as_uint(x[1]);
-      } else {
-        f.k[t][w] = load_small<4>(rc, off);
-      }
-      w += W / 32;
-      f.ks[t][s] = load_u8(rs, krow[t] / 16 + heads + (at + g * (W / 4)) / 32);
+      const int at = seg_at(DK, s);
+      const uint32_t row = krow[t] + head + at / 2;
+      if (seg_width(DK, s) == 128) load_codes<128>(rc, row + (lane >> 4) * 16, f.k[t] + at / 32);
+      else if (seg_width(DK, s) == 64) load_codes<64>(rc, row + (lane >> 4) * 8, f.k[t] + at / 32);
+      else load_codes<32>(rc, row + (lane >> 4) * 4, f.k[t] + at / 32);
     }
   }
+  const uint32_t half = srow / 16 + hk * (DK + DV) / 32 + (lane & 1) * (DK / 32);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
+  for (int i = 0; i < S::kLoads; ++i) f.s[i] = load_small<S::kUnit>(rs, half + i * S::kUnit);
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+#pragma unroll
+    for (int s = 0; s < seg_count(DV); ++s) {
+      const int at = seg_at(DV, s);
+      const uint32_t row = vrow[t] + head + DK / 2 + at / 2;
+      if (seg_width(DV, s) == 128) load_codes<128>(rc, row + (lane & 3) * 16, f.v[t] + at / 32);
+      else if (seg_width(DV, s) == 64) load_codes<64>(rc, row + (lane & 3) * 8, f.v[t] + at / 32);
+      else load_codes<32>(rc, row + (lane & 3) * 4, f.v[t] + at / 32);
+    }
+  }
+}
+
+// V and the scales change lanes through the wave's own part of LDS:
+//   V      [tile][segment][r][g] rows of W / 2 bytes, slot 4g + r of the tile, so that
+//          the 64 lanes write, and for one r read, consecutive bytes;
+//   scales [block][slot], four slots of a block in one word.
+template <int DK, int DV>
+__device__ __forceinline__ void stage(const Frag<DK, DV>& f, uint8_t* lds) {
+  using S = Shape<DK, DV>;
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int t = 0; t < 2; ++t)
 #pragma unroll
     for (int s = 0; s < seg_count(DV); ++s) {
       const int W = seg_width(DV, s), at = seg_at(DV, s);
-      const uint32_t off = vrow[i] + head + DK / 2 + at / 2 + col * (W / 32);
-      f.v[i][s] = W == 128 ? load_small<4>(rc, off) : W == 64 ? load_small<2>(rc, off) : load_small<1>(rc, off);
-      f.vs[i][s] = load_u8(rs, vrow[i] / 16 + heads + DK / 32 + (at + col * (W / 16)) / 32);
+      uint8_t* to = lds + t * 8 * DV + 8 * at + lane * (W / 8);
+      const uint32_t* v = f.v[t] + at / 32;
+      if (W == 128) *reinterpret_cast<uint4*>(to) = make_uint4(v[0], v[1], v[2], v[3]);
+      else if (W == 64) *reinterpret_cast<uint2*>(to) = make_uint2(v[0], v[1]);
+      else *reinterpret_cast<uint32_t*>(to) = v[0];
     }
-  }
+  uint8_t* to = lds + S::kVBytes + (lane & 1) * DK + (lane >> 1);  // 32 bytes a block
+  const int mine = (lane & 1) ? DV / 32 : DK / 32;
+#pragma unroll
+  for (int i = 0; i < S::kScales; ++i)
+    if (DK == DV || i < mine) to[i * 32] = static_cast<uint8_t>(f.s[i / S::kUnit] >> (i % S::kUnit * 8));
+}
+
+// The conversions read a scale's exponent bits alone (checked over all bytes with
+// any sign and mantissa), so a byte of a word becomes a scale by one shift.
+template <int BYTE>
+__device__ __forceinline__ float scale_of(uint32_t w) {
+  return __uint_as_float(BYTE == 3 ? w >> 1 : w << (23 - 8 * BYTE));
+}
+
+// Orders a wave's LDS accesses, which the hardware takes in order, for the compiler.
+__device__ __forceinline__ void wave_lds_order() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
 }
 
 template <int SEL>
@@ -160,8 +217,11 @@ __device__ __forceinline__ void load_q8(const typename Tag::raw* p, u32x4 (&q)[N
 
 template <typename Tag, int NP, int DK, int DV, bool SIDE, bool LISTED>
 __global__ __launch_bounds__(kNT) void attn_kernel(AttnArgs a) {
+  using S = Shape<DK, DV>;
   constexpr int NW = DK / 32, NO = DV / 16, LD = DV + 4;
-  __shared__ float sum_o[kWaves][16][LD];
+  constexpr int kSums = kWaves * 16 * LD * 4, kStages = kWaves * S::kBytes;
+  __shared__ __align__(16) uint8_t lds[kSums > kStages ? kSums : kStages];  // the stages, then the sums
+  float(*sum_o)[16][LD] = reinterpret_cast<float(*)[16][LD]>(lds);
   __shared__ float sum_m[kWaves][16], sum_l[kWaves][16];
 
   // Blocks go round-robin over the 8 XCDs; the blocks of one chunk (its heads)
@@ -174,7 +234,7 @@ __global__ __launch_bounds__(kNT) void attn_kernel(AttnArgs a) {
   const int split = static_cast<int>(chunk_id % a.splits);
   const int32_t seen = kv4_visible(a.c.length, a.count, b, a.c.S, static_cast<int>(bt % a.Tq), a.Tq);
 
-  const int wave = threadIdx.x / kWave, lane = threadIdx.x & 63, g = lane >> 4, col = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = threadIdx.x & 63, g = lane >> 4, col = lane & 15;
   // the lane's query head, and (SIDE) which piece of p it takes
   const int row = SIDE ? col % a.G : rt * 16 + col;
   const int piece = SIDE ? col / a.G : 0;
@@ -227,32 +287,26 @@ __global__ __launch_bounds__(kNT) void attn_kernel(AttnArgs a) {
   const __amdgpu_buffer_rsrc_t all_codes = rsrc(codes, static_cast<int64_t>(limit) * cb);
   const __amdgpu_buffer_rsrc_t all_scales = rsrc(scales, static_cast<int64_t>(limit) * (cb / 16));
   const int32_t* list = LISTED ? a.slots + bt * a.n : nullptr;
+  const int vslot = 4 * ((lane >> 2) & 3) + (lane >> 4);
 
-  auto load = [&](Frag<DK, DV>& f, int64_t j0) {
-    uint32_t krow[2], vrow[8];
-    f.ok = 0;
+  // A listed slot's offset, of entry j0 + lane % 32; read a step before the slots.
+  auto entry = [&](int64_t j0) -> uint32_t {
+    const int64_t j = j0 + (lane & 31);
+    const uint32_t s = j < c1 ? static_cast<uint32_t>(list[j]) : ~0u;
+    return s < static_cast<uint32_t>(limit) ? s * cb : kNowhere;
+  };
+  auto load = [&](Frag<DK, DV>& f, int64_t j0, uint32_t off) {
     if constexpr (LISTED) {
-      auto at = [&](int64_t j) -> uint32_t {
-        const uint32_t s = j < c1 ? static_cast<uint32_t>(list[j]) : ~0u;
-        return s < static_cast<uint32_t>(limit) ? s * cb : kNowhere;
-      };
-#pragma unroll
-      for (int t = 0; t < 2; ++t) krow[t] = at(j0 + 16 * t + col);
-#pragma unroll
-      for (int r = 0; r < 8; ++r) {
-        vrow[r] = at(j0 + (r >> 2) * 16 + 4 * g + (r & 3));
-        f.ok |= (vrow[r] != kNowhere ? 1u : 0u) << r;
-      }
-      load_frag<DK, DV>(f, all_codes, all_scales, krow, vrow, hk);
+      auto from = [&](int l) { return static_cast<uint32_t>(__builtin_amdgcn_ds_bpermute(4 * l, static_cast<int>(off))); };
+      const uint32_t krow[2] = {from(col), from(16 + col)}, vrow[2] = {from(vslot), from(16 + vslot)};
+      load_frag<DK, DV>(f, all_codes, all_scales, krow, vrow, from(lane >> 1), hk);
+      f.ok = static_cast<uint32_t>(__builtin_amdgcn_ballot_w64(off != kNowhere));
     } else {
-#pragma unroll
-      for (int t = 0; t < 2; ++t) krow[t] = (16 * t + col) * cb;
-#pragma unroll
-      for (int r = 0; r < 8; ++r) vrow[r] = ((r >> 2) * 16 + 4 * g + (r & 3)) * cb;
+      const uint32_t krow[2] = {col * cb, (16 + col) * cb}, vrow[2] = {vslot * cb, (16 + vslot) * cb};
       const int64_t rest = max(static_cast<int64_t>(0), limit - j0);
-      load_frag<DK, DV>(f, rsrc(codes + j0 * cb, rest * cb), rsrc(scales + j0 * (cb / 16), rest * (cb / 16)), krow, vrow, hk);
-#pragma unroll
-      for (int r = 0; r < 8; ++r) f.ok |= ((r >> 2) * 16 + 4 * g + (r & 3) < rest ? 1u : 0u) << r;
+      load_frag<DK, DV>(f, rsrc(codes + j0 * cb, rest * cb), rsrc(scales + j0 * (cb / 16), rest * (cb / 16)), krow,
+                        vrow, (lane >> 1) * cb, hk);
+      f.ok = rest >= kTile ? ~0u : (1u << rest) - 1;
     }
   };
 
@@ -262,29 +316,35 @@ __global__ __launch_bounds__(kNT) void attn_kernel(AttnArgs a) {
   float m = -INFINITY, l = 0.0f;
   const float to2 = a.scale * kLog2e;
 
+  uint8_t* mine = lds + wave * S::kBytes;
+  const uint8_t* my_s = mine + S::kVBytes;
   auto compute = [&](const Frag<DK, DV>& f, int64_t j0) {
+    wave_lds_order();
+    stage<DK, DV>(f, mine);
+    wave_lds_order();
     f32x4 s[2] = {f32x4{0, 0, 0, 0}, f32x4{0, 0, 0, 0}};
-    {
-      int w = 0;
 #pragma unroll
-      for (int sg = 0; sg < seg_count(DK); ++sg)
+    for (int sg = 0; sg < seg_count(DK); ++sg) {
+      const int W = seg_width(DK, sg), at = seg_at(DK, sg);
+      const int block = (at + g * (W / 4)) / 32;
+      const float e[2] = {scale_of<0>(my_s[block * 32 + col]), scale_of<0>(my_s[block * 32 + 16 + col])};
 #pragma unroll
-        for (int j = 0; j < seg_width(DK, sg) / 32; ++j, ++w)
+      for (int j = 0; j < W / 32; ++j)
 #pragma unroll
-          for (int t = 0; t < 2; ++t) {
-            const float e = e8m0(f.ks[t][sg]);
-            const uint32_t x = f.k[t][w];
-            const u32x4 k = {cvt2<0>(x, e), cvt2<1>(x, e), cvt2<2>(x, e), cvt2<3>(x, e)};
+        for (int t = 0; t < 2; ++t) {
+          const uint32_t x = f.k[t][at / 32 + j];
+          const u32x4 k = {cvt2<0>(x, e[t]), cvt2<1>(x, e[t]), cvt2<2>(x, e[t]), cvt2<3>(x, e[t])};
 #pragma unroll
-            for (int p = 0; p < NP; ++p) s[t] = mfma(k, q[w][p], s[t]);
-          }
+          for (int p = 0; p < NP; ++p) s[t] = mfma(k, q[at / 32 + j][p], s[t]);
+        }
     }
     float p[8];
 #pragma unroll
     for (int r = 0; r < 8; ++r) p[r] = s[r >> 2][r & 3] * to2;
-    if (__builtin_amdgcn_ballot_w64(f.ok != 0xffu)) {
+    if (f.ok != ~0u) {
+      const uint32_t ok = f.ok >> (4 * g);
 #pragma unroll
-      for (int r = 0; r < 8; ++r) p[r] = (f.ok >> r) & 1u ? p[r] : -INFINITY;
+      for (int r = 0; r < 8; ++r) p[r] = (ok >> ((r >> 2) * 16 + (r & 3))) & 1u ? p[r] : -INFINITY;
     }
     if (a.logits && (SIDE ? piece == 0 : used)) {
       float* to = a.logits + (bh + row) * a.stride + j0 + 4 * g;
@@ -330,17 +390,25 @@ __global__ __launch_bounds__(kNT) void attn_kernel(AttnArgs a) {
     int out = 0;
 #pragma unroll
     for (int sg = 0; sg < seg_count(DV); ++sg) {
-      constexpr int kPairs = 4;
+      const int W = seg_width(DV, sg), at = seg_at(DV, sg);
+      uint32_t v[8];
 #pragma unroll
-      for (int pr = 0; pr < kPairs; ++pr) {
-        if (pr >= seg_width(DV, sg) / 32) break;
+      for (int r = 0; r < 8; ++r) {
+        const uint8_t* from = mine + (r >> 2) * 8 * DV + 8 * at + ((r & 3) * 4 + g) * (W / 2) + col * (W / 32);
+        v[r] = W == 128 ? *reinterpret_cast<const uint32_t*>(from)
+               : W == 64 ? *reinterpret_cast<const uint16_t*>(from) : *from;
+      }
+      const uint8_t* sv = my_s + (DK / 32 + (at + col * (W / 16)) / 32) * 32 + 4 * g;
+      const uint32_t e0 = *reinterpret_cast<const uint32_t*>(sv), e1 = *reinterpret_cast<const uint32_t*>(sv + 16);
+      const float e[8] = {scale_of<0>(e0), scale_of<1>(e0), scale_of<2>(e0), scale_of<3>(e0),
+                          scale_of<0>(e1), scale_of<1>(e1), scale_of<2>(e1), scale_of<3>(e1)};
+#pragma unroll
+      for (int pr = 0; pr < 4; ++pr) {
+        if (pr >= W / 32) break;
         uint32_t y[8];
 #pragma unroll
-        for (int r = 0; r < 8; ++r) {
-          const float e = e8m0(f.vs[r][sg]);
-          y[r] = pr == 0 ? cvt2<0>(f.v[r][sg], e) : pr == 1 ? cvt2<1>(f.v[r][sg], e)
-                 : pr == 2 ? cvt2<2>(f.v[r][sg], e) : cvt2<3>(f.v[r][sg], e);
-        }
+        for (int r = 0; r < 8; ++r)
+          y[r] = pr == 0 ? cvt2<0>(v[r], e[r]) : pr == 1 ? cvt2<1>(v[r], e[r]) : pr == 2 ? cvt2<2>(v[r], e[r]) : cvt2<3>(v[r], e[r]);
         u32x4 lo, hi;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -360,18 +428,28 @@ __global__ __launch_bounds__(kNT) void attn_kernel(AttnArgs a) {
   int64_t j = c0 + wave * kTile;
   if (j < c1) {
     Frag<DK, DV> f0, f1;
-    load(f0, j);
+    uint32_t off = 0;
+    if (LISTED) off = entry(j);
+    load(f0, j, off);
+    if (LISTED) off = entry(j + kStep);
     for (; j < c1; j += 2 * kStep) {
       const bool more = j + kStep < c1;
-      if (more) load(f1, j + kStep);
+      if (more) {
+        load(f1, j + kStep, off);
+        if (LISTED) off = entry(j + 2 * kStep);
+      }
       compute(f0, j);
       if (!more) break;
-      if (j + 2 * kStep < c1) load(f0, j + 2 * kStep);
+      if (j + 2 * kStep < c1) {
+        load(f0, j + 2 * kStep, off);
+        if (LISTED) off = entry(j + 3 * kStep);
+      }
       compute(f1, j + kStep);
     }
   }
 
   // Join the waves (and the pieces of p).
+  __syncthreads();  // the sums lie where the stages were
   l = sum_xor32(sum_xor16(l));
   if (g == 0) {
     sum_m[wave][col] = m;

@@ -56,7 +56,7 @@ __global__ __launch_bounds__(kNT) void indexer_kernel(IndexArgs a) {
   const int t0 = static_cast<int>(bg % a.groups) * a.per, nt = min(a.per, a.Tq - t0);
   const int64_t c0 = blockIdx.x % a.chunks * a.chunk;
   const int64_t c1 = min(c0 + a.chunk, a.span);
-  const int wave = threadIdx.x / kWave, lane = threadIdx.x & 63, g = lane >> 4, r16 = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = threadIdx.x & 63, g = lane >> 4, r16 = lane & 15;
   int32_t limit = 0;
   for (int t = 0; t < nt; ++t) limit = max(limit, kv4_visible(a.c.length, a.count, b, a.c.S, t0 + t, a.Tq));
   const int64_t bt0 = b * a.Tq + t0;
