@@ -37,7 +37,6 @@ namespace {
 
 constexpr int kWaves = kNT / kWave;
 constexpr int kTile = 32;                  // slots a wave takes at once
-constexpr int kStep = kTile * kWaves;      // slots a block takes at once
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kSlack = 8.0f;             // how far a logit may pass the running maximum, in powers of 2
 
@@ -60,8 +59,9 @@ struct AttnArgs {
   const int32_t* slots;  // or null
   const int32_t* count;  // or null
   int Tq, HQ, G, row_tiles;
+  int heads;  // K/V heads a block takes: 4, 2 or 1, its 4 / heads waves of each sharing the slots
   int64_t n, stride;  // slots a query; floats between rows of logits
-  int splits, chunk;  // a chunk is a multiple of kStep slots
+  int splits;         // blocks that share a query's slots
   float scale;
   float* out;
   float* part;    // [B*Tq*HQ][splits][DV] sums, where splits > 1
@@ -98,8 +98,9 @@ struct Shape {
   // their alignment: a half (K's or V's scales) starts at a multiple of it
   static constexpr int kUnit = DK % 128 == 0 && DV % 128 == 0 ? 4 : DK % 64 == 0 && DV % 64 == 0 ? 2 : 1;
   static constexpr int kLoads = (kScales + kUnit - 1) / kUnit;
-  static constexpr int kVBytes = 2 * 16 * DV / 2;
-  static constexpr int kBytes = kVBytes + (DK + DV);  // a multiple of 16
+  // LDS: K, V, scales
+  static constexpr int kV = 2 * 16 * DK / 2, kS = kV + 2 * 16 * DV / 2;
+  static constexpr int kBytes = kS + (DK + DV);  // a multiple of 16
 };
 
 // What a wave has loaded of its 32 slots, two tiles of 16.
@@ -148,7 +149,9 @@ __device__ __forceinline__ void load_frag(Frag<DK, DV>& f, __amdgpu_buffer_rsrc_
   }
 }
 
-// V and the scales change lanes through the wave's own part of LDS:
+// A wave's slots go through its own part of LDS, which leaves their registers to
+// the next ones while these are worked on, and where V and the scales change lanes:
+//   K      [tile][segment][lane], for the lane that wrote it;
 //   V      [tile][segment][r][g] rows of W / 2 bytes, slot 4g + r of the tile, so that
 //          the 64 lanes write, and for one r read, consecutive bytes;
 //   scales [block][slot], four slots of a block in one word.
@@ -156,18 +159,22 @@ template <int DK, int DV>
 __device__ __forceinline__ void stage(const Frag<DK, DV>& f, uint8_t* lds) {
   using S = Shape<DK, DV>;
   const int lane = threadIdx.x & 63;
+  auto put = [&](uint8_t* at_lane0, const uint32_t* v, int W) {
+    uint8_t* to = at_lane0 + lane * (W / 8);
+    if (W == 128) *reinterpret_cast<uint4*>(to) = make_uint4(v[0], v[1], v[2], v[3]);
+    else if (W == 64) *reinterpret_cast<uint2*>(to) = make_uint2(v[0], v[1]);
+    else *reinterpret_cast<uint32_t*>(to) = v[0];
+  };
 #pragma unroll
-  for (int t = 0; t < 2; ++t)
+  for (int t = 0; t < 2; ++t) {
 #pragma unroll
-    for (int s = 0; s < seg_count(DV); ++s) {
-      const int W = seg_width(DV, s), at = seg_at(DV, s);
-      uint8_t* to = lds + t * 8 * DV + 8 * at + lane * (W / 8);
-      const uint32_t* v = f.v[t] + at / 32;
-      if (W == 128) *reinterpret_cast<uint4*>(to) = make_uint4(v[0], v[1], v[2], v[3]);
-      else if (W == 64) *reinterpret_cast<uint2*>(to) = make_uint2(v[0], v[1]);
-      else *reinterpret_cast<uint32_t*>(to) = v[0];
-    }
-  uint8_t* to = lds + S::kVBytes + (lane & 1) * DK + (lane >> 1);  // 32 bytes a block
+    for (int s = 0; s < seg_count(DK); ++s)
+      put(lds + t * 8 * DK + 8 * seg_at(DK, s), f.k[t] + seg_at(DK, s) / 32, seg_width(DK, s));
+#pragma unroll
+    for (int s = 0; s < seg_count(DV); ++s)
+      put(lds + S::kV + t * 8 * DV + 8 * seg_at(DV, s), f.v[t] + seg_at(DV, s) / 32, seg_width(DV, s));
+  }
+  uint8_t* to = lds + S::kS + (lane & 1) * DK + (lane >> 1);  // 32 bytes a block
   const int mine = (lane & 1) ? DV / 32 : DK / 32;
 #pragma unroll
   for (int i = 0; i < S::kScales; ++i)
@@ -200,11 +207,15 @@ __device__ __forceinline__ f32x4 mfma(const u32x4& a, const u32x4& b, f32x4 c) {
   return Mfma16x16x32<BF16>::run(a, b, c);
 }
 
-// 8 consecutive elements of a query row as NP pieces of bf16.
+// 8 elements of a query row, or their negatives, as NP pieces of bf16; zeros where not used.
 template <typename Tag, int NP>
-__device__ __forceinline__ void load_q8(const typename Tag::raw* p, u32x4 (&q)[NP]) {
+__device__ __forceinline__ void split_q8(const typename Tag::raw (&raw)[8], bool used, bool negative, u32x4 (&q)[NP]) {
   float x[8];
-  load_cvt<Tag, 8>(p, x);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    x[j] = used ? to_f32(Tag{}, raw[j]) : 0.0f;
+    x[j] = negative ? -x[j] : x[j];
+  }
 #pragma unroll
   for (int i = 0; i < NP; ++i)
 #pragma unroll
@@ -215,8 +226,15 @@ __device__ __forceinline__ void load_q8(const typename Tag::raw* p, u32x4 (&q)[N
     }
 }
 
+// Waves a SIMD holds: what the registers allow without spills.
+__host__ __device__ constexpr int resident(int NP, int DK, int DV) {
+  if (DK <= 64 || (DK <= 128 && NP == 1)) return 4;
+  if (DK <= 128 || (DV <= 128 && NP == 1)) return 3;
+  return DK <= 192 || NP < 3 ? 2 : 1;
+}
+
 template <typename Tag, int NP, int DK, int DV, bool SIDE, bool LISTED>
-__global__ __launch_bounds__(kNT) void attn_kernel(AttnArgs a) {
+__global__ __launch_bounds__(kNT, resident(NP, DK, DV)) void attn_kernel(AttnArgs a) {
   using S = Shape<DK, DV>;
   constexpr int NW = DK / 32, NO = DV / 16, LD = DV + 4;
   constexpr int kSums = kWaves * 16 * LD * 4, kStages = kWaves * S::kBytes;
@@ -226,55 +244,52 @@ __global__ __launch_bounds__(kNT) void attn_kernel(AttnArgs a) {
 
   // Blocks go round-robin over the 8 XCDs; the blocks of one chunk (its heads)
   // read the same rows, so they go to one XCD, one after another.
-  const int per = a.c.HKV * a.row_tiles;
-  const int64_t i = blockIdx.x / 8, chunk_id = i / per * 8 + blockIdx.x % 8;
-  if (chunk_id >= a.c.B * a.Tq * a.splits) return;
-  const int member = static_cast<int>(i % per), hk = member / a.row_tiles, rt = member % a.row_tiles;
-  const int64_t bt = chunk_id / a.splits, b = bt / a.Tq;
-  const int split = static_cast<int>(chunk_id % a.splits);
-  const int32_t seen = kv4_visible(a.c.length, a.count, b, a.c.S, static_cast<int>(bt % a.Tq), a.Tq);
+  const uint32_t per = a.c.HKV / a.heads * a.row_tiles;
+  const uint32_t i = blockIdx.x / 8, chunk = i / per * 8 + blockIdx.x % 8, member = i % per;
+  const uint32_t bt = chunk / a.splits, b = bt / a.Tq, t = bt % a.Tq;
+  if (b >= a.c.B) return;
+  const int hk0 = member / a.row_tiles * a.heads, rt = member % a.row_tiles, split = chunk % a.splits;
 
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = threadIdx.x & 63, g = lane >> 4, col = lane & 15;
+  const int hk = hk0 + wave % a.heads;  // the wave's K/V head
+  const int share = wave / a.heads, shares = kWaves / a.heads;
+  const int step = kTile * shares * a.splits;  // slots that the head's waves in all blocks take at once
   // the lane's query head, and (SIDE) which piece of p it takes
   const int row = SIDE ? col % a.G : rt * 16 + col;
   const int piece = SIDE ? col / a.G : 0;
   const bool used = SIDE ? piece < 3 : row < a.G;
-  const int64_t bh = bt * a.HQ + hk * a.G;  // the group's first head
+  const int64_t bh = static_cast<int64_t>(bt) * a.HQ + hk * a.G;  // the group's first head
 
+  // the query row, in the order of the K runs; asked for before anything waits
+  typename Tag::raw q_raw[NW][8];
+  {
+    const typename Tag::raw* src = static_cast<const typename Tag::raw*>(a.Q) + (bh + (used ? row : 0)) * DK;
+#pragma unroll
+    for (int s = 0; s < seg_count(DK); ++s) {
+      const int W = seg_width(DK, s), at = seg_at(DK, s);
+#pragma unroll
+      for (int k = 0; k < W / 32; ++k)
+        __builtin_memcpy(q_raw[at / 32 + k], __builtin_assume_aligned(src + at + g * (W / 4) + 8 * k, 16), sizeof(q_raw[0]));
+    }
+  }
+
+  const int32_t seen = kv4_visible(a.c.length, a.count, b, a.c.S, t, a.Tq);
   const int32_t limit = LISTED ? seen : static_cast<int32_t>(min(static_cast<int64_t>(seen), a.n));
-  const int64_t j_end = LISTED ? a.n : limit;
-  const int64_t c0 = static_cast<int64_t>(split) * a.chunk, c1 = min(c0 + a.chunk, j_end);
-  if (c0 >= c1 || limit == 0) {  // nothing here: no sum, and no sums to read
-    const int rows = min(16, a.G - rt * 16);
-    if (a.splits > 1) {
-      if (static_cast<int>(threadIdx.x) < rows)
-        a.ml[(bh + rt * 16 + threadIdx.x) * a.splits + split] = make_float2(-INFINITY, 0.0f);
-    } else {
-      for (int e = threadIdx.x; e < rows * DV; e += kNT)
-        a.out[(bh + rt * 16) * DV + e] = __builtin_nanf("");
-      if (static_cast<int>(threadIdx.x) < rows)
-        a.ml[bh + rt * 16 + threadIdx.x] = make_float2(-INFINITY, 0.0f);
+  // Tiles go to the waves in turn, so that every block has its share of the slots in use.
+  const int64_t j_end = LISTED ? (limit > 0 ? a.n : 0) : limit;
+  const int64_t j_first = static_cast<int64_t>(split) * shares * kTile;
+  const int rows = SIDE ? a.G : min(16, a.G - rt * 16);
+  const int64_t bh0 = static_cast<int64_t>(bt) * a.HQ + hk0 * a.G + rt * 16;  // the block's first query head
+  if (j_first >= j_end) {  // nothing here: no sum, and no sums to read
+    for (int e = threadIdx.x; e < a.heads * rows; e += kNT) {
+      const int64_t h = bh0 + e / rows * a.G + e % rows;
+      a.ml[h * a.splits + split] = make_float2(-INFINITY, 0.0f);
+      if (a.splits == 1)
+        for (int d = 0; d < DV; ++d) a.out[h * DV + d] = __builtin_nanf("");
     }
     return;
   }
 
-  // the query row, in the order of the K runs
-  u32x4 q[NW][NP];
-  {
-    const typename Tag::raw* src = static_cast<const typename Tag::raw*>(a.Q) + (bh + row) * DK;
-    int w = 0;
-#pragma unroll
-    for (int s = 0; s < seg_count(DK); ++s) {
-      const int W = seg_width(DK, s);
-#pragma unroll
-      for (int j = 0; j < W / 32; ++j, ++w) {
-        if (used) load_q8<Tag, NP>(src + seg_at(DK, s) + g * (W / 4) + 8 * j, q[w]);
-        else
-#pragma unroll
-          for (int p = 0; p < NP; ++p) q[w][p] = u32x4{0, 0, 0, 0};
-      }
-    }
-  }
   const uint32_t mask1 = piece >= 1 ? 0xffff0000u : 0u, mask2 = piece >= 2 ? 0xffff0000u : 0u;
 
   const uint32_t cb = a.c.words() * 4;  // bytes of a slot's codes; of its scales: cb / 16
@@ -286,13 +301,13 @@ __global__ __launch_bounds__(kNT) void attn_kernel(AttnArgs a) {
   };
   const __amdgpu_buffer_rsrc_t all_codes = rsrc(codes, static_cast<int64_t>(limit) * cb);
   const __amdgpu_buffer_rsrc_t all_scales = rsrc(scales, static_cast<int64_t>(limit) * (cb / 16));
-  const int32_t* list = LISTED ? a.slots + bt * a.n : nullptr;
+  const int32_t* list = LISTED ? a.slots + static_cast<int64_t>(bt) * a.n : nullptr;
   const int vslot = 4 * ((lane >> 2) & 3) + (lane >> 4);
 
   // A listed slot's offset, of entry j0 + lane % 32; read a step before the slots.
   auto entry = [&](int64_t j0) -> uint32_t {
     const int64_t j = j0 + (lane & 31);
-    const uint32_t s = j < c1 ? static_cast<uint32_t>(list[j]) : ~0u;
+    const uint32_t s = j < j_end ? static_cast<uint32_t>(list[j]) : ~0u;
     return s < static_cast<uint32_t>(limit) ? s * cb : kNowhere;
   };
   auto load = [&](Frag<DK, DV>& f, int64_t j0, uint32_t off) {
@@ -310,29 +325,50 @@ __global__ __launch_bounds__(kNT) void attn_kernel(AttnArgs a) {
     }
   };
 
+  int64_t j = j_first + share * kTile;
+  Frag<DK, DV> f;
+  uint32_t off = LISTED ? entry(j) : 0;
+  if (j < j_end) load(f, j, off);
+
+  u32x4 q[NW][NP];
+#pragma unroll
+  for (int w = 0; w < NW; ++w) split_q8<Tag, NP>(q_raw[w], used, a.scale < 0.0f, q[w]);
+
   f32x4 o[NO];
 #pragma unroll
   for (int i2 = 0; i2 < NO; ++i2) o[i2] = f32x4{0, 0, 0, 0};
   float m = -INFINITY, l = 0.0f;
-  const float to2 = a.scale * kLog2e;
+  // logits in powers of 2; a scale of 0 stays one above it, so that -inf stays -inf
+  const float to2 = fmaxf(fabsf(a.scale) * kLog2e, 1.17549435e-38f);
 
   uint8_t* mine = lds + wave * S::kBytes;
-  const uint8_t* my_s = mine + S::kVBytes;
-  auto compute = [&](const Frag<DK, DV>& f, int64_t j0) {
-    wave_lds_order();
-    stage<DK, DV>(f, mine);
-    wave_lds_order();
+  const uint8_t* my_s = mine + S::kS;
+  auto compute = [&](uint32_t counts, int64_t j0) {
     f32x4 s[2] = {f32x4{0, 0, 0, 0}, f32x4{0, 0, 0, 0}};
 #pragma unroll
     for (int sg = 0; sg < seg_count(DK); ++sg) {
       const int W = seg_width(DK, sg), at = seg_at(DK, sg);
       const int block = (at + g * (W / 4)) / 32;
       const float e[2] = {scale_of<0>(my_s[block * 32 + col]), scale_of<0>(my_s[block * 32 + 16 + col])};
+      uint32_t kw[2][4];
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const uint8_t* from = mine + t * 8 * DK + 8 * at + lane * (W / 8);
+        if (W == 128) {
+          const uint4 x = *reinterpret_cast<const uint4*>(from);
+          kw[t][0] = x.x; kw[t][1] = x.y; kw[t][2] = x.z; kw[t][3] = x.w;
+        } else if (W == 64) {
+          const uint2 x = *reinterpret_cast<const uint2*>(from);
+          kw[t][0] = x.x; kw[t][1] = x.y;
+        } else {
+          kw[t][0] = *reinterpret_cast<const uint32_t*>(from);
+        }
+      }
 #pragma unroll
       for (int j = 0; j < W / 32; ++j)
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-          const uint32_t x = f.k[t][at / 32 + j];
+          const uint32_t x = kw[t][j];
           const u32x4 k = {cvt2<0>(x, e[t]), cvt2<1>(x, e[t]), cvt2<2>(x, e[t]), cvt2<3>(x, e[t])};
 #pragma unroll
           for (int p = 0; p < NP; ++p) s[t] = mfma(k, q[at / 32 + j][p], s[t]);
@@ -340,20 +376,22 @@ __global__ __launch_bounds__(kNT) void attn_kernel(AttnArgs a) {
     }
     float p[8];
 #pragma unroll
-    for (int r = 0; r < 8; ++r) p[r] = s[r >> 2][r & 3] * to2;
-    if (f.ok != ~0u) {
-      const uint32_t ok = f.ok >> (4 * g);
+    for (int r = 0; r < 8; ++r) p[r] = s[r >> 2][r & 3];
+    if (counts != ~0u) {
+      const uint32_t ok = counts >> (4 * g);
 #pragma unroll
       for (int r = 0; r < 8; ++r) p[r] = (ok >> ((r >> 2) * 16 + (r & 3))) & 1u ? p[r] : -INFINITY;
     }
     if (a.logits && (SIDE ? piece == 0 : used)) {
       float* to = a.logits + (bh + row) * a.stride + j0 + 4 * g;
-      *reinterpret_cast<float4*>(to) = make_float4(p[0], p[1], p[2], p[3]);
-      *reinterpret_cast<float4*>(to + 16) = make_float4(p[4], p[5], p[6], p[7]);
+      *reinterpret_cast<float4*>(to) = make_float4(p[0] * to2, p[1] * to2, p[2] * to2, p[3] * to2);
+      *reinterpret_cast<float4*>(to + 16) = make_float4(p[4] * to2, p[5] * to2, p[6] * to2, p[7] * to2);
     }
     // The maximum moves only when a logit passes it by kSlack: exponentials up to
     // 2^8 do no harm in fp32, and most tiles then leave the sums as they are.
-    float top = fmaxf(fmaxf(fmaxf(p[0], p[1]), fmaxf(p[2], p[3])), fmaxf(fmaxf(p[4], p[5]), fmaxf(p[6], p[7])));
+    // (IEEE maxima, one instruction for three; a NaN moves nothing and is in p anyway.)
+    auto max2 = [](float x, float y) { return __builtin_elementwise_maximum(x, y); };
+    const float top = to2 * max2(max2(max2(p[0], p[1]), max2(p[2], p[3])), max2(max2(p[4], p[5]), max2(p[6], p[7])));
     if (__builtin_amdgcn_ballot_w64(top > m + kSlack)) {
       const float next = fmaxf(m, max_xor32(max_xor16(top)));
       const float old = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - next);
@@ -365,7 +403,7 @@ __global__ __launch_bounds__(kNT) void attn_kernel(AttnArgs a) {
     const float ref = m == -INFINITY ? 0.0f : m;
 #pragma unroll
     for (int r = 0; r < 8; ++r) {
-      p[r] = __builtin_amdgcn_exp2f(p[r] - ref);
+      p[r] = __builtin_amdgcn_exp2f(fmaf(p[r], to2, -ref));
       l += p[r];
     }
     constexpr int NX = SIDE ? 1 : 3;
@@ -394,7 +432,7 @@ __global__ __launch_bounds__(kNT) void attn_kernel(AttnArgs a) {
       uint32_t v[8];
 #pragma unroll
       for (int r = 0; r < 8; ++r) {
-        const uint8_t* from = mine + (r >> 2) * 8 * DV + 8 * at + ((r & 3) * 4 + g) * (W / 2) + col * (W / 32);
+        const uint8_t* from = mine + S::kV + (r >> 2) * 8 * DV + 8 * at + ((r & 3) * 4 + g) * (W / 2) + col * (W / 32);
         v[r] = W == 128 ? *reinterpret_cast<const uint32_t*>(from)
                : W == 64 ? *reinterpret_cast<const uint16_t*>(from) : *from;
       }
@@ -425,26 +463,18 @@ __global__ __launch_bounds__(kNT) void attn_kernel(AttnArgs a) {
     }
   };
 
-  int64_t j = c0 + wave * kTile;
-  if (j < c1) {
-    Frag<DK, DV> f0, f1;
-    uint32_t off = 0;
-    if (LISTED) off = entry(j);
-    load(f0, j, off);
-    if (LISTED) off = entry(j + kStep);
-    for (; j < c1; j += 2 * kStep) {
-      const bool more = j + kStep < c1;
-      if (more) {
-        load(f1, j + kStep, off);
-        if (LISTED) off = entry(j + 2 * kStep);
+  if (j < j_end) {
+    if (LISTED) off = entry(j + step);
+    for (; j < j_end; j += step) {
+      const uint32_t counts = f.ok;
+      wave_lds_order();
+      stage<DK, DV>(f, mine);
+      wave_lds_order();
+      if (j + step < j_end) {
+        load(f, j + step, off);
+        if (LISTED) off = entry(j + 2 * step);
       }
-      compute(f0, j);
-      if (!more) break;
-      if (j + 2 * kStep < c1) {
-        load(f0, j + 2 * kStep, off);
-        if (LISTED) off = entry(j + 3 * kStep);
-      }
-      compute(f1, j + kStep);
+      compute(counts, j);
     }
   }
 
@@ -455,49 +485,75 @@ __global__ __launch_bounds__(kNT) void attn_kernel(AttnArgs a) {
     sum_m[wave][col] = m;
     sum_l[wave][col] = l;
   }
-  {
-    int out = 0;
+  if (col < (SIDE ? 3 * a.G : rows)) {
+    float* to = sum_o[wave][col];
 #pragma unroll
     for (int sg = 0; sg < seg_count(DV); ++sg) {
       const int W = seg_width(DV, sg), at = seg_at(DV, sg);
 #pragma unroll
-      for (int i2 = 0; i2 < W / 16; ++i2, ++out)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) sum_o[wave][col][at + (4 * g + r) * (W / 16) + i2] = o[out][r];
+      for (int r = 0; r < 4; ++r) {  // W / 16 columns from at + (4g + r) * W / 16 on
+        float* row_at = to + at + (4 * g + r) * (W / 16);
+        const f32x4* x = o + at / 16;
+        if (W >= 64) {
+          *reinterpret_cast<float4*>(row_at) = make_float4(x[0][r], x[1][r], x[2][r], x[3][r]);
+          if (W == 128) *reinterpret_cast<float4*>(row_at + 4) = make_float4(x[4][r], x[5][r], x[6][r], x[7][r]);
+        } else {
+          *reinterpret_cast<float2*>(row_at) = make_float2(x[0][r], x[1][r]);
+        }
+      }
     }
   }
   __syncthreads();
-  const int rows = SIDE ? a.G : min(16, a.G - rt * 16);
-  for (int e = threadIdx.x; e < rows * DV; e += kNT) {
-    const int rw = e / DV, d = e % DV;
-    float top = sum_m[0][rw];
-#pragma unroll
-    for (int w = 1; w < kWaves; ++w) top = fmaxf(top, sum_m[w][rw]);
+  constexpr int kQuads = DV / 4;
+  for (uint32_t e = threadIdx.x; e < static_cast<uint32_t>(a.heads * rows * kQuads); e += kNT) {
+    const uint32_t hr = e / kQuads, d = e % kQuads * 4, hd = hr / rows, rw = hr % rows;
+    float top = -INFINITY;
+    for (int w = hd; w < kWaves; w += a.heads) top = fmaxf(top, sum_m[w][rw]);
     const float ref = top == -INFINITY ? 0.0f : top;
-    float total = 0.0f, x = 0.0f;
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
+    float total = 0.0f;
+    float4 x = {0, 0, 0, 0};
+    for (int w = hd; w < kWaves; w += a.heads) {
       const float f = __builtin_amdgcn_exp2f(sum_m[w][rw] - ref);
       total += f * sum_l[w][rw];
-      float y = sum_o[w][rw][d];
-      if constexpr (SIDE) y = sum_o[w][rw + 2 * a.G][d] + sum_o[w][rw + a.G][d] + y;
-      x += f * y;
+      float4 y = *reinterpret_cast<const float4*>(&sum_o[w][rw][d]);
+      if constexpr (SIDE) {  // the pieces, the small ones first
+        const float4 y1 = *reinterpret_cast<const float4*>(&sum_o[w][rw + a.G][d]);
+        const float4 y2 = *reinterpret_cast<const float4*>(&sum_o[w][rw + 2 * a.G][d]);
+        y.x += y1.x + y2.x; y.y += y1.y + y2.y; y.z += y1.z + y2.z; y.w += y1.w + y2.w;
+      }
+      x.x += f * y.x; x.y += f * y.y; x.z += f * y.z; x.w += f * y.w;
     }
-    const int64_t h = bh + rt * 16 + rw;
-    if (a.splits > 1) a.part[(h * a.splits + split) * DV + d] = x;
-    else a.out[h * DV + d] = x / total;  // 0 / 0 where no logit is above -inf
+    const int64_t h = bh0 + hd * a.G + rw;
+    if (a.splits > 1) {
+      *reinterpret_cast<float4*>(a.part + (h * a.splits + split) * DV + d) = x;
+    } else {  // 0 / 0 where no logit is above -inf
+      *reinterpret_cast<float4*>(a.out + h * DV + d) = make_float4(x.x / total, x.y / total, x.z / total, x.w / total);
+    }
     if (d == 0) a.ml[h * a.splits + split] = make_float2(top, total);
   }
 }
 
-// One query head's maximum and 1 / sum over its splits.
+// One query head's maximum (0 where it is -inf) and sum over its splits, by 8 lanes.
 __device__ __forceinline__ float2 join_ml(const float2* ml, int splits) {
-  float top = -INFINITY;
-  for (int s = 0; s < splits; ++s) top = fmaxf(top, ml[s].x);
-  const float ref = top == -INFINITY ? 0.0f : top;
-  float total = 0.0f;
-  for (int s = 0; s < splits; ++s) total += __builtin_amdgcn_exp2f(ml[s].x - ref) * ml[s].y;
-  return make_float2(ref, 1.0f / total);
+  const int first = threadIdx.x & 7;
+  float top = -INFINITY, total = 0.0f;
+#pragma unroll 4
+  for (int s = first; s < splits; s += 8) {
+    const float2 x = ml[s];
+    const float most = fmaxf(top, x.x), ref = most == -INFINITY ? 0.0f : most;
+    total = total * __builtin_amdgcn_exp2f(top - ref) + x.y * __builtin_amdgcn_exp2f(x.x - ref);
+    top = most;
+  }
+  float most = top;
+  most = fmaxf(most, dpp_partner<1>(most));
+  most = fmaxf(most, dpp_partner<2>(most));
+  most = fmaxf(most, dpp_partner<4>(most));
+  const float ref = most == -INFINITY ? 0.0f : most;
+  total *= __builtin_amdgcn_exp2f(top - ref);
+  total += dpp_partner<1>(total);
+  total += dpp_partner<2>(total);
+  total += dpp_partner<4>(total);
+  return make_float2(ref, total);
 }
 
 // The first `joins` blocks join the splits of a query head each (joins = 0: there
@@ -506,36 +562,59 @@ __device__ __forceinline__ float2 join_ml(const float2* ml, int splits) {
 // queries, a slot having one thread.  Else one query's, listed ones: two queries
 // never add to one slot at the same time, and a slot that one query lists twice
 // takes the same addend twice, so that the sums have one order.
-__global__ __launch_bounds__(kNT) void finish_kernel(AttnArgs a, int DV, int64_t joins, int t, int64_t per_b) {
+template <int DV>
+__global__ __launch_bounds__(kNT) void finish_kernel(AttnArgs a, int64_t joins, int t, int64_t per_b) {
+  constexpr int kQuads = DV / 4, kGroups = kNT / kQuads;  // of splits, which take turns
   __shared__ float2 head[1024];
+  __shared__ float4 sums[kGroups][kQuads];
   if (blockIdx.x < joins) {
     const int64_t h = blockIdx.x;
     const float2* ml = a.ml + h * a.splits;
     const float2 all = join_ml(ml, a.splits);
+    const int quad = threadIdx.x % kQuads, group = threadIdx.x / kQuads;
+    float4 x = {0, 0, 0, 0};
+    if (group < kGroups) {
+      const float4* part = reinterpret_cast<const float4*>(a.part + h * a.splits * DV) + quad;
+#pragma unroll 4
+      for (int s = group; s < a.splits; s += kGroups) {
+        const float2 y = ml[s];
+        if (y.y == 0.0f) continue;  // a chunk without a sum has left none
+        const float f = __builtin_amdgcn_exp2f(y.x - all.x);
+        const float4 v = part[static_cast<int64_t>(s) * kQuads];
+        x.x += f * v.x; x.y += f * v.y; x.z += f * v.z; x.w += f * v.w;
+      }
+      sums[group][quad] = x;
+    }
+    __syncthreads();
     for (int d = threadIdx.x; d < DV; d += kNT) {
-      float x = 0.0f;
-      for (int s = 0; s < a.splits; ++s)
-        if (ml[s].y != 0.0f)  // a chunk without a sum has left none
-          x += __builtin_amdgcn_exp2f(ml[s].x - all.x) * a.part[(h * a.splits + s) * DV + d];
-      a.out[h * DV + d] = x * all.y;
+      float y = 0.0f;
+      for (int s = 0; s < min(kGroups, a.splits); ++s) y += reinterpret_cast<const float*>(sums[s])[d];
+      a.out[h * DV + d] = y / all.y;  // 0 / 0 where no logit is above -inf
     }
     return;
   }
-  const int64_t blk = blockIdx.x - joins, b = blk / per_b, j = blk % per_b * kNT + threadIdx.x;
+  const uint32_t blk = blockIdx.x - static_cast<uint32_t>(joins), b = blk / static_cast<uint32_t>(per_b);
+  const int64_t j = static_cast<int64_t>(blk % static_cast<uint32_t>(per_b)) * kNT + threadIdx.x;
   float* weight = a.c.weight + b * a.c.S;
   float sum = 0.0f;
   int32_t slot = -1;
   for (int tt = t < 0 ? 0 : t; tt < (t < 0 ? a.Tq : t + 1); ++tt) {
-    const int64_t bt = b * a.Tq + tt;
+    const int64_t bt = static_cast<int64_t>(b) * a.Tq + tt;
     const int32_t seen = kv4_visible(a.c.length, a.count, b, a.c.S, tt, a.Tq);
     __syncthreads();
-    for (int h = threadIdx.x; h < a.HQ; h += kNT) head[h] = join_ml(a.ml + (bt * a.HQ + h) * a.splits, a.splits);
+    for (int h0 = 0; h0 < a.HQ; h0 += kNT / 8) {
+      const int h = h0 + threadIdx.x / 8;
+      const float2 x = join_ml(a.ml + (bt * a.HQ + min(h, a.HQ - 1)) * a.splits, a.splits);
+      if (h < a.HQ && threadIdx.x % 8 == 0) head[h] = make_float2(x.x, 1.0f / x.y);
+    }
     __syncthreads();
     const int32_t s = j >= a.n ? -1 : a.slots ? a.slots[bt * a.n + j] : static_cast<int32_t>(j);
     if (s < 0 || s >= seen) continue;
     slot = s;
+    const float* logits = a.logits + bt * a.HQ * a.stride + j;
+#pragma unroll 8
     for (int h = 0; h < a.HQ; ++h)
-      sum += __builtin_amdgcn_exp2f(a.logits[(bt * a.HQ + h) * a.stride + j] - head[h].x) * head[h].y;
+      sum += __builtin_amdgcn_exp2f(logits[h * a.stride] - head[h].x) * head[h].y;
   }
   if (slot < 0) return;
   if (a.slots) atomicAdd(weight + slot, sum);
@@ -543,7 +622,7 @@ __global__ __launch_bounds__(kNT) void finish_kernel(AttnArgs a, int DV, int64_t
 }
 
 struct Plan {
-  int splits, chunk, row_tiles;
+  int splits, row_tiles, heads;
   bool side;
   int64_t ml, part, logits, total, stride;  // byte offsets; floats a row
 };
@@ -553,16 +632,17 @@ Plan plan_of(const Kv4& c, int64_t Tq, int HQ, int64_t n, bool accumulate) {
   const int G = HQ / c.HKV;
   p.side = G <= 5;
   p.row_tiles = p.side ? 1 : (G + 15) / 16;
-  const int64_t blocks = c.B * Tq * c.HKV * p.row_tiles;
-  const int64_t steps = n > 0 ? (n + kStep - 1) / kStep : 1;
+  p.heads = c.HKV % 4 == 0 ? 4 : c.HKV % 2 == 0 ? 2 : 1;
+  const int64_t blocks = c.B * Tq * (c.HKV / p.heads) * p.row_tiles;
+  const int unit = kTile * (kWaves / p.heads);  // slots that a block takes at once
+  const int64_t steps = n > 0 ? (n + unit - 1) / unit : 1;
   const int cus = device_cus() > 0 ? device_cus() : 256;
-  int64_t splits = blocks > 0 ? (4 * cus + blocks - 1) / blocks : 1;
+    int64_t splits = blocks > 0 ? (2 * cus + blocks - 1) / blocks : 1;
   splits = splits < 1 ? 1 : splits > steps ? steps : splits;
-  p.chunk = static_cast<int>((steps + splits - 1) / splits) * kStep;
-  p.splits = static_cast<int>((steps * kStep + p.chunk - 1) / p.chunk);
+  p.splits = static_cast<int>(splits);
   auto up = [](int64_t v) { return (v + 255) / 256 * 256; };
   const int64_t heads = c.B * Tq * HQ;
-  p.stride = steps * kStep;
+  p.stride = (n + kTile - 1) / kTile * kTile;
   p.ml = 0;
   p.part = up(heads * p.splits * 8);
   p.logits = p.part + (p.splits > 1 ? up(heads * p.splits * c.DV * 4) : 0);
@@ -621,17 +701,17 @@ hipError_t launch_kv4_attn(const Kv4& c, const void* Q, int dtype, const int32_t
   a.HQ = HQ;
   a.G = HQ / c.HKV;
   a.row_tiles = p.row_tiles;
+  a.heads = p.heads;
   a.n = n;
   a.stride = p.stride;
   a.splits = p.splits;
-  a.chunk = p.chunk;
   a.scale = scale;
   a.out = out;
   a.ml = reinterpret_cast<float2*>(base + p.ml);
   a.part = reinterpret_cast<float*>(base + p.part);
   a.logits = accumulate ? reinterpret_cast<float*>(base + p.logits) : nullptr;
   const int64_t chunks = (c.B * Tq * p.splits + 7) / 8 * 8;
-  const int64_t blocks = chunks * c.HKV * p.row_tiles;
+  const int64_t blocks = chunks * (c.HKV / p.heads) * p.row_tiles;
   hipError_t e = dtype == 0   ? launch_type<F32, 3>(a, p.side, blocks, stream)
                  : dtype == 1 ? launch_type<BF16, 1>(a, p.side, blocks, stream)
                               : launch_type<F16, 2>(a, p.side, blocks, stream);
@@ -639,8 +719,15 @@ hipError_t launch_kv4_attn(const Kv4& c, const void* Q, int dtype, const int32_t
   int64_t joins = p.splits > 1 ? c.B * Tq * HQ : 0;
   const int64_t per_b = accumulate ? (n + kNT - 1) / kNT : 0;
   for (int t = slots ? 0 : -1; t < (slots && accumulate ? a.Tq : slots ? 1 : 0); ++t) {
-    if (joins + per_b * c.B > 0)
-      finish_kernel<<<static_cast<uint32_t>(joins + per_b * c.B), kNT, 0, stream>>>(a, c.DV, joins, t, per_b);
+    const uint32_t grid = static_cast<uint32_t>(joins + per_b * c.B);
+    if (grid > 0) switch (c.DV) {
+      case 32: finish_kernel<32><<<grid, kNT, 0, stream>>>(a, joins, t, per_b); break;
+      case 64: finish_kernel<64><<<grid, kNT, 0, stream>>>(a, joins, t, per_b); break;
+      case 96: finish_kernel<96><<<grid, kNT, 0, stream>>>(a, joins, t, per_b); break;
+      case 128: finish_kernel<128><<<grid, kNT, 0, stream>>>(a, joins, t, per_b); break;
+      case 192: finish_kernel<192><<<grid, kNT, 0, stream>>>(a, joins, t, per_b); break;
+      default: finish_kernel<256><<<grid, kNT, 0, stream>>>(a, joins, t, per_b); break;
+    }
     joins = 0;
   }
   return hipGetLastError();
