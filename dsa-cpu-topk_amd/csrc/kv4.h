@@ -55,16 +55,48 @@ __device__ __forceinline__ uint32_t e8m0_of_max(uint32_t maxbits) {
   return static_cast<uint32_t>(min(max(e, 2), 252));
 }
 
-// 8 values as 8 codes: x / scale to the nearest e2m1 (ties to even, 6 beyond
-// it), exact because the scale is a power of two.
-__device__ __forceinline__ uint32_t e2m1_pack8(const float (&x)[8], float scale) {
-  uint32_t w = 0;
-  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[0], x[1], scale, 0);
-  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[2], x[3], scale, 1);
-  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[4], x[5], scale, 2);
-  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[6], x[7], scale, 3);
-  return w;
-}
+// 8 elements as they lie in memory; the bits of their largest magnitude as an
+// fp32's (Inf's or above where one is not finite); their codes, x / scale to the
+// nearest e2m1 (ties to even, 6 beyond it), exact because the scale is a power
+// of two.  16-bit types stay packed in pairs: their magnitudes order as integers.
+template <typename Tag>
+struct Octet {
+  uint32_t w[2 * Tag::kBytes];
+  __device__ __forceinline__ void load(const typename Tag::raw* p) {
+    __builtin_memcpy(w, __builtin_assume_aligned(p, 16), sizeof(w));
+  }
+  __device__ __forceinline__ uint32_t top() const {
+    if constexpr (Tag::kBytes == 4) {
+      uint32_t m = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) m = max(m, w[i] & 0x7fffffffu);
+      return m;
+    } else {
+      typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+      u16x2 m = __builtin_bit_cast(u16x2, w[0] & 0x7fff7fffu);
+#pragma unroll
+      for (int i = 1; i < 4; ++i) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, w[i] & 0x7fff7fffu));
+      return __float_as_uint(to_f32(Tag{}, max(m[0], m[1])));
+    }
+  }
+  __device__ __forceinline__ uint32_t codes(float scale) const {
+    uint32_t c = 0;
+    c = pair<0>(c, scale);
+    c = pair<1>(c, scale);
+    c = pair<2>(c, scale);
+    return pair<3>(c, scale);
+  }
+  template <int I>
+  __device__ __forceinline__ uint32_t pair(uint32_t c, float scale) const {
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    if constexpr (Tag::kBytes == 4)
+      return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, __uint_as_float(w[2 * I]), __uint_as_float(w[2 * I + 1]), scale, I);
+    else if constexpr (__is_same(Tag, BF16))
+      return __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(c, __builtin_bit_cast(bf16x2, w[I]), scale, I);
+    else
+      return __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(c, __builtin_bit_cast(f16x2, w[I]), scale, I);
+  }
+};
 __device__ __forceinline__ void e2m1_unpack8(uint32_t w, float scale, float (&x)[8]) {
   const auto a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, scale, 0);
   const auto b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, scale, 1);

@@ -7,11 +7,37 @@ namespace {
 
 constexpr int kNT = 256;
 
+// How a block's threads cover its tokens: a thread owns word u of a slot (8
+// elements of one head's K or V) for every `step`-th of the block's tokens, so
+// that the head and the source's stride are worked out once, and small slots
+// still take all threads.  words is a multiple of 8, so the 4 lanes of a
+// 32-element block stay 4 neighbours.
+struct Cover {
+  int u, first, step;  // past the slot's words: nothing to do
+  bool is_k;
+  int64_t at, stride;  // elements: of word u in the first token's K or V, from token to token
+};
+__device__ __forceinline__ Cover cover(const Kv4& c, int base) {
+  const int words = c.words(), per_head = (c.DK + c.DV) / 8, kw = c.DK / 8;
+  Cover t;
+  t.step = max(1, kNT / words);
+  t.first = words < kNT ? threadIdx.x / words : 0;
+  t.u = words < kNT ? threadIdx.x - t.first * words : base + threadIdx.x;
+  if (t.first >= t.step) t.u = words;
+  const int h = t.u / per_head, r = t.u - h * per_head;
+  t.is_k = r < kw;
+  t.at = t.is_k ? static_cast<int64_t>(h) * c.DK + r * 8 : static_cast<int64_t>(h) * c.DV + (r - kw) * 8;
+  t.stride = static_cast<int64_t>(c.HKV) * (t.is_k ? c.DK : c.DV);
+  return t;
+}
+
 // ---------------------------------------------------------------------------
-// Append.  A thread owns word u of a slot (8 elements of one head's K or V)
-// and quantises it for the block's tokens; the four lanes of a 32-element
-// block share its largest magnitude.
+// Append, bound by memory: a thread's kAhead tokens are on their way at once
+// (2, 4 and 8 measured 46, 49 and 53 us for 2 x 16384 tokens of 8 heads of 128 in
+// bf16, 187 MB).
 // ---------------------------------------------------------------------------
+constexpr int kAhead = 2, kRowsAhead = 4;
+
 template <typename Tag>
 __global__ __launch_bounds__(kNT) void append_kernel(Kv4 c, const typename Tag::raw* __restrict__ K,
                                                      const typename Tag::raw* __restrict__ V,
@@ -27,38 +53,42 @@ __global__ __launch_bounds__(kNT) void append_kernel(Kv4 c, const typename Tag::
   const int64_t stored = min(many, c.S - have);
   const int64_t i1 = min(i0 + per_block, stored);
 
-  const int words = c.words(), per_head = (c.DK + c.DV) / 8, kw = c.DK / 8;
-  for (int u = threadIdx.x; u < words; u += kNT) {  // words is a multiple of 8
-    const int h = u / per_head, r = u - h * per_head;
-    const bool isk = r < kw;
-    const typename Tag::raw* src =
-        isk ? K + (b * T * c.HKV + h) * c.DK + r * 8 : V + (b * T * c.HKV + h) * c.DV + (r - kw) * 8;
-    const int64_t step = static_cast<int64_t>(c.HKV) * (isk ? c.DK : c.DV);
-    for (int64_t i = i0; i < i1; ++i) {
-      float x[8];
-      load_cvt<Tag, 8>(src + i * step, x);
-      uint32_t m = 0;
+  const int words = c.words();
+  const int64_t slot0 = b * c.S + have;
+  for (int base = 0; base < words; base += kNT) {
+    const Cover t = cover(c, base);
+    if (t.u >= words) continue;
+    const int nb = static_cast<int>(max(static_cast<int64_t>(0), i1 - i0));  // at most kAhead a thread
+    const typename Tag::raw* src = (t.is_k ? K : V) + (b * T + i0) * t.stride + t.at;
+    uint32_t* codes = reinterpret_cast<uint32_t*>(c.codes) + (slot0 + i0) * words + t.u;
+    uint8_t* scales = c.scales + (slot0 + i0) * (words / 4) + t.u / 4;
+    const int stride = static_cast<int>(t.stride);
+    Octet<Tag> x[kAhead];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(x[j]) & 0x7fffffffu);
+    for (int k = 0; k < kAhead; ++k)
+      if (t.first + k * t.step < nb) x[k].load(src + (t.first + k * t.step) * stride);
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const int i = t.first + k * t.step;
+      if (i >= nb) break;  // the same for the 4 lanes of a block
+      uint32_t m = x[k].top();
       m = max(m, dpp_u32<0xB1>(m));  // quad_perm [1,0,3,2]
       m = max(m, dpp_u32<0x4E>(m));  // quad_perm [2,3,0,1]
       const uint32_t s = e8m0_of_max(m);
-      const uint32_t w = s == 255u ? 0u : e2m1_pack8(x, e8m0(s));
-      const int64_t slot = b * c.S + have + i;
-      reinterpret_cast<uint32_t*>(c.codes)[slot * words + u] = w;
-      if ((u & 3) == 0) c.scales[slot * c.scale_bytes() + u / 4] = static_cast<uint8_t>(s);
+      codes[i * words] = s == 255u ? 0u : x[k].codes(e8m0(s));
+      if ((t.u & 3) == 0) scales[i * (words / 4)] = static_cast<uint8_t>(s);
     }
   }
   if (new_idx) {
     const int chunks = c.DI * c.idx_bytes / 16;
     for (int64_t i = i0 * chunks + threadIdx.x; i < i1 * chunks; i += kNT)
-      static_cast<uint4*>(c.k_idx)[(b * c.S + have) * chunks + i] = new_idx[b * T * chunks + i];
+      static_cast<uint4*>(c.k_idx)[slot0 * chunks + i] = new_idx[b * T * chunks + i];
   }
   for (int64_t i = i0 + threadIdx.x; i < i1; i += kNT) {
-    c.position[b * c.S + have + i] = before + static_cast<int32_t>(i);
-    c.weight[b * c.S + have + i] = weight ? weight[b * T + i] : 0.0f;
+    c.position[slot0 + i] = before + static_cast<int32_t>(i);
+    c.weight[slot0 + i] = weight ? weight[b * T + i] : 0.0f;
   }
-  if (update) {  // the sequence's only block
+  if (update && blockIdx.x == 0) {  // the sequence's only block, or no block reads the counters
     __syncthreads();
     if (threadIdx.x == 0) {
       c.length[b] = have + static_cast<int32_t>(stored);
@@ -68,7 +98,7 @@ __global__ __launch_bounds__(kNT) void append_kernel(Kv4 c, const typename Tag::
   }
 }
 
-// The counters of an append that took more than one block a sequence.
+// The counters of an append whose blocks read them.
 __global__ void append_counts_kernel(Kv4 c, const int32_t* __restrict__ count, int64_t T, int restart) {
   const int64_t b = blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x;
   if (b >= c.B) return;
@@ -112,99 +142,23 @@ __global__ __launch_bounds__(kNT) void rows_kernel(Kv4 c, const int32_t* __restr
   const int64_t b = blockIdx.y;
   const int64_t i0 = static_cast<int64_t>(blockIdx.x) * per_block, i1 = min(i0 + per_block, N);
   const int32_t have = kv4_length(c.length, b, c.S);
-  const int words = c.words(), per_head = (c.DK + c.DV) / 8, kw = c.DK / 8;
-  for (int u = threadIdx.x; u < words; u += kNT) {
-    const int h = u / per_head, r = u - h * per_head;
-    const bool isk = r < kw;
-    typename Tag::raw* dst =
-        isk ? K + (b * N * c.HKV + h) * c.DK + r * 8 : V + (b * N * c.HKV + h) * c.DV + (r - kw) * 8;
-    const int64_t step = static_cast<int64_t>(c.HKV) * (isk ? c.DK : c.DV);
-    for (int64_t i = i0; i < i1; ++i) {
+  const int words = c.words();
+  for (int base = 0; base < words; base += kNT) {
+    const Cover t = cover(c, base);
+    if (t.u >= words) continue;
+    typename Tag::raw* dst = (t.is_k ? K : V) + b * N * t.stride + t.at;
+#pragma unroll kRowsAhead
+    for (int64_t i = i0 + t.first; i < i1; i += t.step) {
       const int64_t s = slots ? slots[b * N + i] : i;
       float x[8] = {};
       if (s >= 0 && s < have) {
         const int64_t slot = b * c.S + s;
-        e2m1_unpack8(reinterpret_cast<const uint32_t*>(c.codes)[slot * words + u],
-                     e8m0(c.scales[slot * c.scale_bytes() + u / 4]), x);
+        e2m1_unpack8(reinterpret_cast<const uint32_t*>(c.codes)[slot * words + t.u],
+                     e8m0(c.scales[slot * (words / 4) + t.u / 4]), x);
       }
-      store8<Tag>(dst + i * step, x);
+      store8<Tag>(dst + i * t.stride, x);
     }
   }
-}
-
-// ---------------------------------------------------------------------------
-// Evict.  One block a sequence finds the E = length - keep slots that go: the
-// E smallest keys, the order-preserving bits of the weight, above all of them
-// for a protected (recent) slot; among equals the highest slots go.  Then the
-// i-th kept slot at or past `keep` moves into the i-th freed slot below it: no
-// slot is both read and written, and no more slots move than have to.
-// ---------------------------------------------------------------------------
-constexpr int kET = 1024;
-
-__global__ __launch_bounds__(kET) void evict_select_kernel(Kv4 c, int64_t keep, int64_t recent,
-                                                           int64_t M, int32_t* __restrict__ src,
-                                                           int32_t* __restrict__ dst) {
-  __shared__ uint32_t hist[256];
-  __shared__ uint32_t wsum[kET / kWave];
-  __shared__ uint32_t pick[2];
-  const int64_t b = blockIdx.x;
-  const int32_t n = kv4_length(c.length, b, c.S);
-  const float* weight = c.weight + b * c.S;
-  const int32_t* position = c.position + b * c.S;
-  src += b * M;
-  dst += b * M;
-  if (n <= keep) {
-    for (int64_t i = threadIdx.x; i < M; i += kET) src[i] = dst[i] = -1;
-    return;
-  }
-  const int64_t first_kept = static_cast<int64_t>(c.seen[b]) - recent;
-  auto key_of = [&](int s) {
-    return position[s] >= first_kept ? 0xffffffffu : float_to_key(weight[s]);
-  };
-  uint32_t prefix = 0, want = n - static_cast<int32_t>(keep);  // the want-th smallest is the last to go
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    for (int i = threadIdx.x; i < 256; i += kET) hist[i] = 0;
-    __syncthreads();
-    for (int s = threadIdx.x; s < n; s += kET) {
-      const uint32_t k = key_of(s);
-      if (shift == 24 || (k >> (shift + 8)) == (prefix >> (shift + 8)))
-        atomicAdd(&hist[(k >> shift) & 255u], 1u);
-    }
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      uint32_t below = 0, bin = 0;
-      while (bin < 255 && below + hist[bin] < want) below += hist[bin++];
-      pick[0] = bin;
-      pick[1] = want - below;
-    }
-    __syncthreads();
-    prefix |= pick[0] << shift;
-    want = pick[1];
-    __syncthreads();
-  }
-  // `want` of the slots with key == prefix go: the last ones
-  uint32_t ties = 0, unused;
-  for (int s = threadIdx.x; s < n; s += kET) ties += key_of(s) == prefix;
-  block_exclusive_sum<kET>(ties, wsum, unused);
-  ties = unused;
-  uint32_t tie0 = 0, free0 = 0, away0 = 0;
-  for (int s0 = 0; s0 < n; s0 += kET) {
-    const int s = s0 + threadIdx.x;
-    const uint32_t k = s < n ? key_of(s) : 0u;
-    const bool tie = s < n && k == prefix;
-    uint32_t total;
-    const uint32_t at = tie0 + block_exclusive_sum<kET>(tie, wsum, total);
-    tie0 += total;
-    const bool goes = s < n && (k < prefix || (tie && at >= ties - want));
-    const bool freed = goes && s < keep, away = s < n && !goes && s >= keep;
-    const uint32_t where = block_exclusive_sum<kET>((freed ? 1u : 0u) | (away ? 0x10000u : 0u), wsum, total);
-    if (freed) dst[free0 + (where & 0xffffu)] = s;
-    if (away) src[away0 + (where >> 16)] = s;
-    free0 += total & 0xffffu;
-    away0 += total >> 16;
-  }
-  for (int64_t i = free0 + threadIdx.x; i < M; i += kET) src[i] = dst[i] = -1;
-  if (threadIdx.x == 0) c.length[b] = static_cast<int32_t>(keep);
 }
 
 // Copies `bytes` bytes with the wave.  Rows of a multiple of 16 bytes start at one
@@ -219,12 +173,8 @@ __device__ __forceinline__ void wave_copy(uint8_t* dst, const uint8_t* src, int 
   }
 }
 
-__global__ __launch_bounds__(kNT) void evict_move_kernel(Kv4 c, int64_t M, const int32_t* __restrict__ src,
-                                                         const int32_t* __restrict__ dst) {
-  const int64_t b = blockIdx.y;
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * (kNT / kWave) + threadIdx.x / kWave;
-  if (i >= M || src[b * M + i] < 0) return;
-  const int64_t u = b * c.S + src[b * M + i], v = b * c.S + dst[b * M + i];
+// Slot u's token into slot v, by a wave.
+__device__ __forceinline__ void wave_move(const Kv4& c, int64_t u, int64_t v) {
   const int cb = c.words() * 4, sb = c.scale_bytes(), ib = c.DI * c.idx_bytes;
   wave_copy(c.codes + v * cb, c.codes + u * cb, cb);
   wave_copy(c.scales + v * sb, c.scales + u * sb, sb);
@@ -235,15 +185,205 @@ __global__ __launch_bounds__(kNT) void evict_move_kernel(Kv4 c, int64_t M, const
   }
 }
 
+// ---------------------------------------------------------------------------
+// Evict.  One block a sequence finds the E = length - keep slots that go: the
+// E smallest keys, the order-preserving bits of the weight, above all of them
+// for a protected (recent) slot; among equals the highest slots go.  Then the
+// i-th kept slot at or past `keep` moves into the i-th freed slot below it: no
+// slot is both read and written, and no more slots move than have to.
+//
+// A thread holds VPT neighbouring slots' keys in registers (longer caches are
+// read again in every pass, VPT * 1024 slots at a time).  The E-th smallest key
+// is found by halving the range by 1024: a histogram of the keys between lo and
+// hi, whose bins cut that range evenly, and the bin that holds the E-th; done when
+// the bin's keys all go, or are all equal.  Few keys share a bin of weights spread
+// like real ones, so two passes are the rule, and few lanes add to one bin at once.
+// ---------------------------------------------------------------------------
+constexpr int kET = 1024, kBins = 1024;
+constexpr int kInPlace = 64;  // most moves that the selecting block makes itself
+
+// The block's sum of v before this thread's, and over all (kET threads).
+__device__ __forceinline__ uint32_t evict_scan(uint32_t v, uint32_t* wsum, uint32_t& total) {
+  return block_exclusive_sum<kET>(v, wsum, total);
+}
+
+template <int VPT>
+__global__ __launch_bounds__(kET) void evict_select_kernel(Kv4 c, int64_t keep, int64_t recent,
+                                                           int64_t M, int32_t* __restrict__ src,
+                                                           int32_t* __restrict__ dst) {
+  __shared__ uint32_t hist[kBins];
+  __shared__ uint32_t wsum[kET / kWave], wlo[kET / kWave], whi[kET / kWave];
+  __shared__ uint32_t pick[3];
+  __shared__ int32_t from[kInPlace], to[kInPlace];
+  const int64_t b = blockIdx.x;
+  const int32_t n = kv4_length(c.length, b, c.S);
+  const float* weight = c.weight + b * c.S;
+  const int32_t* position = c.position + b * c.S;
+  src += b * M;
+  dst += b * M;
+  if (n <= keep) {
+    for (int64_t i = threadIdx.x; i < M; i += kET) src[i] = dst[i] = -1;
+    return;
+  }
+  constexpr uint32_t kProtected = 0xffffffffu;  // above every weight's key
+  const int64_t first_kept = static_cast<int64_t>(c.seen[b]) - recent;
+  constexpr int kSpan = VPT * kET;
+  uint32_t key[VPT];
+  auto read = [&](int s0) {  // keys of slots s0 + VPT * thread ..; past n: not looked at
+    const int s = s0 + threadIdx.x * VPT;
+    float w[VPT];
+    int32_t p[VPT];
+    if (s + VPT <= n) {  // 16 bytes at once, at any multiple of 4
+#pragma unroll
+      for (int i = 0; i < VPT; i += 4) {
+        __builtin_memcpy(w + i, weight + s + i, 16);
+        __builtin_memcpy(p + i, position + s + i, 16);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) {
+        w[i] = s + i < n ? weight[s + i] : 0.0f;
+        p[i] = s + i < n ? position[s + i] : 0;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) key[i] = p[i] >= first_kept ? kProtected : float_to_key(w[i]);
+  };
+  const bool once = n <= kSpan;
+  if (once) read(0);
+  auto each = [&](auto f) {  // f(slot, key) for the thread's slots of a span that count
+    for (int s0 = 0; s0 < n; s0 += kSpan) {
+      if (!once) read(s0);
+#pragma unroll
+      for (int i = 0; i < VPT; ++i)
+        if (s0 + static_cast<int>(threadIdx.x) * VPT + i < n) f(key[i]);
+    }
+  };
+
+  const uint32_t E = n - static_cast<int32_t>(keep);
+  uint32_t lo = kProtected, hi = 0, open = 0;  // of the slots that are not protected
+  each([&](uint32_t k) {
+    if (k != kProtected) {
+      lo = min(lo, k);
+      hi = max(hi, k);
+      ++open;
+    }
+  });
+  lo = wave_extreme_u32<false>(lo);
+  hi = wave_extreme_u32<true>(hi);
+  if ((threadIdx.x & 63) == 0) {
+    wlo[threadIdx.x / kWave] = lo;
+    whi[threadIdx.x / kWave] = hi;
+  }
+  uint32_t unprotected;
+  evict_scan(open, wsum, unprotected);  // its barriers publish wlo and whi too
+#pragma unroll
+  for (int w = 0; w < kET / kWave; ++w) {
+    lo = min(lo, wlo[w]);
+    hi = max(hi, whi[w]);
+  }
+  // keys below `lo` go, those above `hi` stay, and of the ties between them `want`
+  uint32_t want = E, ties = 0;
+  if (E > unprotected) {  // more protected than stay: the last of them go too
+    lo = hi = kProtected;
+    want = E - unprotected;
+    ties = n - unprotected;
+  } else {
+    ties = unprotected;
+    while (want != ties && lo != hi) {  // some key between lo and hi goes, and some stays
+      const int shift = max(0, 32 - static_cast<int>(__builtin_clz(hi - lo)) - 10);
+      __syncthreads();
+      hist[threadIdx.x] = 0;
+      __syncthreads();
+      each([&](uint32_t k) {
+        if (k >= lo && k <= hi) atomicAdd(&hist[(k - lo) >> shift], 1u);
+      });
+      __syncthreads();
+      const uint32_t mine = hist[threadIdx.x];
+      uint32_t total;
+      const uint32_t below = evict_scan(mine, wsum, total);
+      if (below < want && want <= below + mine) {
+        pick[0] = threadIdx.x;
+        pick[1] = want - below;
+        pick[2] = mine;
+      }
+      __syncthreads();
+      lo += pick[0] << shift;
+      hi = min(hi, lo + ((1u << shift) - 1));
+      want = pick[1];
+      ties = pick[2];
+    }
+  }
+
+  // The lists, in order of slots.
+  uint32_t tie0 = 0, free0 = 0, away0 = 0, total;
+  for (int s0 = 0; s0 < n; s0 += kSpan) {
+    if (!once) read(s0);
+    const int s = s0 + threadIdx.x * VPT;
+    uint32_t tie = 0;
+    if (want != ties) {
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) tie += s + i < n && key[i] == lo;
+      const uint32_t before = tie0 + evict_scan(tie, wsum, total);
+      tie0 += total;
+      tie = before;
+    }
+    uint64_t freed = 0, away = 0;  // the thread's slots, a bit each
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      if (s + i >= n) continue;
+      bool goes = key[i] < lo || (key[i] <= hi && want == ties);
+      if (want != ties && key[i] == lo) goes = tie++ >= ties - want;
+      if (goes && s + i < keep) freed |= 1ull << i;
+      if (!goes && s + i >= keep) away |= 1ull << i;
+    }
+    uint32_t f = free0 + evict_scan(popc64(freed), wsum, total);
+    free0 += total;
+    uint32_t w = away0 + evict_scan(popc64(away), wsum, total);
+    away0 += total;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      if (freed >> i & 1) {
+        if (M <= kInPlace) to[f] = s + i;
+        dst[f++] = s + i;
+      }
+      if (away >> i & 1) {
+        if (M <= kInPlace) from[w] = s + i;
+        src[w++] = s + i;
+      }
+    }
+  }
+  for (int64_t i = free0 + threadIdx.x; i < M; i += kET) src[i] = dst[i] = -1;
+  if (threadIdx.x == 0) c.length[b] = static_cast<int32_t>(keep);
+  if (M <= kInPlace) {
+    __syncthreads();
+    for (uint32_t i = threadIdx.x / kWave; i < free0; i += kET / kWave) wave_move(c, b * c.S + from[i], b * c.S + to[i]);
+  }
+}
+
+__global__ __launch_bounds__(kNT) void evict_move_kernel(Kv4 c, int64_t M, const int32_t* __restrict__ src,
+                                                         const int32_t* __restrict__ dst) {
+  const int64_t b = blockIdx.y;
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * (kNT / kWave) + threadIdx.x / kWave;
+  if (i >= M || src[b * M + i] < 0) return;
+  wave_move(c, b * c.S + src[b * M + i], b * c.S + dst[b * M + i]);
+}
+
+// Tokens of a block whose threads take `each` of them.
+int tokens_per_block(const Kv4& c, int each) {
+  const int words = c.words();
+  return each * (words < kNT ? kNT / words : 1);
+}
+
 }  // namespace
 
 hipError_t launch_kv4_append(const Kv4& c, const void* K, const void* V, int dtype,
                              const void* new_idx, const float* weight, const int32_t* count, int64_t T,
                              bool restart, hipStream_t stream) {
-  const int per_block = 4;
+  const int per_block = tokens_per_block(c, kAhead);
   const int64_t blocks = (T + per_block - 1) / per_block;
   const dim3 grid(static_cast<uint32_t>(blocks), static_cast<uint32_t>(c.B));
-  const int update = blocks == 1;
+  const int update = blocks == 1 || (restart && blocks > 0);
   const uint4* idx = static_cast<const uint4*>(new_idx);
   if (blocks == 0) {
     // a restart without tokens: the counters alone
@@ -263,7 +403,7 @@ hipError_t launch_kv4_append(const Kv4& c, const void* K, const void* V, int dty
 
 hipError_t launch_kv4_rows(const Kv4& c, const int32_t* slots, int64_t N, int dtype, void* K, void* V,
                            hipStream_t stream) {
-  const int per_block = 4;
+  const int per_block = tokens_per_block(c, kRowsAhead);
   const dim3 grid(static_cast<uint32_t>((N + per_block - 1) / per_block), static_cast<uint32_t>(c.B));
   if (dtype == 0)
     rows_kernel<F32><<<grid, kNT, 0, stream>>>(c, slots, N, per_block, static_cast<float*>(K), static_cast<float*>(V));
@@ -278,9 +418,11 @@ hipError_t launch_kv4_evict(const Kv4& c, int64_t keep, int64_t recent, int32_t*
                             hipStream_t stream) {
   if (keep >= c.S) return hipSuccess;
   const int64_t M = keep < c.S - keep ? keep : c.S - keep;
-  evict_select_kernel<<<static_cast<uint32_t>(c.B), kET, 0, stream>>>(c, keep, recent, M, src, dst);
+  const uint32_t grid = static_cast<uint32_t>(c.B);
+  if (c.S <= 4 * kET) evict_select_kernel<4><<<grid, kET, 0, stream>>>(c, keep, recent, M, src, dst);
+  else evict_select_kernel<16><<<grid, kET, 0, stream>>>(c, keep, recent, M, src, dst);
   hipError_t e = hipGetLastError();
-  if (e != hipSuccess || M == 0) return e;
+  if (e != hipSuccess || M <= kInPlace) return e;
   const int rows = kNT / kWave;
   evict_move_kernel<<<dim3(static_cast<uint32_t>((M + rows - 1) / rows), static_cast<uint32_t>(c.B)), kNT, 0, stream>>>(c, M, src, dst);
   return hipGetLastError();

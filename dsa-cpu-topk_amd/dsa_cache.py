@@ -94,6 +94,7 @@ class KV4Cache:
         def at(x):
             return x.data_ptr() if x is not None else None
 
+        self._workspace = {}  # bytes of kv4_attention's, by its sizes
         self._c = L.Kv4Cache(at(codes), at(scales), at(k_idx), at(length), at(seen), at(lost),
                              at(position), at(weight), B, S, HKV, self.DK, DV, DI,
                              L.dtype_code(idx_dtype))
@@ -132,12 +133,13 @@ def _stored(cache: KV4Cache) -> None:
 
 
 def _ints(x: torch.Tensor | None, shape, name: str, cache: KV4Cache):
-    """An optional int32 tensor and its pointer; contiguous copies where it is not."""
+    """An optional int32 tensor and its pointer; a contiguous copy where it is not."""
     if x is None:
         return None, None
-    assert x.dtype == torch.int32 and tuple(x.shape) == shape and x.device == cache.device, \
+    assert x.dtype is torch.int32 and x.shape == shape and x.device == cache.device, \
         f"{name}: int32 {shape} on {cache.device} (got {x.dtype} {tuple(x.shape)} on {x.device})"
-    x = x.contiguous()
+    if not x.is_contiguous():
+        x = x.contiguous()
     return x, x.data_ptr()
 
 
@@ -172,7 +174,10 @@ def kv4_append(cache: KV4Cache, K: torch.Tensor, V: torch.Tensor, k_idx: torch.T
     _on(cache, K, V)
     assert (k_idx is None) == (cache.k_idx is None), "index keys go with a cache that holds them"
     dt = L.common_dtype(K, V)
-    K, V = L.prep(K, dt), L.prep(V, dt)
+    ptrs = L.ready_ptrs(dt, (K, V))
+    if ptrs is None:
+        K, V = L.prep(K, dt), L.prep(V, dt)
+        ptrs = K.data_ptr(), V.data_ptr()
     if k_idx is not None:
         assert k_idx.shape == (B, T, cache.DI), f"k_idx shape {tuple(k_idx.shape)} != {(B, T, cache.DI)}"
         _on(cache, k_idx)
@@ -184,7 +189,7 @@ def kv4_append(cache: KV4Cache, K: torch.Tensor, V: torch.Tensor, k_idx: torch.T
     count, count_ptr = _ints(count, (B,), "count", cache)
     with L.on_device(cache.device):
         L.check(L.lib().dsa_kv4_append(
-            cache._ref, K.data_ptr(), V.data_ptr(), L.dtype_code(dt),
+            cache._ref, *ptrs, L.dtype_code(dt),
             k_idx.data_ptr() if k_idx is not None else None,
             weight.data_ptr() if weight is not None else None, count_ptr, T, 1 if restart else 0,
             L.stream_ptr(cache.device)), "kv4_append")
@@ -268,32 +273,43 @@ def kv4_attention(cache: KV4Cache, Q: torch.Tensor, *, slots: torch.Tensor | Non
         L.check_out(out, B * Tq * HQ * cache.DV, cache.device)
     acc = 1 if accumulate else 0
     with L.on_device(cache.device):
-        nws = L.lib().dsa_kv4_attention_workspace_bytes(cache._ref, Tq, HQ, 0 if slots is None else 1,
+        lib = L.lib()
+        sizes = (Tq, HQ, slots is None, n, acc)
+        nws = cache._workspace.get(sizes)
+        if nws is None:
+            if len(cache._workspace) >= 64:  # spans of a growing cache
+                cache._workspace.clear()
+            nws = lib.dsa_kv4_attention_workspace_bytes(cache._ref, Tq, HQ, 0 if slots is None else 1,
                                                         n, acc)
-        ws = torch.empty(max(nws, 16), device=cache.device, dtype=torch.uint8)
-        L.check(L.lib().dsa_kv4_attention(
+            cache._workspace[sizes] = nws
+        ws = torch.empty(nws, device=cache.device, dtype=torch.uint8)
+        rc = lib.dsa_kv4_attention(
             cache._ref, Q.data_ptr(), L.dtype_code(dt), slots_ptr, count_ptr, Tq, HQ, n, acc,
-            1.0 / math.sqrt(DK), out.data_ptr(), ws.data_ptr(), nws, L.stream_ptr(cache.device)),
-            "kv4_attention")
+            1.0 / math.sqrt(DK), out.data_ptr(), ws.data_ptr(), nws, L.stream_ptr(cache.device))
+    if rc != L.DSA_OK:
+        L.check(rc, "kv4_attention")
     return out
 
 
-def kv4_evict(cache: KV4Cache, keep: int, recent: int = 0) -> torch.Tensor:
+def kv4_evict(cache: KV4Cache, keep: int, recent: int = 0):
     """Evict every sequence that has more than `keep` slots down to them: the
     `recent` newest tokens stay, then those of the largest accumulated weight
     (among equals the lowest slot).
 
-    Kept slots at or past `keep` move into the freed ones.  Returns them as int32
-    [2,B,M], M = min(keep, S - keep): the slots they came from and went to, in
-    order, -1 past the last (for buffers of the caller's that go by slot)."""
+    Kept slots at or past `keep` move into the freed ones.  Returns (from, to), int32
+    [B,M] each, M = min(keep, S - keep): the slots that moved, in order, -1 past the
+    last (for buffers of the caller's that go by slot)."""
     _stored(cache)
     keep, recent = int(keep), int(recent)
-    moved = torch.empty(2, cache.B, max(0, min(keep, cache.S - keep)), device=cache.device,
-                        dtype=torch.int32)
+    M = max(0, min(keep, cache.S - keep))
+    moved = torch.empty((2, cache.B, M), device=cache.device, dtype=torch.int32)
+    src = moved.data_ptr()
     with L.on_device(cache.device):
-        L.check(L.lib().dsa_kv4_evict(cache._ref, keep, recent, moved[0].data_ptr(),
-                                      moved[1].data_ptr(), L.stream_ptr(cache.device)), "kv4_evict")
-    return moved
+        rc = L.lib().dsa_kv4_evict(cache._ref, keep, recent, src, src + 4 * cache.B * M,
+                                   L.stream_ptr(cache.device))
+    if rc != L.DSA_OK:
+        L.check(rc, "kv4_evict")
+    return moved.unbind(0)
 
 
 def dsa_decode(cache: KV4Cache, q_idx, k_idx, w_idx, Q, K, V, top_k: int, *,

@@ -410,8 +410,8 @@ def test_attention_past_32_bit_offsets(dev):
            (size / total).view(B, 1, 16, D_) * (2.0 ** -16 + 600 * C.U + 1e-5), "whole")
     K, V = D.kv4_rows(cache, (pick + at)[:, 0].contiguous())
     assert torch.equal(K, C.decode(small.codes[..., :64], small.scales[..., :4]).float())
-    moved = D.kv4_evict(cache, S - 5, 0)
-    assert moved.shape == (2, B, 5) and cache.length.tolist() == [S - 5] * B
+    src, dst = D.kv4_evict(cache, S - 5, 0)
+    assert src.shape == dst.shape == (B, 5) and cache.length.tolist() == [S - 5] * B
 
 
 # --- eviction ----------------------------------------------------------------------------------------
@@ -420,7 +420,7 @@ def check_evict(cache, keep, recent, what):
     want = C.evict(cache.length.cpu(), cache.seen.cpu(), cache.position.cpu(), cache.weight.cpu(), keep, recent)
     names = ("codes", "scales", "position", "weight", "k_idx")
     before = {n: getattr(cache, n).clone() for n in names if getattr(cache, n) is not None}
-    moved = D.kv4_evict(cache, keep, recent).cpu()
+    moved = torch.stack(D.kv4_evict(cache, keep, recent)).cpu()
     M = max(0, min(keep, cache.S - keep))
     assert moved.shape == (2, cache.B, M)
     for b, (src, dst, n) in enumerate(want):
