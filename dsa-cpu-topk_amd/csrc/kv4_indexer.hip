@@ -29,8 +29,8 @@ struct IndexArgs {
   const void* w;
   const int32_t* count;
   int Tq, per, groups;  // tokens a block, groups of them a sequence
-  int HI, chunks;
-  int64_t span, chunk;  // slots scored, and of one block
+  int HI, blocks;  // that share a group's slots, a tile to each of their waves in turn
+  int64_t span;    // slots scored
   float* scores;
 };
 
@@ -52,19 +52,17 @@ __global__ __launch_bounds__(kNT) void indexer_kernel(IndexArgs a) {
   constexpr int ROW = DI * Tag::kBytes, NC = ROW / 64;  // bytes of a row, 16-byte pieces of a lane's quarter
   extern __shared__ u32x4 lds[];
   const int nht = (a.HI + 15) / 16;
-  const int64_t bg = blockIdx.x / a.chunks, b = bg / a.groups;
+  const uint32_t bg = blockIdx.x / a.blocks, b = bg / a.groups;
   const int t0 = static_cast<int>(bg % a.groups) * a.per, nt = min(a.per, a.Tq - t0);
-  const int64_t c0 = blockIdx.x % a.chunks * a.chunk;
-  const int64_t c1 = min(c0 + a.chunk, a.span);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = threadIdx.x & 63, g = lane >> 4, r16 = lane & 15;
-  int32_t limit = 0;
+  int32_t limit = 0;  // slots that some token of the group sees
   for (int t = 0; t < nt; ++t) limit = max(limit, kv4_visible(a.c.length, a.count, b, a.c.S, t0 + t, a.Tq));
-  const int64_t bt0 = b * a.Tq + t0;
-  if (c0 >= limit) {
-    for (int t = 0; t < nt; ++t)
-      for (int64_t s = c0 + threadIdx.x; s < c1; s += kNT) a.scores[(bt0 + t) * a.span + s] = -INFINITY;
-    return;
-  }
+  const int64_t bt0 = static_cast<int64_t>(b) * a.Tq + t0;
+  const int64_t end = min(a.span, static_cast<int64_t>(limit));
+  constexpr int kTile = 16 * KB;
+  const int64_t step = static_cast<int64_t>(a.blocks) * kWaves * kTile;
+  int64_t s = static_cast<int64_t>(blockIdx.x % a.blocks * kWaves + wave) * kTile;
+  const bool busy = static_cast<int64_t>(blockIdx.x % a.blocks) * kWaves * kTile < end;  // one of the block's waves is
 
   const char* keys = static_cast<const char*>(a.c.k_idx) + b * a.c.S * ROW;
   auto load = [&](u32x4 (&k)[KB][NC], int64_t s0) {  // rows past the last visible one give zeros
@@ -76,9 +74,6 @@ __global__ __launch_bounds__(kNT) void indexer_kernel(IndexArgs a) {
         k[kb][c] = __builtin_bit_cast(u32x4, buffer_load_f32x4(r, (16 * kb + r16) * ROW + g * (ROW / 4) + c * 16, 0, 0));
   };
   u32x4 k0[KB][NC], k1[KB][NC];
-  constexpr int64_t kStep = 16 * KB * kWaves;
-  int64_t s = c0 + wave * 16 * KB;
-  const int64_t end = min(c1, static_cast<int64_t>(limit));
   if (s < end) load(k0, s);
 
   const char* q = static_cast<const char*>(a.q) + bt0 * a.HI * ROW;
@@ -90,11 +85,11 @@ __global__ __launch_bounds__(kNT) void indexer_kernel(IndexArgs a) {
     if (h < a.HI) x = *reinterpret_cast<const u32x4*>(q + (static_cast<int64_t>(t) * a.HI + h) * ROW + g * (ROW / 4) + c * 16);
     return x;
   };
-  if constexpr (IN_LDS) {
+  if (busy && IN_LDS) {
     for (int i = wave; i < nt * nht * NC; i += kWaves)
       lds[i * 64 + lane] = piece(i / (nht * NC), i / NC % nht, i % NC);
   }
-  for (int i = threadIdx.x; i < nt * nht * 16; i += kNT) {
+  for (int i = threadIdx.x; busy && i < nt * nht * 16; i += kNT) {
     const int t = i / (nht * 16), h = i % (nht * 16);
     weights[i] = h < a.HI ? to_f32(Tag{}, w[t * a.HI + h]) : 0.0f;
   }
@@ -133,20 +128,21 @@ __global__ __launch_bounds__(kNT) void indexer_kernel(IndexArgs a) {
       }
       const int64_t at = s0 + 16 * g + r16;
       const int32_t seen = kv4_visible(a.c.length, a.count, b, a.c.S, t0 + t, a.Tq);
-      if (g < KB && at < c1) a.scores[(bt0 + t) * a.span + at] = at < seen ? mine : -INFINITY;
+      if (g < KB && at < a.span) a.scores[(bt0 + t) * a.span + at] = at < seen ? mine : -INFINITY;
     }
   };
-  for (; s < end; s += 2 * kStep) {
-    if (s + kStep < end) load(k1, s + kStep);
+  while (s < end) {
+    if (s + step < end) load(k1, s + step);
     compute(k0, s);
-    if (s + kStep >= end) break;
-    if (s + 2 * kStep < end) load(k0, s + 2 * kStep);
-    compute(k1, s + kStep);
+    s += step;
+    if (s >= end) break;
+    if (s + step < end) load(k0, s + step);
+    compute(k1, s);
+    s += step;
   }
-  // what the waves' whole tiles did not reach
-  const int64_t done = c0 + (end - c0 + 16 * KB - 1) / (16 * KB) * (16 * KB);
-  for (int t = 0; t < nt; ++t)
-    for (int64_t at = done + threadIdx.x; at < c1; at += kNT) a.scores[(bt0 + t) * a.span + at] = -INFINITY;
+  for (; s < a.span; s += step)  // the tiles that nothing sees
+    for (int t = 0; t < nt; ++t)
+      if (lane < kTile && s + lane < a.span) a.scores[(bt0 + t) * a.span + s + lane] = -INFINITY;
 }
 
 template <typename Tag, int DI>
@@ -162,13 +158,12 @@ hipError_t launch_di(IndexArgs a, hipStream_t stream) {
   const bool in_lds = a.per * row_lds <= kMaxLds;
   const int step = 16 * KB * kWaves;
   const int64_t rows = a.c.B * a.groups, steps = (a.span + step - 1) / step;
+  // two blocks a compute unit (1, 2, 3, 4 and 8 measured 18.6, 15.1, 16.7, 16.6 and
+  // 19.3 us for 8 x 32768 slots, 64 heads of 128 in bf16)
   const int cus = device_cus() > 0 ? device_cus() : 256;
-  int64_t chunks = (4 * cus + rows - 1) / rows;
-  chunks = chunks < 1 ? 1 : chunks > steps ? steps : chunks;
-  const int64_t per_chunk = (steps + chunks - 1) / chunks;
-  a.chunk = per_chunk * step;
-  a.chunks = static_cast<int>((steps + per_chunk - 1) / per_chunk);
-  const uint32_t grid = static_cast<uint32_t>(rows * a.chunks);
+  const int64_t blocks = (2 * cus + rows - 1) / rows;
+  a.blocks = static_cast<int>(blocks < 1 ? 1 : blocks > steps ? steps : blocks);
+  const uint32_t grid = static_cast<uint32_t>(rows * a.blocks);
   if (in_lds)
     indexer_kernel<Tag, DI, KB, true><<<grid, kNT, a.per * row_lds, stream>>>(a);
   else
