@@ -89,7 +89,8 @@ class KV4Cache:
         self.length, self.seen, self.lost = length, seen, lost
         self.position, self.weight = position, weight
         self.B, self.S, self.HKV, self.DK, self.DV, self.DI = B, S, HKV, DK or 0, DV, DI
-        self.device, self.idx_dtype = device, idx_dtype
+        self.device, self.index, self.idx_dtype = device, device.index, idx_dtype
+        self.scale = 1.0 / math.sqrt(self.DK) if self.DK else 0.0
 
         def at(x):
             return x.data_ptr() if x is not None else None
@@ -132,26 +133,43 @@ def _stored(cache: KV4Cache) -> None:
     assert cache.codes is not None, "this cache holds index keys only"
 
 
-def _ints(x: torch.Tensor | None, shape, name: str, cache: KV4Cache):
-    """An optional int32 tensor and its pointer; a contiguous copy where it is not."""
-    if x is None:
-        return None, None
-    assert x.dtype is torch.int32 and x.shape == shape and x.device == cache.device, \
+def _ints(x: torch.Tensor, shape, name: str, cache: KV4Cache) -> torch.Tensor:
+    """An int32 tensor of the caller's; a contiguous copy where it is not."""
+    assert x.dtype is torch.int32 and x.shape == shape and x.get_device() == cache.index, \
         f"{name}: int32 {shape} on {cache.device} (got {x.dtype} {tuple(x.shape)} on {x.device})"
-    if not x.is_contiguous():
-        x = x.contiguous()
-    return x, x.data_ptr()
+    return x if x.is_contiguous() else x.contiguous()
 
 
-def _on(cache: KV4Cache, *xs: torch.Tensor) -> None:
+def _ready(dtype: torch.dtype, cache: KV4Cache, *xs: torch.Tensor):
+    """`xs` as the kernels take them (L.prep) and their pointers."""
     for x in xs:
-        assert x.device == cache.device, f"inputs must be on the cache's GPU {cache.device} (got {x.device})"
+        assert x.get_device() == cache.index, \
+            f"inputs must be on the cache's GPU {cache.device} (got {x.device})"
+    ptrs = L.ready_ptrs(dtype, xs)
+    if ptrs is None:
+        xs = [L.prep(x, dtype) for x in xs]
+        ptrs = [x.data_ptr() for x in xs]
+    return xs, ptrs
 
 
 def _span(cache: KV4Cache, span: int | None) -> int:
-    n = cache.S if span is None else int(span)
+    if span is None:
+        return cache.S
+    n = int(span)
     assert 0 <= n <= cache.S, f"span={n} outside [0, S={cache.S}]"
     return n
+
+
+def _call(cache: KV4Cache, what: str, fn, *args) -> None:
+    """fn(cache, *args, stream) on the cache's GPU.  Single-token calls are bound by
+    the host, so the usual case enters no context."""
+    if torch.cuda.current_device() == cache.index:
+        rc = fn(cache._ref, *args, L.stream_ptr(cache.device))
+    else:
+        with torch.cuda.device(cache.device):
+            rc = fn(cache._ref, *args, L.stream_ptr(cache.device))
+    if rc != L.DSA_OK:
+        L.check(rc, what)
 
 
 def kv4_append(cache: KV4Cache, K: torch.Tensor, V: torch.Tensor, k_idx: torch.Tensor | None = None,
@@ -171,28 +189,21 @@ def kv4_append(cache: KV4Cache, K: torch.Tensor, V: torch.Tensor, k_idx: torch.T
         f"K shape {tuple(K.shape)} != {(cache.B, T, cache.HKV, cache.DK)}"
     assert V.shape == (cache.B, T, cache.HKV, cache.DV), \
         f"V shape {tuple(V.shape)} != {(cache.B, T, cache.HKV, cache.DV)}"
-    _on(cache, K, V)
     assert (k_idx is None) == (cache.k_idx is None), "index keys go with a cache that holds them"
     dt = L.common_dtype(K, V)
-    ptrs = L.ready_ptrs(dt, (K, V))
-    if ptrs is None:
-        K, V = L.prep(K, dt), L.prep(V, dt)
-        ptrs = K.data_ptr(), V.data_ptr()
+    kv, (k_ptr, v_ptr) = _ready(dt, cache, K, V)
+    idx_ptr = weight_ptr = count_ptr = None
     if k_idx is not None:
         assert k_idx.shape == (B, T, cache.DI), f"k_idx shape {tuple(k_idx.shape)} != {(B, T, cache.DI)}"
-        _on(cache, k_idx)
-        k_idx = L.prep(k_idx, cache.idx_dtype)
+        k_idx, (idx_ptr,) = _ready(cache.idx_dtype, cache, k_idx)
     if weight is not None:
         assert weight.shape == (B, T), f"weight shape {tuple(weight.shape)} != {(B, T)}"
-        _on(cache, weight)
-        weight = L.prep(weight, torch.float32)
-    count, count_ptr = _ints(count, (B,), "count", cache)
-    with L.on_device(cache.device):
-        L.check(L.lib().dsa_kv4_append(
-            cache._ref, *ptrs, L.dtype_code(dt),
-            k_idx.data_ptr() if k_idx is not None else None,
-            weight.data_ptr() if weight is not None else None, count_ptr, T, 1 if restart else 0,
-            L.stream_ptr(cache.device)), "kv4_append")
+        weight, (weight_ptr,) = _ready(torch.float32, cache, weight)
+    if count is not None:
+        count = _ints(count, (B,), "count", cache)
+        count_ptr = count.data_ptr()
+    _call(cache, "kv4_append", L.lib().dsa_kv4_append, k_ptr, v_ptr, L.dtype_code(dt), idx_ptr,
+          weight_ptr, count_ptr, T, 1 if restart else 0)
 
 
 def kv4_rows(cache: KV4Cache, slots: torch.Tensor | None = None, *, span: int | None = None,
@@ -202,15 +213,18 @@ def kv4_rows(cache: KV4Cache, slots: torch.Tensor | None = None, *, span: int | 
     slots int32 [B,N], or the first `span` slots (default all).  Slots that hold
     nothing give zeros.  Exact in fp32 and bf16."""
     _stored(cache)
-    N = slots.shape[1] if slots is not None else _span(cache, span)
-    assert slots is None or span is None, "slots or span, not both"
-    slots, slots_ptr = _ints(slots, (cache.B, N), "slots", cache)
+    slots_ptr = None
+    if slots is not None:
+        assert span is None, "slots or span, not both"
+        N = slots.shape[1]
+        slots = _ints(slots, (cache.B, N), "slots", cache)
+        slots_ptr = slots.data_ptr()
+    else:
+        N = _span(cache, span)
     code = L.dtype_code(dtype)
-    K = torch.empty(cache.B, N, cache.HKV, cache.DK, device=cache.device, dtype=dtype)
-    V = torch.empty(cache.B, N, cache.HKV, cache.DV, device=cache.device, dtype=dtype)
-    with L.on_device(cache.device):
-        L.check(L.lib().dsa_kv4_rows(cache._ref, slots_ptr, N, code, K.data_ptr(), V.data_ptr(),
-                                     L.stream_ptr(cache.device)), "kv4_rows")
+    K = torch.empty((cache.B, N, cache.HKV, cache.DK), device=cache.device, dtype=dtype)
+    V = torch.empty((cache.B, N, cache.HKV, cache.DV), device=cache.device, dtype=dtype)
+    _call(cache, "kv4_rows", L.lib().dsa_kv4_rows, slots_ptr, N, code, K.data_ptr(), V.data_ptr())
     return K, V
 
 
@@ -227,15 +241,15 @@ def kv4_indexer_scores(cache: KV4Cache, q_idx: torch.Tensor, w_idx: torch.Tensor
     B, Tq, HI, DI = q_idx.shape
     assert (B, DI) == (cache.B, cache.DI), f"q_idx shape {tuple(q_idx.shape)}: B={cache.B}, DI={cache.DI}"
     assert w_idx.shape == (B, Tq, HI), f"w_idx shape {tuple(w_idx.shape)} != {(B, Tq, HI)}"
-    _on(cache, q_idx, w_idx)
     n = _span(cache, span)
-    q_idx, w_idx = L.prep(q_idx, cache.idx_dtype), L.prep(w_idx, cache.idx_dtype)
-    count, count_ptr = _ints(count, (B,), "count", cache)
-    scores = torch.empty(B, Tq, n, device=cache.device, dtype=torch.float32)
-    with L.on_device(cache.device):
-        L.check(L.lib().dsa_kv4_indexer_scores(
-            cache._ref, q_idx.data_ptr(), w_idx.data_ptr(), count_ptr, Tq, HI, n, scores.data_ptr(),
-            L.stream_ptr(cache.device)), "kv4_indexer_scores")
+    qw, (q_ptr, w_ptr) = _ready(cache.idx_dtype, cache, q_idx, w_idx)
+    count_ptr = None
+    if count is not None:
+        count = _ints(count, (B,), "count", cache)
+        count_ptr = count.data_ptr()
+    scores = torch.empty((B, Tq, n), device=cache.device, dtype=torch.float32)
+    _call(cache, "kv4_indexer_scores", L.lib().dsa_kv4_indexer_scores, q_ptr, w_ptr, count_ptr, Tq,
+          HI, n, scores.data_ptr())
     return scores
 
 
@@ -255,39 +269,38 @@ def kv4_attention(cache: KV4Cache, Q: torch.Tensor, *, slots: torch.Tensor | Non
     _stored(cache)
     B, Tq, HQ, DK = Q.shape
     assert (B, DK) == (cache.B, cache.DK), f"Q shape {tuple(Q.shape)}: B={cache.B}, DK={cache.DK}"
-    _on(cache, Q)
-    n = _span(cache, span)
+    slots_ptr = count_ptr = None
     if slots is not None:
         assert slots.dim() == 3, "slots: int32 [B, Tq, k]"
         assert span is None, "slots or span, not both"
         n = slots.shape[2]
-        slots, slots_ptr = _ints(slots, (B, Tq, n), "slots", cache)
+        slots = _ints(slots, (B, Tq, n), "slots", cache)
+        slots_ptr = slots.data_ptr()
     else:
-        slots_ptr = None
-    count, count_ptr = _ints(count, (B,), "count", cache)
+        n = _span(cache, span)
+    if count is not None:
+        count = _ints(count, (B,), "count", cache)
+        count_ptr = count.data_ptr()
     dt = L.common_dtype(Q)
-    Q = L.prep(Q, dt)
+    q, (q_ptr,) = _ready(dt, cache, Q)
     if out is None:
-        out = torch.empty(B, Tq, HQ, cache.DV, device=cache.device, dtype=torch.float32)
+        out = torch.empty((B, Tq, HQ, cache.DV), device=cache.device, dtype=torch.float32)
     else:
         L.check_out(out, B * Tq * HQ * cache.DV, cache.device)
     acc = 1 if accumulate else 0
-    with L.on_device(cache.device):
-        lib = L.lib()
-        sizes = (Tq, HQ, slots is None, n, acc)
-        nws = cache._workspace.get(sizes)
-        if nws is None:
-            if len(cache._workspace) >= 64:  # spans of a growing cache
-                cache._workspace.clear()
+    lib = L.lib()
+    sizes = (Tq, HQ, slots is None, n, acc)
+    nws = cache._workspace.get(sizes)
+    if nws is None:
+        if len(cache._workspace) >= 64:  # spans of a growing cache
+            cache._workspace.clear()
+        with L.on_device(cache.device):
             nws = lib.dsa_kv4_attention_workspace_bytes(cache._ref, Tq, HQ, 0 if slots is None else 1,
                                                         n, acc)
-            cache._workspace[sizes] = nws
-        ws = torch.empty(nws, device=cache.device, dtype=torch.uint8)
-        rc = lib.dsa_kv4_attention(
-            cache._ref, Q.data_ptr(), L.dtype_code(dt), slots_ptr, count_ptr, Tq, HQ, n, acc,
-            1.0 / math.sqrt(DK), out.data_ptr(), ws.data_ptr(), nws, L.stream_ptr(cache.device))
-    if rc != L.DSA_OK:
-        L.check(rc, "kv4_attention")
+        cache._workspace[sizes] = nws
+    ws = torch.empty(nws, device=cache.device, dtype=torch.uint8)
+    _call(cache, "kv4_attention", lib.dsa_kv4_attention, q_ptr, L.dtype_code(dt), slots_ptr, count_ptr,
+          Tq, HQ, n, acc, cache.scale, out.data_ptr(), ws.data_ptr(), nws)
     return out
 
 
@@ -304,11 +317,7 @@ def kv4_evict(cache: KV4Cache, keep: int, recent: int = 0):
     M = max(0, min(keep, cache.S - keep))
     moved = torch.empty((2, cache.B, M), device=cache.device, dtype=torch.int32)
     src = moved.data_ptr()
-    with L.on_device(cache.device):
-        rc = L.lib().dsa_kv4_evict(cache._ref, keep, recent, src, src + 4 * cache.B * M,
-                                   L.stream_ptr(cache.device))
-    if rc != L.DSA_OK:
-        L.check(rc, "kv4_evict")
+    _call(cache, "kv4_evict", L.lib().dsa_kv4_evict, keep, recent, src, src + 4 * cache.B * M)
     return moved.unbind(0)
 
 
