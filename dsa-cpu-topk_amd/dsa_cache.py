@@ -43,7 +43,15 @@ class KV4Cache:
     no free slot (check() raises where there are any); weight: attention weight
     accumulated by kv4_attention.  Made from buffers in use, what is not given
     starts as after an append of `length` tokens.  A cache of index keys alone
-    (codes None) serves kv4_indexer_scores."""
+    (codes None) serves kv4_indexer_scores.  The calls go by the buffers' addresses:
+    write into a buffer (cache.length.copy_(...)), it cannot be replaced."""
+
+    _BUFFERS = ("codes", "scales", "k_idx", "length", "seen", "lost", "position", "weight")
+
+    def __setattr__(self, name, value):
+        if name in self._BUFFERS and name in self.__dict__:
+            raise AttributeError(f"KV4Cache.{name} is written in place, not replaced")
+        super().__setattr__(name, value)
 
     def __init__(self, codes: torch.Tensor | None, scales: torch.Tensor | None,
                  length: torch.Tensor, k_idx: torch.Tensor | None = None,
@@ -332,17 +340,21 @@ def dsa_decode(cache: KV4Cache, q_idx, k_idx, w_idx, Q, K, V, top_k: int, *,
     K [B,Tq,HKV,DK]  V [B,Tq,HKV,DV].  Exactly top_k slots a token (the lowest
     slot wins ties), all it sees where it sees fewer.  span: no sequence has more
     slots than that in use (default S); where top_k >= span all of them are
-    attended to and nothing is scored.  The cache needs room for the Tq tokens:
-    keep + Tq <= S in steady state."""
+    attended to and nothing is scored.  The cache needs room for the Tq tokens
+    (keep + Tq <= S is checked; without keep, cache.check() says whether some were lost)."""
     assert top_k >= 1, "top_k must be >= 1"
     n = _span(cache, span)
-    kv4_append(cache, K, V, k_idx, count=count)
-    slots = None
-    if top_k < n:
-        scores = kv4_indexer_scores(cache, q_idx, w_idx, span=n, count=count)
-        _, slots = topk_indices(scores, int(top_k))
-    out = kv4_attention(cache, Q, slots=slots, span=None if slots is not None else n, count=count,
-                        accumulate=keep is not None)
     if keep is not None:
-        kv4_evict(cache, keep, recent)
+        assert keep + Q.shape[1] <= cache.S, \
+            f"keep={keep} slots and {Q.shape[1]} new tokens do not fit S={cache.S}"
+    with L.on_device(cache.device):
+        kv4_append(cache, K, V, k_idx, count=count)
+        slots = None
+        if top_k < n:
+            scores = kv4_indexer_scores(cache, q_idx, w_idx, span=n, count=count)
+            _, slots = topk_indices(scores, int(top_k))
+        out = kv4_attention(cache, Q, slots=slots, span=None if slots is not None else n,
+                            count=count, accumulate=keep is not None)
+        if keep is not None:
+            kv4_evict(cache, keep, recent)
     return out

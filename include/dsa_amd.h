@@ -507,7 +507,8 @@ int dsa_kv4_indexer_scores(const dsa_kv4_cache* cache, const void* q_idx, const 
  * query sees count for nothing, one listed twice counts twice.  A query that
  * sees no slot gets O = NaN, as dsa_sparse_attn_threshold's empty rows do.
  *   accumulate != 0: weight[b,s] += sum over t and h of p[b,t,h,s], with the same
- * result in every run.
+ * result in every run (over listed slots that takes a launch for each of the Tq
+ * tokens).
  *   fp32 logits, softmax and sums; fp32 operands enter the matrix instructions
  * whole, as bf16 pieces.
  *   Q [B,Tq,HQ,DK] of dtype (fp32, bf16, fp16), out [B,Tq,HQ,DV] fp32, 16-byte

@@ -75,8 +75,9 @@ def indexer(k_idx, length, q, w, count=None, span=None):
     return score.masked_fill(~ok, -math.inf), bound
 
 
-def attention(codes, scales, DK, length, Q, slots=None, span=None, count=None):
-    """(O float64 [B,Tq,HQ,DV], its bound, added weight [B,S], its bound)."""
+def attention(codes, scales, DK, length, Q, slots=None, span=None, count=None, dtype=None):
+    """(O float64 [B,Tq,HQ,DV], its bound, added weight [B,S], its bound); dtype: what the
+    kernel had Q in, where that is not Q's here."""
     B, S, HKV = codes.shape[:3]
     Tq, HQ = Q.shape[1:3]
     G = HQ // HKV
@@ -101,7 +102,7 @@ def attention(codes, scales, DK, length, Q, slots=None, span=None, count=None):
                 V = decode(codes[b, at, h, DK // 2:], scales[b, at, h, DK // 32:])
                 q = Q[b, t, h * G:(h + 1) * G].double()
                 lg = q @ K.t().contiguous() / math.sqrt(DK)
-                d = ((PIECES[Q.dtype] * DK + 3) * U * (q.abs() @ K.abs().t().contiguous()) / math.sqrt(DK)).amax(-1, keepdim=True)
+                d = ((PIECES[dtype or Q.dtype] * DK + 3) * U * (q.abs() @ K.abs().t().contiguous()) / math.sqrt(DK)).amax(-1, keepdim=True)
                 p = torch.softmax(lg, -1)
                 O[b, t, h * G:(h + 1) * G] = p @ V
                 rel = 2 * d + d * d + 16 * U

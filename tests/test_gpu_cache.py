@@ -8,6 +8,7 @@ import math
 import pytest
 import torch
 
+import _dsa_lib as L
 import cache_oracle as C
 import dsa_cache as D
 from helpers import say
@@ -606,6 +607,55 @@ def test_two_streams_at_once(dev):
         assert all(torch.equal(a, b) for a, b in zip(got[i], want))
 
 
+@pytest.mark.parametrize("scale", [-0.125, 0.0, 0.5])
+@pytest.mark.parametrize("HQ", [2, 16])
+def test_any_finite_scale(dev, scale, HQ):
+    """The C entry's scale: of either sign, and 0 (a plain mean of the visible slots)."""
+    g = gen(dev, 70)
+    cache = filled(dev, 2, 90, 1, 64, 64, [77, 2], 71)
+    Q = randn(g, 2, 1, HQ, 64)
+    out, lib = torch.empty(2, 1, HQ, 64, device=dev), L.lib()
+    nws = lib.dsa_kv4_attention_workspace_bytes(cache._ref, 1, HQ, 0, 90, 1)
+    ws = torch.empty(nws, device=dev, dtype=torch.uint8)
+    before = cache.weight.clone()
+    args = (cache._ref, Q.data_ptr(), L.DSA_F32, None, None, 1, HQ, 90, 1, scale, out.data_ptr(), ws.data_ptr())
+    assert lib.dsa_kv4_attention(*args, nws - 1, L.stream_ptr(dev)) == L.DSA_EINVAL
+    L.check(lib.dsa_kv4_attention(*args, nws, L.stream_ptr(dev)), "attention")
+    # the same logits come of Q * scale * sqrt(64) at the usual scale
+    O, lim, add, addlim = C.attention(cache.codes, cache.scales, 64, cache.length, Q.double() * scale * 8, dtype=F32)
+    within(out, O, lim, "out")
+    w = before.double() + add
+    within(cache.weight, w, addlim + 2 * C.U * w.abs(), "weights")
+
+
+def test_buffers_stay(dev):
+    cache = filled(dev, 2, 20, 1, 32, 32, [20, 4])
+    for name in D.KV4Cache._BUFFERS:
+        with pytest.raises(AttributeError):
+            setattr(cache, name, None)
+    cache.length.copy_(ints(dev, [5, 0]))  # back to an earlier token
+    Q = randn(gen(dev, 1), 2, 1, 2, 32)
+    O, lim, _, _ = C.attention(cache.codes, cache.scales, 32, ints(dev, [5, 0]), Q)
+    within(D.kv4_attention(cache, Q), O, lim, "out")
+
+
+def test_nothing_in_nothing_out(dev):
+    """No sequences, no tokens: empty results, and nothing changes."""
+    none = D.KV4Cache.empty(0, 8, 2, 64, 64, 32, device=dev)
+    z = lambda *s: torch.zeros(s, device=dev)  # noqa: E731
+    D.kv4_append(none, z(0, 3, 2, 64), z(0, 3, 2, 64), z(0, 3, 32))
+    assert D.kv4_attention(none, z(0, 1, 4, 64), accumulate=True).shape == (0, 1, 4, 64)
+    assert D.kv4_indexer_scores(none, z(0, 1, 4, 32), z(0, 1, 4)).shape == (0, 1, 8)
+    assert D.kv4_rows(none)[0].shape == (0, 8, 2, 64) and D.kv4_evict(none, 4)[0].shape == (0, 4)
+    cache = filled(dev, 2, 20, 2, 64, 64, [20, 4], DI=32)
+    before = [getattr(cache, n).clone() for n in D.KV4Cache._BUFFERS]
+    D.kv4_append(cache, z(2, 0, 2, 64), z(2, 0, 2, 64), z(2, 0, 32))
+    assert D.kv4_attention(cache, z(2, 0, 4, 64), accumulate=True).shape == (2, 0, 4, 64)
+    assert D.kv4_indexer_scores(cache, z(2, 0, 4, 32), z(2, 0, 4)).shape == (2, 0, 20)
+    D.kv4_evict(cache, 20)
+    assert all(same(a, getattr(cache, n)) for a, n in zip(before, D.KV4Cache._BUFFERS))
+
+
 def test_python_refusals(dev):
     cache = D.KV4Cache.empty(2, 16, 2, 64, 32, 32, device=dev)
     K, V, ki = (torch.zeros(2, 1, *s, device=dev) for s in ((2, 64), (2, 32), (32,)))
@@ -625,6 +675,7 @@ def test_python_refusals(dev):
         lambda: D.kv4_evict(cache, 4, 5),
         lambda: D.kv4_evict(cache, -1),
         lambda: D.dsa_decode(cache, *[K] * 6, top_k=0),
+        lambda: D.dsa_decode(cache, *[K] * 6, top_k=4, keep=16),  # no room for a token
         lambda: D.KV4Cache(cache.codes[:, ::2], cache.scales[:, ::2], cache.length, DK=64),
         lambda: D.KV4Cache(cache.codes, cache.scales, cache.length.long(), DK=64),
         lambda: D.KV4Cache.empty(1, 4, 1, 48, 32, device=dev),
