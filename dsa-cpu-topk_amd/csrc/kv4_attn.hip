@@ -62,6 +62,7 @@ struct AttnArgs {
   int heads;  // K/V heads a block takes: 4, 2 or 1, its 4 / heads waves of each sharing the slots
   int64_t n, stride;  // slots a query; floats between rows of logits
   int splits;         // blocks that share a query's slots
+  int join_cols;      // columns of a head that a joining block takes
   float scale;
   float* out;
   float* part;    // [B*Tq*HQ][splits][DV] sums, where splits > 1
@@ -533,12 +534,12 @@ __global__ __launch_bounds__(kNT, resident(NP, DK, DV)) void attn_kernel(AttnArg
   }
 }
 
-// One query head's maximum (0 where it is -inf) and sum over its splits, by 8 lanes.
+// One query head's maximum (0 where it is -inf) and sum over its splits, by 8 or 64 lanes.
+template <int LANES>
 __device__ __forceinline__ float2 join_ml(const float2* ml, int splits) {
-  const int first = threadIdx.x & 7;
   float top = -INFINITY, total = 0.0f;
 #pragma unroll 4
-  for (int s = first; s < splits; s += 8) {
+  for (int s = threadIdx.x % LANES; s < splits; s += LANES) {
     const float2 x = ml[s];
     const float most = fmaxf(top, x.x), ref = most == -INFINITY ? 0.0f : most;
     total = total * __builtin_amdgcn_exp2f(top - ref) + x.y * __builtin_amdgcn_exp2f(x.x - ref);
@@ -548,48 +549,55 @@ __device__ __forceinline__ float2 join_ml(const float2* ml, int splits) {
   most = fmaxf(most, dpp_partner<1>(most));
   most = fmaxf(most, dpp_partner<2>(most));
   most = fmaxf(most, dpp_partner<4>(most));
+  if (LANES == 64) most = max_xor32(max_xor16(fmaxf(most, dpp_partner<8>(most))));
   const float ref = most == -INFINITY ? 0.0f : most;
   total *= __builtin_amdgcn_exp2f(top - ref);
   total += dpp_partner<1>(total);
   total += dpp_partner<2>(total);
   total += dpp_partner<4>(total);
+  if (LANES == 64) total = sum_xor32(sum_xor16(total + dpp_partner<8>(total)));
   return make_float2(ref, total);
 }
 
-// The first `joins` blocks join the splits of a query head each (joins = 0: there
-// is one split, or they are joined already); the others add query t's
+constexpr int kMaxSplits = 512;  // what a joining block keeps factors of
+
+// The first `joins` blocks join the splits of a.join_cols columns of a query head each
+// (joins = 0: there is one split, or they are joined already); the others add query t's
 // probabilities onto the weights of kNT slots of a sequence.  t < 0: of all
 // queries, a slot having one thread.  Else one query's, listed ones: two queries
 // never add to one slot at the same time, and a slot that one query lists twice
 // takes the same addend twice, so that the sums have one order.
-template <int DV>
 __global__ __launch_bounds__(kNT) void finish_kernel(AttnArgs a, int64_t joins, int t, int64_t per_b) {
-  constexpr int kQuads = DV / 4, kGroups = kNT / kQuads;  // of splits, which take turns
   __shared__ float2 head[1024];
-  __shared__ float4 sums[kGroups][kQuads];
+  __shared__ float4 sums[kNT];
+  __shared__ float factor[kMaxSplits];
   if (blockIdx.x < joins) {
-    const int64_t h = blockIdx.x;
-    const float2* ml = a.ml + h * a.splits;
-    const float2 all = join_ml(ml, a.splits);
-    const int quad = threadIdx.x % kQuads, group = threadIdx.x / kQuads;
-    float4 x = {0, 0, 0, 0};
-    if (group < kGroups) {
-      const float4* part = reinterpret_cast<const float4*>(a.part + h * a.splits * DV) + quad;
-#pragma unroll 4
-      for (int s = group; s < a.splits; s += kGroups) {
-        const float2 y = ml[s];
-        if (y.y == 0.0f) continue;  // a chunk without a sum has left none
-        const float f = __builtin_amdgcn_exp2f(y.x - all.x);
-        const float4 v = part[static_cast<int64_t>(s) * kQuads];
-        x.x += f * v.x; x.y += f * v.y; x.z += f * v.z; x.w += f * v.w;
-      }
-      sums[group][quad] = x;
+    const uint32_t cols = a.join_cols, parts = a.c.DV / cols, h = blockIdx.x / parts, d0 = blockIdx.x % parts * cols;
+    const float2* ml = a.ml + static_cast<int64_t>(h) * a.splits;
+    const float2 all = join_ml<64>(ml, a.splits);
+    for (int s = threadIdx.x; s < a.splits; s += kNT) {
+      const float2 x = ml[s];
+      factor[s] = x.y == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(x.x - all.x);
     }
     __syncthreads();
-    for (int d = threadIdx.x; d < DV; d += kNT) {
+    // groups of threads take the splits in turn, a thread 4 columns
+    const uint32_t quads = cols / 4, groups = kNT / quads, quad = threadIdx.x % quads, group = threadIdx.x / quads;
+    const float* part = a.part + static_cast<int64_t>(h) * a.splits * a.c.DV + d0 + quad * 4;
+    float4 x = {0, 0, 0, 0};
+#pragma unroll 4
+    for (int s = group; s < a.splits && group < groups; s += groups) {
+      const float f = factor[s];
+      if (f == 0.0f) continue;  // a block without a sum has left none
+      const float4 v = *reinterpret_cast<const float4*>(part + static_cast<int64_t>(s) * a.c.DV);
+      x.x += f * v.x; x.y += f * v.y; x.z += f * v.z; x.w += f * v.w;
+    }
+    sums[threadIdx.x] = x;
+    __syncthreads();
+    if (threadIdx.x < cols) {
       float y = 0.0f;
-      for (int s = 0; s < min(kGroups, a.splits); ++s) y += reinterpret_cast<const float*>(sums[s])[d];
-      a.out[h * DV + d] = y / all.y;  // 0 / 0 where no logit is above -inf
+      for (uint32_t s = 0; s < min(groups, static_cast<uint32_t>(a.splits)); ++s)
+        y += reinterpret_cast<const float*>(sums + s * quads)[threadIdx.x];
+      a.out[static_cast<int64_t>(h) * a.c.DV + d0 + threadIdx.x] = y / all.y;  // 0 / 0 where no logit is above -inf
     }
     return;
   }
@@ -604,7 +612,7 @@ __global__ __launch_bounds__(kNT) void finish_kernel(AttnArgs a, int64_t joins, 
     __syncthreads();
     for (int h0 = 0; h0 < a.HQ; h0 += kNT / 8) {
       const int h = h0 + threadIdx.x / 8;
-      const float2 x = join_ml(a.ml + (bt * a.HQ + min(h, a.HQ - 1)) * a.splits, a.splits);
+      const float2 x = join_ml<8>(a.ml + (bt * a.HQ + min(h, a.HQ - 1)) * a.splits, a.splits);
       if (h < a.HQ && threadIdx.x % 8 == 0) head[h] = make_float2(x.x, 1.0f / x.y);
     }
     __syncthreads();
@@ -632,16 +640,25 @@ Plan plan_of(const Kv4& c, int64_t Tq, int HQ, int64_t n, bool accumulate) {
   const int G = HQ / c.HKV;
   p.side = G <= 5;
   p.row_tiles = p.side ? 1 : (G + 15) / 16;
-  p.heads = c.HKV % 4 == 0 ? 4 : c.HKV % 2 == 0 ? 2 : 1;
+  // Up to 8 turns of four waves on one head's slots cost less than the launch that
+  // would join splits (255 listed slots, 8 heads of 64, fp32, 4 sequences: 11.3 us
+  // with it, 8.8 without).  (Whether weights are accumulated does not enter: it
+  // changes no bit of the output.)
+  const bool alone = n <= 8 * kTile * kWaves;
+  // Four neighbouring heads a block read whole rows of the cache together; few blocks
+  // of one that have no splits finish sooner (us with four / one: 64 x 1024 slots of
+  // 8 heads of 128 19.6 / 16.6, 256 x 512 of 8 of 64 17.3 / 19.6).
+  const int cus = device_cus() > 0 ? device_cus() : 256;
+  const bool few = c.B * Tq * c.HKV * p.row_tiles <= 4 * cus;
+  p.heads = alone && few ? 1 : c.HKV % 4 == 0 ? 4 : c.HKV % 2 == 0 ? 2 : 1;
   const int64_t blocks = c.B * Tq * (c.HKV / p.heads) * p.row_tiles;
   const int unit = kTile * (kWaves / p.heads);  // slots that a block takes at once
   const int64_t steps = n > 0 ? (n + unit - 1) / unit : 1;
-  const int cus = device_cus() > 0 ? device_cus() : 256;
-    int64_t splits = blocks > 0 ? (2 * cus + blocks - 1) / blocks : 1;
-  splits = splits < 1 ? 1 : splits > steps ? steps : splits;
-  // Up to 8 turns of the waves cost less than the launch that would join their
-  // splits (129 slots of 4 heads of 32: 10.6 us with it, 8.1 without).
-  if (steps <= 8) splits = 1;
+  // Two blocks a compute unit: 1, 2, 4 and 8 measured 108, 94, 93 and 109 us for
+  // 16 x 32768 slots, 16.1, 12.9, 14.4 and 15.1 us for 16 x 4096.
+  int64_t splits = alone || blocks < 1 ? 1 : (2 * cus + blocks - 1) / blocks;
+  splits = splits > steps ? steps : splits;
+  splits = splits > kMaxSplits ? kMaxSplits : splits;
   p.splits = static_cast<int>(splits);
   auto up = [](int64_t v) { return (v + 255) / 256 * 256; };
   const int64_t heads = c.B * Tq * HQ;
@@ -708,6 +725,10 @@ hipError_t launch_kv4_attn(const Kv4& c, const void* Q, int dtype, const int32_t
   a.n = n;
   a.stride = p.stride;
   a.splits = p.splits;
+  // many splits are joined by more blocks (1 x 32768 slots, 256 splits of 8 heads:
+  // 27.9 us by the head, 16.8 by 32 columns; 128 heads of 16 sequences, 4 splits:
+  // 38.6 and 44.4)
+  a.join_cols = p.splits > 32 ? 32 : c.DV;
   a.scale = scale;
   a.out = out;
   a.ml = reinterpret_cast<float2*>(base + p.ml);
@@ -719,18 +740,11 @@ hipError_t launch_kv4_attn(const Kv4& c, const void* Q, int dtype, const int32_t
                  : dtype == 1 ? launch_type<BF16, 1>(a, p.side, blocks, stream)
                               : launch_type<F16, 2>(a, p.side, blocks, stream);
   if (e != hipSuccess) return e;
-  int64_t joins = p.splits > 1 ? c.B * Tq * HQ : 0;
+  int64_t joins = p.splits > 1 ? c.B * Tq * HQ * (c.DV / a.join_cols) : 0;
   const int64_t per_b = accumulate ? (n + kNT - 1) / kNT : 0;
   for (int t = slots ? 0 : -1; t < (slots && accumulate ? a.Tq : slots ? 1 : 0); ++t) {
     const uint32_t grid = static_cast<uint32_t>(joins + per_b * c.B);
-    if (grid > 0) switch (c.DV) {
-      case 32: finish_kernel<32><<<grid, kNT, 0, stream>>>(a, joins, t, per_b); break;
-      case 64: finish_kernel<64><<<grid, kNT, 0, stream>>>(a, joins, t, per_b); break;
-      case 96: finish_kernel<96><<<grid, kNT, 0, stream>>>(a, joins, t, per_b); break;
-      case 128: finish_kernel<128><<<grid, kNT, 0, stream>>>(a, joins, t, per_b); break;
-      case 192: finish_kernel<192><<<grid, kNT, 0, stream>>>(a, joins, t, per_b); break;
-      default: finish_kernel<256><<<grid, kNT, 0, stream>>>(a, joins, t, per_b); break;
-    }
+    if (grid > 0) finish_kernel<<<grid, kNT, 0, stream>>>(a, joins, t, per_b);
     joins = 0;
   }
   return hipGetLastError();

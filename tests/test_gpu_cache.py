@@ -253,7 +253,7 @@ def attend(cache, Q, what, **kw):
     w = before.double() + add
     within(cache.weight, w, addlim + (times + 1) * C.U * w.abs(), what + " weights")
     again = D.kv4_attention(cache, Q, **kw)
-    assert torch.equal(torch.nan_to_num(again), torch.nan_to_num(out)), "another result without the weights"
+    assert same(torch.nan_to_num(again), torch.nan_to_num(out)), "another result without the weights"
     return out
 
 
@@ -321,7 +321,7 @@ def test_attention_over_listed_slots(dev, dtype, k, Tq, HQ, HKV, DH):
     wide[..., :k] = slots
     Q = randn(g, B, Tq, HQ, DH, dtype=dtype)
     a, b = D.kv4_attention(cache, Q, slots=wide[..., :k]), D.kv4_attention(cache, Q, slots=slots)
-    assert torch.equal(torch.nan_to_num(a), torch.nan_to_num(b))  # a view of a wider list
+    assert same(torch.nan_to_num(a), torch.nan_to_num(b))  # a view of a wider list
     attend(cache, Q, "long list", slots=torch.randint(0, 500, (B, Tq, 3000), generator=g, device=dev, dtype=torch.int32))
 
 
