@@ -587,7 +587,8 @@ int dsa_kv4_indexer_scores(const dsa_kv4_cache* cache, const void* q_idx, const 
 
 int64_t dsa_kv4_attention_workspace_bytes(const dsa_kv4_cache* cache, int64_t Tq, int HQ, int listed,
                                           int64_t n, int accumulate) {
-  if (check_kv4_attention(cache, Tq, HQ, listed != 0, n, "kv4_attention_workspace_bytes") != DSA_OK) return 0;
+  const int rc = check_kv4_attention(cache, Tq, HQ, listed != 0, n, "kv4_attention_workspace_bytes");
+  if (rc != DSA_OK) return rc;
   return dsa::kv4_attn_workspace(kv4_of(cache), Tq, HQ, n, accumulate != 0);
 }
 

@@ -132,7 +132,7 @@ class KV4Cache:
 
     def check(self) -> None:
         """RuntimeError if a token found no free slot (waits for the GPU)."""
-        if self.lost is not None and int(self.lost.max()) > 0:
+        if self.lost is not None and self.B and int(self.lost.max()) > 0:
             raise RuntimeError(f"KV4Cache: {int(self.lost.sum())} tokens found no free slot "
                                f"(S={self.S}): evict before appending")
 
@@ -166,6 +166,37 @@ def _span(cache: KV4Cache, span: int | None) -> int:
     n = int(span)
     assert 0 <= n <= cache.S, f"span={n} outside [0, S={cache.S}]"
     return n
+
+
+def _queries(cache: KV4Cache, Q: torch.Tensor):
+    _stored(cache)
+    assert Q.dim() == 4 and (Q.shape[0], Q.shape[3]) == (cache.B, cache.DK), \
+        f"Q shape {tuple(Q.shape)}: B={cache.B}, DK={cache.DK}"
+    return Q.shape
+
+
+def _index_queries(cache: KV4Cache, q_idx: torch.Tensor, w_idx: torch.Tensor):
+    assert cache.k_idx is not None, "this cache holds no index keys"
+    assert q_idx.dim() == 4 and (q_idx.shape[0], q_idx.shape[3]) == (cache.B, cache.DI), \
+        f"q_idx shape {tuple(q_idx.shape)}: B={cache.B}, DI={cache.DI}"
+    assert 1 <= q_idx.shape[2] <= 256, f"HI={q_idx.shape[2]} outside [1,256]"
+    assert w_idx.shape == q_idx.shape[:3], f"w_idx shape {tuple(w_idx.shape)} != {tuple(q_idx.shape[:3])}"
+    return q_idx.shape
+
+
+def _workspace_bytes(cache: KV4Cache, Tq: int, HQ: int, listed: bool, n: int, acc: int) -> int:
+    """What dsa_kv4_attention needs of these sizes; raises where it would refuse them."""
+    sizes = (Tq, HQ, listed, n, acc)
+    nws = cache._workspace.get(sizes)
+    if nws is None:
+        if len(cache._workspace) >= 64:  # spans of a growing cache
+            cache._workspace.clear()
+        with L.on_device(cache.device):
+            nws = L.lib().dsa_kv4_attention_workspace_bytes(cache._ref, Tq, HQ, int(listed), n, acc)
+        if nws < 0:
+            L.check(nws, "kv4_attention")
+        cache._workspace[sizes] = nws
+    return nws
 
 
 def _call(cache: KV4Cache, what: str, fn, *args) -> None:
@@ -224,6 +255,7 @@ def kv4_rows(cache: KV4Cache, slots: torch.Tensor | None = None, *, span: int | 
     slots_ptr = None
     if slots is not None:
         assert span is None, "slots or span, not both"
+        assert slots.dim() == 2, "slots: int32 [B, N]"
         N = slots.shape[1]
         slots = _ints(slots, (cache.B, N), "slots", cache)
         slots_ptr = slots.data_ptr()
@@ -245,10 +277,7 @@ def kv4_indexer_scores(cache: KV4Cache, q_idx: torch.Tensor, w_idx: torch.Tensor
     q_idx [B,Tq,HI,DI], w_idx [B,Tq,HI].  span: only the first span slots (default
     all S).  count int32 [B]: how many of the Tq are tokens, as kv4_append's; the
     others' rows are -inf."""
-    assert cache.k_idx is not None, "this cache holds no index keys"
-    B, Tq, HI, DI = q_idx.shape
-    assert (B, DI) == (cache.B, cache.DI), f"q_idx shape {tuple(q_idx.shape)}: B={cache.B}, DI={cache.DI}"
-    assert w_idx.shape == (B, Tq, HI), f"w_idx shape {tuple(w_idx.shape)} != {(B, Tq, HI)}"
+    B, Tq, HI, _ = _index_queries(cache, q_idx, w_idx)
     n = _span(cache, span)
     qw, (q_ptr, w_ptr) = _ready(cache.idx_dtype, cache, q_idx, w_idx)
     count_ptr = None
@@ -274,9 +303,7 @@ def kv4_attention(cache: KV4Cache, Q: torch.Tensor, *, slots: torch.Tensor | Non
     count int32 [B]: how many of the Tq are tokens; the others see nothing.
     accumulate: add each slot's probabilities, over tokens and heads, to
     cache.weight (what kv4_evict goes by)."""
-    _stored(cache)
-    B, Tq, HQ, DK = Q.shape
-    assert (B, DK) == (cache.B, cache.DK), f"Q shape {tuple(Q.shape)}: B={cache.B}, DK={cache.DK}"
+    B, Tq, HQ, _ = _queries(cache, Q)
     slots_ptr = count_ptr = None
     if slots is not None:
         assert slots.dim() == 3, "slots: int32 [B, Tq, k]"
@@ -297,15 +324,7 @@ def kv4_attention(cache: KV4Cache, Q: torch.Tensor, *, slots: torch.Tensor | Non
         L.check_out(out, B * Tq * HQ * cache.DV, cache.device)
     acc = 1 if accumulate else 0
     lib = L.lib()
-    sizes = (Tq, HQ, slots is None, n, acc)
-    nws = cache._workspace.get(sizes)
-    if nws is None:
-        if len(cache._workspace) >= 64:  # spans of a growing cache
-            cache._workspace.clear()
-        with L.on_device(cache.device):
-            nws = lib.dsa_kv4_attention_workspace_bytes(cache._ref, Tq, HQ, 0 if slots is None else 1,
-                                                        n, acc)
-        cache._workspace[sizes] = nws
+    nws = _workspace_bytes(cache, Tq, HQ, slots is not None, n, acc)
     ws = torch.empty(nws, device=cache.device, dtype=torch.uint8)
     _call(cache, "kv4_attention", lib.dsa_kv4_attention, q_ptr, L.dtype_code(dt), slots_ptr, count_ptr,
           Tq, HQ, n, acc, cache.scale, out.data_ptr(), ws.data_ptr(), nws)
@@ -344,13 +363,20 @@ def dsa_decode(cache: KV4Cache, q_idx, k_idx, w_idx, Q, K, V, top_k: int, *,
     (keep + Tq <= S is checked; without keep, cache.check() says whether some were lost)."""
     assert top_k >= 1, "top_k must be >= 1"
     n = _span(cache, span)
+    # what the later calls would refuse, before the first one changes the cache
+    B, Tq, HQ, _ = _queries(cache, Q)
+    assert K.shape[:2] == (B, Tq), f"K shape {tuple(K.shape)}: {Tq} tokens in Q"
+    listed = top_k < n
+    if listed:
+        assert _index_queries(cache, q_idx, w_idx)[1] == Tq, f"q_idx shape {tuple(q_idx.shape)}: {Tq} tokens in Q"
     if keep is not None:
-        assert keep + Q.shape[1] <= cache.S, \
-            f"keep={keep} slots and {Q.shape[1]} new tokens do not fit S={cache.S}"
+        assert 0 <= recent <= keep, f"keep={keep} recent={recent} must be 0 <= recent <= keep"
+        assert keep + Tq <= cache.S, f"keep={keep} slots and {Tq} new tokens do not fit S={cache.S}"
+    _workspace_bytes(cache, Tq, HQ, listed, int(top_k) if listed else n, 0 if keep is None else 1)
     with L.on_device(cache.device):
         kv4_append(cache, K, V, k_idx, count=count)
         slots = None
-        if top_k < n:
+        if listed:
             scores = kv4_indexer_scores(cache, q_idx, w_idx, span=n, count=count)
             _, slots = topk_indices(scores, int(top_k))
         out = kv4_attention(cache, Q, slots=slots, span=None if slots is not None else n,

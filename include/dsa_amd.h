@@ -517,7 +517,8 @@ int dsa_kv4_indexer_scores(const dsa_kv4_cache* cache, const void* q_idx, const 
  *   (else DSA_EUNSUPPORTED).
  *   workspace: device memory of dsa_kv4_attention_workspace_bytes, 16-byte
  *   aligned, used by no other work until the launches complete, contents on entry
- *   free (a smaller one is refused).  Needs the device (its compute-unit count).
+ *   free (a smaller one is refused).  Needs the device (its compute-unit count);
+ *   a negative status where the sizes are refused.
  */
 int64_t dsa_kv4_attention_workspace_bytes(const dsa_kv4_cache* cache, int64_t Tq, int HQ, int listed,
                                           int64_t n, int accumulate);

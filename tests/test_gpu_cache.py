@@ -656,6 +656,39 @@ def test_nothing_in_nothing_out(dev):
     assert all(same(a, getattr(cache, n)) for a, n in zip(before, D.KV4Cache._BUFFERS))
 
 
+def test_refused_steps_change_nothing(dev):
+    """A step that one of its later calls would refuse is refused before the append."""
+    g = gen(dev, 72)
+    cache = filled(dev, 2, 40, 2, 64, 64, [20, 4], 73, 32)
+    q, ki, w, Q, K, V = step_inputs(g, 2, 1, 4, 32, 4, 2, 64, 64, BF16)
+    odd = filled(dev, 2, 40, 1, 160, 160, [20, 4], 74)  # no attention kernel for it
+    caches = [cache, odd]
+    before = [[getattr(c, n).clone() for n in D.KV4Cache._BUFFERS if getattr(c, n) is not None] for c in caches]
+    wide = randn(g, 2, 1, 257, 32)
+    rows = randn(g, 2, 1, 1, 160)
+    for args, kw in [((q, ki, w, Q, K, V, 8), dict(keep=30, recent=31)),
+                     ((q, ki, w, Q, K, V, 8), dict(keep=-1)),
+                     ((q, ki, w, Q, K, V, 8), dict(span=41)),
+                     ((q, ki, w, Q[:, :, :3], K, V, 8), {}),
+                     ((q, ki, w, Q[..., :32], K, V, 8), {}),
+                     ((q, ki, w, Q.expand(2, 2, 4, 64), K, V, 8), {}),
+                     ((q, ki, w[..., :3], Q, K, V, 8), {}),
+                     ((q[..., :16], ki, w, Q, K, V, 8), {}),
+                     ((wide, ki, wide[..., 0], Q, K, V, 8), {}),
+                     ((q.expand(2, 2, 4, 32), ki, w.expand(2, 2, 4), Q, K, V, 8), {})]:
+        with pytest.raises(AssertionError):
+            D.dsa_decode(cache, *args, **kw)
+    with pytest.raises(AssertionError):  # scores of a cache without index keys
+        D.dsa_decode(odd, q, None, w, rows, rows, rows, 8)
+    with pytest.raises(L.DSAUnsupported):
+        D.dsa_decode(odd, q, None, w, rows, rows, rows, 40)
+    for c, old in zip(caches, before):
+        now = [getattr(c, n) for n in D.KV4Cache._BUFFERS if getattr(c, n) is not None]
+        assert all(same(a, b) for a, b in zip(now, old))
+    D.dsa_decode(cache, q, ki, w, Q, K, V, 8, keep=30, recent=30)
+    assert cache.length.tolist() == [21, 5]
+
+
 def test_python_refusals(dev):
     cache = D.KV4Cache.empty(2, 16, 2, 64, 32, 32, device=dev)
     K, V, ki = (torch.zeros(2, 1, *s, device=dev) for s in ((2, 64), (2, 32), (32,)))
