@@ -3,8 +3,8 @@
 Each case calls one public entry point the way a program does: the whole
 forward (dsa_attention), the lightning indexer (lightning_indexer), the
 per-row select (topk_threshold) and the precomputed-threshold attention.
-Every call is a forward pass over whole sequences: the library has no
-backward and no single-token entry point.  Inputs are N(0,1) with indexer
+Every call is a forward pass over whole sequences (operators.py has the
+decode ones); the library has no backward.  Inputs are N(0,1) with indexer
 weights N(0,1)/sqrt(HI), the distributions the repository's benchmark and
 tests use.
 
