@@ -589,7 +589,7 @@ int64_t dsa_kv4_attention_workspace_bytes(const dsa_kv4_cache* cache, int64_t Tq
                                           int64_t n, int accumulate) {
   const int rc = check_kv4_attention(cache, Tq, HQ, listed != 0, n, "kv4_attention_workspace_bytes");
   if (rc != DSA_OK) return rc;
-  return dsa::kv4_attn_workspace(kv4_of(cache), Tq, HQ, n, accumulate != 0);
+  return dsa::kv4_attn_workspace(kv4_of(cache), Tq, HQ, listed != 0, n, accumulate != 0);
 }
 
 int dsa_kv4_attention(const dsa_kv4_cache* cache, const void* Q, int dtype, const int32_t* slots,
@@ -606,7 +606,7 @@ int dsa_kv4_attention(const dsa_kv4_cache* cache, const void* Q, int dtype, cons
   if (!aligned16(Q) || !aligned16(out)) return fail(DSA_EINVAL, "kv4_attention: Q and out must be 16-byte aligned");
   if (!aligned4(slots) || !aligned4(count)) return fail(DSA_EINVAL, "kv4_attention: slots and count must be 4-byte aligned");
   const dsa::Kv4 c = kv4_of(cache);
-  const int64_t need = dsa::kv4_attn_workspace(c, Tq, HQ, n, accumulate != 0);
+  const int64_t need = dsa::kv4_attn_workspace(c, Tq, HQ, slots != nullptr, n, accumulate != 0);
   if (need > 0 && (!workspace || !aligned16(workspace) || workspace_bytes < need))
     return fail(DSA_EINVAL, "kv4_attention: needs a 16-byte aligned workspace of %lld bytes (got %lld)", (long long)need, (long long)workspace_bytes);
   return hip_status(dsa::launch_kv4_attn(c, Q, dtype, slots, count, Tq, HQ, n, accumulate != 0, scale, out,

@@ -127,7 +127,7 @@ hipError_t launch_kv4_indexer(const Kv4& c, const void* q, const void* w, int dt
 // Attention over the cache (kv4_attn.hip): n slots a query, those of `slots`
 // [B, Tq, n] or (null) the first n.
 bool kv4_attn_supported(int DK, int DV);
-int64_t kv4_attn_workspace(const Kv4& c, int64_t Tq, int HQ, int64_t n, bool accumulate);
+int64_t kv4_attn_workspace(const Kv4& c, int64_t Tq, int HQ, bool listed, int64_t n, bool accumulate);
 hipError_t launch_kv4_attn(const Kv4& c, const void* Q, int dtype, const int32_t* slots,
                            const int32_t* count, int64_t Tq, int HQ, int64_t n, bool accumulate,
                            float scale, float* out, void* ws, hipStream_t stream);

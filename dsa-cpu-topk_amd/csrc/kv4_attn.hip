@@ -3,8 +3,8 @@
 //   O = sum p V,   weight[b, slot] += sum over queries and heads of p
 //
 // One pass over the cache with a running maximum and sum.  A wave takes 32 slots
-// at a time of one K/V head and up to 16 query heads of its group, on
-// v_mfma_f32_16x16x32_bf16:
+// at a time of one K/V head and up to 16 rows, query heads of its group (of all
+// tokens together where they attend to the same slots), on v_mfma_f32_16x16x32_bf16:
 //
 //   S^T[slot, head] = K Q^T    A: a lane holds 8-element runs of one slot's K row,
 //                              converted from e2m1 with their scale by one
@@ -22,7 +22,7 @@
 // lanes that take them.
 //
 // fp32 operands enter as bf16 pieces: Q as one (bf16), two (fp16) or three (fp32),
-// p as three, which hold its 24 bits.  For up to 5 heads of a group the three
+// p as three, which hold its 24 bits.  For up to 5 rows the three
 // pieces of p stand side by side in the 16 columns (Q is repeated there, so each
 // lane has the p whose piece it takes) and one instruction takes them all.
 //
@@ -39,6 +39,8 @@
 // instructions a tile).  Short calls are bound by latency: 1.2 us to the sequence's
 // length, 1-2 to its first rows, 0.5 a tile, 0.5-2 to join a block's waves, 3-6 for
 // the second launch.
+#include <type_traits>
+
 #include "dsa_launch.h"
 #include "kv4.h"
 #include "tile_common.h"
@@ -69,7 +71,8 @@ struct AttnArgs {
   const void* Q;
   const int32_t* slots;  // or null
   const int32_t* count;  // or null
-  int Tq, HQ, G, row_tiles;
+  int Tq, HQ, G;
+  int row_tiles;  // tiles of 16 rows
   int heads;  // K/V heads a block takes: 4, 2 or 1, its 4 / heads waves of each sharing the slots
   int64_t n, stride;  // slots a query; floats between rows of logits
   int splits;         // blocks that share a query's slots
@@ -121,7 +124,7 @@ struct Frag {
   uint32_t k[2][DK / 32];  // a quarter of the row of slot lane % 16
   uint32_t v[2][DV / 32];  // a quarter of the row of slot 4 * (lane / 4 % 4) + lane / 16
   uint32_t s[Shape<DK, DV>::kLoads];  // K's (even lanes) or V's scales of slot lane / 2 of the 32
-  uint32_t ok;  // bit i: slot i counts
+  uint32_t ok;  // bit i: slot i counts (for the block's one token)
 };
 
 constexpr uint32_t kNowhere = 0x80000000u;  // past any sequence's codes: such loads give zeros
@@ -240,15 +243,20 @@ __device__ __forceinline__ void split_q8(const typename Tag::raw (&raw)[8], bool
 }
 
 // Waves a SIMD holds: what the registers allow without spills.
-__host__ __device__ constexpr int resident(int NP, int DK, int DV) {
-  if (DK <= 64 || (DK <= 128 && NP == 1)) return 4;
+__host__ __device__ constexpr int resident(int NP, int DK, int DV, bool side) {
+  if (DK <= 64 || (DK <= 128 && NP == 1 && side)) return 4;
   if (DK <= 128 || (DV <= 128 && NP == 1)) return 3;
   return DK <= 192 || NP < 3 ? 2 : 1;
 }
 
-template <typename Tag, int NP, int DK, int DV, bool SIDE, bool LISTED>
-__global__ __launch_bounds__(kNT, resident(NP, DK, DV)) void attn_kernel(AttnArgs a) {
+// A block's rows: one token's heads over the first slots or over listed ones, or
+// all tokens' heads over the first slots.
+enum Rows { kOne, kListed, kTokens };
+
+template <typename Tag, int NP, int DK, int DV, bool SIDE, Rows ROWS>
+__global__ __launch_bounds__(kNT, resident(NP, DK, DV, SIDE)) void attn_kernel(AttnArgs a) {
   using S = Shape<DK, DV>;
+  constexpr bool LISTED = ROWS == kListed, MANY = ROWS == kTokens;
   constexpr int NW = DK / 32, NO = DV / 16, LD = DV + 4;
   constexpr int kSums = kWaves * 16 * LD * 4, kStages = kWaves * S::kBytes;
   __shared__ __align__(16) uint8_t lds[kSums > kStages ? kSums : kStages];  // the stages, then the sums
@@ -259,7 +267,7 @@ __global__ __launch_bounds__(kNT, resident(NP, DK, DV)) void attn_kernel(AttnArg
   // read the same rows, so they go to one XCD, one after another.
   const uint32_t per = a.c.HKV / a.heads * a.row_tiles;
   const uint32_t i = blockIdx.x / 8, chunk = i / per * 8 + blockIdx.x % 8, member = i % per;
-  const uint32_t bt = chunk / a.splits, b = bt / a.Tq, t = bt % a.Tq;
+  const uint32_t groups = MANY ? 1 : a.Tq, bg = chunk / a.splits, b = bg / groups, t0 = bg % groups;
   if (b >= a.c.B) return;
   const int hk0 = member / a.row_tiles * a.heads, rt = member % a.row_tiles, split = chunk % a.splits;
 
@@ -267,16 +275,24 @@ __global__ __launch_bounds__(kNT, resident(NP, DK, DV)) void attn_kernel(AttnArg
   const int hk = hk0 + wave % a.heads;  // the wave's K/V head
   const int share = wave / a.heads, shares = kWaves / a.heads;
   const int step = kTile * shares * a.splits;  // slots that the head's waves in all blocks take at once
-  // the lane's query head, and (SIDE) which piece of p it takes
-  const int row = SIDE ? col % a.G : rt * 16 + col;
-  const int piece = SIDE ? col / a.G : 0;
-  const bool used = SIDE ? piece < 3 : row < a.G;
-  const int64_t bh = static_cast<int64_t>(bt) * a.HQ + hk * a.G;  // the group's first head
+  // the lane's row, a token's query head, and (SIDE) which piece of p it takes
+  const int all_rows = MANY ? a.Tq * a.G : a.G;
+  const int row = SIDE ? col % all_rows : rt * 16 + col;
+  const int piece = SIDE ? col / all_rows : 0;
+  const bool used = SIDE ? piece < 3 : row < all_rows;
+  auto token_of = [&](int r) { return MANY ? r / a.G : 0; };
+  // where row r of head hd stands in [B, Tq, HQ]
+  const uint32_t bh = (b * a.Tq + t0) * a.HQ;  // all rows are fewer than 2^23
+  auto head_of = [&](int hd, int r) -> uint32_t {
+    const int t = token_of(r);
+    return bh + t * a.HQ + hd * a.G + (r - t * a.G);
+  };
+  const uint32_t my_head = head_of(hk, used ? row : 0);
 
   // the query row, in the order of the K runs; asked for before anything waits
   typename Tag::raw q_raw[NW][8];
   {
-    const typename Tag::raw* src = static_cast<const typename Tag::raw*>(a.Q) + (bh + (used ? row : 0)) * DK;
+    const typename Tag::raw* src = static_cast<const typename Tag::raw*>(a.Q) + static_cast<int64_t>(my_head) * DK;
 #pragma unroll
     for (int s = 0; s < seg_count(DK); ++s) {
       const int W = seg_width(DK, s), at = seg_at(DK, s);
@@ -286,16 +302,28 @@ __global__ __launch_bounds__(kNT, resident(NP, DK, DV)) void attn_kernel(AttnArg
     }
   }
 
-  const int32_t seen = kv4_visible(a.c.length, a.count, b, a.c.S, t, a.Tq);
-  const int32_t limit = LISTED ? seen : static_cast<int32_t>(min(static_cast<int64_t>(seen), a.n));
+  // `limit` slots for some of the block's rows (their last token sees the most),
+  // `my_limit` for the lane's own.
+  int32_t limit, my_limit;
+  if constexpr (!MANY) {
+    limit = kv4_visible(a.c.length, a.count, b, a.c.S, t0, a.Tq);
+    if (!LISTED) limit = static_cast<int32_t>(min(static_cast<int64_t>(limit), a.n));
+    my_limit = limit;
+  } else {
+    const int32_t n = a.count ? max(0, min(a.count[b], a.Tq)) : a.Tq, have = kv4_length(a.c.length, b, a.c.S) - n + 1;
+    const int32_t most = static_cast<int32_t>(a.n);
+    const int first = token_of(rt * 16), last = min(token_of(min(rt * 16 + 16, all_rows) - 1), n - 1);
+    limit = last >= first ? max(0, min(have + last, most)) : 0;
+    const int mine = token_of(used ? row : rt * 16);
+    my_limit = mine < n ? max(0, min(have + mine, most)) : 0;
+  }
   // Tiles go to the waves in turn, so that every block has its share of the slots in use.
   const int64_t j_end = LISTED ? (limit > 0 ? a.n : 0) : limit;
   const int64_t j_first = static_cast<int64_t>(split) * shares * kTile;
-  const int rows = SIDE ? a.G : min(16, a.G - rt * 16);
-  const int64_t bh0 = static_cast<int64_t>(bt) * a.HQ + hk0 * a.G + rt * 16;  // the block's first query head
+  const int rows = SIDE ? all_rows : min(16, all_rows - rt * 16);
   if (j_first >= j_end) {  // nothing here: no sum, and no sums to read
     for (int e = threadIdx.x; e < a.heads * rows; e += kNT) {
-      const int64_t h = bh0 + e / rows * a.G + e % rows;
+      const int64_t h = head_of(hk0 + e / rows, rt * 16 + e % rows);
       a.ml[h * a.splits + split] = make_float2(-INFINITY, 0.0f);
       if (a.splits == 1)
         for (int d = 0; d < DV; ++d) a.out[h * DV + d] = __builtin_nanf("");
@@ -314,7 +342,7 @@ __global__ __launch_bounds__(kNT, resident(NP, DK, DV)) void attn_kernel(AttnArg
   };
   const __amdgpu_buffer_rsrc_t all_codes = rsrc(codes, static_cast<int64_t>(limit) * cb);
   const __amdgpu_buffer_rsrc_t all_scales = rsrc(scales, static_cast<int64_t>(limit) * (cb / 16));
-  const int32_t* list = LISTED ? a.slots + static_cast<int64_t>(bt) * a.n : nullptr;
+  const int32_t* list = LISTED ? a.slots + (static_cast<int64_t>(b) * a.Tq + t0) * a.n : nullptr;
   const int vslot = 4 * ((lane >> 2) & 3) + (lane >> 4);
 
   // A listed slot's offset, of entry j0 + lane % 32; read a step before the slots.
@@ -332,9 +360,9 @@ __global__ __launch_bounds__(kNT, resident(NP, DK, DV)) void attn_kernel(AttnArg
     } else {
       const uint32_t krow[2] = {col * cb, (16 + col) * cb}, vrow[2] = {vslot * cb, (16 + vslot) * cb};
       const int64_t rest = max(static_cast<int64_t>(0), limit - j0);
+      if (!MANY) f.ok = rest >= kTile ? ~0u : (1u << rest) - 1;
       load_frag<DK, DV>(f, rsrc(codes + j0 * cb, rest * cb), rsrc(scales + j0 * (cb / 16), rest * (cb / 16)), krow,
                         vrow, (lane >> 1) * cb, hk);
-      f.ok = rest >= kTile ? ~0u : (1u << rest) - 1;
     }
   };
 
@@ -356,7 +384,7 @@ __global__ __launch_bounds__(kNT, resident(NP, DK, DV)) void attn_kernel(AttnArg
 
   uint8_t* mine = lds + wave * S::kBytes;
   const uint8_t* my_s = mine + S::kS;
-  auto compute = [&](uint32_t counts, int64_t j0) {
+  auto compute = [&](uint32_t ok_all, int64_t j0) {
     f32x4 s[2] = {f32x4{0, 0, 0, 0}, f32x4{0, 0, 0, 0}};
 #pragma unroll
     for (int sg = 0; sg < seg_count(DK); ++sg) {
@@ -390,13 +418,36 @@ __global__ __launch_bounds__(kNT, resident(NP, DK, DV)) void attn_kernel(AttnArg
     float p[8];
 #pragma unroll
     for (int r = 0; r < 8; ++r) p[r] = s[r >> 2][r & 3];
-    if (counts != ~0u) {
+    const int32_t rest = my_limit - static_cast<int32_t>(j0);
+    const uint32_t counts = !MANY ? ok_all : rest >= kTile ? ~0u : rest <= 0 ? 0u : (1u << rest) - 1;
+    if (MANY ? __builtin_amdgcn_ballot_w64(counts != ~0u) != 0 : counts != ~0u) {
       const uint32_t ok = counts >> (4 * g);
 #pragma unroll
       for (int r = 0; r < 8; ++r) p[r] = (ok >> ((r >> 2) * 16 + (r & 3))) & 1u ? p[r] : -INFINITY;
+      // A value that is NaN meets p = 0 in the rows that do not see it: such blocks
+      // become zeros here, and NaN the sums of the rows that do.
+      if constexpr (MANY) {
+#pragma unroll
+        for (int bl = 0; bl < DV / 32; ++bl) {
+          uint8_t* at = mine + S::kS + (DK / 32 + bl) * 32 + (lane & 31);
+          const bool nan = *at == 255;
+          const uint32_t bad = static_cast<uint32_t>(__builtin_amdgcn_ballot_w64(nan));
+          if (bad == 0) continue;
+          if (nan) *at = 0;
+          if ((bad & counts) == 0) continue;
+#pragma unroll
+          for (int sg = 0; sg < seg_count(DV); ++sg)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if ((seg_at(DV, sg) + (4 * g + r) * (seg_width(DV, sg) / 16)) / 32 == bl)
+#pragma unroll
+                for (int i2 = 0; i2 < seg_width(DV, sg) / 16; ++i2) o[seg_at(DV, sg) / 16 + i2][r] = __builtin_nanf("");
+        }
+        wave_lds_order();
+      }
     }
     if (a.logits && (SIDE ? piece == 0 : used)) {
-      float* to = a.logits + (bh + row) * a.stride + j0 + 4 * g;
+      float* to = a.logits + my_head * a.stride + j0 + 4 * g;
       *reinterpret_cast<float4*>(to) = make_float4(p[0] * to2, p[1] * to2, p[2] * to2, p[3] * to2);
       *reinterpret_cast<float4*>(to + 16) = make_float4(p[4] * to2, p[5] * to2, p[6] * to2, p[7] * to2);
     }
@@ -479,7 +530,7 @@ __global__ __launch_bounds__(kNT, resident(NP, DK, DV)) void attn_kernel(AttnArg
   if (j < j_end) {
     if (LISTED) off = entry(j + step);
     for (; j < j_end; j += step) {
-      const uint32_t counts = f.ok;
+      const uint32_t ok_all = MANY ? 0u : f.ok;
       wave_lds_order();
       stage<DK, DV>(f, mine);
       wave_lds_order();
@@ -487,7 +538,7 @@ __global__ __launch_bounds__(kNT, resident(NP, DK, DV)) void attn_kernel(AttnArg
         load(f, j + step, off);
         if (LISTED) off = entry(j + 2 * step);
       }
-      compute(counts, j);
+      compute(ok_all, j);
     }
   }
 
@@ -498,7 +549,7 @@ __global__ __launch_bounds__(kNT, resident(NP, DK, DV)) void attn_kernel(AttnArg
     sum_m[wave][col] = m;
     sum_l[wave][col] = l;
   }
-  if (col < (SIDE ? 3 * a.G : rows)) {
+  if (col < (SIDE ? 3 * rows : rows)) {
     float* to = sum_o[wave][col];
 #pragma unroll
     for (int sg = 0; sg < seg_count(DV); ++sg) {
@@ -530,13 +581,13 @@ __global__ __launch_bounds__(kNT, resident(NP, DK, DV)) void attn_kernel(AttnArg
       total += f * sum_l[w][rw];
       float4 y = *reinterpret_cast<const float4*>(&sum_o[w][rw][d]);
       if constexpr (SIDE) {  // the pieces, the small ones first
-        const float4 y1 = *reinterpret_cast<const float4*>(&sum_o[w][rw + a.G][d]);
-        const float4 y2 = *reinterpret_cast<const float4*>(&sum_o[w][rw + 2 * a.G][d]);
+        const float4 y1 = *reinterpret_cast<const float4*>(&sum_o[w][rw + rows][d]);
+        const float4 y2 = *reinterpret_cast<const float4*>(&sum_o[w][rw + 2 * rows][d]);
         y.x += y1.x + y2.x; y.y += y1.y + y2.y; y.z += y1.z + y2.z; y.w += y1.w + y2.w;
       }
       x.x += f * y.x; x.y += f * y.y; x.z += f * y.z; x.w += f * y.w;
     }
-    const int64_t h = bh0 + hd * a.G + rw;
+    const int64_t h = head_of(hk0 + hd, rt * 16 + rw);
     if (a.splits > 1) {
       *reinterpret_cast<float4*>(a.part + (h * a.splits + split) * DV + d) = x;
     } else {  // 0 / 0 where no logit is above -inf
@@ -643,27 +694,34 @@ __global__ __launch_bounds__(kNT) void finish_kernel(AttnArgs a, int64_t joins, 
 
 struct Plan {
   int splits, row_tiles, heads;
-  bool side;
+  bool side, many;
   int64_t ml, part, logits, total, stride;  // byte offsets; floats a row
 };
 
-Plan plan_of(const Kv4& c, int64_t Tq, int HQ, int64_t n, bool accumulate) {
+Plan plan_of(const Kv4& c, int64_t Tq, int HQ, bool listed, int64_t n, bool accumulate) {
   Plan p;
-  const int G = HQ / c.HKV;
-  p.side = G <= 5;
-  p.row_tiles = p.side ? 1 : (G + 15) / 16;
+  const int64_t G = HQ / c.HKV, tiles = (G + 15) / 16;  // of 16 rows, one token's
   // Up to 8 turns of four waves on one head's slots cost less than the launch that
   // would join splits (255 listed slots, 8 heads of 64, fp32, 4 sequences: 11.3 us
   // with it, 8.8 without).  (Whether weights are accumulated does not enter: it
   // changes no bit of the output.)
   const bool alone = n <= 8 * kTile * kWaves;
+  const int cus = device_cus() > 0 ? device_cus() : 256;
+  const bool few = c.B * Tq * c.HKV * tiles <= 4 * cus;
+  // Tokens that attend to the same slots, all but the last few, share a block's rows
+  // where that leaves fewer tiles of rows (us with / without: 16 x 16384 slots of 8
+  // heads of 128, groups of 4, 2 tokens 59 / 80, 4 tokens 62 / 137; 2 x 4096 slots, 64
+  // tokens 42 / 83), unless there are few blocks of one turn anyway (4 x 500 slots of
+  // 8 heads of 64 in fp32, 2 tokens 11.3 / 8.8).
+  p.many = !listed && (Tq * G + 15) / 16 < Tq * tiles && !(alone && few);
+  const int64_t rows = p.many ? Tq * G : G, groups = p.many ? c.B : c.B * Tq;
+  p.side = rows <= 5;
+  p.row_tiles = static_cast<int>((rows + 15) / 16);
   // Four neighbouring heads a block read whole rows of the cache together; few blocks
   // of one that have no splits finish sooner (us with four / one: 64 x 1024 slots of
   // 8 heads of 128 19.6 / 16.6, 256 x 512 of 8 of 64 17.3 / 19.6).
-  const int cus = device_cus() > 0 ? device_cus() : 256;
-  const bool few = c.B * Tq * c.HKV * p.row_tiles <= 4 * cus;
   p.heads = alone && few ? 1 : c.HKV % 4 == 0 ? 4 : c.HKV % 2 == 0 ? 2 : 1;
-  const int64_t blocks = c.B * Tq * (c.HKV / p.heads) * p.row_tiles;
+  const int64_t blocks = groups * (c.HKV / p.heads) * p.row_tiles;
   const int unit = kTile * (kWaves / p.heads);  // slots that a block takes at once
   const int64_t steps = n > 0 ? (n + unit - 1) / unit : 1;
   // Two blocks a compute unit: 1, 2, 4 and 8 measured 108, 94, 93 and 109 us for
@@ -683,28 +741,29 @@ Plan plan_of(const Kv4& c, int64_t Tq, int HQ, int64_t n, bool accumulate) {
 }
 
 template <typename Tag, int NP, int DK, int DV>
-hipError_t launch_dims(const AttnArgs& a, bool side, int64_t blocks, hipStream_t stream) {
+hipError_t launch_dims(const AttnArgs& a, const Plan& p, int64_t blocks, hipStream_t stream) {
   const uint32_t grid = static_cast<uint32_t>(blocks);
-  if (a.slots) {
-    if (side) attn_kernel<Tag, NP, DK, DV, true, true><<<grid, kNT, 0, stream>>>(a);
-    else attn_kernel<Tag, NP, DK, DV, false, true><<<grid, kNT, 0, stream>>>(a);
-  } else {
-    if (side) attn_kernel<Tag, NP, DK, DV, true, false><<<grid, kNT, 0, stream>>>(a);
-    else attn_kernel<Tag, NP, DK, DV, false, false><<<grid, kNT, 0, stream>>>(a);
-  }
+  auto run = [&](auto side) {
+    constexpr bool SIDE = decltype(side)::value;
+    if (a.slots) attn_kernel<Tag, NP, DK, DV, SIDE, kListed><<<grid, kNT, 0, stream>>>(a);
+    else if (p.many) attn_kernel<Tag, NP, DK, DV, SIDE, kTokens><<<grid, kNT, 0, stream>>>(a);
+    else attn_kernel<Tag, NP, DK, DV, SIDE, kOne><<<grid, kNT, 0, stream>>>(a);
+  };
+  if (p.side) run(std::true_type{});
+  else run(std::false_type{});
   return hipGetLastError();
 }
 
 template <typename Tag, int NP>
-hipError_t launch_type(const AttnArgs& a, bool side, int64_t blocks, hipStream_t stream) {
-  if (a.c.DK != a.c.DV) return launch_dims<Tag, NP, 192, 128>(a, side, blocks, stream);
+hipError_t launch_type(const AttnArgs& a, const Plan& p, int64_t blocks, hipStream_t stream) {
+  if (a.c.DK != a.c.DV) return launch_dims<Tag, NP, 192, 128>(a, p, blocks, stream);
   switch (a.c.DK) {
-    case 32: return launch_dims<Tag, NP, 32, 32>(a, side, blocks, stream);
-    case 64: return launch_dims<Tag, NP, 64, 64>(a, side, blocks, stream);
-    case 96: return launch_dims<Tag, NP, 96, 96>(a, side, blocks, stream);
-    case 128: return launch_dims<Tag, NP, 128, 128>(a, side, blocks, stream);
-    case 192: return launch_dims<Tag, NP, 192, 192>(a, side, blocks, stream);
-    default: return launch_dims<Tag, NP, 256, 256>(a, side, blocks, stream);
+    case 32: return launch_dims<Tag, NP, 32, 32>(a, p, blocks, stream);
+    case 64: return launch_dims<Tag, NP, 64, 64>(a, p, blocks, stream);
+    case 96: return launch_dims<Tag, NP, 96, 96>(a, p, blocks, stream);
+    case 128: return launch_dims<Tag, NP, 128, 128>(a, p, blocks, stream);
+    case 192: return launch_dims<Tag, NP, 192, 192>(a, p, blocks, stream);
+    default: return launch_dims<Tag, NP, 256, 256>(a, p, blocks, stream);
   }
 }
 
@@ -715,14 +774,14 @@ bool kv4_attn_supported(int DK, int DV) {
   return DK == DV && (DK == 32 || DK == 64 || DK == 96 || DK == 128 || DK == 192 || DK == 256);
 }
 
-int64_t kv4_attn_workspace(const Kv4& c, int64_t Tq, int HQ, int64_t n, bool accumulate) {
-  return plan_of(c, Tq, HQ, n, accumulate).total;
+int64_t kv4_attn_workspace(const Kv4& c, int64_t Tq, int HQ, bool listed, int64_t n, bool accumulate) {
+  return plan_of(c, Tq, HQ, listed, n, accumulate).total;
 }
 
 hipError_t launch_kv4_attn(const Kv4& c, const void* Q, int dtype, const int32_t* slots,
                            const int32_t* count, int64_t Tq, int HQ, int64_t n, bool accumulate,
                            float scale, float* out, void* ws, hipStream_t stream) {
-  const Plan p = plan_of(c, Tq, HQ, n, accumulate);
+  const Plan p = plan_of(c, Tq, HQ, slots != nullptr, n, accumulate);
   char* base = static_cast<char*>(ws);
   AttnArgs a;
   a.c = c;
@@ -746,11 +805,11 @@ hipError_t launch_kv4_attn(const Kv4& c, const void* Q, int dtype, const int32_t
   a.ml = reinterpret_cast<float2*>(base + p.ml);
   a.part = reinterpret_cast<float*>(base + p.part);
   a.logits = accumulate ? reinterpret_cast<float*>(base + p.logits) : nullptr;
-  const int64_t chunks = (c.B * Tq * p.splits + 7) / 8 * 8;
+  const int64_t chunks = ((p.many ? c.B : c.B * Tq) * p.splits + 7) / 8 * 8;
   const int64_t blocks = chunks * (c.HKV / p.heads) * p.row_tiles;
-  hipError_t e = dtype == 0   ? launch_type<F32, 3>(a, p.side, blocks, stream)
-                 : dtype == 1 ? launch_type<BF16, 1>(a, p.side, blocks, stream)
-                              : launch_type<F16, 2>(a, p.side, blocks, stream);
+  hipError_t e = dtype == 0   ? launch_type<F32, 3>(a, p, blocks, stream)
+                 : dtype == 1 ? launch_type<BF16, 1>(a, p, blocks, stream)
+                              : launch_type<F16, 2>(a, p, blocks, stream);
   if (e != hipSuccess) return e;
   int64_t joins = p.splits > 1 ? c.B * Tq * HQ * (c.DV / a.join_cols) : 0;
   const int64_t per_b = accumulate ? (n + kNT - 1) / kNT : 0;

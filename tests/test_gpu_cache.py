@@ -335,6 +335,38 @@ def test_attention_of_listed_all_is_attention(dev):
     assert torch.isnan(D.kv4_attention(cache, Q, slots=slots[..., :0])).all()
 
 
+@pytest.mark.parametrize("HQ, HKV, DK, DV, Tq, dtype", [
+    (1, 1, 64, 64, 2, F32), (2, 2, 128, 128, 5, BF16), (8, 2, 64, 64, 2, F16), (8, 4, 32, 32, 3, F32),
+    (12, 2, 128, 128, 7, BF16), (5, 1, 96, 96, 3, BF16), (12, 4, 192, 128, 11, F16), (3, 3, 256, 256, 33, BF16),
+    (20, 1, 64, 64, 4, F32), (4, 1, 192, 192, 40, F32)])
+def test_attention_of_tokens_together(dev, HQ, HKV, DK, DV, Tq, dtype):
+    """Tokens that share the cache's tiles: their own last slots on both sides of a
+    tile's edge, row tiles that begin inside a token's heads, padded batches."""
+    cache = filled(dev, 5, 1100, HKV, DK, DV, [1100, 1056 + Tq // 2, 1025, Tq - 1, 0], 46)
+    Q = randn(gen(dev, 47), 5, Tq, HQ, DK, dtype=dtype)
+    attend(cache, Q, "all tokens")
+    attend(cache, Q, "padded", count=ints(dev, [Tq, 1, Tq - 1, 1, 0]))
+    attend(cache, Q, "the first slots", span=1057)
+
+
+@pytest.mark.parametrize("D_", [32, 128, 192])
+def test_nan_of_tokens_together(dev, D_):
+    """A later token's NaN value, and an earlier one's, among tokens that share tiles:
+    NaN exactly in the blocks of 32 of the queries that see it."""
+    g, Tq, n = gen(dev, 48), 6, 1058
+    cache = filled(dev, 1, 1100, 2, D_, D_, [n], 49)
+    per = D_ // 32
+    cache.scales[0, n - 2, 0, per] = 255       # V of the last token but one: block 0 of head 0
+    cache.scales[0, n - 5, 1, 2 * per - 1] = 255  # V of the second: the last block of head 1
+    cache.scales[0, n - 1, 1, 0] = 255         # K of the last: its own query of head 1 alone
+    out = D.kv4_attention(cache, randn(g, 1, Tq, 4, D_)).view(Tq, 2, 2, per, 32)
+    want = torch.zeros(Tq, 2, 2, per, 32, dtype=torch.bool, device=dev)
+    want[Tq - 2:, 0, :, 0] = True
+    want[1:, 1, :, per - 1] = True
+    want[Tq - 1, 1] = True
+    assert torch.equal(torch.isnan(out), want)
+
+
 def test_attention_nan_where_it_belongs(dev):
     """A NaN block of a later token's or an unlisted slot reaches no other query; a seen one does."""
     g = gen(dev, 43)
