@@ -719,8 +719,10 @@ Plan plan_of(const Kv4& c, int64_t Tq, int HQ, bool listed, int64_t n, bool accu
   p.row_tiles = static_cast<int>((rows + 15) / 16);
   // Four neighbouring heads a block read whole rows of the cache together; few blocks
   // of one that have no splits finish sooner (us with four / one: 64 x 1024 slots of
-  // 8 heads of 128 19.6 / 16.6, 256 x 512 of 8 of 64 17.3 / 19.6).
-  p.heads = alone && few ? 1 : c.HKV % 4 == 0 ? 4 : c.HKV % 2 == 0 ? 2 : 1;
+  // 8 heads of 128 19.6 / 16.6, 256 x 512 of 8 of 64 17.3 / 19.6), and so does it where
+  // the rows are gathered (2048 listed slots of 32 x 4 heads of 128 19.5 / 18.7, 256 x 4
+  // of 64 55.5 / 41.3, 16 x 4 with groups of 16 22.4 / 16.6; of 64 x 8 49 / 53).
+  p.heads = listed || (alone && few) ? 1 : c.HKV % 4 == 0 ? 4 : c.HKV % 2 == 0 ? 2 : 1;
   const int64_t blocks = groups * (c.HKV / p.heads) * p.row_tiles;
   const int unit = kTile * (kWaves / p.heads);  // slots that a block takes at once
   const int64_t steps = n > 0 ? (n + unit - 1) / unit : 1;
