@@ -80,7 +80,7 @@ struct AttnArgs {
   float scale;
   float* out;
   float* part;    // [B*Tq*HQ][splits][DV] sums, where splits > 1
-  float2* ml;     // [B*Tq*HQ][splits] maximum (in powers of 2) and sum of exponentials
+  float2* ml;     // [B*Tq*HQ][splits] maximum (in powers of 2) and sum of exponentials, or null
   float* logits;  // [B*Tq*HQ][stride], in powers of 2, or null
 };
 
@@ -324,7 +324,7 @@ __global__ __launch_bounds__(kNT, resident(NP, DK, DV, SIDE)) void attn_kernel(A
   if (j_first >= j_end) {  // nothing here: no sum, and no sums to read
     for (int e = threadIdx.x; e < a.heads * rows; e += kNT) {
       const int64_t h = head_of(hk0 + e / rows, rt * 16 + e % rows);
-      a.ml[h * a.splits + split] = make_float2(-INFINITY, 0.0f);
+      if (a.ml) a.ml[h * a.splits + split] = make_float2(-INFINITY, 0.0f);
       if (a.splits == 1)
         for (int d = 0; d < DV; ++d) a.out[h * DV + d] = __builtin_nanf("");
     }
@@ -593,7 +593,7 @@ __global__ __launch_bounds__(kNT, resident(NP, DK, DV, SIDE)) void attn_kernel(A
     } else {  // 0 / 0 where no logit is above -inf
       *reinterpret_cast<float4*>(a.out + h * DV + d) = make_float4(x.x / total, x.y / total, x.z / total, x.w / total);
     }
-    if (d == 0) a.ml[h * a.splits + split] = make_float2(top, total);
+    if (d == 0 && a.ml) a.ml[h * a.splits + split] = make_float2(top, total);
   }
 }
 
@@ -735,8 +735,8 @@ Plan plan_of(const Kv4& c, int64_t Tq, int HQ, bool listed, int64_t n, bool accu
   auto up = [](int64_t v) { return (v + 255) / 256 * 256; };
   const int64_t heads = c.B * Tq * HQ;
   p.stride = (n + kTile - 1) / kTile * kTile;
-  p.ml = 0;
-  p.part = up(heads * p.splits * 8);
+  p.ml = 0;  // one split without weights needs nothing
+  p.part = p.splits > 1 || accumulate ? up(heads * p.splits * 8) : 0;
   p.logits = p.part + (p.splits > 1 ? up(heads * p.splits * c.DV * 4) : 0);
   p.total = p.logits + (accumulate ? up(heads * p.stride * 4) : 0);
   return p;
@@ -804,7 +804,7 @@ hipError_t launch_kv4_attn(const Kv4& c, const void* Q, int dtype, const int32_t
   a.join_cols = p.splits > 32 ? 32 : c.DV;
   a.scale = scale;
   a.out = out;
-  a.ml = reinterpret_cast<float2*>(base + p.ml);
+  a.ml = p.total > 0 ? reinterpret_cast<float2*>(base + p.ml) : nullptr;
   a.part = reinterpret_cast<float*>(base + p.part);
   a.logits = accumulate ? reinterpret_cast<float*>(base + p.logits) : nullptr;
   const int64_t chunks = ((p.many ? c.B : c.B * Tq) * p.splits + 7) / 8 * 8;

@@ -325,9 +325,9 @@ def kv4_attention(cache: KV4Cache, Q: torch.Tensor, *, slots: torch.Tensor | Non
     acc = 1 if accumulate else 0
     lib = L.lib()
     nws = _workspace_bytes(cache, Tq, HQ, slots is not None, n, acc)
-    ws = torch.empty(nws, device=cache.device, dtype=torch.uint8)
+    ws = torch.empty(nws, device=cache.device, dtype=torch.uint8) if nws else None
     _call(cache, "kv4_attention", lib.dsa_kv4_attention, q_ptr, L.dtype_code(dt), slots_ptr, count_ptr,
-          Tq, HQ, n, acc, cache.scale, out.data_ptr(), ws.data_ptr(), nws)
+          Tq, HQ, n, acc, cache.scale, out.data_ptr(), ws.data_ptr() if nws else None, nws)
     return out
 
 
