@@ -3,7 +3,7 @@
 //
 // Measured: 2 x 16384 tokens of 8 heads of 128 in bf16 in (187 MB) 46 us and back
 // out (170 MB) 27 us, 4.9 TB/s together where a copy reaches 5.2; eviction's select
-// 8.6 us for 32 sequences of 2049 slots with the one slot that moves, 11.8 for 8 of
+// 7.2 us for 32 sequences of 2049 slots with the one slot that moves, 10.8 for 8 of
 // 4099, a chain of passes over registers, histogram and scans; its moves 5.2 us for
 // 8 x 760 slots.
 #include "kv4.h"
@@ -228,19 +228,16 @@ __global__ __launch_bounds__(kET) void evict_select_kernel(Kv4 c, int64_t keep, 
   const int32_t* position = c.position + b * c.S;
   src += b * M;
   dst += b * M;
-  if (n <= keep) {
-    for (int64_t i = threadIdx.x; i < M; i += kET) src[i] = dst[i] = -1;
-    return;
-  }
   constexpr uint32_t kProtected = 0xffffffffu;  // above every weight's key
   const int64_t first_kept = static_cast<int64_t>(c.seen[b]) - recent;
+  const int32_t S = static_cast<int32_t>(c.S);
   constexpr int kSpan = VPT * kET;
   uint32_t key[VPT];
-  auto read = [&](int s0) {  // keys of slots s0 + VPT * thread ..; past n: not looked at
+  auto read = [&](int s0) {  // keys of slots s0 + VPT * thread .., which may be past n
     const int s = s0 + threadIdx.x * VPT;
     float w[VPT];
     int32_t p[VPT];
-    if (s + VPT <= n) {  // 16 bytes at once, at any multiple of 4
+    if (s + VPT <= S) {  // 16 bytes at once, at any multiple of 4
 #pragma unroll
       for (int i = 0; i < VPT; i += 4) {
         __builtin_memcpy(w + i, weight + s + i, 16);
@@ -249,15 +246,19 @@ __global__ __launch_bounds__(kET) void evict_select_kernel(Kv4 c, int64_t keep, 
     } else {
 #pragma unroll
       for (int i = 0; i < VPT; ++i) {
-        w[i] = s + i < n ? weight[s + i] : 0.0f;
-        p[i] = s + i < n ? position[s + i] : 0;
+        w[i] = s + i < S ? weight[s + i] : 0.0f;
+        p[i] = s + i < S ? position[s + i] : 0;
       }
     }
 #pragma unroll
     for (int i = 0; i < VPT; ++i) key[i] = p[i] >= first_kept ? kProtected : float_to_key(w[i]);
   };
+  read(0);  // on its way together with the length
+  if (n <= keep) {
+    for (int64_t i = threadIdx.x; i < M; i += kET) src[i] = dst[i] = -1;
+    return;
+  }
   const bool once = n <= kSpan;
-  if (once) read(0);
   auto each = [&](auto f) {  // f(slot, key) for the thread's slots of a span that count
     for (int s0 = 0; s0 < n; s0 += kSpan) {
       if (!once) read(s0);
@@ -344,10 +345,11 @@ __global__ __launch_bounds__(kET) void evict_select_kernel(Kv4 c, int64_t keep, 
       if (goes && s + i < keep) freed |= 1ull << i;
       if (!goes && s + i >= keep) away |= 1ull << i;
     }
-    uint32_t f = free0 + evict_scan(popc64(freed), wsum, total);
-    free0 += total;
-    uint32_t w = away0 + evict_scan(popc64(away), wsum, total);
-    away0 += total;
+    // both counts of a span in one sum, 16 bits each (kSpan <= 2^14)
+    const uint32_t before = evict_scan(popc64(freed) | popc64(away) << 16, wsum, total);
+    uint32_t f = free0 + (before & 0xffffu), w = away0 + (before >> 16);
+    free0 += total & 0xffffu;
+    away0 += total >> 16;
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
       if (freed >> i & 1) {
