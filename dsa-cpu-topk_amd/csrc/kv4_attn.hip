@@ -698,7 +698,8 @@ struct Plan {
   int64_t ml, part, logits, total, stride;  // byte offsets; floats a row
 };
 
-Plan plan_of(const Kv4& c, int64_t Tq, int HQ, bool listed, int64_t n, bool accumulate) {
+// pieces: of Q (resident); the most splits come of the fewest.
+Plan plan_of(const Kv4& c, int64_t Tq, int HQ, bool listed, int64_t n, bool accumulate, int pieces) {
   Plan p;
   const int64_t G = HQ / c.HKV, tiles = (G + 15) / 16;  // of 16 rows, one token's
   // Up to 8 turns of four waves on one head's slots cost less than the launch that
@@ -727,8 +728,10 @@ Plan plan_of(const Kv4& c, int64_t Tq, int HQ, bool listed, int64_t n, bool accu
   const int unit = kTile * (kWaves / p.heads);  // slots that a block takes at once
   const int64_t steps = n > 0 ? (n + unit - 1) / unit : 1;
   // Two blocks a compute unit: 1, 2, 4 and 8 measured 108, 94, 93 and 109 us for
-  // 16 x 32768 slots, 16.1, 12.9, 14.4 and 15.1 us for 16 x 4096.
-  int64_t splits = alone || blocks < 1 ? 1 : (2 * cus + blocks - 1) / blocks;
+  // 16 x 32768 slots, 16.1, 12.9, 14.4 and 15.1 us for 16 x 4096.  One where a second
+  // would wait (4 x 8192 slots, 16 heads on 4 of 256 in fp32: 24.4 us with two, 17.9).
+  const int at_once = resident(pieces, c.DK, c.DV, p.side) < 2 ? 1 : 2;
+  int64_t splits = alone || blocks < 1 ? 1 : (at_once * cus + blocks - 1) / blocks;
   splits = splits > steps ? steps : splits;
   splits = splits > kMaxSplits ? kMaxSplits : splits;
   p.splits = static_cast<int>(splits);
@@ -777,13 +780,13 @@ bool kv4_attn_supported(int DK, int DV) {
 }
 
 int64_t kv4_attn_workspace(const Kv4& c, int64_t Tq, int HQ, bool listed, int64_t n, bool accumulate) {
-  return plan_of(c, Tq, HQ, listed, n, accumulate).total;
+  return plan_of(c, Tq, HQ, listed, n, accumulate, 1).total;
 }
 
 hipError_t launch_kv4_attn(const Kv4& c, const void* Q, int dtype, const int32_t* slots,
                            const int32_t* count, int64_t Tq, int HQ, int64_t n, bool accumulate,
                            float scale, float* out, void* ws, hipStream_t stream) {
-  const Plan p = plan_of(c, Tq, HQ, slots != nullptr, n, accumulate);
+  const Plan p = plan_of(c, Tq, HQ, slots != nullptr, n, accumulate, dtype == 0 ? 3 : dtype == 1 ? 1 : 2);
   char* base = static_cast<char*>(ws);
   AttnArgs a;
   a.c = c;
