@@ -115,13 +115,22 @@ __global__ __launch_bounds__(kNT) void indexer_kernel(IndexArgs a) {
           for (int kb = 0; kb < KB; ++kb) acc[kb] = mfma16<Tag>(x, k[kb][c], acc[kb]);
         }
         const float4 wv = *reinterpret_cast<const float4*>(weights + (t * nht + ht) * 16 + 4 * g);
+        // Rows past HI are zeros, and 0 * Inf is NaN there: they stay out of the sum.
+        const int heads = a.HI - 16 * ht;
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb) {
           // the IEEE maximum: a NaN stays one
-          sum[kb] = fmaf(wv.x, __builtin_elementwise_maximum(acc[kb][0], 0.0f), sum[kb]);
-          sum[kb] = fmaf(wv.y, __builtin_elementwise_maximum(acc[kb][1], 0.0f), sum[kb]);
-          sum[kb] = fmaf(wv.z, __builtin_elementwise_maximum(acc[kb][2], 0.0f), sum[kb]);
-          sum[kb] = fmaf(wv.w, __builtin_elementwise_maximum(acc[kb][3], 0.0f), sum[kb]);
+          f32x4 r;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) r[i] = __builtin_elementwise_maximum(acc[kb][i], 0.0f);
+          if (heads < 16) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) r[i] = 4 * g + i < heads ? r[i] : 0.0f;
+          }
+          sum[kb] = fmaf(wv.x, r[0], sum[kb]);
+          sum[kb] = fmaf(wv.y, r[1], sum[kb]);
+          sum[kb] = fmaf(wv.z, r[2], sum[kb]);
+          sum[kb] = fmaf(wv.w, r[3], sum[kb]);
         }
       }
       float mine = 0.0f;  // lane group g stores the slots of tile g
