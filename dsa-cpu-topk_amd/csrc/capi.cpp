@@ -167,6 +167,23 @@ int check_kv4_attention(const dsa_kv4_cache* c, int64_t Tq, int HQ, bool listed,
   return DSA_OK;
 }
 
+// dtype: of q_idx and w_idx, the cache's idx_dtype or fp32.
+int kv4_indexer(const dsa_kv4_cache* cache, const void* q_idx, const void* w_idx, int dtype,
+                const int32_t* count, int64_t Tq, int HI, int64_t span, float* scores, void* stream) {
+  int rc = check_kv4(cache, false, true, "kv4_indexer");
+  if (rc != DSA_OK) return rc;
+  if (HI < 1 || HI > 256) return fail(DSA_EINVAL, "kv4_indexer: HI=%d outside [1,256]", HI);
+  if (Tq < 0 || Tq > kMaxElems) return fail(DSA_EINVAL, "kv4_indexer: Tq=%lld", (long long)Tq);
+  if (span < 0 || span > cache->S) return fail(DSA_EINVAL, "kv4_indexer: span=%lld outside [0, S=%lld]", (long long)span, (long long)cache->S);
+  if (cache->B * Tq * span == 0) return DSA_OK;
+  if (cache->B * Tq >= (int64_t{1} << 23)) return fail(DSA_EINVAL, "kv4_indexer: B*Tq=%lld must be < 2^23", (long long)(cache->B * Tq));
+  if (!q_idx || !w_idx || !scores) return fail(DSA_EINVAL, "kv4_indexer: null pointer");
+  if (!aligned16(q_idx) || !aligned4(scores) || !aligned4(count)) return fail(DSA_EINVAL, "kv4_indexer: q_idx must be 16-byte aligned, scores and count 4-byte");
+  return hip_status(dsa::launch_kv4_indexer(kv4_of(cache), q_idx, w_idx, dtype, cache->idx_dtype, count, Tq, HI,
+                                            span, scores, static_cast<hipStream_t>(stream)),
+                    "dsa_kv4_indexer_scores");
+}
+
 }  // namespace
 
 extern "C" {
@@ -571,18 +588,13 @@ int dsa_kv4_rows(const dsa_kv4_cache* cache, const int32_t* slots, int64_t N, in
 int dsa_kv4_indexer_scores(const dsa_kv4_cache* cache, const void* q_idx, const void* w_idx,
                            const int32_t* count, int64_t Tq, int HI, int64_t span, float* scores,
                            void* stream) {
-  int rc = check_kv4(cache, false, true, "kv4_indexer");
-  if (rc != DSA_OK) return rc;
-  if (HI < 1 || HI > 256) return fail(DSA_EINVAL, "kv4_indexer: HI=%d outside [1,256]", HI);
-  if (Tq < 0 || Tq > kMaxElems) return fail(DSA_EINVAL, "kv4_indexer: Tq=%lld", (long long)Tq);
-  if (span < 0 || span > cache->S) return fail(DSA_EINVAL, "kv4_indexer: span=%lld outside [0, S=%lld]", (long long)span, (long long)cache->S);
-  if (cache->B * Tq * span == 0) return DSA_OK;
-  if (cache->B * Tq >= (int64_t{1} << 23)) return fail(DSA_EINVAL, "kv4_indexer: B*Tq=%lld must be < 2^23", (long long)(cache->B * Tq));
-  if (!q_idx || !w_idx || !scores) return fail(DSA_EINVAL, "kv4_indexer: null pointer");
-  if (!aligned16(q_idx) || !aligned4(scores) || !aligned4(count)) return fail(DSA_EINVAL, "kv4_indexer: q_idx must be 16-byte aligned, scores and count 4-byte");
-  return hip_status(dsa::launch_kv4_indexer(kv4_of(cache), q_idx, w_idx, cache->idx_dtype, count, Tq, HI, span,
-                                            scores, static_cast<hipStream_t>(stream)),
-                    "dsa_kv4_indexer_scores");
+  return kv4_indexer(cache, q_idx, w_idx, cache ? cache->idx_dtype : DSA_F32, count, Tq, HI, span, scores, stream);
+}
+
+int dsa_kv4_indexer_scores_f32(const dsa_kv4_cache* cache, const float* q_idx, const float* w_idx,
+                               const int32_t* count, int64_t Tq, int HI, int64_t span, float* scores,
+                               void* stream) {
+  return kv4_indexer(cache, q_idx, w_idx, DSA_F32, count, Tq, HI, span, scores, stream);
 }
 
 int64_t dsa_kv4_attention_workspace_bytes(const dsa_kv4_cache* cache, int64_t Tq, int HQ, int listed,

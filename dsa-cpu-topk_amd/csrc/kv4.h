@@ -119,8 +119,9 @@ hipError_t launch_kv4_rows(const Kv4& c, const int32_t* slots, int64_t N, int dt
 hipError_t launch_kv4_evict(const Kv4& c, int64_t keep, int64_t recent, int32_t* src, int32_t* dst,
                             hipStream_t stream);
 
-// Indexer scores [B, Tq, span] (kv4_indexer.hip); dtype as the cache's index keys.
-hipError_t launch_kv4_indexer(const Kv4& c, const void* q, const void* w, int dtype,
+// Indexer scores [B, Tq, span] (kv4_indexer.hip); dtype (of q and w): key_dtype (the
+// cache's) or fp32.
+hipError_t launch_kv4_indexer(const Kv4& c, const void* q, const void* w, int dtype, int key_dtype,
                               const int32_t* count, int64_t Tq, int HI, int64_t span, float* scores,
                               hipStream_t stream);
 

@@ -11,11 +11,13 @@
 // and one sum over the four lane groups ends a slot.
 //
 // fp32 takes the fp32 matrix instruction (its 157 TFLOP/s are about what 64 heads
-// of 128 need at the memory's rate, fewer heads need less).
+// of 128 need at the memory's rate, fewer heads need less).  fp32 queries over 16-bit
+// keys take it too: the keys are read as they are and widened in registers, so that
+// no operand is rounded.
 //
 // Measured: 8 sequences of up to 32768 slots, 64 heads of 128, bf16 (62 MB): 14.9 us,
 // 4.1 TB/s; the loads alone 13.7.  Full ones in fp32: 8 heads of 64 14.7 us, 4.6 TB/s;
-// 64 heads of 128 46 us, bound by the matrix instruction.
+// 64 heads of 128 46 us, bound by the matrix instruction; over bf16 keys 11.5 and 47.
 #include "dsa_launch.h"
 #include "kv4.h"
 #include "tile_common.h"
@@ -50,10 +52,28 @@ __device__ __forceinline__ f32x4 mfma16(const u32x4& a, const u32x4& b, f32x4 ac
   }
 }
 
-template <typename Tag, int DI, int KB, bool IN_LDS>
+// Piece c of a lane's quarter of a key row, as the matrix instruction's type Tag.
+template <typename Tag, typename Key, int NK>
+__device__ __forceinline__ u32x4 key_piece(const u32x4 (&k)[NK], int c) {
+  if constexpr (__is_same(Tag, Key)) {
+    return k[c];
+  } else {
+    u32x4 x;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t w = k[c / 2][c % 2 * 2 + i / 2];
+      x[i] = __float_as_uint(to_f32(Key{}, static_cast<uint16_t>(i % 2 ? w >> 16 : w)));
+    }
+    return x;
+  }
+}
+
+// Tag: the type of q and w; Key: of the cached keys, the same or (Tag fp32) a 16-bit one.
+template <typename Tag, typename Key, int DI, int KB, bool IN_LDS>
 __global__ __launch_bounds__(kNT) void indexer_kernel(IndexArgs a) {
   using raw = typename Tag::raw;
   constexpr int ROW = DI * Tag::kBytes, NC = ROW / 64;  // bytes of a row, 16-byte pieces of a lane's quarter
+  constexpr int KROW = DI * Key::kBytes, NK = KROW / 64;  // of the keys
   extern __shared__ u32x4 lds[];
   const int nht = (a.HI + 15) / 16;
   const uint32_t bg = blockIdx.x / a.blocks, b = bg / a.groups;
@@ -68,16 +88,16 @@ __global__ __launch_bounds__(kNT) void indexer_kernel(IndexArgs a) {
   int64_t s = static_cast<int64_t>(blockIdx.x % a.blocks * kWaves + wave) * kTile;
   const bool busy = static_cast<int64_t>(blockIdx.x % a.blocks) * kWaves * kTile < end;  // one of the block's waves is
 
-  const char* keys = static_cast<const char*>(a.c.k_idx) + b * a.c.S * ROW;
-  auto load = [&](u32x4 (&k)[KB][NC], int64_t s0) {  // rows past the last visible one give zeros
-    const __amdgpu_buffer_rsrc_t r = rows_rsrc(keys, s0, limit, ROW);
+  const char* keys = static_cast<const char*>(a.c.k_idx) + b * a.c.S * KROW;
+  auto load = [&](u32x4 (&k)[KB][NK], int64_t s0) {  // rows past the last visible one give zeros
+    const __amdgpu_buffer_rsrc_t r = rows_rsrc(keys, s0, limit, KROW);
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-      for (int c = 0; c < NC; ++c)
-        k[kb][c] = __builtin_bit_cast(u32x4, buffer_load_f32x4(r, (16 * kb + r16) * ROW + g * (ROW / 4) + c * 16, 0, 0));
+      for (int c = 0; c < NK; ++c)
+        k[kb][c] = __builtin_bit_cast(u32x4, buffer_load_f32x4(r, (16 * kb + r16) * KROW + g * (KROW / 4) + c * 16, 0, 0));
   };
-  u32x4 k0[KB][NC], k1[KB][NC];
+  u32x4 k0[KB][NK], k1[KB][NK];
   if (s < end) load(k0, s);
 
   const char* q = static_cast<const char*>(a.q) + bt0 * a.HI * ROW;
@@ -99,7 +119,7 @@ __global__ __launch_bounds__(kNT) void indexer_kernel(IndexArgs a) {
   }
   __syncthreads();
 
-  auto compute = [&](const u32x4 (&k)[KB][NC], int64_t s0) {
+  auto compute = [&](const u32x4 (&k)[KB][NK], int64_t s0) {
     for (int t = 0; t < nt; ++t) {
       float sum[KB];
 #pragma unroll
@@ -112,7 +132,7 @@ __global__ __launch_bounds__(kNT) void indexer_kernel(IndexArgs a) {
         for (int c = 0; c < NC; ++c) {
           const u32x4 x = IN_LDS ? lds[((t * nht + ht) * NC + c) * 64 + lane] : piece(t, ht, c);
 #pragma unroll
-          for (int kb = 0; kb < KB; ++kb) acc[kb] = mfma16<Tag>(x, k[kb][c], acc[kb]);
+          for (int kb = 0; kb < KB; ++kb) acc[kb] = mfma16<Tag>(x, key_piece<Tag, Key>(k[kb], c), acc[kb]);
         }
         const float4 wv = *reinterpret_cast<const float4*>(weights + (t * nht + ht) * 16 + 4 * g);
         // Rows past HI are zeros, and 0 * Inf is NaN there: they stay out of the sum.
@@ -158,11 +178,11 @@ __global__ __launch_bounds__(kNT) void indexer_kernel(IndexArgs a) {
       if (lane < kTile && s + lane < a.span) a.scores[(bt0 + t) * a.span + s + lane] = -INFINITY;
 }
 
-template <typename Tag, int DI>
+template <typename Tag, typename Key, int DI>
 hipError_t launch_di(IndexArgs a, hipStream_t stream) {
-  constexpr int ROW = DI * Tag::kBytes;
+  constexpr int ROW = DI * Tag::kBytes, KROW = DI * Key::kBytes;
   // 32 registers of keys a stage, at most the 4 tiles that 4 lane groups store
-  constexpr int KB = ROW <= 128 ? 4 : ROW <= 256 ? 2 : 1;
+  constexpr int KB = KROW <= 128 ? 4 : KROW <= 256 ? 2 : 1;
   const int nht = (a.HI + 15) / 16;
   const int row_lds = nht * 16 * (ROW + 4);  // of one token
   a.per = a.Tq < kTokens ? a.Tq : kTokens;
@@ -178,29 +198,29 @@ hipError_t launch_di(IndexArgs a, hipStream_t stream) {
   a.blocks = static_cast<int>(blocks < 1 ? 1 : blocks > steps ? steps : blocks);
   const uint32_t grid = static_cast<uint32_t>(rows * a.blocks);
   if (in_lds)
-    indexer_kernel<Tag, DI, KB, true><<<grid, kNT, a.per * row_lds, stream>>>(a);
+    indexer_kernel<Tag, Key, DI, KB, true><<<grid, kNT, a.per * row_lds, stream>>>(a);
   else
-    indexer_kernel<Tag, DI, KB, false><<<grid, kNT, nht * 64, stream>>>(a);
+    indexer_kernel<Tag, Key, DI, KB, false><<<grid, kNT, nht * 64, stream>>>(a);
   return hipGetLastError();
 }
 
-template <typename Tag>
+template <typename Tag, typename Key>
 hipError_t launch_tag(const IndexArgs& a, hipStream_t stream) {
   switch (a.c.DI) {
     case 16:
-      if constexpr (Tag::kBytes == 4) return launch_di<Tag, 16>(a, stream);
+      if constexpr (Key::kBytes == 4) return launch_di<Tag, Key, 16>(a, stream);
       return hipErrorNotSupported;
-    case 32: return launch_di<Tag, 32>(a, stream);
-    case 64: return launch_di<Tag, 64>(a, stream);
-    case 128: return launch_di<Tag, 128>(a, stream);
-    default: return launch_di<Tag, 256>(a, stream);
+    case 32: return launch_di<Tag, Key, 32>(a, stream);
+    case 64: return launch_di<Tag, Key, 64>(a, stream);
+    case 128: return launch_di<Tag, Key, 128>(a, stream);
+    default: return launch_di<Tag, Key, 256>(a, stream);
   }
 }
 
 }  // namespace
 
-hipError_t launch_kv4_indexer(const Kv4& c, const void* q, const void* w, int dtype, const int32_t* count,
-                              int64_t Tq, int HI, int64_t span, float* scores, hipStream_t stream) {
+hipError_t launch_kv4_indexer(const Kv4& c, const void* q, const void* w, int dtype, int key_dtype,
+                              const int32_t* count, int64_t Tq, int HI, int64_t span, float* scores, hipStream_t stream) {
   IndexArgs a;
   a.c = c;
   a.q = q;
@@ -210,7 +230,10 @@ hipError_t launch_kv4_indexer(const Kv4& c, const void* q, const void* w, int dt
   a.HI = HI;
   a.span = span;
   a.scores = scores;
-  return dtype == 0 ? launch_tag<F32>(a, stream) : dtype == 1 ? launch_tag<BF16>(a, stream) : launch_tag<F16>(a, stream);
+  if (dtype != key_dtype) return key_dtype == 1 ? launch_tag<F32, BF16>(a, stream) : launch_tag<F32, F16>(a, stream);
+  return dtype == 0   ? launch_tag<F32, F32>(a, stream)
+         : dtype == 1 ? launch_tag<BF16, BF16>(a, stream)
+                      : launch_tag<F16, F16>(a, stream);
 }
 
 }  // namespace dsa

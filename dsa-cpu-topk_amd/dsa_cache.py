@@ -119,7 +119,7 @@ class KV4Cache:
     @classmethod
     def empty(cls, B: int, S: int, HKV: int, DK: int, DV: int, DI: int = 0,
               idx_dtype: torch.dtype = torch.bfloat16, device="cuda") -> "KV4Cache":
-        """A cache with nothing in it (DI = 0: without index keys)."""
+        """A cache with nothing in it (DI = 0: without index keys, which are held in idx_dtype)."""
         assert DK > 0 and DV > 0 and DK % 32 == 0 and DV % 32 == 0, \
             f"DK={DK} DV={DV} must be multiples of 32"
         dev = torch.device(device)
@@ -217,7 +217,8 @@ def kv4_append(cache: KV4Cache, K: torch.Tensor, V: torch.Tensor, k_idx: torch.T
     """Quantise T new tokens a sequence into the cache's next slots.
 
     K [B,T,HKV,DK], V [B,T,HKV,DV] (fp32, bf16 or fp16), k_idx [B,T,DI] where the
-    cache holds index keys.  count int32 [B]: how many of the T are tokens (a
+    cache holds index keys, stored in the type of its buffer (idx_dtype: other types
+    are rounded to it, past fp16's range to Inf).  count int32 [B]: how many of the T are tokens (a
     padded batch; default all).  weight fp32 [B,T]: the new slots' first weights,
     e.g. what a prompt's own attention gave them (default 0).  restart: the
     sequences begin anew, at slot 0 and position 0 (a new batch of prompts).
@@ -274,19 +275,22 @@ def kv4_indexer_scores(cache: KV4Cache, q_idx: torch.Tensor, w_idx: torch.Tensor
     keys: [B,Tq,span] fp32, -inf where a token does not see the slot (its own and
     the earlier slots it sees, the later tokens' it does not).
 
-    q_idx [B,Tq,HI,DI], w_idx [B,Tq,HI].  span: only the first span slots (default
+    q_idx [B,Tq,HI,DI], w_idx [B,Tq,HI].  Types other than the cached keys' (or each
+    other's) go as fp32: nothing is rounded to the keys' type.  span: only the first span slots (default
     all S).  count int32 [B]: how many of the Tq are tokens, as kv4_append's; the
     others' rows are -inf."""
     B, Tq, HI, _ = _index_queries(cache, q_idx, w_idx)
     n = _span(cache, span)
-    qw, (q_ptr, w_ptr) = _ready(cache.idx_dtype, cache, q_idx, w_idx)
+    dt, fn = cache.idx_dtype, L.lib().dsa_kv4_indexer_scores
+    if q_idx.dtype is not dt or w_idx.dtype is not dt:
+        dt, fn = torch.float32, L.lib().dsa_kv4_indexer_scores_f32
+    qw, (q_ptr, w_ptr) = _ready(dt, cache, q_idx, w_idx)
     count_ptr = None
     if count is not None:
         count = _ints(count, (B,), "count", cache)
         count_ptr = count.data_ptr()
     scores = torch.empty((B, Tq, n), device=cache.device, dtype=torch.float32)
-    _call(cache, "kv4_indexer_scores", L.lib().dsa_kv4_indexer_scores, q_ptr, w_ptr, count_ptr, Tq,
-          HI, n, scores.data_ptr())
+    _call(cache, "kv4_indexer_scores", fn, q_ptr, w_ptr, count_ptr, Tq, HI, n, scores.data_ptr())
     return scores
 
 

@@ -490,13 +490,17 @@ int dsa_kv4_rows(const dsa_kv4_cache* cache, const int32_t* slots, int64_t N, in
  * (null: Tq) of the Tq queries are tokens, those from n on see nothing.
  * scores [B,Tq,span] fp32: the first span slots.  fp32 sums.
  *   q_idx [B,Tq,HI,DI] (16-byte aligned), w_idx [B,Tq,HI], of the cache's
- *   idx_dtype; 1 <= HI <= 256; span <= S; B*Tq < 2^23.
+ *   idx_dtype (_f32: of fp32, whatever the cache's; no operand is rounded);
+ *   1 <= HI <= 256; span <= S; B*Tq < 2^23.
  * Replaces: nothing (the reference's indexer, lightning_indexer.py:54-125, is
  *   the square [B,T,T]).
  */
 int dsa_kv4_indexer_scores(const dsa_kv4_cache* cache, const void* q_idx, const void* w_idx,
                            const int32_t* count, int64_t Tq, int HI, int64_t span, float* scores,
                            void* stream);
+int dsa_kv4_indexer_scores_f32(const dsa_kv4_cache* cache, const float* q_idx, const float* w_idx,
+                               const int32_t* count, int64_t Tq, int HI, int64_t span, float* scores,
+                               void* stream);
 
 /*
  * Attention of each sequence's last Tq tokens over the cache:

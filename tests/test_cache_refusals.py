@@ -1,0 +1,21 @@
+"""CPU: what else the 4-bit cache's C entries refuse before any HIP call."""
+from __future__ import annotations
+
+import pytest
+
+import _dsa_lib as L
+from test_cache_host import CALLS, FAKE, cache, call, put
+
+
+@pytest.mark.parametrize("changes, needle", [
+    (dict(_0=None), "null"), (dict(_0=FAKE + 8), "aligned"), (dict(_1=None), "null"), (dict(_3=-1), "Tq"),
+    (dict(_4=0), "HI"), (dict(_4=257), "HI"), (dict(_5=65), "span"), (dict(_6=None), "null"),
+])
+def test_fp32_indexer_refusals(changes, needle):
+    name, args = "dsa_kv4_indexer_scores_f32", CALLS["dsa_kv4_indexer_scores"]
+    rc, msg = call(name, cache(), *put(args, **changes))
+    assert rc == L.DSA_EINVAL and needle in msg, (rc, msg)
+    assert call(name, None, *args)[0] == L.DSA_EINVAL
+    assert call(name, cache(DI=16), *args)[0] == L.DSA_EUNSUPPORTED  # 16 bits have no kernel of 16
+    assert call(name, cache(k_idx=None), *args)[0] == L.DSA_EINVAL
+    assert call(name, cache(), *put(args, _3=0))[0] == L.DSA_OK

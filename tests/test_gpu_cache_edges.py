@@ -6,9 +6,10 @@ import math
 import pytest
 import torch
 
+import cache_oracle as C
 import dsa_cache as D
 from helpers import say
-from test_gpu_cache import BF16, F16, F32, gen, ints, randn
+from test_gpu_cache import BF16, F16, F32, filled, gen, ints, randn, within
 
 pytestmark = pytest.mark.gpu
 
@@ -36,3 +37,31 @@ def test_infinite_index_keys(dev, dtype, HI, DI):
     assert got[0, 1, 69].item() == -inf and got[0, 0, 69].item() == -inf  # the second token sees it, the first does not
     keep = [s for s in range(S - 1) if s not in (5, 6, 7)]
     assert torch.equal(got[..., keep], clean[..., keep])
+
+
+@pytest.mark.parametrize("cached", [BF16, F16])
+@pytest.mark.parametrize("q_dtype, w_dtype", [(F32, F32), (None, F32), (F32, None), (BF16, F16), (torch.float64, F32)])
+@pytest.mark.parametrize("HI, DI, Tq", [(4, 32, 1), (17, 64, 3), (64, 128, 2), (9, 256, 1), (250, 128, 1)])
+def test_mixed_types_of_the_indexer(dev, cached, q_dtype, w_dtype, HI, DI, Tq):
+    """Queries and weights of another type than the cached keys' lose none of their bits:
+    mixed types go as fp32 (None: the cache's own)."""
+    q_dtype, w_dtype = q_dtype or cached, w_dtype or cached
+    say("mixed", cached, q_dtype, w_dtype, HI, DI, Tq)
+    lengths, S = [333, 40, 1, 0], 333
+    cache = filled(dev, 4, S, 1, 32, 32, lengths, 1, DI, cached)
+    g = gen(dev, HI)
+    q, w = randn(g, 4, Tq, HI, DI, dtype=q_dtype), randn(g, 4, Tq, HI, dtype=w_dtype)
+    if q_dtype is F32:
+        q[0] *= 1e5  # past fp16's range
+    for kw in ({}, dict(count=ints(dev, [Tq, 1, 0, 1]), span=300)):
+        want, lim = C.indexer(torch.nan_to_num(cache.k_idx), cache.length, q.float(), w.float(), **kw)
+        within(D.kv4_indexer_scores(cache, q, w, **kw), want, lim, "scores")
+
+
+def test_infinite_keys_and_mixed_types(dev):
+    g, S, HI = gen(dev, 1), 40, 12
+    q, w, k = randn(g, 1, 1, HI, 64).abs() + 0.5, randn(g, 1, 1, HI).abs(), randn(g, 1, S, 64, dtype=BF16)
+    k[0, 3, 9], k[0, 4, 9], k[0, 5, 63] = math.inf, -math.inf, math.nan
+    got = D.kv4_indexer_scores(D.KV4Cache(None, None, ints(dev, [S]), k), q, w)[0, 0]
+    assert got[3].item() == math.inf and got[4].item() == 0.0 and torch.isnan(got[5])
+    assert torch.isfinite(got[6:]).all()
