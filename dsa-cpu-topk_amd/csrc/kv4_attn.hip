@@ -52,6 +52,7 @@ constexpr int kWaves = kNT / kWave;
 constexpr int kTile = 32;                  // slots a wave takes at once
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kSlack = 8.0f;             // how far a logit may pass the running maximum, in powers of 2
+constexpr float kNoSum = -1.0f;            // a split's sum of exponentials where it has no slots
 
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 
@@ -324,7 +325,7 @@ __global__ __launch_bounds__(kNT, resident(NP, DK, DV, SIDE)) void attn_kernel(A
   if (j_first >= j_end) {  // nothing here: no sum, and no sums to read
     for (int e = threadIdx.x; e < a.heads * rows; e += kNT) {
       const int64_t h = head_of(hk0 + e / rows, rt * 16 + e % rows);
-      if (a.ml) a.ml[h * a.splits + split] = make_float2(-INFINITY, 0.0f);
+      if (a.ml) a.ml[h * a.splits + split] = make_float2(-INFINITY, kNoSum);
       if (a.splits == 1)
         for (int d = 0; d < DV; ++d) a.out[h * DV + d] = __builtin_nanf("");
     }
@@ -598,6 +599,7 @@ __global__ __launch_bounds__(kNT, resident(NP, DK, DV, SIDE)) void attn_kernel(A
 }
 
 // One query head's maximum (0 where it is -inf) and sum over its splits, by 8 or 64 lanes.
+// (A split without slots adds kNoSum * 2^-inf.)
 template <int LANES>
 __device__ __forceinline__ float2 join_ml(const float2* ml, int splits) {
   float top = -INFINITY, total = 0.0f;
@@ -640,7 +642,7 @@ __global__ __launch_bounds__(kNT) void finish_kernel(AttnArgs a, int64_t joins, 
     const float2 all = join_ml<64>(ml, a.splits);
     for (int s = threadIdx.x; s < a.splits; s += kNT) {
       const float2 x = ml[s];
-      factor[s] = x.y == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(x.x - all.x);
+      factor[s] = x.y == kNoSum ? kNoSum : __builtin_amdgcn_exp2f(x.x - all.x);
     }
     __syncthreads();
     // groups of threads take the splits in turn, a thread 4 columns
@@ -650,7 +652,7 @@ __global__ __launch_bounds__(kNT) void finish_kernel(AttnArgs a, int64_t joins, 
 #pragma unroll 4
     for (int s = group; s < a.splits && group < groups; s += groups) {
       const float f = factor[s];
-      if (f == 0.0f) continue;  // a block without a sum has left none
+      if (f == kNoSum) continue;  // such a block has left none; a factor of 0 keeps a NaN one
       const float4 v = *reinterpret_cast<const float4*>(part + static_cast<int64_t>(s) * a.c.DV);
       x.x += f * v.x; x.y += f * v.y; x.z += f * v.z; x.w += f * v.w;
     }

@@ -65,3 +65,27 @@ def test_infinite_keys_and_mixed_types(dev):
     got = D.kv4_indexer_scores(D.KV4Cache(None, None, ints(dev, [S]), k), q, w)[0, 0]
     assert got[3].item() == math.inf and got[4].item() == 0.0 and torch.isnan(got[5])
     assert torch.isfinite(got[6:]).all()
+
+
+# --- attention ---------------------------------------------------------------------------------------
+@pytest.mark.parametrize("HQ", [1, 16])
+@pytest.mark.parametrize("low", [-2048.0, -2.0 ** 100])
+@pytest.mark.parametrize("listed", [False, True])
+def test_nan_value_beside_a_far_larger_logit(dev, HQ, low, listed):
+    """A visible slot's NaN value is NaN in the output however small its probability
+    (0 * NaN), also where blocks share a long cache and its block's sums weigh nothing."""
+    S, D_ = 5000, 64
+    say("far below", HQ, low, listed)
+    K, V = torch.zeros(1, S, 1, D_, device=dev), torch.ones(1, S, 1, D_, device=dev)
+    K[..., 0] = low
+    K[0, 7] = 0
+    V[0, 4000, 0, 3] = math.nan  # the first 32 columns
+    cache = D.KV4Cache.empty(1, S, 1, D_, D_, device=dev)
+    D.kv4_append(cache, K, V)
+    Q = torch.zeros(1, 1, HQ, D_, device=dev)
+    Q[..., 0] = 8.0 if low > -1e6 else 2.0 ** 100
+    slots = torch.arange(S, device=dev, dtype=torch.int32).flip(0).expand(1, 1, S) if listed else None
+    out = D.kv4_attention(cache, Q, slots=slots)
+    assert torch.isnan(out[..., :32]).all() and bool((out[..., 32:] == 1).all())
+    cache.length.fill_(4000)  # the NaN is behind the last slot
+    assert bool((D.kv4_attention(cache, Q, slots=slots) == 1).all())
