@@ -82,6 +82,7 @@ _SIGNATURES = {
     "dsa_kv4_attention_workspace_bytes": ([_P, _I64, _I, _I, _I64, _I], _I64),
     "dsa_kv4_attention": ([_P, _P, _I, _P, _P, _I64, _I, _I64, _I, _F, _P, _P, _I64, _P], _I),
     "dsa_kv4_evict": ([_P, _I64, _I64, _P, _P, _P], _I),
+    "dsa_kv4_make_room": ([_P, _P, _I64, _I64, _P, _P, _P], _I),
 }
 
 

@@ -639,4 +639,17 @@ int dsa_kv4_evict(const dsa_kv4_cache* cache, int64_t keep, int64_t recent, int3
                     "dsa_kv4_evict");
 }
 
+int dsa_kv4_make_room(const dsa_kv4_cache* cache, const int32_t* count, int64_t T, int64_t recent,
+                      int32_t* src, int32_t* dst, void* stream) {
+  int rc = check_kv4(cache, true, false, "kv4_make_room");
+  if (rc != DSA_OK) return rc;
+  if (T < 0 || T > cache->S || recent < 0)
+    return fail(DSA_EINVAL, "kv4_make_room: T=%lld outside [0, S=%lld] or recent=%lld negative", (long long)T, (long long)cache->S, (long long)recent);
+  if (cache->B == 0 || T == 0) return DSA_OK;
+  if (!src || !dst) return fail(DSA_EINVAL, "kv4_make_room: null pointer");
+  if (!aligned4(src) || !aligned4(dst) || !aligned4(count)) return fail(DSA_EINVAL, "kv4_make_room: src, dst and count must be 4-byte aligned");
+  return hip_status(dsa::launch_kv4_make_room(kv4_of(cache), count, T, recent, src, dst, static_cast<hipStream_t>(stream)),
+                    "dsa_kv4_make_room");
+}
+
 }  // extern "C"

@@ -118,6 +118,9 @@ hipError_t launch_kv4_rows(const Kv4& c, const int32_t* slots, int64_t N, int dt
 // Down to `keep` slots a sequence; src, dst [B, M], M = min(keep, S - keep).
 hipError_t launch_kv4_evict(const Kv4& c, int64_t keep, int64_t recent, int32_t* src, int32_t* dst,
                             hipStream_t stream);
+// Down to S - count[b] (null: T) slots; src, dst [B, T].
+hipError_t launch_kv4_make_room(const Kv4& c, const int32_t* count, int64_t T, int64_t recent, int32_t* src,
+                                int32_t* dst, hipStream_t stream);
 
 // Indexer scores [B, Tq, span] (kv4_indexer.hip); dtype (of q and w): key_dtype (the
 // cache's) or fp32.

@@ -214,10 +214,12 @@ __device__ __forceinline__ uint32_t evict_scan(uint32_t v, uint32_t* wsum, uint3
   return block_exclusive_sum<kET>(v, wsum, total);
 }
 
+// What stays of a sequence: `keep` slots, or (room) as many as leave count[b] (or
+// null: `keep`) of the S free.
 template <int VPT>
-__global__ __launch_bounds__(kET) void evict_select_kernel(Kv4 c, int64_t keep, int64_t recent,
-                                                           int64_t M, int32_t* __restrict__ src,
-                                                           int32_t* __restrict__ dst) {
+__global__ __launch_bounds__(kET) void evict_select_kernel(Kv4 c, int64_t keep, int64_t recent, bool room,
+                                                           const int32_t* __restrict__ count, int64_t M,
+                                                           int32_t* __restrict__ src, int32_t* __restrict__ dst) {
   __shared__ uint32_t hist[kBins];
   __shared__ uint32_t wsum[kET / kWave], wlo[kET / kWave], whi[kET / kWave];
   __shared__ uint32_t pick[3];
@@ -254,6 +256,7 @@ __global__ __launch_bounds__(kET) void evict_select_kernel(Kv4 c, int64_t keep, 
     for (int i = 0; i < VPT; ++i) key[i] = p[i] >= first_kept ? kProtected : float_to_key(w[i]);
   };
   read(0);  // on its way together with the length
+  if (room) keep = c.S - (count ? max(static_cast<int64_t>(0), min(static_cast<int64_t>(count[b]), keep)) : keep);
   if (n <= keep) {
     for (int64_t i = threadIdx.x; i < M; i += kET) src[i] = dst[i] = -1;
     return;
@@ -423,18 +426,33 @@ hipError_t launch_kv4_rows(const Kv4& c, const int32_t* slots, int64_t N, int dt
   return hipGetLastError();
 }
 
-hipError_t launch_kv4_evict(const Kv4& c, int64_t keep, int64_t recent, int32_t* src, int32_t* dst,
-                            hipStream_t stream) {
-  if (keep >= c.S) return hipSuccess;
-  const int64_t M = keep < c.S - keep ? keep : c.S - keep;
+namespace {
+
+hipError_t launch_evict(const Kv4& c, int64_t keep, int64_t recent, bool room, const int32_t* count,
+                        int64_t M, int32_t* src, int32_t* dst, hipStream_t stream) {
   const uint32_t grid = static_cast<uint32_t>(c.B);
-  if (c.S <= 4 * kET) evict_select_kernel<4><<<grid, kET, 0, stream>>>(c, keep, recent, M, src, dst);
-  else evict_select_kernel<16><<<grid, kET, 0, stream>>>(c, keep, recent, M, src, dst);
+  if (c.S <= 4 * kET) evict_select_kernel<4><<<grid, kET, 0, stream>>>(c, keep, recent, room, count, M, src, dst);
+  else evict_select_kernel<16><<<grid, kET, 0, stream>>>(c, keep, recent, room, count, M, src, dst);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || M <= kInPlace) return e;
   const int rows = kNT / kWave;
   evict_move_kernel<<<dim3(static_cast<uint32_t>((M + rows - 1) / rows), static_cast<uint32_t>(c.B)), kNT, 0, stream>>>(c, M, src, dst);
   return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_kv4_evict(const Kv4& c, int64_t keep, int64_t recent, int32_t* src, int32_t* dst,
+                            hipStream_t stream) {
+  if (keep >= c.S) return hipSuccess;
+  return launch_evict(c, keep, recent, false, nullptr, keep < c.S - keep ? keep : c.S - keep, src, dst, stream);
+}
+
+// No more slots move than are freed, T at most.
+hipError_t launch_kv4_make_room(const Kv4& c, const int32_t* count, int64_t T, int64_t recent, int32_t* src,
+                                int32_t* dst, hipStream_t stream) {
+  if (T == 0) return hipSuccess;
+  return launch_evict(c, T, recent, true, count, T, src, dst, stream);
 }
 
 }  // namespace dsa

@@ -211,18 +211,8 @@ def _call(cache: KV4Cache, what: str, fn, *args) -> None:
         L.check(rc, what)
 
 
-def kv4_append(cache: KV4Cache, K: torch.Tensor, V: torch.Tensor, k_idx: torch.Tensor | None = None,
-               *, count: torch.Tensor | None = None, weight: torch.Tensor | None = None,
-               restart: bool = False) -> None:
-    """Quantise T new tokens a sequence into the cache's next slots.
-
-    K [B,T,HKV,DK], V [B,T,HKV,DV] (fp32, bf16 or fp16), k_idx [B,T,DI] where the
-    cache holds index keys, stored in the type of its buffer (idx_dtype: other types
-    are rounded to it, past fp16's range to Inf).  count int32 [B]: how many of the T are tokens (a
-    padded batch; default all).  weight fp32 [B,T]: the new slots' first weights,
-    e.g. what a prompt's own attention gave them (default 0).  restart: the
-    sequences begin anew, at slot 0 and position 0 (a new batch of prompts).
-    Tokens past slot S - 1 are not stored but counted in cache.lost."""
+def _append_args(cache: KV4Cache, K, V, k_idx, count, weight):
+    """dsa_kv4_append's arguments up to T, and what they point into."""
     _stored(cache)
     B, T = K.shape[:2]
     assert K.shape == (cache.B, T, cache.HKV, cache.DK), \
@@ -242,8 +232,23 @@ def kv4_append(cache: KV4Cache, K: torch.Tensor, V: torch.Tensor, k_idx: torch.T
     if count is not None:
         count = _ints(count, (B,), "count", cache)
         count_ptr = count.data_ptr()
-    _call(cache, "kv4_append", L.lib().dsa_kv4_append, k_ptr, v_ptr, L.dtype_code(dt), idx_ptr,
-          weight_ptr, count_ptr, T, 1 if restart else 0)
+    return (k_ptr, v_ptr, L.dtype_code(dt), idx_ptr, weight_ptr, count_ptr, T), (kv, k_idx, weight, count)
+
+
+def kv4_append(cache: KV4Cache, K: torch.Tensor, V: torch.Tensor, k_idx: torch.Tensor | None = None,
+               *, count: torch.Tensor | None = None, weight: torch.Tensor | None = None,
+               restart: bool = False) -> None:
+    """Quantise T new tokens a sequence into the cache's next slots.
+
+    K [B,T,HKV,DK], V [B,T,HKV,DV] (fp32, bf16 or fp16), k_idx [B,T,DI] where the
+    cache holds index keys, stored in the type of its buffer (idx_dtype: other types
+    are rounded to it, past fp16's range to Inf).  count int32 [B]: how many of the T are tokens (a
+    padded batch; default all).  weight fp32 [B,T]: the new slots' first weights,
+    e.g. what a prompt's own attention gave them (default 0).  restart: the
+    sequences begin anew, at slot 0 and position 0 (a new batch of prompts).
+    Tokens past slot S - 1 are not stored but counted in cache.lost."""
+    args, held = _append_args(cache, K, V, k_idx, count, weight)
+    _call(cache, "kv4_append", L.lib().dsa_kv4_append, *args, 1 if restart else 0)
 
 
 def kv4_rows(cache: KV4Cache, slots: torch.Tensor | None = None, *, span: int | None = None,
@@ -352,6 +357,13 @@ def kv4_evict(cache: KV4Cache, keep: int, recent: int = 0):
     return moved.unbind(0)
 
 
+def _make_room(cache: KV4Cache, count_ptr: int | None, Tq: int, recent: int) -> None:
+    """Evict what leaves no room for the next append: down to S - count[b] (default S - Tq)."""
+    moved = torch.empty((2, cache.B, Tq), device=cache.device, dtype=torch.int32)
+    src = moved.data_ptr()
+    _call(cache, "kv4_make_room", L.lib().dsa_kv4_make_room, count_ptr, Tq, recent, src, src + 4 * cache.B * Tq)
+
+
 def dsa_decode(cache: KV4Cache, q_idx, k_idx, w_idx, Q, K, V, top_k: int, *,
                span: int | None = None, count: torch.Tensor | None = None,
                keep: int | None = None, recent: int = 0) -> torch.Tensor:
@@ -363,8 +375,9 @@ def dsa_decode(cache: KV4Cache, q_idx, k_idx, w_idx, Q, K, V, top_k: int, *,
     K [B,Tq,HKV,DK]  V [B,Tq,HKV,DV].  Exactly top_k slots a token (the lowest
     slot wins ties), all it sees where it sees fewer.  span: no sequence has more
     slots than that in use (default S); where top_k >= span all of them are
-    attended to and nothing is scored.  The cache needs room for the Tq tokens
-    (keep + Tq <= S is checked; without keep, cache.check() says whether some were lost)."""
+    attended to and nothing is scored.  With keep (keep + Tq <= S) a sequence that has
+    no room for its new tokens, after a prompt, is evicted down to it before the append;
+    without, the caller sees to the room and cache.check() says whether tokens were lost."""
     assert top_k >= 1, "top_k must be >= 1"
     n = _span(cache, span)
     # what the later calls would refuse, before the first one changes the cache
@@ -378,7 +391,10 @@ def dsa_decode(cache: KV4Cache, q_idx, k_idx, w_idx, Q, K, V, top_k: int, *,
         assert keep + Tq <= cache.S, f"keep={keep} slots and {Tq} new tokens do not fit S={cache.S}"
     _workspace_bytes(cache, Tq, HQ, listed, int(top_k) if listed else n, 0 if keep is None else 1)
     with L.on_device(cache.device):
-        kv4_append(cache, K, V, k_idx, count=count)
+        args, held = _append_args(cache, K, V, k_idx, count, None)
+        if keep is not None:
+            _make_room(cache, args[5], Tq, int(recent))
+        _call(cache, "kv4_append", L.lib().dsa_kv4_append, *args, 0)
         slots = None
         if listed:
             scores = kv4_indexer_scores(cache, q_idx, w_idx, span=n, count=count)

@@ -544,6 +544,14 @@ int dsa_kv4_attention(const dsa_kv4_cache* cache, const void* Q, int dtype, cons
 int dsa_kv4_evict(const dsa_kv4_cache* cache, int64_t keep, int64_t recent, int32_t* src,
                   int32_t* dst, void* stream);
 
+/*
+ * Room for the next append: the same for every sequence that has more than
+ * S - count[b] slots (count null: S - T; values outside [0, T] count as the nearer
+ * end), down to as many; the others stay as they are.  src, dst [B, T], 0 <= T <= S.
+ */
+int dsa_kv4_make_room(const dsa_kv4_cache* cache, const int32_t* count, int64_t T, int64_t recent,
+                      int32_t* src, int32_t* dst, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

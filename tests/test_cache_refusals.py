@@ -19,3 +19,18 @@ def test_fp32_indexer_refusals(changes, needle):
     assert call(name, cache(DI=16), *args)[0] == L.DSA_EUNSUPPORTED  # 16 bits have no kernel of 16
     assert call(name, cache(k_idx=None), *args)[0] == L.DSA_EINVAL
     assert call(name, cache(), *put(args, _3=0))[0] == L.DSA_OK
+
+
+ROOM = (None, 4, 2, FAKE, FAKE, None)
+
+
+@pytest.mark.parametrize("changes", [dict(_1=-1), dict(_1=65), dict(_2=-1), dict(_3=None), dict(_4=None),
+                                     dict(_3=FAKE + 2), dict(_4=FAKE + 1), dict(_0=FAKE + 2)])
+def test_make_room_refusals(changes):
+    name = "dsa_kv4_make_room"
+    rc, msg = call(name, cache(), *put(ROOM, **changes))
+    assert rc == L.DSA_EINVAL and msg, (rc, msg)
+    assert call(name, None, *ROOM)[0] == L.DSA_EINVAL
+    assert call(name, cache(codes=None), *ROOM)[0] == L.DSA_EINVAL
+    assert call(name, cache(), *put(ROOM, _1=0))[0] == L.DSA_OK
+    assert call(name, cache(B=0), *ROOM)[0] == L.DSA_OK

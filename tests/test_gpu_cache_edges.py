@@ -6,10 +6,12 @@ import math
 import pytest
 import torch
 
+import _dsa_lib as L
 import cache_oracle as C
 import dsa_cache as D
 from helpers import say
-from test_gpu_cache import BF16, F16, F32, filled, gen, ints, randn, within
+from test_gpu_cache import BF16, F16, F32, filled, gen, ints, randn, same, step_inputs, within
+from topk_threshold import topk_indices
 
 pytestmark = pytest.mark.gpu
 
@@ -89,3 +91,116 @@ def test_nan_value_beside_a_far_larger_logit(dev, HQ, low, listed):
     assert torch.isnan(out[..., :32]).all() and bool((out[..., 32:] == 1).all())
     cache.length.fill_(4000)  # the NaN is behind the last slot
     assert bool((D.kv4_attention(cache, Q, slots=slots) == 1).all())
+
+
+# --- the step ----------------------------------------------------------------------------------------
+NAMES = ("codes", "scales", "length", "k_idx", "position", "weight", "seen", "lost")
+
+
+def copy_of(c):
+    return D.KV4Cache(*(getattr(c, n).clone() for n in NAMES[:4]),
+                      **{n: getattr(c, n).clone() for n in NAMES[4:]}, DK=c.DK)
+
+
+@pytest.mark.parametrize("S, length, Tq, keep, recent", [
+    (10, 10, 1, 6, 2), (10, 9, 2, 6, 0), (10, 10, 2, 8, 8), (300, 300, 3, 100, 7), (300, 298, 3, 297, 0),
+    (400, 390, 70, 200, 20), (20000, 19999, 2, 17000, 64),
+])
+def test_step_of_a_full_cache(dev, S, length, Tq, keep, recent):
+    """A prompt that left no room: the step first evicts down to it, so that every new
+    token is stored and sees itself."""
+    say("full", S, length, Tq, keep)
+    g = gen(dev, S + Tq)
+    cache = filled(dev, 1, S, 2, 64, 64, [length], S, 32)
+    apart = copy_of(cache)
+    x = step_inputs(g, 1, Tq, 4, 32, 4, 2, 64, 64, BF16)
+    k = min(8, S - 1)
+    out = D.dsa_decode(cache, *x, top_k=k, keep=keep, recent=recent)
+    D.kv4_evict(apart, S - Tq, recent)
+    D.kv4_append(apart, x[4], x[5], x[1])
+    assert int(apart.length) == S and not int(apart.lost)
+    _, slots = topk_indices(D.kv4_indexer_scores(apart, x[0], x[2]), k)
+    want = D.kv4_attention(apart, x[3], slots=slots, accumulate=True)
+    D.kv4_evict(apart, keep, recent)
+    assert same(out, want)
+    for n in NAMES:
+        assert same(getattr(cache, n), getattr(apart, n)), n
+    cache.check()
+
+
+@pytest.mark.parametrize("S, Tq", [(40, 3), (40, 40), (500, 100), (17000, 2)])
+def test_room_is_made_by_sequence(dev, S, Tq):
+    """Each sequence down to S - its own tokens; those with room stay as they are, and so
+    does what no kept slot moves into."""
+    lengths = [S, S - 1, S - Tq, S - Tq + 1 if Tq > 1 else S, S, 0, S]
+    counts = [Tq, 1, Tq, Tq, 0, Tq, Tq + 9]
+    for count in (counts, None):
+        cache = filled(dev, 7, S, 2, 32, 32, lengths, S + Tq, 32)
+        moved = torch.empty(2, 7, Tq, device=dev, dtype=torch.int32)
+        names = ("codes", "scales", "k_idx", "position", "weight")
+        before = {n: getattr(cache, n).clone() for n in names}
+        want = []
+        for b in range(7):
+            one = slice(b, b + 1)
+            room = S - (Tq if count is None else min(count[b], Tq))
+            want += C.evict(cache.length[one].cpu(), cache.seen[one].cpu(), cache.position[one].cpu(),
+                            cache.weight[one].cpu(), room, 2)
+        n = ints(dev, count) if count else None
+        L.check(L.lib().dsa_kv4_make_room(cache._ref, n.data_ptr() if count else None, Tq, 2, moved[0].data_ptr(),
+                                          moved[1].data_ptr(), L.stream_ptr(dev)), "room")
+        for b, (src, dst, length) in enumerate(want):
+            assert moved[0, b].tolist() == src + [-1] * (Tq - len(src)), b
+            assert moved[1, b].tolist() == dst + [-1] * (Tq - len(dst)), b
+            assert int(cache.length[b]) == length
+            for x in before.values():
+                if src:
+                    x[b, torch.tensor(dst, device=dev)] = x[b, torch.tensor(src, device=dev)].clone()
+        for name, x in before.items():
+            assert same(getattr(cache, name), x), name
+
+
+def test_steps_of_a_padded_full_batch(dev):
+    """Room is made for a sequence's own tokens alone, and a captured step makes it too."""
+    g, S, lengths = gen(dev, 90), 60, [60, 59, 60, 20]
+    args = (3, 4, 32, 4, 2, 64, 64, BF16)
+    caches = [filled(dev, 4, S, 2, 64, 64, lengths, 91, 32) for _ in range(2)]
+    x, count = step_inputs(g, 4, *args), ints(dev, [3, 1, 0, 2])
+    kw = dict(top_k=9, count=count, keep=57, recent=3)
+    warm = filled(dev, 4, S, 2, 64, 64, lengths, 91, 32)
+    D.dsa_decode(warm, *x, **kw)
+    assert not warm.lost.any() and warm.seen.tolist() == [63, 60, 60, 22] and warm.length.tolist() == [57, 57, 57, 22]
+    for b, n in enumerate([3, 1, 0, 2]):  # the newest tokens are there
+        assert set(range(lengths[b], lengths[b] + n)) <= set(warm.position[b, :int(warm.length[b])].tolist())
+    torch.cuda.synchronize()
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        out = D.dsa_decode(caches[0], *x, **kw)
+    for i in range(6):
+        for t, new in zip(x, step_inputs(g, 4, *args)):
+            t.copy_(new)
+        if i == 3:  # full again
+            for c in caches:
+                c.length.fill_(S)
+        gr.replay()
+        got = out.clone()
+        torch.randn(500, 500, device=dev).sum()
+        want = D.dsa_decode(caches[1], *x, **kw)
+        torch.cuda.synchronize()
+        assert same(torch.nan_to_num(got), torch.nan_to_num(want)), i
+        for n in NAMES:
+            assert same(getattr(caches[0], n), getattr(caches[1], n)), (i, n)
+    caches[1].check()
+
+
+def test_refused_steps_of_a_full_cache_make_no_room(dev):
+    """What the append refuses is refused before room is made for it."""
+    g = gen(dev, 95)
+    cache = filled(dev, 2, 40, 2, 64, 64, [40, 39], 96, 32)
+    before = [getattr(cache, n).clone() for n in NAMES]
+    q, ki, w, Q, K, V = step_inputs(g, 2, 2, 4, 32, 4, 2, 64, 64, BF16)
+    for args, kw in [((q, None, w, Q, K, V, 8), {}), ((q, ki[..., :16], w, Q, K, V, 8), {}),
+                     ((q, ki, w, Q, K, V[:, :1], 8), {}), ((q, ki, w, Q, K[..., :32], V, 8), {}),
+                     ((q, ki, w, Q, K, V, 8), dict(count=torch.ones(2, device=dev)))]:
+        with pytest.raises(AssertionError):
+            D.dsa_decode(cache, *args, keep=30, **kw)
+    assert all(same(getattr(cache, n), old) for n, old in zip(NAMES, before))
