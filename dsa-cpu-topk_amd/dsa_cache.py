@@ -148,11 +148,15 @@ def _ints(x: torch.Tensor, shape, name: str, cache: KV4Cache) -> torch.Tensor:
     return x if x.is_contiguous() else x.contiguous()
 
 
-def _ready(dtype: torch.dtype, cache: KV4Cache, *xs: torch.Tensor):
-    """`xs` as the kernels take them (L.prep) and their pointers."""
+def _here(cache: KV4Cache, *xs: torch.Tensor) -> None:
     for x in xs:
         assert x.get_device() == cache.index, \
             f"inputs must be on the cache's GPU {cache.device} (got {x.device})"
+
+
+def _ready(dtype: torch.dtype, cache: KV4Cache, *xs: torch.Tensor):
+    """`xs` as the kernels take them (L.prep) and their pointers."""
+    _here(cache, *xs)
     ptrs = L.ready_ptrs(dtype, xs)
     if ptrs is None:
         xs = [L.prep(x, dtype) for x in xs]
@@ -384,8 +388,10 @@ def dsa_decode(cache: KV4Cache, q_idx, k_idx, w_idx, Q, K, V, top_k: int, *,
     B, Tq, HQ, _ = _queries(cache, Q)
     assert K.shape[:2] == (B, Tq), f"K shape {tuple(K.shape)}: {Tq} tokens in Q"
     listed = top_k < n
+    _here(cache, Q)
     if listed:
         assert _index_queries(cache, q_idx, w_idx)[1] == Tq, f"q_idx shape {tuple(q_idx.shape)}: {Tq} tokens in Q"
+        _here(cache, q_idx, w_idx)
     if keep is not None:
         assert 0 <= recent <= keep, f"keep={keep} recent={recent} must be 0 <= recent <= keep"
         assert keep + Tq <= cache.S, f"keep={keep} slots and {Tq} new tokens do not fit S={cache.S}"

@@ -204,3 +204,25 @@ def test_refused_steps_of_a_full_cache_make_no_room(dev):
         with pytest.raises(AssertionError):
             D.dsa_decode(cache, *args, keep=30, **kw)
     assert all(same(getattr(cache, n), old) for n, old in zip(NAMES, before))
+
+
+def test_steps_refused_for_a_device_or_for_room_change_nothing(dev):
+    g = gen(dev, 92)
+    cache = filled(dev, 2, 40, 2, 64, 64, [20, 4], 93, 32)
+    before = [getattr(cache, n).clone() for n in NAMES]
+    x = step_inputs(g, 2, 1, 4, 32, 4, 2, 64, 64, BF16)
+    for i in range(6):
+        bad = [t.cpu() if j == i else t for j, t in enumerate(x)]
+        with pytest.raises(AssertionError, match="cache's GPU"):
+            D.dsa_decode(cache, *bad, 8)
+    with pytest.raises(AssertionError, match="cache's GPU"):
+        D.kv4_attention(cache, x[3].cpu())
+    with pytest.raises(AssertionError, match="cache's GPU"):
+        D.kv4_indexer_scores(cache, x[0], x[2].cpu())
+    with pytest.raises(AssertionError, match="count"):
+        D.dsa_decode(cache, *x, 8, count=torch.ones(2, dtype=torch.int32))
+    with pytest.raises(AssertionError, match="do not fit"):
+        D.dsa_decode(cache, *x, 8, keep=40)
+    assert all(same(getattr(cache, n), old) for n, old in zip(NAMES, before))
+    D.dsa_decode(cache, *x, 8, keep=39)
+    assert cache.length.tolist() == [21, 5]
