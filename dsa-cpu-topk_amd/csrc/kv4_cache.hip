@@ -16,7 +16,7 @@ constexpr int kNT = 256;
 // How a block's threads cover its tokens: a thread owns word u of a slot (8
 // elements of one head's K or V) for every `step`-th of the block's tokens, so
 // that the head and the source's stride are worked out once, and small slots
-// still take all threads.  words is a multiple of 8, so the 4 lanes of a
+// still take all threads.  words is a multiple of 4, so the 4 lanes of a
 // 32-element block stay 4 neighbours.
 struct Cover {
   int u, first, step;  // past the slot's words: nothing to do
@@ -167,24 +167,23 @@ __global__ __launch_bounds__(kNT) void rows_kernel(Kv4 c, const int32_t* __restr
   }
 }
 
-// Copies `bytes` bytes with the wave.  Rows of a multiple of 16 bytes start at one
-// too; the others are scales, few bytes and an odd number for some DK + DV.
+// Copies `bytes` bytes, a multiple of Unit's, with the wave.
+template <typename Unit>
 __device__ __forceinline__ void wave_copy(uint8_t* dst, const uint8_t* src, int bytes) {
-  const int lane = threadIdx.x & (kWave - 1);
-  if (bytes % 16 == 0) {
-    for (int i = lane; i < bytes / 16; i += kWave)
-      reinterpret_cast<uint4*>(dst)[i] = reinterpret_cast<const uint4*>(src)[i];
-  } else {
-    for (int i = lane; i < bytes; i += kWave) dst[i] = src[i];
-  }
+  const int n = bytes / static_cast<int>(sizeof(Unit));
+  for (int i = threadIdx.x & (kWave - 1); i < n; i += kWave)
+    reinterpret_cast<Unit*>(dst)[i] = reinterpret_cast<const Unit*>(src)[i];
 }
 
 // Slot u's token into slot v, by a wave.
 __device__ __forceinline__ void wave_move(const Kv4& c, int64_t u, int64_t v) {
   const int cb = c.words() * 4, sb = c.scale_bytes(), ib = c.DI * c.idx_bytes;
-  wave_copy(c.codes + v * cb, c.codes + u * cb, cb);
-  wave_copy(c.scales + v * sb, c.scales + u * sb, sb);
-  if (c.k_idx) wave_copy(static_cast<uint8_t*>(c.k_idx) + v * ib, static_cast<uint8_t*>(c.k_idx) + u * ib, ib);
+  // codes and index keys are 16-byte aligned, in rows of multiples of it; scales are
+  // 4-byte aligned, few bytes and an odd number for some DK + DV
+  wave_copy<uint4>(c.codes + v * cb, c.codes + u * cb, cb);
+  if (sb % 4 == 0) wave_copy<uint32_t>(c.scales + v * sb, c.scales + u * sb, sb);
+  else wave_copy<uint8_t>(c.scales + v * sb, c.scales + u * sb, sb);
+  if (c.k_idx) wave_copy<uint4>(static_cast<uint8_t*>(c.k_idx) + v * ib, static_cast<uint8_t*>(c.k_idx) + u * ib, ib);
   if ((threadIdx.x & (kWave - 1)) == 0) {
     c.position[v] = c.position[u];
     c.weight[v] = c.weight[u];

@@ -226,3 +226,21 @@ def test_steps_refused_for_a_device_or_for_room_change_nothing(dev):
     assert all(same(getattr(cache, n), old) for n, old in zip(NAMES, before))
     D.dsa_decode(cache, *x, 8, keep=39)
     assert cache.length.tolist() == [21, 5]
+
+
+@pytest.mark.parametrize("keep", [40, 390])  # moves by a launch of their own, and by the selecting block
+def test_scales_at_any_multiple_of_four_bytes(dev, keep):
+    """The C entries take scales that are 4-byte aligned, also where a slot's are 16 bytes."""
+    S = 400
+    cache = filled(dev, 2, S, 4, 64, 64, [S, S - 7], 94, 32)
+    room = torch.zeros(cache.scales.numel() + 16, device=dev, dtype=torch.uint8)
+    for shift in (4, 8, 12):
+        apart = copy_of(cache)
+        moved = room[shift:shift + cache.scales.numel()]
+        moved.copy_(cache.scales.flatten())
+        c = copy_of(cache)
+        D.kv4_evict(apart, keep, 5)
+        out = torch.empty(2, 2, min(keep, S - keep), device=dev, dtype=torch.int32)
+        c._c.scales = moved.data_ptr()
+        L.check(L.lib().dsa_kv4_evict(c._ref, keep, 5, out[0].data_ptr(), out[1].data_ptr(), L.stream_ptr(dev)), "evict")
+        assert same(moved, apart.scales.flatten()) and same(c.codes, apart.codes), shift
