@@ -175,7 +175,7 @@ int kv4_indexer(const dsa_kv4_cache* cache, const void* q_idx, const void* w_idx
   if (HI < 1 || HI > 256) return fail(DSA_EINVAL, "kv4_indexer: HI=%d outside [1,256]", HI);
   if (Tq < 0 || Tq > kMaxElems) return fail(DSA_EINVAL, "kv4_indexer: Tq=%lld", (long long)Tq);
   if (span < 0 || span > cache->S) return fail(DSA_EINVAL, "kv4_indexer: span=%lld outside [0, S=%lld]", (long long)span, (long long)cache->S);
-  if (cache->B * Tq * span == 0) return DSA_OK;
+  if (cache->B == 0 || Tq == 0 || span == 0) return DSA_OK;
   if (cache->B * Tq >= (int64_t{1} << 23)) return fail(DSA_EINVAL, "kv4_indexer: B*Tq=%lld must be < 2^23", (long long)(cache->B * Tq));
   if (!q_idx || !w_idx || !scores) return fail(DSA_EINVAL, "kv4_indexer: null pointer");
   if (!aligned16(q_idx) || !aligned4(scores) || !aligned4(count)) return fail(DSA_EINVAL, "kv4_indexer: q_idx must be 16-byte aligned, scores and count 4-byte");

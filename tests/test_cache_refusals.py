@@ -34,3 +34,13 @@ def test_make_room_refusals(changes):
     assert call(name, cache(codes=None), *ROOM)[0] == L.DSA_EINVAL
     assert call(name, cache(), *put(ROOM, _1=0))[0] == L.DSA_OK
     assert call(name, cache(B=0), *ROOM)[0] == L.DSA_OK
+
+
+@pytest.mark.parametrize("name", ["dsa_kv4_indexer_scores", "dsa_kv4_indexer_scores_f32"])
+@pytest.mark.parametrize("B, Tq, span", [(16, 1 << 30, 1 << 30), (1 << 15, 1 << 30, 1 << 19), (1, 1 << 23, 64)])
+def test_sizes_of_the_indexer_whose_product_overflows(name, B, Tq, span):
+    """B * Tq * span is 2^64 in the first two."""
+    c = cache(B=B, S=1 << 30, codes=None)
+    rc, msg = call(name, c, *put(CALLS["dsa_kv4_indexer_scores"], _3=Tq, _5=span))
+    assert rc == L.DSA_EINVAL and "2^23" in msg, (rc, msg)
+    assert call(name, c, *put(CALLS["dsa_kv4_indexer_scores"], _3=Tq, _5=0))[0] == L.DSA_OK
