@@ -559,7 +559,8 @@ int dsa_kv4_append(const dsa_kv4_cache* cache, const void* K, const void* V, int
   int rc = check_kv4(cache, true, false, "kv4_append");
   if (rc != DSA_OK) return rc;
   if (!dtype_ok(dtype)) return fail(DSA_EINVAL, "kv4_append: unknown dtype %d", dtype);
-  if (T < 0 || T >= (int64_t{1} << 25)) return fail(DSA_EINVAL, "kv4_append: T=%lld outside [0, 2^25)", (long long)T);
+  // two tokens a block of 256 threads, and a launch holds fewer than 2^32
+  if (T < 0 || T >= (int64_t{1} << 25) - 1) return fail(DSA_EINVAL, "kv4_append: T=%lld outside [0, 2^25 - 1)", (long long)T);
   if ((k_idx != nullptr) != (cache->k_idx != nullptr) && cache->B * T != 0)
     return fail(DSA_EINVAL, "kv4_append: index keys go with a cache that holds them");
   // with T = 0 there is nothing to do but a restart's counters

@@ -468,7 +468,7 @@ typedef struct dsa_kv4_cache {
  *   K [B,T,HKV,DK], V [B,T,HKV,DV] of dtype (fp32, bf16, fp16); k_idx [B,T,DI] of
  *   the cache's idx_dtype, null exactly where the cache holds none; weight [B,T]
  *   fp32, the new slots' first weights (null: 0).  16-byte aligned (weight and
- *   count 4).  T < 2^25.
+ *   count 4).  T < 2^25 - 1.
  */
 int dsa_kv4_append(const dsa_kv4_cache* cache, const void* K, const void* V, int dtype,
                    const void* k_idx, const float* weight, const int32_t* count, int64_t T,

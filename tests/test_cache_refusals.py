@@ -44,3 +44,9 @@ def test_sizes_of_the_indexer_whose_product_overflows(name, B, Tq, span):
     rc, msg = call(name, c, *put(CALLS["dsa_kv4_indexer_scores"], _3=Tq, _5=span))
     assert rc == L.DSA_EINVAL and "2^23" in msg, (rc, msg)
     assert call(name, c, *put(CALLS["dsa_kv4_indexer_scores"], _3=Tq, _5=0))[0] == L.DSA_OK
+
+
+def test_append_of_more_blocks_than_a_launch_holds():
+    """Two tokens a block of 256 threads: 2^25 - 1 of them are 2^32 threads."""
+    rc, msg = call("dsa_kv4_append", cache(), *put(CALLS["dsa_kv4_append"], _6=(1 << 25) - 1))
+    assert rc == L.DSA_EINVAL and "T=" in msg, (rc, msg)
