@@ -10,7 +10,7 @@ import _dsa_lib as L
 import cache_oracle as C
 import dsa_cache as D
 from helpers import say
-from test_gpu_cache import BF16, F16, F32, filled, gen, ints, randn, same, step_inputs, within
+from test_gpu_cache import BF16, F16, F32, attend, check_evict, filled, gen, ints, randn, same, step_inputs, within
 from topk_threshold import topk_indices
 
 pytestmark = pytest.mark.gpu
@@ -244,3 +244,45 @@ def test_scales_at_any_multiple_of_four_bytes(dev, keep):
         c._c.scales = moved.data_ptr()
         L.check(L.lib().dsa_kv4_evict(c._ref, keep, 5, out[0].data_ptr(), out[1].data_ptr(), L.stream_ptr(dev)), "evict")
         assert same(moved, apart.scales.flatten()) and same(c.codes, apart.codes), shift
+
+
+# --- sizes -------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("HQ, HKV, D_, Tq, listed", [(1024, 1024, 32, 1, 0), (1024, 1, 64, 1, 0), (1024, 4, 32, 3, 0),
+                                                     (1024, 2, 32, 1, 90), (1023, 341, 64, 2, 50)])
+def test_attention_of_the_most_heads(dev, HQ, HKV, D_, Tq, listed):
+    say("most heads", HQ, HKV, D_, Tq, listed)
+    g = gen(dev, HQ + HKV)
+    cache = filled(dev, 2, 70, HKV, D_, D_, [70, 33], 97)
+    slots = torch.randint(-2, 72, (2, Tq, listed), generator=g, device=dev, dtype=torch.int32) if listed else None
+    attend(cache, randn(g, 2, Tq, HQ, D_, dtype=BF16), "out", slots=slots)
+
+
+def test_steps_of_nothing_and_of_one_slot(dev):
+    """No sequences, no tokens, and a cache whose one slot each step takes over."""
+    g = gen(dev, 98)
+    none = D.KV4Cache.empty(0, 8, 2, 64, 64, 32, device=dev)
+    assert D.dsa_decode(none, *step_inputs(g, 0, 1, 4, 32, 4, 2, 64, 64, BF16), 4, keep=7).shape == (0, 1, 4, 64)
+    cache = filled(dev, 2, 20, 2, 64, 64, [20, 4], 99, 32)
+    assert D.dsa_decode(cache, *step_inputs(g, 2, 0, 4, 32, 4, 2, 64, 64, BF16), 4, keep=20).shape == (2, 0, 4, 64)
+    assert cache.length.tolist() == [20, 4] and not cache.lost.any()
+    one = D.KV4Cache.empty(2, 1, 2, 64, 64, 32, device=dev)
+    x = step_inputs(g, 2, 1, 4, 32, 4, 2, 64, 64, BF16)
+    D.kv4_append(one, x[4], x[5], x[1])
+    for i in range(3):
+        x = step_inputs(g, 2, 1, 4, 32, 4, 2, 64, 64, BF16)
+        out = D.dsa_decode(one, *x, 1, keep=0)
+        V = C.decode(*C.quantise(x[5])).repeat_interleave(2, 2)
+        assert torch.equal(out.double(), V)  # p = 1
+        assert one.length.tolist() == [0, 0] and one.seen.tolist() == [i + 2] * 2 and not one.lost.any()
+
+
+@pytest.mark.parametrize("S, T", [(300, 200)])
+def test_rows_of_the_widest_heads(dev, S, T):
+    """DK and DV up to 1024, which append, rows and eviction take."""
+    g = gen(dev, 100)
+    cache = D.KV4Cache.empty(2, S, 3, 1024, 32, device=dev)
+    K, V = randn(g, 2, T, 3, 1024, dtype=BF16), randn(g, 2, T, 3, 32, dtype=BF16)
+    D.kv4_append(cache, K, V, weight=torch.rand(2, T, generator=g, device=dev))
+    k, v = D.kv4_rows(cache, span=T)
+    assert torch.equal(k.double(), C.decode(*C.quantise(K))) and torch.equal(v.double(), C.decode(*C.quantise(V)))
+    check_evict(cache, 90, 7, "wide")
