@@ -44,7 +44,8 @@ class KV4Cache:
     accumulated by kv4_attention.  Made from buffers in use, what is not given
     starts as after an append of `length` tokens.  A cache of index keys alone
     (codes None) serves kv4_indexer_scores.  The calls go by the buffers' addresses:
-    write into a buffer (cache.length.copy_(...)), it cannot be replaced."""
+    write into a buffer (cache.length.copy_(...), and seen with it where tokens are
+    taken back), it cannot be replaced."""
 
     _BUFFERS = ("codes", "scales", "k_idx", "length", "seen", "lost", "position", "weight")
 

@@ -429,7 +429,8 @@ int64_t dsa_fused_max_T(void);
  * The keys and values of B sequences, S slots each, in OCP MXFP4: e2m1 codes
  * (0, 1/2, 1, 3/2, 2, 3, 4, 6 with a sign; the even element of a pair in the
  * low nibble) and one E8M0 scale byte, 2^(byte-127), per 32 elements of a head's
- * row.  A slot holds one token; the slots in use are 0 .. length-1, in no
+ * row: 2 .. 252, so that the values are normal fp32 numbers, or 255, NaN (append
+ * writes no others; what the calls make of others is not defined).  A slot holds one token; the slots in use are 0 .. length-1, in no
  * particular order of positions once something was evicted.  The buffers are
  * device memory of the caller's, dense row-major, in this struct on the host,
  * which is read before the call returns.  A call that writes the cache and any
@@ -459,7 +460,8 @@ typedef struct dsa_kv4_cache {
  * Append: token i of sequence b goes into slot length[b] + i, for i < count[b]
  * (count null: T).  With restart != 0 the sequences begin anew, at slot 0 and
  * position 0.  Then length, seen and lost are brought up to date; tokens past
- * slot S - 1 are counted in lost and not stored.  Slots behind the last token
+ * slot S - 1 are counted in lost and not stored: their queries would count other
+ * slots as their own (dsa_kv4_make_room evicts what leaves no room).  Slots behind the last token
  * keep what they hold.
  *   A block of 32 elements gets the least scale 2^e with max|x| < 7 * 2^e (so no
  * element is off by more than half of the widest step, 2^e), 2^-125 <= 2^e <=
@@ -514,7 +516,8 @@ int dsa_kv4_indexer_scores_f32(const dsa_kv4_cache* cache, const float* q_idx, c
  * result in every run (over listed slots that takes a launch for each of the Tq
  * tokens).
  *   fp32 logits, softmax and sums; fp32 operands enter the matrix instructions
- * whole, as bf16 pieces.
+ * whole, as bf16 pieces.  The sums are divided last: exponentials go up to 2^8, so
+ * that 2^8 n max|V| must stay below fp32's range.
  *   Q [B,Tq,HQ,DK] of dtype (fp32, bf16, fp16), out [B,Tq,HQ,DV] fp32, 16-byte
  *   aligned; HQ a multiple of HKV, at most 1024; without slots n <= S;
  *   B*Tq*HQ < 2^23; B*n < 2^31; DK = DV in {32, 64, 96, 128, 192, 256} or DK 192 with DV 128
