@@ -83,6 +83,13 @@ _SIGNATURES = {
     "dsa_kv4_attention": ([_P, _P, _I, _P, _P, _I64, _I, _I64, _I, _F, _P, _P, _I64, _P], _I),
     "dsa_kv4_evict": ([_P, _I64, _I64, _P, _P, _P], _I),
     "dsa_kv4_make_room": ([_P, _P, _I64, _I64, _P, _P, _P], _I),
+    "dsa_window_attention": ([_P, _P, _P, _I, _P, _I64, _I64, _I, _I, _I, _I64, _I64, _I64, _I64, _I64,
+                              _F, _P, _P], _I),
+    "dsa_kv8_append": ([_P, _P, _P, _P, _I, _I64, _I, _I64, _I64, _I64, _P, _P, _I64, _I, _I, _P, _P,
+                        _P, _P, _P], _I),
+    "dsa_kv8_rows": ([_P, _P, _I64, _I, _P, _P, _P], _I),
+    "dsa_kv8_attention_workspace_bytes": ([_P, _I64, _I, _I64, _I64, _I64], _I64),
+    "dsa_kv8_attention": ([_P, _P, _I, _P, _I64, _I, _I64, _I64, _I64, _F, _P, _P, _I64, _P], _I),
 }
 
 
@@ -92,6 +99,13 @@ class Kv4Cache(ctypes.Structure):
     _fields_ = [(n, _P) for n in ("codes", "scales", "k_idx", "length", "seen", "lost", "position",
                                   "weight")] \
         + [("B", _I64), ("S", _I64)] + [(n, _I) for n in ("HKV", "DK", "DV", "DI", "idx_dtype")]
+
+
+class Kv8Cache(ctypes.Structure):
+    """dsa_kv8_cache: the buffers and sizes of a paged 8-bit cache."""
+
+    _fields_ = [(n, _P) for n in ("codes", "scales", "pages", "length", "lost")] \
+        + [(n, _I64) for n in ("B", "NP", "max_pages")] + [(n, _I) for n in ("HKV", "DK", "DV", "page")]
 
 
 _CPU_SIGNATURES = {

@@ -11,6 +11,7 @@
 #include "../../include/dsa_amd.h"
 #include "dsa_launch.h"
 #include "kv4.h"
+#include "kv8.h"
 
 namespace {
 
@@ -165,6 +166,58 @@ int check_kv4_attention(const dsa_kv4_cache* c, int64_t Tq, int HQ, bool listed,
   if (!dsa::kv4_attn_supported(c->DK, c->DV))
     return fail(DSA_EUNSUPPORTED, "%s: no kernel for DK=%d DV=%d (equal ones of 32, 64, 96, 128, 192, 256, or 192 with 128)", who, c->DK, c->DV);
   return DSA_OK;
+}
+
+// The paged 8-bit cache.
+int check_kv8(const dsa_kv8_cache* c, const char* who) {
+  if (!c) return fail(DSA_EINVAL, "%s: null cache", who);
+  if (c->B < 0 || c->B > 65535) return fail(DSA_EINVAL, "%s: B=%lld outside [0, 65535]", who, (long long)c->B);
+  if (c->NP < 1 || c->max_pages < 1 || c->NP > kMaxElems || c->max_pages > kMaxElems)
+    return fail(DSA_EINVAL, "%s: NP=%lld max_pages=%lld outside [1, 2^31)", who, (long long)c->NP, (long long)c->max_pages);
+  if (c->page < 64 || c->page > 65536 || !pow2(c->page)) return fail(DSA_EINVAL, "%s: page=%d must be 64 * 2^j, at most 65536", who, c->page);
+  if (c->max_pages * c->page > kMaxElems - 255)
+    return fail(DSA_EINVAL, "%s: max_pages*page = %lld slots must be at most 2^31 - 256", who, (long long)(c->max_pages * c->page));
+  if (c->HKV < 1 || c->HKV > 1024) return fail(DSA_EINVAL, "%s: HKV=%d outside [1,1024]", who, c->HKV);
+  if (!dsa::kv8_supported(c->DK, c->DV))
+    return fail(DSA_EUNSUPPORTED, "%s: no kernel for DK=%d DV=%d (equal ones of 32, 64, 96, 128, 192, 256, or 192 with 128)", who, c->DK, c->DV);
+  if (c->B == 0) return DSA_OK;
+  if (!c->codes || !c->scales || !c->pages || !c->length || !c->lost) return fail(DSA_EINVAL, "%s: null cache buffer", who);
+  if (!aligned16(c->codes) || (reinterpret_cast<uintptr_t>(c->scales) & 1u)) return fail(DSA_EINVAL, "%s: codes must be 16-byte aligned, scales 2-byte", who);
+  if (!aligned4(c->pages) || !aligned4(c->length) || !aligned4(c->lost)) return fail(DSA_EINVAL, "%s: pages, length and lost must be 4-byte aligned", who);
+  return DSA_OK;
+}
+
+dsa::Kv8 kv8_of(const dsa_kv8_cache* c) {
+  dsa::Kv8 k;
+  k.codes = c->codes;
+  k.scales = c->scales;
+  k.pages = c->pages;
+  k.length = c->length;
+  k.lost = c->lost;
+  k.B = c->B;
+  k.NP = c->NP;
+  k.max_pages = c->max_pages;
+  k.HKV = c->HKV;
+  k.DK = c->DK;
+  k.DV = c->DV;
+  k.page_shift = __builtin_ctz(static_cast<unsigned>(c->page)) - 6;
+  return k;
+}
+
+int check_kv8_attention(const dsa_kv8_cache* c, int64_t Tq, int HQ, int64_t n, int64_t window, int64_t sinks, const char* who) {
+  const int rc = check_kv8(c, who);
+  if (rc != DSA_OK) return rc;
+  if (HQ < 1 || HQ > 1024 || HQ % c->HKV) return fail(DSA_EINVAL, "%s: HQ=%d must be a multiple of HKV=%d, at most 1024", who, HQ, c->HKV);
+  if (Tq < 0 || Tq > kMaxElems || c->B * Tq * HQ >= (int64_t{1} << 23)) return fail(DSA_EINVAL, "%s: Tq=%lld: B*Tq*HQ must be < 2^23", who, (long long)Tq);
+  if (n < 0 || n > c->max_pages * c->page) return fail(DSA_EINVAL, "%s: n=%lld outside [0, %lld]", who, (long long)n, (long long)(c->max_pages * c->page));
+  if (window < 0 || sinks < 0) return fail(DSA_EINVAL, "%s: window=%lld sinks=%lld must not be negative", who, (long long)window, (long long)sinks);
+  return DSA_OK;
+}
+
+// Consecutive tokens `ld` elements apart, each of `row` elements.
+bool stride_ok(int64_t ld, int64_t row, int dtype) {
+  const int64_t bytes = dtype == DSA_F32 ? 4 : 2;
+  return ld >= row && ld <= (int64_t{1} << 24) && ld * bytes % 16 == 0;
 }
 
 // dtype: of q_idx and w_idx, the cache's idx_dtype or fp32.
@@ -651,6 +704,130 @@ int dsa_kv4_make_room(const dsa_kv4_cache* cache, const int32_t* count, int64_t 
   if (!aligned4(src) || !aligned4(dst) || !aligned4(count)) return fail(DSA_EINVAL, "kv4_make_room: src, dst and count must be 4-byte aligned");
   return hip_status(dsa::launch_kv4_make_room(kv4_of(cache), count, T, recent, src, dst, static_cast<hipStream_t>(stream)),
                     "dsa_kv4_make_room");
+}
+
+int dsa_window_attention(const void* Q, const void* K, const void* V, int dtype, const int32_t* count,
+                         int64_t B, int64_t T, int HQ, int HKV, int D, int64_t ldq, int64_t ldk,
+                         int64_t ldv, int64_t window, int64_t sinks, float scale, void* out,
+                         void* stream) {
+  if (!dtype_ok(dtype)) return fail(DSA_EINVAL, "window_attention: unknown dtype %d", dtype);
+  if (B < 0 || T < 0 || T > kMaxElems - 256 || B > kMaxElems) return fail(DSA_EINVAL, "window_attention: B=%lld T=%lld", (long long)B, (long long)T);
+  if (HKV < 1 || HQ < 1 || HQ > 1024 || HQ % HKV) return fail(DSA_EINVAL, "window_attention: HQ=%d must be a multiple of HKV=%d, at most 1024", HQ, HKV);
+  if (!dsa::window_attn_supported(D)) return fail(DSA_EUNSUPPORTED, "window_attention: no kernel for D=%d (32, 64, 128, 256)", D);
+  if (window < 1 || sinks < 0) return fail(DSA_EINVAL, "window_attention: window=%lld must be >= 1 and sinks=%lld >= 0", (long long)window, (long long)sinks);
+  if (!std::isfinite(scale)) return fail(DSA_EINVAL, "window_attention: scale must be finite");
+  if (!stride_ok(ldq, static_cast<int64_t>(HQ) * D, dtype) || !stride_ok(ldk, static_cast<int64_t>(HKV) * D, dtype) ||
+      !stride_ok(ldv, static_cast<int64_t>(HKV) * D, dtype))
+    return fail(DSA_EINVAL, "window_attention: strides %lld %lld %lld must hold a token's heads, be multiples of 16 bytes and at most 2^24", (long long)ldq, (long long)ldk, (long long)ldv);
+  // a launch holds 2^32 threads of 256 a block, the batch's heads filled up to 8
+  if ((B + 7) * HQ * ((T + 63) / 64) >= (int64_t{1} << 24)) return fail(DSA_EINVAL, "window_attention: (B+7)*HQ*ceil(T/64) must be < 2^24");
+  if (B * T == 0) return DSA_OK;
+  if (!Q || !K || !V || !out) return fail(DSA_EINVAL, "window_attention: null pointer");
+  if (!aligned16(Q) || !aligned16(K) || !aligned16(V) || !aligned16(out) || !aligned4(count))
+    return fail(DSA_EINVAL, "window_attention: Q, K, V and out must be 16-byte aligned, count 4-byte");
+  dsa::WindowArgs a;
+  a.Q = Q;
+  a.K = K;
+  a.V = V;
+  a.out = out;
+  a.count = count;
+  a.B = B;
+  a.ldq = ldq;
+  a.ldk = ldk;
+  a.ldv = ldv;
+  a.T = static_cast<int>(T);
+  a.HQ = HQ;
+  a.HKV = HKV;
+  a.D = D;
+  a.window = static_cast<int>(window < T ? window : T);
+  a.sinks = static_cast<int>(sinks < T ? sinks : T);
+  a.scale = scale;
+  return hip_status(dsa::launch_window_attn(a, dtype, static_cast<hipStream_t>(stream)), "dsa_window_attention");
+}
+
+int dsa_kv8_append(const dsa_kv8_cache* cache, const void* K, const void* V, const void* Q, int dtype,
+                   int64_t T, int HQ, int64_t ldk, int64_t ldv, int64_t ldq, const float* cos,
+                   const float* sin, int64_t table_rows, int R, int pairs, const int32_t* start,
+                   const int32_t* count, void* K_out, void* Q_out, void* stream) {
+  const int rc = check_kv8(cache, "kv8_append");
+  if (rc != DSA_OK) return rc;
+  if (!dtype_ok(dtype)) return fail(DSA_EINVAL, "kv8_append: unknown dtype %d", dtype);
+  if (T < 0 || T > kMaxElems || cache->B * cache->HKV * (T / 64 + 2) >= (int64_t{1} << 23))
+    return fail(DSA_EINVAL, "kv8_append: T=%lld: B*HKV*(T/64 + 2) must be < 2^23", (long long)T);
+  if ((Q == nullptr) != (Q_out == nullptr) && cache->B * T > 0) return fail(DSA_EINVAL, "kv8_append: Q goes with Q_out");
+  if (R < 0 || R > cache->DK || R % 16) return fail(DSA_EINVAL, "kv8_append: R=%d must be a multiple of 16, at most DK=%d", R, cache->DK);
+  if (R > 0 && table_rows < cache->max_pages * cache->page)
+    return fail(DSA_EINVAL, "kv8_append: the tables' %lld rows must cover the %lld slots", (long long)table_rows, (long long)(cache->max_pages * cache->page));
+  if (!stride_ok(ldk, static_cast<int64_t>(cache->HKV) * cache->DK, dtype) || !stride_ok(ldv, static_cast<int64_t>(cache->HKV) * cache->DV, dtype))
+    return fail(DSA_EINVAL, "kv8_append: strides %lld %lld must hold a token's heads, be multiples of 16 bytes and at most 2^24", (long long)ldk, (long long)ldv);
+  if (Q) {
+    if (HQ < 1 || HQ > 1024) return fail(DSA_EINVAL, "kv8_append: HQ=%d outside [1,1024]", HQ);
+    if (!stride_ok(ldq, static_cast<int64_t>(HQ) * cache->DK, dtype))
+      return fail(DSA_EINVAL, "kv8_append: stride %lld of Q must hold a token's heads, be a multiple of 16 bytes and at most 2^24", (long long)ldq);
+    if (cache->B * T * HQ * (cache->DK / 8) > kMaxElems) return fail(DSA_EINVAL, "kv8_append: B*T*HQ*DK/8 must be < 2^31");
+  }
+  if (cache->B == 0) return DSA_OK;
+  if (T > 0 && (!K || !V || (R > 0 && (!cos || !sin)))) return fail(DSA_EINVAL, "kv8_append: null pointer");
+  if (!aligned16(K) || !aligned16(V) || !aligned16(Q) || !aligned16(cos) || !aligned16(sin) || !aligned16(K_out) || !aligned16(Q_out))
+    return fail(DSA_EINVAL, "kv8_append: K, V, Q, the tables and the outputs must be 16-byte aligned");
+  if (!aligned4(start) || !aligned4(count)) return fail(DSA_EINVAL, "kv8_append: start and count must be 4-byte aligned");
+  dsa::Kv8Append a;
+  a.K = K;
+  a.V = V;
+  a.Q = Q;
+  a.K_out = K_out;
+  a.Q_out = Q_out;
+  a.ldk = ldk;
+  a.ldv = ldv;
+  a.ldq = ldq;
+  a.cos = cos;
+  a.sin = sin;
+  a.start = start;
+  a.count = count;
+  a.T = T;
+  a.HQ = HQ;
+  a.R = R;
+  a.pairs = pairs;
+  return hip_status(dsa::launch_kv8_append(kv8_of(cache), a, dtype, static_cast<hipStream_t>(stream)), "dsa_kv8_append");
+}
+
+int dsa_kv8_rows(const dsa_kv8_cache* cache, const int32_t* slots, int64_t N, int dtype, void* K, void* V,
+                 void* stream) {
+  const int rc = check_kv8(cache, "kv8_rows");
+  if (rc != DSA_OK) return rc;
+  if (!dtype_ok(dtype)) return fail(DSA_EINVAL, "kv8_rows: unknown dtype %d", dtype);
+  if (N < 0 || N > kMaxElems || cache->B * N > kMaxElems || cache->B * N * cache->HKV * ((cache->DK + cache->DV) / 8) > kMaxElems)
+    return fail(DSA_EINVAL, "kv8_rows: N=%lld: B*N*HKV*(DK+DV)/8 must be < 2^31", (long long)N);
+  if (cache->B == 0 || N == 0) return DSA_OK;
+  if (!K || !V) return fail(DSA_EINVAL, "kv8_rows: null pointer");
+  if (!aligned16(K) || !aligned16(V) || !aligned4(slots)) return fail(DSA_EINVAL, "kv8_rows: K and V must be 16-byte aligned, slots 4-byte");
+  return hip_status(dsa::launch_kv8_rows(kv8_of(cache), slots, N, dtype, K, V, static_cast<hipStream_t>(stream)), "dsa_kv8_rows");
+}
+
+int64_t dsa_kv8_attention_workspace_bytes(const dsa_kv8_cache* cache, int64_t Tq, int HQ, int64_t n,
+                                          int64_t window, int64_t sinks) {
+  const int rc = check_kv8_attention(cache, Tq, HQ, n, window, sinks, "kv8_attention_workspace_bytes");
+  if (rc != DSA_OK) return rc;
+  return dsa::kv8_attn_workspace(kv8_of(cache), Tq, HQ, n, window, sinks);
+}
+
+int dsa_kv8_attention(const dsa_kv8_cache* cache, const void* Q, int dtype, const int32_t* count, int64_t Tq,
+                      int HQ, int64_t n, int64_t window, int64_t sinks, float scale, void* out,
+                      void* workspace, int64_t workspace_bytes, void* stream) {
+  const int rc = check_kv8_attention(cache, Tq, HQ, n, window, sinks, "kv8_attention");
+  if (rc != DSA_OK) return rc;
+  if (!dtype_ok(dtype)) return fail(DSA_EINVAL, "kv8_attention: unknown dtype %d", dtype);
+  if (!std::isfinite(scale)) return fail(DSA_EINVAL, "kv8_attention: scale must be finite");
+  if (cache->B == 0 || Tq == 0) return DSA_OK;
+  if (!Q || !out) return fail(DSA_EINVAL, "kv8_attention: null pointer");
+  if (!aligned16(Q) || !aligned16(out) || !aligned4(count)) return fail(DSA_EINVAL, "kv8_attention: Q and out must be 16-byte aligned, count 4-byte");
+  const dsa::Kv8 c = kv8_of(cache);
+  const int64_t need = dsa::kv8_attn_workspace(c, Tq, HQ, n, window, sinks);
+  if (need > 0 && (!workspace || !aligned16(workspace) || workspace_bytes < need))
+    return fail(DSA_EINVAL, "kv8_attention: needs a 16-byte aligned workspace of %lld bytes (got %lld)", (long long)need, (long long)workspace_bytes);
+  return hip_status(dsa::launch_kv8_attn(c, Q, dtype, count, Tq, HQ, n, window, sinks, scale, out, workspace,
+                                         static_cast<hipStream_t>(stream)),
+                    "dsa_kv8_attention");
 }
 
 }  // extern "C"

@@ -78,8 +78,9 @@ struct TileLds {
   static constexpr int NCH = D / 8;  // 16-byte chunks per row
   static constexpr int BYTES = KT * D * 2;
   // K is read as 16-byte A fragments by 16 consecutive rows at one chunk:
-  // row % NCH spreads them over NCH chunk positions.
-  static __device__ __forceinline__ int swz_k(int r) { return r & (NCH - 1); }
+  // row % NCH spreads them over NCH chunk positions (16 of them take all banks,
+  // and rows 16 apart, which a lane reads from one offset, keep their swizzle).
+  static __device__ __forceinline__ int swz_k(int r) { return r & ((NCH < 16 ? NCH : 16) - 1); }
   // V is read by the transposing 8-byte reads: 4 consecutive rows at one
   // chunk pair {2m, 2m+1} per 16-lane group; 2*(r % (NCH/2)) keeps the pair
   // together and moves it per row.

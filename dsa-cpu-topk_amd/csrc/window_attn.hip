@@ -1,0 +1,551 @@
+// window_attn.hip -- attention of prompts over a sliding window and the first tokens
+// (gfx950).
+//
+//   O[b,t,h,:] = sum_s p_s V[b,s,h/G,:],  p = softmax_s(<Q[b,t,h], K[b,s,h/G]> scale)
+// over s <= t with s > t - window or s < sinks.
+//
+// A block takes 128 queries of one head (64 of 256 dimensions), a wave 32, and walks the tiles of 64 keys that
+// any of them sees: those of the first tokens, then those of the window.  K and V go to
+// LDS by DMA, two buffers each, the products run transposed,
+//   S^T = K . Q^T,  O^T = V^T . P^T,
+// so that P goes from the first product's registers into the second one's, and the
+// softmax is one pass with a running maximum and sum in fp32.
+#include <type_traits>
+
+#include "kv8.h"
+#include "tile_common.h"
+
+namespace dsa {
+namespace {
+
+struct Win {
+  const void *Q, *K, *V;
+  void* out;
+  const int32_t* count;
+  int64_t B, ldq, ldk, ldv;
+  int T, HQ, G, window, sinks;
+  float scale_log2;
+};
+
+// What of the tiles of KT keys a block of TQ queries from t0 on walks.
+struct Walk {
+  int n;            // tokens of the sequence
+  int first, near;  // tiles of the first tokens: 0 .. first - 1, then near, near + 1, ...
+  int total;
+  __device__ __forceinline__ int tile(int v) const { return v < first ? v : near + v - first; }
+};
+template <int TQ, int KT>
+__device__ __forceinline__ Walk walk_of(const Win& a, int64_t b, int t0) {
+  Walk w;
+  w.n = a.count ? max(0, min(a.count[b], a.T)) : a.T;
+  if (t0 >= w.n) {
+    w.first = w.near = w.total = 0;
+    return w;
+  }
+  w.near = max(0, t0 - a.window + 1) / KT;
+  w.first = min((a.sinks + KT - 1) / KT, w.near);
+  w.total = w.first + (min(t0 + TQ, w.n) - 1) / KT - w.near + 1;
+  return w;
+}
+
+// Block -> (tile of queries, batch, head): the tiles of one K/V head go to one XCD (block
+// i starts on XCD i % 8), the latest, which see most, first.
+template <int TQ>
+__device__ __forceinline__ bool place(const Win& a, int& t0, int64_t& b, int& h) {
+  const int ntile = (a.T + TQ - 1) / TQ, HKV = a.HQ / a.G;
+  const int64_t pairs = a.B * HKV;  // (b, K/V head)
+  const int64_t lanes = (pairs + 7) / 8;
+  int64_t i = blockIdx.x;
+  const int64_t x = i % 8;
+  i /= 8;
+  const int hh = static_cast<int>(i % a.G);
+  i /= a.G;
+  const int64_t pair = i % lanes * 8 + x;
+  t0 = (ntile - 1 - static_cast<int>(i / lanes)) * TQ;
+  if (pair >= pairs) return false;
+  b = pair / HKV;
+  h = static_cast<int>(pair % HKV) * a.G + hh;
+  return true;
+}
+template <int TQ>
+int64_t blocks_of(const Win& a) {
+  const int64_t ntile = (a.T + TQ - 1) / TQ;
+  return (a.B * (a.HQ / a.G) + 7) / 8 * 8 * a.G * ntile;
+}
+
+__device__ __forceinline__ bool finite_f32(float x) { return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u; }
+// Bit 15 of each half that is Inf or NaN.
+template <typename Tag>
+__device__ __forceinline__ uint32_t odd_halves(uint32_t w) {
+  constexpr uint32_t kExp = __is_same(Tag, BF16) ? 0x7f807f80u : 0x7c007c00u, kOne = __is_same(Tag, BF16) ? 0x00800080u : 0x04000400u;
+  return ((w & kExp) + kOne) & 0x80008000u;
+}
+
+template <typename Tag>
+__device__ __forceinline__ void store4(typename Tag::raw* to, f32x4 y) {
+  if constexpr (Tag::kBytes == 4) {
+    *reinterpret_cast<f32x4*>(to) = y;
+  } else if constexpr (__is_same(Tag, BF16)) {
+    typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+    *reinterpret_cast<bf16x4*>(to) = __builtin_convertvector(y, bf16x4);
+  } else {
+    typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+    *reinterpret_cast<f16x4*>(to) = __builtin_convertvector(y, f16x4);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// 16-bit inputs: 16x16x32 products.  P is rounded to the inputs' type for the second
+// one and for the sum it is divided by (an output of that type holds no more).
+//
+// What a query does not see must not reach it, NaN and Inf included.  Keys are
+// masked by a select of the logit.  In V a product with a p of 0 would carry them, which
+// shows in the result: a block whose result is not finite is run again with V's
+// non-finite elements taken out of the product and added to the rows that see them.
+// ---------------------------------------------------------------------------
+template <typename Tag, int D, int QT>
+__global__ __launch_bounds__(kNT, D == 256 ? 1 : 2) void window_kernel(Win a) {
+  using raw = typename Tag::raw;
+  using M = Mfma16x16x32<Tag>;
+  using L = TileLds<D>;
+  constexpr int TQ = 64 * QT, NKS = D / 32, NDT = D / 16;
+  constexpr int KJ = D == 256 ? 1 : 4;           // 16-key tiles whose K fragments are read at once
+  constexpr int VG = NDT < 4 ? NDT : 4;          // 16-dim tiles whose V fragments are
+  constexpr int PW = L::BYTES / 1024 / (kNT / kWave);
+  __shared__ __align__(16) uint8_t k0[L::BYTES], k1[L::BYTES], v0[L::BYTES], v1[L::BYTES];
+
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int lane = lane_id(), g = lane >> 4, c16 = lane & 15;
+  int t0, h;
+  int64_t b;
+  if (!place<TQ>(a, t0, b, h)) return;
+  const Walk walk = walk_of<TQ, kKT>(a, b, t0);
+  const int T = a.T, n = walk.n, window = a.window, sinks = a.sinks;
+  const int tw = t0 + 16 * QT * wave, wave_last = min(tw + 16 * QT - 1, n - 1);
+  raw* const out = static_cast<raw*>(a.out) + (b * T * a.HQ + h) * D;
+
+  const raw* Qb = static_cast<const raw*>(a.Q) + b * T * a.ldq + static_cast<int64_t>(h) * D;
+  const char* const kbase = reinterpret_cast<const char*>(static_cast<const raw*>(a.K) + b * T * a.ldk + static_cast<int64_t>(h / a.G) * D);
+  const char* const vbase = reinterpret_cast<const char*>(static_cast<const raw*>(a.V) + b * T * a.ldv + static_cast<int64_t>(h / a.G) * D);
+  const uint32_t krow = static_cast<uint32_t>(a.ldk) * 2u, vrow = static_cast<uint32_t>(a.ldv) * 2u;
+  uint32_t koff[PW], voff[PW];  // of this wave's 16-byte chunks within a tile
+#pragma unroll
+  for (int i = 0; i < PW; ++i) {
+    const int P = (wave * PW + i) * 64 + lane, r = P / L::NCH, pc = P % L::NCH;
+    koff[i] = static_cast<uint32_t>(r) * krow + 16u * static_cast<uint32_t>(pc ^ L::swz_k(r));
+    voff[i] = static_cast<uint32_t>(r) * vrow + 16u * static_cast<uint32_t>(pc ^ L::swz_v(r));
+  }
+  // rows past the sequence read as zeros
+  auto fetch = [&](int kt, DSA_LDS uint8_t* kd, DSA_LDS uint8_t* vd) __attribute__((always_inline)) {
+    dma_tile<PW>(rows_rsrc(kbase, kt * kKT, n, krow), koff, kd, wave);
+    dma_tile<PW>(rows_rsrc(vbase, kt * kKT, n, vrow), voff, vd, wave);
+  };
+  DSA_LDS uint8_t* const kl0 = (DSA_LDS uint8_t*)k0;
+  DSA_LDS uint8_t* const kl1 = (DSA_LDS uint8_t*)k1;
+  DSA_LDS uint8_t* const vl0 = (DSA_LDS uint8_t*)v0;
+  DSA_LDS uint8_t* const vl1 = (DSA_LDS uint8_t*)v1;
+
+  u32x4 qf[QT][NKS];
+  int tq[QT];
+#pragma unroll
+  for (int qt = 0; qt < QT; ++qt) {
+    tq[qt] = tw + 16 * qt + c16;
+    const raw* q = Qb + min(tq[qt], T - 1) * a.ldq;
+#pragma unroll
+    for (int ks = 0; ks < NKS; ++ks) qf[qt][ks] = *reinterpret_cast<const u32x4*>(q + 32 * ks + 8 * g);
+  }
+  int kofs[NKS], vofs[NDT];  // LDS reads within a tile
+#pragma unroll
+  for (int ks = 0; ks < NKS; ++ks) kofs[ks] = c16 * (2 * D) + 16 * ((4 * ks + g) ^ L::swz_k(c16));
+  {
+    const int vr = 4 * g + (c16 >> 2);
+#pragma unroll
+    for (int dt = 0; dt < NDT; ++dt)
+      vofs[dt] = vr * (2 * D) + 16 * ((2 * dt + ((c16 & 3) >> 1)) ^ L::swz_v(vr)) + 8 * (c16 & 1);
+  }
+
+  f32x4 o[NDT][QT];
+  float m[QT], lpart[QT];
+  auto run = [&](auto careful) __attribute__((always_inline)) {
+    constexpr bool CAREFUL = decltype(careful)::value;
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) {
+      m[qt] = -INFINITY;
+      lpart[qt] = 0.0f;
+#pragma unroll
+      for (int dt = 0; dt < NDT; ++dt) o[dt][qt] = f32x4{0, 0, 0, 0};
+    }
+    auto compute = [&](auto masked, int s0, const DSA_LDS uint8_t* kl, const DSA_LDS uint8_t* vl) __attribute__((always_inline)) {
+      constexpr bool MASKED = decltype(masked)::value;
+      f32x4 st[4][QT];
+      __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+      for (int jp = 0; jp < 4; jp += KJ) {
+        u32x4 ka[KJ][NKS];
+#pragma unroll
+        for (int jj = 0; jj < KJ; ++jj)
+#pragma unroll
+          for (int ks = 0; ks < NKS; ++ks)
+            ka[jj][ks] = *reinterpret_cast<const DSA_LDS u32x4*>(kl + kofs[ks] + 16 * (jp + jj) * (2 * D));
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int jj = 0; jj < KJ; ++jj) {
+#pragma unroll
+          for (int qt = 0; qt < QT; ++qt) st[jp + jj][qt] = f32x4{0, 0, 0, 0};
+#pragma unroll
+          for (int ks = 0; ks < NKS; ++ks)
+#pragma unroll
+            for (int qt = 0; qt < QT; ++qt) st[jp + jj][qt] = M::run(ka[jj][ks], qf[qt][ks], st[jp + jj][qt]);
+        }
+      }
+      __builtin_amdgcn_s_setprio(0);
+      u32x4 pf[QT][2];
+      bool grow = false;
+      float alpha[QT];
+      uint32_t ok[QT];  // bit 4j + r: key s0 + 16j + 4g + r is seen
+#pragma unroll
+      for (int qt = 0; qt < QT; ++qt) {
+        float mx = -INFINITY;
+        ok[qt] = 0xffffu;
+        if constexpr (MASKED) {
+          ok[qt] = 0;
+          const int far = tq[qt] - s0 - 4 * g, near = far - window, sink = sinks - s0 - 4 * g;
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const int s = 16 * (e >> 2) + (e & 3);
+            const bool yes = s <= far && (s > near || s < sink);
+            ok[qt] |= yes ? 1u << e : 0u;
+            st[e >> 2][qt][e & 3] = yes ? st[e >> 2][qt][e & 3] * a.scale_log2 : -INFINITY;
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) st[e >> 2][qt][e & 3] *= a.scale_log2;
+        }
+#pragma unroll
+        for (int e = 0; e < 16; ++e) mx = fmaxf(mx, st[e >> 2][qt][e & 3]);
+        mx = max_xor32(max_xor16(mx));
+        // the maximum moves when a tile's passes it by 2^8: p then stays far below overflow
+        const bool up = mx > m[qt] + 8.f;
+        const float m_new = up ? mx : m[qt];
+        alpha[qt] = up ? __builtin_amdgcn_exp2f(m[qt] - m_new) : 1.f;
+        grow |= up && m[qt] != -INFINITY;
+        m[qt] = m_new;
+        const float ref = m_new == -INFINITY ? 0.f : m_new;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) st[e >> 2][qt][e & 3] = __builtin_amdgcn_exp2f(st[e >> 2][qt][e & 3] - ref);
+#pragma unroll
+        for (int jj = 0; jj < 2; ++jj)
+          pf[qt][jj] = u32x4{M::pack(st[2 * jj][qt][0], st[2 * jj][qt][1]), M::pack(st[2 * jj][qt][2], st[2 * jj][qt][3]),
+                             M::pack(st[2 * jj + 1][qt][0], st[2 * jj + 1][qt][1]), M::pack(st[2 * jj + 1][qt][2], st[2 * jj + 1][qt][3])};
+      }
+      if (ballot(grow)) {
+#pragma unroll
+        for (int qt = 0; qt < QT; ++qt) {
+          lpart[qt] *= alpha[qt];
+#pragma unroll
+          for (int dt = 0; dt < NDT; ++dt) o[dt][qt] *= alpha[qt];
+        }
+      }
+#pragma unroll
+      for (int jj = 0; jj < 2; ++jj)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+          for (int qt = 0; qt < QT; ++qt) lpart[qt] = M::dot2_ones(pf[qt][jj][e], lpart[qt]);
+      uint32_t odd = 0;
+      __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+      for (int dg = 0; dg < NDT; dg += VG) {
+        u32x4 vfrag[VG][2];
+#pragma unroll
+        for (int d = 0; d < VG; ++d)
+#pragma unroll
+          for (int jj = 0; jj < 2; ++jj) {
+            const DSA_LDS uint8_t* va = vl + vofs[dg + d] + 32 * jj * (2 * D);
+            const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((DSA_LDS s16x4*)va);
+            const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((DSA_LDS s16x4*)(va + 16 * (2 * D)));
+            const uint2 l2 = __builtin_bit_cast(uint2, lo), h2 = __builtin_bit_cast(uint2, hi);
+            vfrag[d][jj] = u32x4{l2.x, l2.y, h2.x, h2.y};
+            if constexpr (CAREFUL) {
+#pragma unroll
+              for (int w = 0; w < 4; ++w) {
+                const uint32_t bad = odd_halves<Tag>(vfrag[d][jj][w]);
+                odd |= bad;
+                vfrag[d][jj][w] &= ~((bad >> 15) * 0xffffu);
+              }
+            }
+          }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int d = 0; d < VG; ++d)
+#pragma unroll
+          for (int jj = 0; jj < 2; ++jj)
+#pragma unroll
+            for (int qt = 0; qt < QT; ++qt) o[dg + d][qt] = M::run(vfrag[d][jj], pf[qt][jj], o[dg + d][qt]);
+      }
+      __builtin_amdgcn_s_setprio(0);
+      if constexpr (CAREFUL) {
+        if (ballot(odd != 0)) {
+          const raw* v = reinterpret_cast<const raw*>(vbase) + static_cast<int64_t>(s0) * a.ldv;
+          for (int s = 0; s < min(kKT, n - s0); ++s) {  // key s0 + s: lane group s / 4 % 4, entry 4 (s / 16) + s % 4
+            const int from = ((s >> 2) & 3) * 16 + c16;
+#pragma unroll
+            for (int qt = 0; qt < QT; ++qt) {
+              float mine = 0.0f;  // this lane's p of entry 4 (s / 16) + s % 4, as the product took it
+#pragma unroll
+              for (int e = 0; e < 16; ++e) {
+                const uint32_t w = pf[qt][e >> 3][(e >> 1) & 3];
+                const float pe = to_f32(Tag{}, static_cast<uint16_t>(e & 1 ? w >> 16 : w & 0xffffu));
+                mine = e == 4 * (s >> 4) + (s & 3) ? pe : mine;
+              }
+              const float p = __shfl(mine, from, kWave);
+              const bool yes = static_cast<uint32_t>(__shfl(static_cast<int>(ok[qt]), from, kWave)) >> (4 * (s >> 4) + (s & 3)) & 1u;
+#pragma unroll
+              for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                  const float x = to_f32(Tag{}, v[s * a.ldv + 16 * dt + 4 * g + r]);
+                  if (yes && !finite_f32(x)) o[dt][qt][r] += p * x;
+                }
+            }
+          }
+        }
+      }
+    };
+    if (walk.total > 0) fetch(walk.tile(0), kl0, vl0);
+    __builtin_amdgcn_sched_barrier(0);
+    wait_dma_keep<0>();
+    block_sync_lds();
+    auto step = [&](int v, DSA_LDS uint8_t* kc, DSA_LDS uint8_t* vc, DSA_LDS uint8_t* kn, DSA_LDS uint8_t* vn) __attribute__((always_inline)) {
+      if (v + 1 < walk.total) fetch(walk.tile(v + 1), kn, vn);
+      __builtin_amdgcn_sched_barrier(0);
+      const int s0 = walk.tile(v) * kKT, s1 = s0 + kKT - 1;
+      if (s0 <= wave_last && (s1 > tw - window || s0 < sinks)) {
+        if (s1 <= tw && (s0 > wave_last - window || s1 < sinks)) compute(std::false_type{}, s0, kc, vc);
+        else compute(std::true_type{}, s0, kc, vc);
+      }
+      wait_dma_keep<0>();
+      block_sync_lds();
+    };
+    for (int v = 0; v < walk.total; v += 2) {
+      step(v, kl0, vl0, kl1, vl1);
+      if (v + 1 < walk.total) step(v + 1, kl1, vl1, kl0, vl0);
+    }
+  };
+
+  run(std::false_type{});
+  bool odd = false;
+#pragma unroll
+  for (int qt = 0; qt < QT; ++qt) {
+    if (tq[qt] >= n) continue;
+#pragma unroll
+    for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) odd |= !finite_f32(o[dt][qt][r]);
+  }
+  if (__syncthreads_or(odd)) run(std::true_type{});
+
+#pragma unroll
+  for (int qt = 0; qt < QT; ++qt) {
+    const float l = sum_xor32(sum_xor16(lpart[qt]));
+    if (tq[qt] >= T) continue;
+    const float inv = tq[qt] < n ? 1.f / l : __builtin_nanf("");  // no token: sees nothing
+    raw* to = out + static_cast<int64_t>(tq[qt]) * a.HQ * D;
+#pragma unroll
+    for (int dt = 0; dt < NDT; ++dt) store4<Tag>(to + 16 * dt + 4 * g, o[dt][qt] * inv);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// fp32: 16x16x4 fp32 products, 64 queries a block (a wave 16).  Tiles of KT keys; rows
+// lie in LDS as they are, padded by 4 elements so that neither reading hits a bank twice.
+// K-slots: element i of a lane's 16 bytes of K is step i (dims 16kk + 4g + i), token
+// 16j + 4g + r is step r of P's.
+// ---------------------------------------------------------------------------
+template <int D, int KT>
+__global__ __launch_bounds__(kNT) void window_f32_kernel(Win a) {
+  constexpr int TQ = 64, NKK = D / 16, NDT = D / 16, NJ = KT / 16, LD = D + 4;
+  __shared__ __align__(16) float kt_[KT * LD], vt_[KT * LD];
+  const int tid = threadIdx.x, wave = tid >> 6, lane = lane_id(), g = lane >> 4, c16 = lane & 15;
+  int t0, h;
+  int64_t b;
+  if (!place<TQ>(a, t0, b, h)) return;
+  const Walk walk = walk_of<TQ, KT>(a, b, t0);
+  const int T = a.T, n = walk.n, window = a.window, sinks = a.sinks;
+  const int tw = t0 + 16 * wave, wave_last = min(tw + 15, n - 1), tq = tw + c16;
+  const float* kb = static_cast<const float*>(a.K) + b * T * a.ldk + static_cast<int64_t>(h / a.G) * D;
+  const float* vb = static_cast<const float*>(a.V) + b * T * a.ldv + static_cast<int64_t>(h / a.G) * D;
+  f32x4 q[NKK];
+  {
+    const float* src = static_cast<const float*>(a.Q) + (b * T + min(tq, T - 1)) * a.ldq + static_cast<int64_t>(h) * D;
+#pragma unroll
+    for (int kk = 0; kk < NKK; ++kk) q[kk] = *reinterpret_cast<const f32x4*>(src + 16 * kk + 4 * g);
+  }
+  f32x4 o[NDT];
+  float m, l;
+  auto run = [&](auto careful) __attribute__((always_inline)) {
+    constexpr bool CAREFUL = decltype(careful)::value;
+    m = -INFINITY;
+    l = 0.0f;
+#pragma unroll
+    for (int d = 0; d < NDT; ++d) o[d] = f32x4{0, 0, 0, 0};
+    for (int v = 0; v < walk.total; ++v) {
+      const int s0 = walk.tile(v) * KT, s1 = s0 + KT - 1;
+      __syncthreads();
+      for (int i = tid; i < KT * D / 4; i += kNT) {
+        const int r = i / (D / 4), d = i % (D / 4) * 4;
+        f32x4 x{0, 0, 0, 0}, y{0, 0, 0, 0};
+        if (s0 + r < n) {
+          x = *reinterpret_cast<const f32x4*>(kb + (s0 + r) * a.ldk + d);
+          y = *reinterpret_cast<const f32x4*>(vb + (s0 + r) * a.ldv + d);
+        }
+        *reinterpret_cast<f32x4*>(kt_ + r * LD + d) = x;
+        *reinterpret_cast<f32x4*>(vt_ + r * LD + d) = y;
+      }
+      __syncthreads();
+      if (s0 > wave_last || (s1 <= tw - window && s0 >= sinks)) continue;
+      f32x4 st[NJ];
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+        st[j] = f32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int kk = 0; kk < NKK; ++kk) {
+          const f32x4 x = *reinterpret_cast<const f32x4*>(kt_ + (16 * j + c16) * LD + 16 * kk + 4 * g);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) st[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[i], q[kk][i], st[j], 0, 0, 0);
+        }
+      }
+      const bool inner = s1 <= tw && (s0 > wave_last - window || s1 < sinks);
+      uint32_t ok = 0xffffu;
+      if (!inner) {
+        ok = 0;
+        const int far = tq - s0 - 4 * g, near = far - window, sink = sinks - s0 - 4 * g;
+#pragma unroll
+        for (int e = 0; e < 4 * NJ; ++e) {
+          const int s = 16 * (e >> 2) + (e & 3);
+          ok |= s <= far && (s > near || s < sink) ? 1u << e : 0u;
+        }
+      }
+      float top = -INFINITY;
+#pragma unroll
+      for (int e = 0; e < 4 * NJ; ++e) {
+        const float x = st[e >> 2][e & 3] * a.scale_log2;
+        st[e >> 2][e & 3] = ok >> e & 1u ? x : -INFINITY;
+        top = fmaxf(top, st[e >> 2][e & 3]);
+      }
+      top = max_xor32(max_xor16(top));
+      if (ballot(top > m + 8.f)) {
+        const float next = fmaxf(m, top);
+        const float fall = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - next);
+        m = next;
+        l *= fall;
+#pragma unroll
+        for (int d = 0; d < NDT; ++d) o[d] *= fall;
+      }
+      const float ref = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+      for (int e = 0; e < 4 * NJ; ++e) {
+        st[e >> 2][e & 3] = __builtin_amdgcn_exp2f(st[e >> 2][e & 3] - ref);
+        l += st[e >> 2][e & 3];
+      }
+      bool odd = false;
+#pragma unroll
+      for (int j = 0; j < NJ; ++j)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float* row = vt_ + (16 * j + 4 * g + r) * LD + c16;
+#pragma unroll
+          for (int d = 0; d < NDT; ++d) {
+            float x = row[16 * d];
+            if constexpr (CAREFUL) {
+              odd |= !finite_f32(x);
+              x = finite_f32(x) ? x : 0.0f;
+            }
+            o[d] = __builtin_amdgcn_mfma_f32_16x16x4f32(x, st[j][r], o[d], 0, 0, 0);
+          }
+        }
+      if constexpr (CAREFUL) {
+        if (ballot(odd)) {
+          for (int s = 0; s < min(KT, n - s0); ++s) {
+            const int from = ((s >> 2) & 3) * 16 + c16, e0 = 4 * (s >> 4) + (s & 3);
+            float mine = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 4 * NJ; ++e) mine = e == e0 ? st[e >> 2][e & 3] : mine;
+            const float p = __shfl(mine, from, kWave);
+            const bool yes = static_cast<uint32_t>(__shfl(static_cast<int>(ok), from, kWave)) >> e0 & 1u;
+#pragma unroll
+            for (int d = 0; d < NDT; ++d)
+#pragma unroll
+              for (int r = 0; r < 4; ++r) {
+                const float x = vt_[s * LD + 16 * d + 4 * g + r];
+                if (yes && !finite_f32(x)) o[d][r] += p * x;
+              }
+          }
+        }
+      }
+    }
+  };
+  run(std::false_type{});
+  bool odd = false;
+  if (tq < n) {
+#pragma unroll
+    for (int d = 0; d < NDT; ++d)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) odd |= !finite_f32(o[d][r]);
+  }
+  if (__syncthreads_or(odd)) run(std::true_type{});
+  l = sum_xor32(sum_xor16(l));
+  if (tq >= T) return;
+  const float inv = tq < n ? 1.0f / l : __builtin_nanf("");
+  float* to = static_cast<float*>(a.out) + ((b * T + tq) * a.HQ + h) * D;
+#pragma unroll
+  for (int d = 0; d < NDT; ++d) store4<F32>(to + 16 * d + 4 * g, o[d] * inv);
+}
+
+template <typename Tag>
+hipError_t launch_16(const Win& w, int D, hipStream_t stream) {
+  const dim3 grid(static_cast<uint32_t>(D == 256 ? blocks_of<64>(w) : blocks_of<128>(w)));
+  switch (D) {
+    case 32: window_kernel<Tag, 32, 2><<<grid, kNT, 0, stream>>>(w); break;
+    case 64: window_kernel<Tag, 64, 2><<<grid, kNT, 0, stream>>>(w); break;
+    case 128: window_kernel<Tag, 128, 2><<<grid, kNT, 0, stream>>>(w); break;
+    default: window_kernel<Tag, 256, 1><<<grid, kNT, 0, stream>>>(w);  // registers
+  }
+  return hipGetLastError();
+}
+
+}  // namespace
+
+bool window_attn_supported(int D) { return D == 32 || D == 64 || D == 128 || D == 256; }
+
+hipError_t launch_window_attn(const WindowArgs& a, int dtype, hipStream_t stream) {
+  if (a.B == 0 || a.T == 0) return hipSuccess;
+  Win w;
+  w.Q = a.Q;
+  w.K = a.K;
+  w.V = a.V;
+  w.out = a.out;
+  w.count = a.count;
+  w.B = a.B;
+  w.ldq = a.ldq;
+  w.ldk = a.ldk;
+  w.ldv = a.ldv;
+  w.T = a.T;
+  w.HQ = a.HQ;
+  w.G = a.HQ / a.HKV;
+  w.window = a.window;
+  w.sinks = a.sinks;
+  w.scale_log2 = a.scale * 1.4426950408889634f;
+  if (dtype == 1) return launch_16<BF16>(w, a.D, stream);
+  if (dtype == 2) return launch_16<F16>(w, a.D, stream);
+  const dim3 grid(static_cast<uint32_t>(blocks_of<64>(w)));
+  switch (a.D) {
+    case 32: window_f32_kernel<32, 64><<<grid, kNT, 0, stream>>>(w); break;
+    case 64: window_f32_kernel<64, 64><<<grid, kNT, 0, stream>>>(w); break;
+    case 128: window_f32_kernel<128, 64><<<grid, kNT, 0, stream>>>(w); break;
+    default: window_f32_kernel<256, 32><<<grid, kNT, 0, stream>>>(w);
+  }
+  return hipGetLastError();
+}
+
+}  // namespace dsa

@@ -555,6 +555,121 @@ int dsa_kv4_evict(const dsa_kv4_cache* cache, int64_t keep, int64_t recent, int3
 int dsa_kv4_make_room(const dsa_kv4_cache* cache, const int32_t* count, int64_t T, int64_t recent,
                       int32_t* src, int32_t* dst, void* stream);
 
+/*
+ * ---- Windowed attention of prompts ------------------------------------------
+ *
+ *   out[b,t,h,:] = sum_s p[b,t,h,s] V[b,s,h/G,:],
+ *   p[b,t,h,:] = softmax_s(<Q[b,t,h], K[b,s,h/G]> * scale),  G = HQ / HKV,
+ * over s <= t with s > t - window or s < sinks: a sliding window, and the first
+ * tokens, which stay visible (window >= T: plain causal attention).  count [B]
+ * (null: T): how many of a sequence's T rows are tokens; the others see nothing and
+ * get NaN, as empty rows do everywhere here.  What a query does not see does not
+ * reach its result, NaN and Inf included.
+ *   out [B,T,HQ,D] of dtype: fp32 arithmetic throughout for fp32; 16-bit types round
+ * p to their type for its product with V and for the sum it is divided by.
+ *   Q [B,T,HQ,D], K, V [B,T,HKV,D] of dtype (fp32, bf16, fp16), consecutive tokens
+ *   ldq / ldk / ldv elements apart (at least HQ*D, HKV*D, HKV*D; a batch element spans
+ *   T of them), e.g. the columns of one projection's output.
+ * No reference counterpart: its attention sees what the indexer selects.
+ * Constraints: D in {32, 64, 128, 256}; HQ a multiple of HKV, at most 1024;
+ *   window >= 1, sinks >= 0; T < 2^31 - 256; strides below 2^24 elements, in bytes
+ *   multiples of 16; pointers 16-byte aligned, count 4; (B+7)*HQ*ceil(T/64) < 2^24.
+ */
+int dsa_window_attention(const void* Q, const void* K, const void* V, int dtype, const int32_t* count,
+                         int64_t B, int64_t T, int HQ, int HKV, int D, int64_t ldq, int64_t ldk,
+                         int64_t ldv, int64_t window, int64_t sinks, float scale, void* out,
+                         void* stream);
+
+/*
+ * ---- A paged cache held in 8 bits -------------------------------------------
+ *
+ * Keys and values in OCP e4m3 with one E8M0 scale byte, 2^(byte-127), 10 .. 247, for
+ * each block of 64 tokens of one head, K and V apart.  The blocks lie in the pages of a
+ * pool that many sequences share; sequence b's slot s, which holds its token at
+ * position s, is slot s % page of page pages[b][s / page]:
+ *   codes [NP, HKV, page/64, 64*(DK+DV)]   of a block: K [64][DK], then V [DV][64], a
+ *     dimension's tokens t in the order of (t/4%4)*16 + t/16*4 + t%4 (that of the
+ *     matrix products)
+ *   scales [NP, HKV, page/64, 2]           the block's K's, then its V's
+ * A page id outside [0, NP) names no page: nothing is read or written there, its slots
+ * hold nothing.  Pages that no visible slot lies on (behind a window) need no id.  The
+ * buffers are device memory of the caller's, in this struct on the host, which is read
+ * before the call returns.  A call that writes pages and any other call on them need
+ * the order of one stream or an event between them.  Two sequences may share pages that
+ * are only read; blocks that a call writes belong to one sequence.  Values of length
+ * outside [0, max_pages*page] count as the nearer end.
+ * No reference counterpart: it has no cache.
+ * Constraints: B <= 65535; 1 <= NP, max_pages; page = 64 * 2^j <= 65536;
+ *   max_pages*page <= 2^31 - 256; 1 <= HKV <= 1024; DK = DV in {32, 64, 96, 128, 192,
+ *   256} or DK 192 with DV 128 (else DSA_EUNSUPPORTED); codes 16-byte aligned, scales
+ *   2-byte, the others 4-byte.
+ */
+typedef struct dsa_kv8_cache {
+  uint8_t* codes;
+  uint8_t* scales;
+  const int32_t* pages; /* [B, max_pages] page ids                       */
+  int32_t* length;      /* [B] slots in use                              */
+  int32_t* lost;        /* [B] tokens that found no slot or no page      */
+  int64_t B, NP, max_pages;
+  int HKV, DK, DV, page;
+} dsa_kv8_cache;
+
+/*
+ * Append with the position rotation on the way: token i of sequence b has position and
+ * slot start[b] + i (start null: length[b] + i).  Its keys, and Q where it is given,
+ * are rotated: of the first R dimensions the pairs (j, j + R/2), or with pairs != 0
+ * the neighbours (2j, 2j + 1), become
+ *   (a cos - b sin, b cos + a sin),  cos, sin [table rows][R/2] fp32 at the position,
+ * in fp32, each product and sum rounded once.  R = 0: nothing is rotated.  The first count[b]
+ * (null: T) tokens go into the cache; then length[b] = start[b] + count[b], at most
+ * the last slot's end, and lost[b] counts those that found no slot or no page.
+ *   A block's scale is the least 2^e (from 2^-117 on) with max|x| <= 448 * 2^e over its
+ * new finite values, and not below the block's scale so far where it holds tokens of
+ * before; x / 2^e rounds to the nearest e4m3, ties to even, Inf and NaN become NaN.
+ * Where the scale grows, the held tokens' codes are rounded to it.  Slots behind the
+ * last token keep their codes.  (Magnitudes from 1.9375 * 2^127 on read back as Inf.)
+ *   K [B,T,HKV,DK], V [B,T,HKV,DV], Q [B,T,HQ,DK] (null exactly where Q_out is) of dtype
+ *   (fp32, bf16, fp16), consecutive tokens ldk / ldv / ldq elements apart; K_out
+ *   [B,T,HKV,DK] (null: not wanted) and Q_out [B,T,HQ,DK], dense, of dtype: the rotated
+ *   rows of all T, NaN for positions past the last slot.
+ *   R a multiple of 16, at most DK; the tables hold max_pages*page rows at least.
+ *   16-byte aligned (start and count 4); strides in bytes multiples of 16, at most 2^24
+ *   elements; B*HKV*(T/64 + 2) < 2^23, B*T*HQ*DK/8 < 2^31.
+ */
+int dsa_kv8_append(const dsa_kv8_cache* cache, const void* K, const void* V, const void* Q, int dtype,
+                   int64_t T, int HQ, int64_t ldk, int64_t ldv, int64_t ldq, const float* cos,
+                   const float* sin, int64_t table_rows, int R, int pairs, const int32_t* start,
+                   const int32_t* count, void* K_out, void* Q_out, void* stream);
+
+/*
+ * The values that N slots of each sequence stand for, K [B,N,HKV,DK] and V [B,N,HKV,DV] of
+ * dtype (exact in fp32 and bf16; fp16 rounds, to Inf past its range): slots [B,N], or
+ * 0 .. N-1 where null.  Slots outside [0, length) give zeros.  K and V 16-byte aligned;
+ * B*N*HKV*(DK+DV)/8 < 2^31.
+ */
+int dsa_kv8_rows(const dsa_kv8_cache* cache, const int32_t* slots, int64_t N, int dtype, void* K, void* V,
+                 void* stream);
+
+/*
+ * Attention of each sequence's last Tq tokens over the cache, as dsa_window_attention's of
+ * the tokens at positions length[b] - count[b] + t, t < count[b] (count null: Tq; the
+ * others see nothing: NaN), over the slots among the first n.  window 0: all of them.
+ *   fp32 logits, softmax and sums; the cache's values enter the products unrounded; Q
+ * and p as f16 with a power of two for each row of Q (16-bit types) or as two such
+ * pieces (fp32: 22 bits and more).
+ *   Q [B,Tq,HQ,DK], out [B,Tq,HQ,DV] of dtype (fp32, bf16, fp16), 16-byte aligned; HQ a
+ *   multiple of HKV, at most 1024; n <= max_pages*page; B*Tq*HQ < 2^23.
+ *   workspace: device memory of dsa_kv8_attention_workspace_bytes, 16-byte aligned, used
+ *   by no other work until the launches complete, contents on entry free (a smaller one
+ *   is refused).  Needs the device (its compute-unit count); a negative status where the
+ *   sizes are refused.
+ */
+int64_t dsa_kv8_attention_workspace_bytes(const dsa_kv8_cache* cache, int64_t Tq, int HQ, int64_t n,
+                                          int64_t window, int64_t sinks);
+int dsa_kv8_attention(const dsa_kv8_cache* cache, const void* Q, int dtype, const int32_t* count, int64_t Tq,
+                      int HQ, int64_t n, int64_t window, int64_t sinks, float scale, void* out,
+                      void* workspace, int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
