@@ -361,13 +361,20 @@ def _plain_window(s):
 
 
 # --- the framework's calls -----------------------------------------------------------------------
-def _framework():
-    pkg = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "dsa-cpu-topk_amd")
-    if pkg not in sys.path:
-        sys.path.insert(0, pkg)
-    import dsa_paged
+_module = None
 
-    return dsa_paged
+
+def _framework():
+    """The framework's module, imported once, as a program does."""
+    global _module
+    if _module is None:
+        pkg = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "dsa-cpu-topk_amd")
+        if pkg not in sys.path:
+            sys.path.insert(0, pkg)
+        import dsa_paged
+
+        _module = dsa_paged
+    return _module
 
 
 def _held(s):
