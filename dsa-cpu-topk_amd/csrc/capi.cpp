@@ -796,8 +796,8 @@ int dsa_kv8_rows(const dsa_kv8_cache* cache, const int32_t* slots, int64_t N, in
   const int rc = check_kv8(cache, "kv8_rows");
   if (rc != DSA_OK) return rc;
   if (!dtype_ok(dtype)) return fail(DSA_EINVAL, "kv8_rows: unknown dtype %d", dtype);
-  if (N < 0 || N > kMaxElems || cache->B * N > kMaxElems || cache->B * N * cache->HKV * ((cache->DK + cache->DV) / 8) > kMaxElems)
-    return fail(DSA_EINVAL, "kv8_rows: N=%lld: B*N*HKV*(DK+DV)/8 must be < 2^31", (long long)N);
+  if (N < 0 || N > kMaxElems || cache->B * cache->HKV * ((N + 63) / 64) >= (int64_t{1} << 24))
+    return fail(DSA_EINVAL, "kv8_rows: N=%lld: B*HKV*ceil(N/64) must be < 2^24", (long long)N);
   if (cache->B == 0 || N == 0) return DSA_OK;
   if (!K || !V) return fail(DSA_EINVAL, "kv8_rows: null pointer");
   if (!aligned16(K) || !aligned16(V) || !aligned4(slots)) return fail(DSA_EINVAL, "kv8_rows: K and V must be 16-byte aligned, slots 4-byte");

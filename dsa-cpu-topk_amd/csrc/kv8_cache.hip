@@ -1,5 +1,6 @@
 // kv8_cache.hip -- what goes into the paged 8-bit cache and comes back out of it
 // (gfx950).
+#include "dsa_launch.h"
 #include "kv8.h"
 
 namespace dsa {
@@ -20,32 +21,56 @@ __device__ __forceinline__ float turn_b(float a, float b, float c, float s) {
   return x + y;
 }
 
-// Elements d0 .. d0+7 of the row at `p` (one head of one token), rotated by table row `at`.
-template <typename Tag>
-__device__ __forceinline__ void load_rotated(const typename Tag::raw* p, int d0, int R, bool pairs,
-                                             const float* cos, const float* sin, int64_t at, float (&x)[8]) {
-  load_cvt<Tag, 8>(p + d0, x);
-  if (d0 >= R) return;
-  const int half = R / 2;
+// A thread takes 16 elements of a row, unit u: elements lo .. lo+7 and hi .. hi+7, which are
+// the pairs where halves turn; neighbouring units are neighbours in memory.
+struct Unit {
+  int lo, hi;
+  bool turn_lo, turn_hi;
+};
+__device__ __forceinline__ Unit unit_of(int u, int D, int R, bool pairs) {
+  if (!pairs && 16 * u < R) return {8 * u, 8 * u + R / 2, true, true};
+  const int from = pairs ? 0 : R, lo = from + 8 * u - from / 2, hi = lo + (D - from) / 2;
+  return {lo, hi, lo < R, hi < R};
+}
+struct Angles {
+  float c[8], s[8];
+};
+__device__ __forceinline__ void load_angles(const Kv8Append& a, const Unit& un, int64_t at, Angles& g) {
+  const int64_t row = at * (a.R / 2);
+  if (!a.pairs) {
+    if (!un.turn_lo) return;
+    load_f32<8>(a.cos + row + un.lo, g.c);
+    load_f32<8>(a.sin + row + un.lo, g.s);
+    return;
+  }
+  if (un.turn_lo) {
+    *reinterpret_cast<f32x4*>(g.c) = *reinterpret_cast<const f32x4*>(a.cos + row + un.lo / 2);
+    *reinterpret_cast<f32x4*>(g.s) = *reinterpret_cast<const f32x4*>(a.sin + row + un.lo / 2);
+  }
+  if (un.turn_hi) {
+    *reinterpret_cast<f32x4*>(g.c + 4) = *reinterpret_cast<const f32x4*>(a.cos + row + un.hi / 2);
+    *reinterpret_cast<f32x4*>(g.s + 4) = *reinterpret_cast<const f32x4*>(a.sin + row + un.hi / 2);
+  }
+}
+__device__ __forceinline__ void turn_pairs(float (&x)[8], const float* c, const float* s) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float a = x[2 * i], b = x[2 * i + 1];
+    x[2 * i] = turn_a(a, b, c[i], s[i]);
+    x[2 * i + 1] = turn_b(a, b, c[i], s[i]);
+  }
+}
+__device__ __forceinline__ void turn(float (&lo)[8], float (&hi)[8], const Angles& g, const Unit& un, bool pairs) {
   if (pairs) {
-    float c[4], s[4];
-    load_f32<4>(cos + at * half + d0 / 2, c);
-    load_f32<4>(sin + at * half + d0 / 2, s);
+    if (un.turn_lo) turn_pairs(lo, g.c, g.s);
+    if (un.turn_hi) turn_pairs(hi, g.c + 4, g.s + 4);
+  } else if (un.turn_lo) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float a = x[2 * i], b = x[2 * i + 1];
-      x[2 * i] = turn_a(a, b, c[i], s[i]);
-      x[2 * i + 1] = turn_b(a, b, c[i], s[i]);
+    for (int i = 0; i < 8; ++i) {
+      const float a = lo[i], b = hi[i];
+      lo[i] = turn_a(a, b, g.c[i], g.s[i]);
+      hi[i] = turn_b(a, b, g.c[i], g.s[i]);
     }
-  } else {
-    const bool low = d0 < half;
-    const int j = low ? d0 : d0 - half;
-    float y[8], c[8], s[8];
-    load_cvt<Tag, 8>(p + (low ? d0 + half : d0 - half), y);
-    load_f32<8>(cos + at * half + j, c);
-    load_f32<8>(sin + at * half + j, s);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = low ? turn_a(x[i], y[i], c[i], s[i]) : turn_b(y[i], x[i], c[i], s[i]);
   }
 }
 
@@ -103,13 +128,13 @@ __device__ __forceinline__ Span span_of(const Kv8& c, const Kv8Append& a, int64_
 
 // Sequence b's counters, by one block: length, and the tokens past the last slot or
 // on a page that is none.
-__device__ void update_counts(const Kv8& c, const Span& s, int64_t b) {
+__device__ __forceinline__ void update_counts(const Kv8& c, const Span& s, int64_t b) {
   __shared__ int32_t bad;
   if (threadIdx.x == 0) bad = 0;
   __syncthreads();
   const int shift = c.page_shift + 6;
   int32_t mine = 0;
-  for (int64_t p = (s.have >> shift) + threadIdx.x; p << shift < s.end; p += kNT) {
+  for (int64_t p = (s.have >> shift) + threadIdx.x; p << shift < s.end; p += blockDim.x) {
     const int32_t id = c.pages[b * c.max_pages + p];
     if (id < 0 || id >= c.NP)
       mine += static_cast<int32_t>(min(s.end, (p + 1) << shift) - max(s.have, p << shift));
@@ -122,169 +147,336 @@ __device__ void update_counts(const Kv8& c, const Span& s, int64_t b) {
   }
 }
 
-// One block of threads takes one block of 64 slots of one head: rotates, finds the
-// scales, encodes, writes.  Thread (r, ch) holds elements 8 ch .. 8 ch + 7 of tokens
-// r, r + RP, ...
-template <int D>
-struct Tile {
-  static constexpr int kChunks = D / 8, kRows = kNT / kChunks, kPasses = (kBlk + kRows - 1) / kRows;
-};
-
-template <typename Tag, int DK, int DV>
-__global__ __launch_bounds__(kNT) void append_kernel(Kv8 c, Kv8Append a, int nblk, uint32_t kv_blocks, int update) {
-  using raw = typename Tag::raw;
-  using TK = Tile<DK>;
-  using TV = Tile<DV>;
-  constexpr int kRowBytes = 80;  // of a dimension's 64 codes in LDS
-  __shared__ uint32_t tops[2][4];
-  __shared__ __align__(16) uint8_t vt[DV * kRowBytes];
-  const float* cos = a.cos;
-  const float* sin = a.sin;
-  const int64_t S = c.slots();
-
-  if (blockIdx.x >= kv_blocks) {  // the queries, 8 elements a thread
-    const int64_t items = c.B * a.T * a.HQ * TK::kChunks;
-    const int64_t i = (blockIdx.x - kv_blocks) * static_cast<int64_t>(kNT) + threadIdx.x;
-    if (i >= items) return;
-    const int d0 = static_cast<int>(i % TK::kChunks) * 8;
-    const int64_t row = i / TK::kChunks, h = row % a.HQ, bt = row / a.HQ, b = bt / a.T;
-    const int64_t at = span_of(c, a, b).have + bt % a.T;
-    float x[8];
-    load_rotated<Tag>(static_cast<const raw*>(a.Q) + bt * a.ldq + h * DK, d0, a.R, a.pairs, cos, sin, min(at, S - 1), x);
-    if (at >= S) {
+// f = 2^(old - new) for codes whose scale grows.
+__device__ __forceinline__ float fall_of(uint32_t old_byte, uint32_t new_byte) {
+  return new_byte - old_byte > 40 ? 0.0f : __uint_as_float((127u + old_byte - new_byte) << 23);
+}
+__device__ __forceinline__ uint2 encode8(const float (&x)[8], float inverse) {
+  return make_uint2(encode4(scaled(x[0], inverse), scaled(x[1], inverse), scaled(x[2], inverse), scaled(x[3], inverse)),
+                    encode4(scaled(x[4], inverse), scaled(x[5], inverse), scaled(x[6], inverse), scaled(x[7], inverse)));
+}
+__device__ __forceinline__ void make_nan(float (&x)[8]) {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) x[k] = __builtin_nanf("");
-    }
-    store8<Tag>(static_cast<raw*>(a.Q_out) + row * DK + d0, x);
-    return;
-  }
+  for (int i = 0; i < 8; ++i) x[i] = __builtin_nanf("");
+}
+// Of a dimension's 16 words of V, word w holds tokens t .. t + 3.
+__device__ __forceinline__ int word_token(int w) { return (w & 3) * 16 + (w >> 2) * 4; }
 
-  const int h = blockIdx.x % c.HKV;
-  const uint32_t rest = blockIdx.x / c.HKV;
+// A block of threads takes the heads [h0, h1) of one block of 64 slots, one after
+// another, and then their share of the query heads, with the angles of its tokens in
+// registers.  Of K a thread has one unit of some tokens; of V 4 tokens by 8
+// dimensions, which it turns into words of 4 tokens (a word of the cache has one owner,
+// so bytes that stay are merged without a barrier, and a wave writes whole rows of 64).
+template <typename Tag, int DK, int DV>
+__global__ __launch_bounds__(kNT) void append_kernel(Kv8 c, Kv8Append a, int nblk, int groups, int update) {
+  using raw = typename Tag::raw;
+  constexpr int NU = DK / 16, kRows = kNT / NU, kPasses = (kBlk + kRows - 1) / kRows;
+  constexpr int kItems = 2 * DV, kTurns = (kItems + kNT - 1) / kNT;  // of V: 16 words by DV / 8 dimensions' eights
+  __shared__ uint32_t tops[2][2][4];
+  const int64_t S = c.slots();
+  const int grp = blockIdx.x % groups;
+  const uint32_t rest = blockIdx.x / groups;
   const int64_t b = rest / nblk;
   const Span s = span_of(c, a, b);
   const int64_t blk = (s.have >> 6) + rest % nblk, first = blk * kBlk;
   // the call's tokens on this block: all, and those that are stored
   const int lo = static_cast<int>(max(s.have - first, int64_t{0}));
   const int all = static_cast<int>(min(s.have + a.T - first, int64_t{kBlk}));
-  const int64_t at_block = first < s.end ? kv8_block(c, b, blk, h) : -1;
-  const int hi = at_block >= 0 ? static_cast<int>(min(s.end - first, int64_t{kBlk})) : lo;
-  uint8_t* const codes = c.codes + at_block * c.block_bytes();
+  const int64_t row0 = b * a.T - s.have + first;  // the call's row of the block's token 0
+  const bool pairs = a.pairs != 0;
 
-  float k[TK::kPasses][8], v[TV::kPasses][8];
-  uint32_t top_k = 0, top_v = 0;
-  {
-    const int ch = threadIdx.x % TK::kChunks, r0 = threadIdx.x / TK::kChunks;
-    const raw* src = static_cast<const raw*>(a.K) + (b * a.T - s.have + first) * a.ldk + static_cast<int64_t>(h) * DK;
+  const int u = threadIdx.x % NU, r0 = threadIdx.x / NU;
+  const Unit un = unit_of(u, DK, a.R, pairs);
+  Angles ang[kPasses];
 #pragma unroll
-    for (int p = 0; p < TK::kPasses; ++p) {
-      const int t = r0 + p * TK::kRows;
-      if (r0 >= TK::kRows || t < lo || t >= all || (t >= hi && !a.K_out)) continue;
-      load_rotated<Tag>(src + t * a.ldk, ch * 8, a.R, a.pairs, cos, sin, min(first + t, S - 1), k[p]);
-      if (a.K_out) {
-        float y[8];
+  for (int p = 0; p < kPasses; ++p) {
+    const int t = r0 + p * kRows;
+    if (r0 < kRows && t >= lo && t < all) load_angles(a, un, min(first + t, S - 1), ang[p]);
+  }
+
+  const int h0 = c.HKV * grp / groups, h1 = c.HKV * (grp + 1) / groups;
+  for (int h = h0; h < h1; ++h) {
+    const int64_t at = first < s.end ? kv8_block(c, b, blk, h) : -1;
+    const int hi = at >= 0 ? static_cast<int>(min(s.end - first, int64_t{kBlk})) : lo;
+    uint8_t* const codes = c.codes + at * c.block_bytes();
+    uint8_t* const scale_at = c.scales + at * 2;
+    uint32_t top_k = 0, top_v = 0, old_k = 0, old_v = 0;
+    float k0[kPasses][8], k1[kPasses][8], v[kTurns][4][8];
+    const raw* const ksrc = static_cast<const raw*>(a.K) + row0 * a.ldk + static_cast<int64_t>(h) * DK;
+    const raw* const vsrc = static_cast<const raw*>(a.V) + row0 * a.ldv + static_cast<int64_t>(h) * DV;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] = first + t < S ? k[p][i] : __builtin_nanf("");
-        store8<Tag>(static_cast<raw*>(a.K_out) + ((b * a.T - s.have + first + t) * c.HKV + h) * DK + ch * 8, y);
+    for (int p = 0; p < kPasses; ++p) {
+      const int t = r0 + p * kRows;
+      if (r0 >= kRows || t < lo || t >= (a.K_out ? all : hi)) continue;
+      load_cvt<Tag, 8>(ksrc + t * a.ldk + un.lo, k0[p]);
+      load_cvt<Tag, 8>(ksrc + t * a.ldk + un.hi, k1[p]);
+    }
+#pragma unroll
+    for (int p = 0; p < kTurns; ++p) {
+      const int i = threadIdx.x + p * kNT, d = (i >> 6) * 32 + (i & 3) * 8, t = word_token((i >> 2) & 15);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+#pragma unroll
+        for (int x = 0; x < 8; ++x) v[p][e][x] = 0.0f;
+        if (i < kItems && t + e >= lo && t + e < hi) load_cvt<Tag, 8>(vsrc + (t + e) * a.ldv + d, v[p][e]);
       }
+    }
+    if (lo > 0 && lo < hi) {
+      old_k = scale_at[0];
+      old_v = scale_at[1];
+    }
+#pragma unroll
+    for (int p = 0; p < kPasses; ++p) {
+      const int t = r0 + p * kRows;
+      if (r0 >= kRows || t < lo || t >= (a.K_out ? all : hi)) continue;
+      turn(k0[p], k1[p], ang[p], un, pairs);
       if (t < hi) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) top_k = max(top_k, finite_bits(k[p][i]));
+        for (int i = 0; i < 8; ++i) top_k = max(top_k, max(finite_bits(k0[p][i]), finite_bits(k1[p][i])));
+      }
+      if (a.K_out) {
+        raw* to = static_cast<raw*>(a.K_out) + ((row0 + t) * c.HKV + h) * DK;
+        if (first + t >= S) {
+          make_nan(k0[p]);
+          make_nan(k1[p]);
+        }
+        store8<Tag>(to + un.lo, k0[p]);
+        store8<Tag>(to + un.hi, k1[p]);
       }
     }
-  }
-  if (lo < hi) {  // the same for the whole block
-    {
-      const int ch = threadIdx.x % TV::kChunks, r0 = threadIdx.x / TV::kChunks;
-      const raw* src = static_cast<const raw*>(a.V) + (b * a.T - s.have + first) * a.ldv + static_cast<int64_t>(h) * DV;
+    if (lo >= hi) continue;  // the same for the whole block
 #pragma unroll
-      for (int p = 0; p < TV::kPasses; ++p) {
-        const int t = r0 + p * TV::kRows;
-        if (r0 >= TV::kRows || t < lo || t >= hi) continue;
-        load_cvt<Tag, 8>(src + t * a.ldv + ch * 8, v[p]);
+    for (int p = 0; p < kTurns; ++p)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) top_v = max(top_v, finite_bits(v[p][i]));
-      }
-    }
-    uint8_t* const scale_at = c.scales + at_block * 2;
-    const uint32_t old_k = lo > 0 ? scale_at[0] : 0u, old_v = lo > 0 ? scale_at[1] : 0u;
+      for (int e = 0; e < 4; ++e)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top_v = max(top_v, finite_bits(v[p][e][i]));
     top_k = wave_max_bits(top_k);
     top_v = wave_max_bits(top_v);
+    uint32_t(&top)[2][4] = tops[h & 1];
     if ((threadIdx.x & 63) == 0) {
-      tops[0][threadIdx.x >> 6] = top_k;
-      tops[1][threadIdx.x >> 6] = top_v;
+      top[0][threadIdx.x >> 6] = top_k;
+      top[1][threadIdx.x >> 6] = top_v;
     }
-    __syncthreads();  // the old scales have been read
-    const uint32_t new_k = max(old_k, kv8_scale(max(max(tops[0][0], tops[0][1]), max(tops[0][2], tops[0][3]))));
-    const uint32_t new_v = max(old_v, kv8_scale(max(max(tops[1][0], tops[1][1]), max(tops[1][2], tops[1][3]))));
-    if (threadIdx.x == 0) {
-      scale_at[0] = static_cast<uint8_t>(new_k);
-      scale_at[1] = static_cast<uint8_t>(new_v);
-    }
+    __syncthreads();  // the old scales have been read; the next head writes the other tops
+    const uint32_t new_k = max(old_k, kv8_scale(max(max(top[0][0], top[0][1]), max(top[0][2], top[0][3]))));
+    const uint32_t new_v = max(old_v, kv8_scale(max(max(top[1][0], top[1][1]), max(top[1][2], top[1][3]))));
+    if (threadIdx.x == 0) *reinterpret_cast<uint16_t*>(scale_at) = static_cast<uint16_t>(new_k | new_v << 8);
     // Held tokens whose block's scale grows are rounded again, to the new one.
     if (lo > 0 && new_k > old_k) {
-      const float f = new_k - old_k > 40 ? 0.0f : __uint_as_float((127u + old_k - new_k) << 23);
+      const float f = fall_of(old_k, new_k);
       for (int i = threadIdx.x; i < lo * DK / 4; i += kNT) {
         uint32_t* w = reinterpret_cast<uint32_t*>(codes) + i;
         *w = rescale4(*w, f);
       }
     }
-    if (lo > 0 && new_v > old_v) {
-      const float f = new_v - old_v > 40 ? 0.0f : __uint_as_float((127u + old_v - new_v) << 23);
-      for (int i = threadIdx.x; i < DV * kBlk / 4; i += kNT) {
-        const int t = (i & 3) * 16 + ((i >> 2) & 3) * 4;  // word i of the rows: tokens t .. t + 3
-        if (t >= lo) continue;
-        uint32_t* w = reinterpret_cast<uint32_t*>(codes + kBlk * DK) + i;
-        const uint32_t was = *w, now = rescale4(was, f);
-        const uint32_t keep = lo - t >= 4 ? 0xffffffffu : (1u << (8 * (lo - t))) - 1u;
-        *w = (now & keep) | (was & ~keep);
-      }
-    }
     {
-      const int ch = threadIdx.x % TK::kChunks, r0 = threadIdx.x / TK::kChunks;
       const float f = kv8_inverse(new_k);
 #pragma unroll
-      for (int p = 0; p < TK::kPasses; ++p) {
-        const int t = r0 + p * TK::kRows;
-        if (r0 >= TK::kRows || t < lo || t >= hi) continue;
-        float y[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] = scaled(k[p][i], f);
-        *reinterpret_cast<uint2*>(codes + t * DK + ch * 8) =
-            make_uint2(encode4(y[0], y[1], y[2], y[3]), encode4(y[4], y[5], y[6], y[7]));
+      for (int p = 0; p < kPasses; ++p) {
+        const int t = r0 + p * kRows;
+        if (r0 >= kRows || t < lo || t >= hi) continue;
+        *reinterpret_cast<uint2*>(codes + t * DK + un.lo) = encode8(k0[p], f);
+        *reinterpret_cast<uint2*>(codes + t * DK + un.hi) = encode8(k1[p], f);
       }
     }
-    {  // V changes from rows of tokens to rows of dimensions through LDS
-      const int ch = threadIdx.x % TV::kChunks, r0 = threadIdx.x / TV::kChunks;
-      const float f = kv8_inverse(new_v);
+    const float f = kv8_inverse(new_v), fall = fall_of(old_v, new_v);
+    const bool grows = lo > 0 && new_v > old_v;
 #pragma unroll
-      for (int p = 0; p < TV::kPasses; ++p) {
-        const int t = r0 + p * TV::kRows;
-        if (r0 >= TV::kRows || t < lo || t >= hi) continue;
-        float y[8];
+    for (int p = 0; p < kTurns; ++p) {
+      const int i = threadIdx.x + p * kNT, d = (i >> 6) * 32 + (i & 3) * 8, w = (i >> 2) & 15, t = word_token(w);
+      if (i >= kItems || t >= hi || (t + 4 <= lo && !grows)) continue;
+      uint2 q[4];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] = scaled(v[p][i], f);
-        const uint32_t w[2] = {encode4(y[0], y[1], y[2], y[3]), encode4(y[4], y[5], y[6], y[7])};
+      for (int e = 0; e < 4; ++e) q[e] = encode8(v[p][e], f);
+      uint32_t* const to = reinterpret_cast<uint32_t*>(codes + kBlk * DK + d * kBlk) + w;
+      uint32_t out[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i)  // dimension 8 ch + i in row i * chunks + ch: no two lanes on a bank
-          vt[(i * TV::kChunks + ch) * kRowBytes + v_place(t)] = static_cast<uint8_t>(w[i >> 2] >> (8 * (i & 3)));
+      for (int half = 0; half < 2; ++half) {  // 4 tokens by 4 dimensions change places
+        const uint32_t q0 = half ? q[0].y : q[0].x, q1 = half ? q[1].y : q[1].x, q2 = half ? q[2].y : q[2].x, q3 = half ? q[3].y : q[3].x;
+        const uint32_t a01 = __builtin_amdgcn_perm(q1, q0, 0x05010400u), a23 = __builtin_amdgcn_perm(q3, q2, 0x05010400u);
+        const uint32_t b01 = __builtin_amdgcn_perm(q1, q0, 0x07030602u), b23 = __builtin_amdgcn_perm(q3, q2, 0x07030602u);
+        out[4 * half] = __builtin_amdgcn_perm(a23, a01, 0x05040100u);
+        out[4 * half + 1] = __builtin_amdgcn_perm(a23, a01, 0x07060302u);
+        out[4 * half + 2] = __builtin_amdgcn_perm(b23, b01, 0x05040100u);
+        out[4 * half + 3] = __builtin_amdgcn_perm(b23, b01, 0x07060302u);
       }
+      if (t < lo || t + 4 > hi) {  // some bytes are others'
+        uint32_t held = 0, fresh = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          held |= t + e < lo ? 0xffu << (8 * e) : 0u;
+          fresh |= t + e >= lo && t + e < hi ? 0xffu << (8 * e) : 0u;
+        }
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
+          const uint32_t was = to[x * (kBlk / 4)];
+          const uint32_t kept = grows ? rescale4(was, fall) : was;
+          out[x] = (out[x] & fresh) | (kept & held) | (was & ~(held | fresh));
+        }
+      }
+#pragma unroll
+      for (int x = 0; x < 8; ++x) to[x * (kBlk / 4)] = out[x];
     }
-    __syncthreads();  // also: held codes have been rewritten before bytes go in beside them
-    uint8_t* const to = codes + kBlk * DK;
-    if (hi - lo == kBlk) {
-      for (int i = threadIdx.x; i < DV * 4; i += kNT) {
-        const int d = i >> 2, row = (d & 7) * TV::kChunks + (d >> 3);
-        reinterpret_cast<uint4*>(to)[i] = *reinterpret_cast<const uint4*>(vt + row * kRowBytes + (i & 3) * 16);
-      }
-    } else {  // bytes: the others' stay as they are
-      for (int i = threadIdx.x; i < DV * (hi - lo); i += kNT) {
-        const int d = i % DV, t = lo + i / DV, row = (d & 7) * TV::kChunks + (d >> 3);
-        to[d * kBlk + v_place(t)] = vt[row * kRowBytes + v_place(t)];
+  }
+
+  if (a.Q_out) {
+    const int q0 = static_cast<int>(static_cast<int64_t>(a.HQ) * grp / groups), q1 = static_cast<int>(static_cast<int64_t>(a.HQ) * (grp + 1) / groups);
+    const raw* __restrict__ const from = static_cast<const raw*>(a.Q);
+    raw* __restrict__ const to = static_cast<raw*>(a.Q_out);
+#pragma unroll
+    for (int p = 0; p < kPasses; ++p) {
+      const int t = r0 + p * kRows;
+      if (r0 >= kRows || t < lo || t >= all) continue;
+      const raw* src = from + (row0 + t) * a.ldq;
+      raw* dst = to + (row0 + t) * a.HQ * DK;
+#pragma unroll 4
+      for (int h = q0; h < q1; ++h) {
+        float x[8], y[8];
+        load_cvt<Tag, 8>(src + static_cast<int64_t>(h) * DK + un.lo, x);
+        load_cvt<Tag, 8>(src + static_cast<int64_t>(h) * DK + un.hi, y);
+        turn(x, y, ang[p], un, pairs);
+        if (first + t >= S) {
+          make_nan(x);
+          make_nan(y);
+        }
+        store8<Tag>(dst + static_cast<int64_t>(h) * DK + un.lo, x);
+        store8<Tag>(dst + static_cast<int64_t>(h) * DK + un.hi, y);
       }
     }
   }
-  if (update && h == 0 && rest % nblk == 0) update_counts(c, s, b);
+  if (update && grp == 0 && rest % nblk == 0) update_counts(c, s, b);
+}
+
+// Few tokens (a decode step): a block of threads takes a sequence whole, so that one launch also
+// changes its length.  A wave takes the K or the V of one head, a unit of one token a
+// lane, then units of the queries; what does not depend on the position is loaded before the
+// position is known.
+constexpr int kFew = 4;  // tokens, by 16 units: a wave
+template <typename Tag, int DK, int DV>
+__global__ __launch_bounds__(1024) void append_few_kernel(Kv8 c, Kv8Append a) {
+  using raw = typename Tag::raw;
+  constexpr int NU = DK / 16;
+  const int64_t b = blockIdx.x, S = c.slots();
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = lane_id(), waves = blockDim.x >> 6;
+  const int T = static_cast<int>(a.T), items = 2 * c.HKV, q_items = a.Q_out ? T * a.HQ * NU : 0;
+  const bool pairs = a.pairs != 0;
+  const int u = lane % 16, tok = lane / 16;
+  float x[8], y[8], qx[8], qy[8];
+  auto load_item = [&](int item) __attribute__((always_inline)) {
+    const int h = item >> 1, is_v = item & 1;
+    if (item >= items || tok >= T || 16 * u >= (is_v ? DV : DK)) return;
+    const Unit un = is_v ? unit_of(u, DV, 0, false) : unit_of(u, DK, a.R, pairs);
+    const raw* src = is_v ? static_cast<const raw*>(a.V) + (b * T + tok) * a.ldv + static_cast<int64_t>(h) * DV
+                          : static_cast<const raw*>(a.K) + (b * T + tok) * a.ldk + static_cast<int64_t>(h) * DK;
+    load_cvt<Tag, 8>(src + un.lo, x);
+    load_cvt<Tag, 8>(src + un.hi, y);
+  };
+  auto load_query = [&](int i) __attribute__((always_inline)) {
+    if (i >= q_items) return;
+    const int row = i / NU;
+    const Unit un = unit_of(i % NU, DK, a.R, pairs);
+    const raw* src = static_cast<const raw*>(a.Q) + (b * T + row / a.HQ) * a.ldq + static_cast<int64_t>(row % a.HQ) * DK;
+    load_cvt<Tag, 8>(src + un.lo, qx);
+    load_cvt<Tag, 8>(src + un.hi, qy);
+  };
+  load_item(wave);
+  load_query(threadIdx.x);
+  const Span s = span_of(c, a, b);
+  const int64_t blk0 = s.have / kBlk;
+  // the first item's place and scales, ahead of the queries
+  const int64_t at0 = s.have < s.end && wave < items ? kv8_block(c, b, blk0, wave >> 1) : -1;
+  const uint32_t old0 = at0 >= 0 ? c.scales[at0 * 2 + (wave & 1)] : 0u;
+
+  for (int i = threadIdx.x; i < q_items; i += blockDim.x) {
+    if (i != static_cast<int>(threadIdx.x)) load_query(i);
+    const int row = i / NU, t = row / a.HQ;
+    const Unit un = unit_of(i % NU, DK, a.R, pairs);
+    Angles g;
+    load_angles(a, un, min(s.have + t, S - 1), g);
+    turn(qx, qy, g, un, pairs);
+    if (s.have + t >= S) {
+      make_nan(qx);
+      make_nan(qy);
+    }
+    raw* to = static_cast<raw*>(a.Q_out) + (b * T * a.HQ + row) * DK;
+    store8<Tag>(to + un.lo, qx);
+    store8<Tag>(to + un.hi, qy);
+  }
+
+  const int nblk = static_cast<int>((s.have + T - 1) / kBlk - blk0) + 1;
+  for (int item = wave; item < items; item += waves) {
+    if (item != wave) load_item(item);
+    const int h = item >> 1, is_v = item & 1;
+    const bool has = tok < T && 16 * u < (is_v ? DV : DK);
+    const Unit un = is_v ? unit_of(u, DV, 0, false) : unit_of(u, DK, a.R, pairs);
+    uint32_t top = 0;
+    if (has) {
+      if (!is_v) {
+        Angles g;
+        load_angles(a, un, min(s.have + tok, S - 1), g);
+        turn(x, y, g, un, pairs);
+        if (a.K_out) {
+          if (s.have + tok >= S) {
+            make_nan(x);
+            make_nan(y);
+          }
+          raw* to = static_cast<raw*>(a.K_out) + ((b * T + tok) * c.HKV + h) * DK;
+          store8<Tag>(to + un.lo, x);
+          store8<Tag>(to + un.hi, y);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) top = max(top, max(finite_bits(x[i]), finite_bits(y[i])));
+    }
+    for (int n = 0; n < nblk; ++n) {  // the one or two blocks that the tokens lie on
+      const int64_t first = (blk0 + n) * kBlk;
+      if (first >= s.end) break;
+      const bool known = item == wave && n == 0;
+      const int64_t at = known ? at0 : kv8_block(c, b, blk0 + n, h);
+      const int lo = static_cast<int>(max(s.have - first, int64_t{0}));
+      const int hi = static_cast<int>(min(s.end - first, int64_t{kBlk}));
+      if (at < 0 || lo >= hi) continue;  // the same for the whole wave
+      uint8_t* const codes = c.codes + at * c.block_bytes() + (is_v ? kBlk * DK : 0);
+      uint8_t* const scale_at = c.scales + at * 2 + is_v;
+      const int t = static_cast<int>(s.have + tok - first);
+      const bool mine = has && t >= lo && t < hi;
+      const uint32_t old = lo == 0 ? 0u : known ? old0 : *scale_at;
+      const uint32_t now = max(old, kv8_scale(wave_max_bits(mine ? top : 0u)));
+      if (lane == 0) *scale_at = static_cast<uint8_t>(now);
+      if (lo > 0 && now > old) {  // the block's held tokens, 4 codes a lane
+        const float f = fall_of(old, now);
+        for (int i = lane; i < (is_v ? DV * kBlk : lo * DK) / 4; i += kWave) {
+          const int first_t = is_v ? word_token(i & 15) : 0;
+          if (is_v && first_t >= lo) continue;
+          uint32_t* w = reinterpret_cast<uint32_t*>(codes) + i;
+          const uint32_t was = *w, keep = is_v && lo - first_t < 4 ? (1u << (8 * (lo - first_t))) - 1u : 0xffffffffu;
+          *w = (rescale4(was, f) & keep) | (was & ~keep);
+        }
+        __threadfence();  // before bytes go in beside them
+      }
+      if (!mine) continue;
+      const uint2 p = encode8(x, kv8_inverse(now)), q = encode8(y, kv8_inverse(now));
+      if (!is_v) {
+        *reinterpret_cast<uint2*>(codes + t * DK + un.lo) = p;
+        *reinterpret_cast<uint2*>(codes + t * DK + un.hi) = q;
+      } else {
+        const uint32_t w[4] = {p.x, p.y, q.x, q.y};
+        uint8_t* to = codes + v_place(t);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) to[((i < 8 ? un.lo : un.hi) + (i & 7)) * kBlk] = static_cast<uint8_t>(w[i >> 2] >> (8 * (i & 3)));
+      }
+    }
+  }
+  __syncthreads();  // every wave has read the length
+  if (threadIdx.x == 0) {
+    int32_t lost = static_cast<int32_t>(s.many - (s.end - s.have));
+    for (int n = 0; n < nblk && (blk0 + n) * kBlk < s.end; ++n)
+      if (kv8_block(c, b, blk0 + n, 0) < 0)
+        lost += static_cast<int32_t>(min(s.end, (blk0 + n + 1) * kBlk) - max(s.have, (blk0 + n) * kBlk));
+    c.length[b] = static_cast<int32_t>(s.end);
+    if (lost) c.lost[b] += lost;
+  }
 }
 
 // The counters of an append whose blocks read them.
@@ -292,56 +484,123 @@ __global__ __launch_bounds__(kNT) void append_counts_kernel(Kv8 c, Kv8Append a) 
   update_counts(c, span_of(c, a, blockIdx.x), blockIdx.x);
 }
 
-// Slots back as values, 8 elements of one head's K or V a thread; zeros for a slot
-// that holds nothing.
+// Slots back as values; zeros for a slot that holds nothing.  A block of threads takes 64
+// entries of a list, one head.  Where they are one block's slots in order (as
+// the first N slots are, and runs that begin with a block), a thread takes 4 tokens by 8
+// dimensions of V from words of 4 tokens; else it gathers bytes.
+__device__ __forceinline__ void decode8(uint32_t w0, uint32_t w1, float f, float (&x)[8]) {
+  const f32x2 a = __builtin_amdgcn_cvt_pk_f32_fp8(w0, false), b = __builtin_amdgcn_cvt_pk_f32_fp8(w0, true);
+  const f32x2 c = __builtin_amdgcn_cvt_pk_f32_fp8(w1, false), d = __builtin_amdgcn_cvt_pk_f32_fp8(w1, true);
+  x[0] = a[0] * f; x[1] = a[1] * f; x[2] = b[0] * f; x[3] = b[1] * f;
+  x[4] = c[0] * f; x[5] = c[1] * f; x[6] = d[0] * f; x[7] = d[1] * f;
+}
+
 template <typename Tag>
-__global__ __launch_bounds__(kNT) void rows_kernel(Kv8 c, const int32_t* __restrict__ slots, int64_t N,
+__global__ __launch_bounds__(kNT) void rows_kernel(Kv8 c, const int32_t* __restrict__ slots, int64_t N, uint32_t lists,
                                                    typename Tag::raw* __restrict__ K, typename Tag::raw* __restrict__ V) {
-  const int kc = c.DK / 8, per = kc + c.DV / 8;
-  const int64_t i = blockIdx.x * static_cast<int64_t>(kNT) + threadIdx.x;
-  if (i >= c.B * N * c.HKV * per) return;
-  const int ch = static_cast<int>(i % per);
-  const int64_t row = i / per, bn = row / c.HKV, b = bn / N;
-  const int h = static_cast<int>(row % c.HKV);
-  const int64_t slot = slots ? static_cast<int64_t>(slots[bn]) : bn % N;
-  float x[8] = {};
-  if (slot >= 0 && slot < kv8_length(c, b)) {
-    const int64_t at = kv8_block(c, b, slot >> 6, h);
+  __shared__ int32_t slot_of[kBlk];
+  __shared__ bool in_order;
+  const int h = blockIdx.x % c.HKV;
+  const uint32_t rest = blockIdx.x / c.HKV;
+  const int64_t b = rest / lists, n0 = static_cast<int64_t>(rest % lists) * kBlk;
+  const int many = static_cast<int>(min(N - n0, int64_t{kBlk}));
+  const int32_t length = kv8_length(c, b);
+  if (threadIdx.x < kBlk) {  // the first wave
+    const int i = min(static_cast<int>(threadIdx.x), many - 1);
+    const int32_t mine = slots ? slots[b * N + n0 + i] : static_cast<int32_t>(n0 + i);
+    slot_of[threadIdx.x] = mine;
+    const bool runs = ballot(mine != __builtin_amdgcn_readfirstlane(mine) + i) == 0;
+    if (threadIdx.x == 0) in_order = runs;
+  }
+  __syncthreads();
+  const int32_t first = slot_of[0];
+  const bool run = in_order && first >= 0 && first < length && first % kBlk == 0;
+  const int kc = c.DK / 8, vc = c.DV / 8;
+  if (run) {
+    const int64_t at = kv8_block(c, b, first >> 6, h);
+    const uint8_t* codes = c.codes + at * c.block_bytes();
+    const int held = at < 0 ? 0 : min(many, length - first);  // entries that hold something
+    const float fk = at < 0 ? 0.0f : __uint_as_float(static_cast<uint32_t>(c.scales[at * 2]) << 23);
+    const float fv = at < 0 ? 0.0f : __uint_as_float(static_cast<uint32_t>(c.scales[at * 2 + 1]) << 23);
+    for (int i = threadIdx.x; i < many * kc; i += kNT) {
+      const int t = i / kc, d = i % kc * 8;
+      float x[8] = {};
+      if (t < held) {
+        const uint2 w = *reinterpret_cast<const uint2*>(codes + t * c.DK + d);
+        decode8(w.x, w.y, fk, x);
+      }
+      store8<Tag>(K + ((b * N + n0 + t) * c.HKV + h) * c.DK + d, x);
+    }
+    for (int i = threadIdx.x; i < 16 * vc; i += kNT) {
+      const int d = (i >> 6) * 32 + (i & 3) * 8, w = (i >> 2) & 15, t = word_token(w);
+      if (t >= many) continue;
+      uint32_t q[8] = {};
+      if (t < held) {
+        const uint32_t* from = reinterpret_cast<const uint32_t*>(codes + kBlk * c.DK + d * kBlk) + w;
+#pragma unroll
+        for (int x = 0; x < 8; ++x) q[x] = from[x * (kBlk / 4)];
+      }
+      uint32_t o[2][4];  // 4 dimensions by 4 tokens change places
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const uint32_t a01 = __builtin_amdgcn_perm(q[4 * half + 1], q[4 * half], 0x05010400u), a23 = __builtin_amdgcn_perm(q[4 * half + 3], q[4 * half + 2], 0x05010400u);
+        const uint32_t b01 = __builtin_amdgcn_perm(q[4 * half + 1], q[4 * half], 0x07030602u), b23 = __builtin_amdgcn_perm(q[4 * half + 3], q[4 * half + 2], 0x07030602u);
+        o[half][0] = __builtin_amdgcn_perm(a23, a01, 0x05040100u);
+        o[half][1] = __builtin_amdgcn_perm(a23, a01, 0x07060302u);
+        o[half][2] = __builtin_amdgcn_perm(b23, b01, 0x05040100u);
+        o[half][3] = __builtin_amdgcn_perm(b23, b01, 0x07060302u);
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (t + e >= many) break;
+        float x[8] = {};
+        if (t + e < held) decode8(o[0][e], o[1][e], fv, x);
+        store8<Tag>(V + ((b * N + n0 + t + e) * c.HKV + h) * c.DV + d, x);
+      }
+    }
+    return;
+  }
+  for (int i = threadIdx.x; i < many * (kc + vc); i += kNT) {
+    const int t = i / (kc + vc), ch = i % (kc + vc);
+    const int32_t slot = slot_of[t];
+    const int64_t row = (b * N + n0 + t) * c.HKV + h;
+    float x[8] = {};
+    const int64_t at = slot >= 0 && slot < length ? kv8_block(c, b, slot >> 6, h) : -1;
     if (at >= 0) {
       const uint8_t* codes = c.codes + at * c.block_bytes();
-      const int t = static_cast<int>(slot & 63);
-      uint32_t w[2];
+      const float f = __uint_as_float(static_cast<uint32_t>(c.scales[at * 2 + (ch < kc ? 0 : 1)]) << 23);
       if (ch < kc) {
-        const uint2 u = *reinterpret_cast<const uint2*>(codes + t * c.DK + ch * 8);
-        w[0] = u.x;
-        w[1] = u.y;
+        const uint2 w = *reinterpret_cast<const uint2*>(codes + (slot & 63) * c.DK + ch * 8);
+        decode8(w.x, w.y, f, x);
       } else {
-        const uint8_t* from = codes + kBlk * c.DK + (ch - kc) * 8 * kBlk + v_place(t);
+        const uint8_t* from = codes + kBlk * c.DK + (ch - kc) * 8 * kBlk + v_place(slot & 63);
+        uint32_t w[2];
 #pragma unroll
         for (int j = 0; j < 2; ++j)
           w[j] = from[(4 * j) * kBlk] | from[(4 * j + 1) * kBlk] << 8 | from[(4 * j + 2) * kBlk] << 16 |
                  static_cast<uint32_t>(from[(4 * j + 3) * kBlk]) << 24;
-      }
-      const float f = __uint_as_float(static_cast<uint32_t>(c.scales[at * 2 + (ch < kc ? 0 : 1)]) << 23);
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const f32x2 a = __builtin_amdgcn_cvt_pk_f32_fp8(w[j], false), d = __builtin_amdgcn_cvt_pk_f32_fp8(w[j], true);
-        x[4 * j] = a[0] * f; x[4 * j + 1] = a[1] * f; x[4 * j + 2] = d[0] * f; x[4 * j + 3] = d[1] * f;
+        decode8(w[0], w[1], f, x);
       }
     }
+    if (ch < kc) store8<Tag>(K + row * c.DK + ch * 8, x);
+    else store8<Tag>(V + row * c.DV + (ch - kc) * 8, x);
   }
-  if (ch < kc) store8<Tag>(K + row * c.DK + ch * 8, x);
-  else store8<Tag>(V + row * c.DV + (ch - kc) * 8, x);
 }
 
 template <typename Tag, int DK, int DV>
 hipError_t append_dims(const Kv8& c, const Kv8Append& a, hipStream_t stream) {
+  if (a.T <= kFew) {
+    const int64_t items = 2 * c.HKV + (a.Q_out ? a.T * a.HQ * (DK / 16) / kWave : 0);
+    const int waves = items >= 16 ? 16 : items >= 8 ? 8 : 4;
+    append_few_kernel<Tag, DK, DV><<<static_cast<uint32_t>(c.B), waves * kWave, 0, stream>>>(c, a);
+    return hipGetLastError();
+  }
   const int nblk = static_cast<int>((a.T + kBlk - 2) / kBlk + 1);
-  const uint32_t kv = static_cast<uint32_t>(c.B * c.HKV * nblk);
-  const int64_t q_items = a.Q_out ? c.B * a.T * a.HQ * (DK / 8) : 0;
-  const uint32_t grid = kv + static_cast<uint32_t>((q_items + kNT - 1) / kNT);
+  // the angles are loaded once for the heads of a group: as many as leave four blocks a compute unit
+  const int64_t want = 16 * int64_t{device_cus() > 0 ? device_cus() : 256}, blocks = c.B * nblk;
+  const int groups = static_cast<int>(blocks * c.HKV <= want ? c.HKV : (want + blocks - 1) / blocks);
+  append_kernel<Tag, DK, DV><<<static_cast<uint32_t>(blocks * groups), kNT, 0, stream>>>(c, a, nblk, groups, a.start != nullptr);
   // where the blocks read the length to find their place, a launch of its own changes it
-  append_kernel<Tag, DK, DV><<<grid, kNT, 0, stream>>>(c, a, nblk, kv, a.start != nullptr);
   if (!a.start) append_counts_kernel<<<static_cast<uint32_t>(c.B), kNT, 0, stream>>>(c, a);
   return hipGetLastError();
 }
@@ -377,11 +636,11 @@ hipError_t launch_kv8_append(const Kv8& c, const Kv8Append& a, int dtype, hipStr
 hipError_t launch_kv8_rows(const Kv8& c, const int32_t* slots, int64_t N, int dtype, void* K, void* V,
                            hipStream_t stream) {
   if (c.B == 0 || N == 0) return hipSuccess;
-  const int64_t items = c.B * N * c.HKV * ((c.DK + c.DV) / 8);
-  const uint32_t grid = static_cast<uint32_t>((items + kNT - 1) / kNT);
-  if (dtype == 0) rows_kernel<F32><<<grid, kNT, 0, stream>>>(c, slots, N, static_cast<float*>(K), static_cast<float*>(V));
-  else if (dtype == 1) rows_kernel<BF16><<<grid, kNT, 0, stream>>>(c, slots, N, static_cast<uint16_t*>(K), static_cast<uint16_t*>(V));
-  else rows_kernel<F16><<<grid, kNT, 0, stream>>>(c, slots, N, static_cast<uint16_t*>(K), static_cast<uint16_t*>(V));
+  const uint32_t lists = static_cast<uint32_t>((N + kBlk - 1) / kBlk);
+  const uint32_t grid = static_cast<uint32_t>(c.B * lists * c.HKV);
+  if (dtype == 0) rows_kernel<F32><<<grid, kNT, 0, stream>>>(c, slots, N, lists, static_cast<float*>(K), static_cast<float*>(V));
+  else if (dtype == 1) rows_kernel<BF16><<<grid, kNT, 0, stream>>>(c, slots, N, lists, static_cast<uint16_t*>(K), static_cast<uint16_t*>(V));
+  else rows_kernel<F16><<<grid, kNT, 0, stream>>>(c, slots, N, lists, static_cast<uint16_t*>(K), static_cast<uint16_t*>(V));
   return hipGetLastError();
 }
 

@@ -645,7 +645,7 @@ int dsa_kv8_append(const dsa_kv8_cache* cache, const void* K, const void* V, con
  * The values that N slots of each sequence stand for, K [B,N,HKV,DK] and V [B,N,HKV,DV] of
  * dtype (exact in fp32 and bf16; fp16 rounds, to Inf past its range): slots [B,N], or
  * 0 .. N-1 where null.  Slots outside [0, length) give zeros.  K and V 16-byte aligned;
- * B*N*HKV*(DK+DV)/8 < 2^31.
+ * B*HKV*ceil(N/64) < 2^24.
  */
 int dsa_kv8_rows(const dsa_kv8_cache* cache, const int32_t* slots, int64_t N, int dtype, void* K, void* V,
                  void* stream);

@@ -88,7 +88,7 @@ def test_append_refusals(changes, needle):
 
 
 @pytest.mark.parametrize("changes, needle", [
-    (dict(_1=-1), "N="), (dict(_1=1 << 40), "N="), (dict(_1=1 << 25), "2^31"), (dict(_2=L.DSA_FP8), "dtype"),
+    (dict(_1=-1), "N="), (dict(_1=1 << 40), "N="), (dict(_1=1 << 28), "2^24"), (dict(_2=L.DSA_FP8), "dtype"),
     (dict(_3=None), "null"), (dict(_4=None), "null"), (dict(_3=FAKE + 8), "aligned"), (dict(_0=FAKE + 2), "aligned"),
 ])
 def test_rows_refusals(changes, needle):
