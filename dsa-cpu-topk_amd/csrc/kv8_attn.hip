@@ -674,9 +674,12 @@ Plan plan_of(const Kv8& c, int64_t Tq, int HQ, int64_t n, int64_t window, int64_
     most = near < most ? near : most;
   }
   const int64_t steps = most > waves ? (most + waves - 1) / waves : 1;
-  const int64_t blocks = c.B * c.HKV * p.row_tiles;
+  // as many splits as all run at once: the chunks go over 8 XCDs in equal numbers, and
+  // one that waits for a place doubles the time (2 x 33 blocks an XCD of 2 x 32 places:
+  // 35 us for what takes 20 in 60)
   const int64_t room = (c.DK <= 128 ? 2 : 1) * int64_t{device_cus() > 0 ? device_cus() : 256};
-  int64_t splits = blocks < 1 || blocks >= room ? 1 : room / blocks;
+  const int64_t chunks = rows < 1 ? 0 : room / p.row_tiles / 8 * 8, pairs = c.B * c.HKV;
+  int64_t splits = pairs < 1 || pairs >= chunks ? 1 : chunks / pairs;
   splits = splits > steps ? steps : splits;
   p.splits = static_cast<int>(splits > kMaxSplits ? kMaxSplits : splits);
   auto up = [](int64_t v) { return (v + 255) / 256 * 256; };

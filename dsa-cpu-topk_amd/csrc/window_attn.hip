@@ -10,6 +10,8 @@
 //   S^T = K . Q^T,  O^T = V^T . P^T,
 // so that P goes from the first product's registers into the second one's, and the
 // softmax is one pass with a running maximum and sum in fp32.
+#include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include "kv8.h"
@@ -24,7 +26,8 @@ struct Win {
   const int32_t* count;
   int64_t B, ldq, ldk, ldv;
   int T, HQ, G, window, sinks;
-  float scale_log2;
+  float scale_log2;  // positive: times a masked -Inf it is one
+  uint32_t flip;     // Q's sign bits, where the scale is negative
 };
 
 // What of the tiles of KT keys a block of TQ queries from t0 on walks.
@@ -73,6 +76,17 @@ int64_t blocks_of(const Win& a) {
   return (a.B * (a.HQ / a.G) + 7) / 8 * 8 * a.G * ntile;
 }
 
+__device__ __forceinline__ float mul(float x, float y) {  // rounded by itself
+#pragma clang fp contract(off)
+  return x * y;
+}
+// 2^(x scale - ref).  An fma keeps x scale whole, where ref, the maximum's product, was
+// rounded: at logits of 2^28 and more all p of a row are then beyond or below a 16-bit
+// type, which leaves no finite result, and the careful pass rounds each as ref was.
+template <bool CAREFUL>
+__device__ __forceinline__ float weight(float x, float scale, float ref) {
+  return __builtin_amdgcn_exp2f(CAREFUL ? mul(x, scale) - ref : fmaf(x, scale, -ref));
+}
 __device__ __forceinline__ bool finite_f32(float x) { return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u; }
 // Bit 15 of each half that is Inf or NaN.
 template <typename Tag>
@@ -110,7 +124,6 @@ __global__ __launch_bounds__(kNT, D == 256 ? 1 : 2) void window_kernel(Win a) {
   using L = TileLds<D>;
   constexpr int TQ = 64 * QT, NKS = D / 32, NDT = D / 16;
   constexpr int KJ = D == 256 ? 1 : 4;           // 16-key tiles whose K fragments are read at once
-  constexpr int VG = NDT < 4 ? NDT : 4;          // 16-dim tiles whose V fragments are
   constexpr int PW = L::BYTES / 1024 / (kNT / kWave);
   __shared__ __align__(16) uint8_t k0[L::BYTES], k1[L::BYTES], v0[L::BYTES], v1[L::BYTES];
 
@@ -152,7 +165,7 @@ __global__ __launch_bounds__(kNT, D == 256 ? 1 : 2) void window_kernel(Win a) {
     tq[qt] = tw + 16 * qt + c16;
     const raw* q = Qb + min(tq[qt], T - 1) * a.ldq;
 #pragma unroll
-    for (int ks = 0; ks < NKS; ++ks) qf[qt][ks] = *reinterpret_cast<const u32x4*>(q + 32 * ks + 8 * g);
+    for (int ks = 0; ks < NKS; ++ks) qf[qt][ks] = *reinterpret_cast<const u32x4*>(q + 32 * ks + 8 * g) ^ a.flip;
   }
   int kofs[NKS], vofs[NDT];  // LDS reads within a tile
 #pragma unroll
@@ -168,6 +181,7 @@ __global__ __launch_bounds__(kNT, D == 256 ? 1 : 2) void window_kernel(Win a) {
   float m[QT], lpart[QT];
   auto run = [&](auto careful) __attribute__((always_inline)) {
     constexpr bool CAREFUL = decltype(careful)::value;
+    constexpr int VG = NDT < 4 || CAREFUL ? 2 : 4;  // 16-dim tiles whose V fragments are read at once
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt) {
       m[qt] = -INFINITY;
@@ -215,15 +229,12 @@ __global__ __launch_bounds__(kNT, D == 256 ? 1 : 2) void window_kernel(Win a) {
             const int s = 16 * (e >> 2) + (e & 3);
             const bool yes = s <= far && (s > near || s < sink);
             ok[qt] |= yes ? 1u << e : 0u;
-            st[e >> 2][qt][e & 3] = yes ? st[e >> 2][qt][e & 3] * a.scale_log2 : -INFINITY;
+            st[e >> 2][qt][e & 3] = yes ? st[e >> 2][qt][e & 3] : -INFINITY;
           }
-        } else {
-#pragma unroll
-          for (int e = 0; e < 16; ++e) st[e >> 2][qt][e & 3] *= a.scale_log2;
         }
 #pragma unroll
         for (int e = 0; e < 16; ++e) mx = fmaxf(mx, st[e >> 2][qt][e & 3]);
-        mx = max_xor32(max_xor16(mx));
+        mx = mul(max_xor32(max_xor16(mx)), a.scale_log2);
         // the maximum moves when a tile's passes it by 2^8: p then stays far below overflow
         const bool up = mx > m[qt] + 8.f;
         const float m_new = up ? mx : m[qt];
@@ -232,7 +243,7 @@ __global__ __launch_bounds__(kNT, D == 256 ? 1 : 2) void window_kernel(Win a) {
         m[qt] = m_new;
         const float ref = m_new == -INFINITY ? 0.f : m_new;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) st[e >> 2][qt][e & 3] = __builtin_amdgcn_exp2f(st[e >> 2][qt][e & 3] - ref);
+        for (int e = 0; e < 16; ++e) st[e >> 2][qt][e & 3] = weight<CAREFUL>(st[e >> 2][qt][e & 3], a.scale_log2, ref);
 #pragma unroll
         for (int jj = 0; jj < 2; ++jj)
           pf[qt][jj] = u32x4{M::pack(st[2 * jj][qt][0], st[2 * jj][qt][1]), M::pack(st[2 * jj][qt][2], st[2 * jj][qt][3]),
@@ -321,7 +332,7 @@ __global__ __launch_bounds__(kNT, D == 256 ? 1 : 2) void window_kernel(Win a) {
       __builtin_amdgcn_sched_barrier(0);
       const int s0 = walk.tile(v) * kKT, s1 = s0 + kKT - 1;
       if (s0 <= wave_last && (s1 > tw - window || s0 < sinks)) {
-        if (s1 <= tw && (s0 > wave_last - window || s1 < sinks)) compute(std::false_type{}, s0, kc, vc);
+        if (!CAREFUL && s1 <= tw && (s0 > wave_last - window || s1 < sinks)) compute(std::false_type{}, s0, kc, vc);
         else compute(std::true_type{}, s0, kc, vc);
       }
       wait_dma_keep<0>();
@@ -337,7 +348,9 @@ __global__ __launch_bounds__(kNT, D == 256 ? 1 : 2) void window_kernel(Win a) {
   bool odd = false;
 #pragma unroll
   for (int qt = 0; qt < QT; ++qt) {
+    const float l = sum_xor32(sum_xor16(lpart[qt]));
     if (tq[qt] >= n) continue;
+    odd |= !(l > 0.0f && finite_f32(l));
 #pragma unroll
     for (int dt = 0; dt < NDT; ++dt)
 #pragma unroll
@@ -357,149 +370,301 @@ __global__ __launch_bounds__(kNT, D == 256 ? 1 : 2) void window_kernel(Win a) {
 }
 
 // ---------------------------------------------------------------------------
-// fp32: 16x16x4 fp32 products, 64 queries a block (a wave 16).  Tiles of KT keys; rows
-// lie in LDS as they are, padded by 4 elements so that neither reading hits a bank twice.
-// K-slots: element i of a lane's 16 bytes of K is step i (dims 16kk + 4g + i), token
-// 16j + 4g + r is step r of P's.
+// fp32: every operand as three bf16 pieces (8 bits each, to the nearest: 24 together),
+// six of the nine products (those dropped are below 2^-25 of the whole) on the 16-bit
+// matrix instructions: 96 cycles where the fp32 ones take 256.  K and V are split once for
+// a block's queries, on the way into LDS; the next tile's rows wait in registers.
+//
+// Pieces of Inf are no numbers, and a p of 0 carries a NaN or Inf of V: a block whose result
+// is not finite is run again on the fp32 matrix instructions, with V's non-finite elements
+// taken out of the product and added to the rows that see them.
 // ---------------------------------------------------------------------------
-template <int D, int KT>
-__global__ __launch_bounds__(kNT) void window_f32_kernel(Win a) {
-  constexpr int TQ = 64, NKK = D / 16, NDT = D / 16, NJ = KT / 16, LD = D + 4;
-  __shared__ __align__(16) float kt_[KT * LD], vt_[KT * LD];
-  const int tid = threadIdx.x, wave = tid >> 6, lane = lane_id(), g = lane >> 4, c16 = lane & 15;
+struct Three {
+  uint32_t h, m, l;  // two elements' pieces
+};
+__device__ __forceinline__ Three split3(float x, float y) {
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  Three t;
+  t.h = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{x, y}), bf16x2));
+  x -= __uint_as_float(t.h << 16);
+  y -= __uint_as_float(t.h & 0xffff0000u);
+  t.m = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{x, y}), bf16x2));
+  x -= __uint_as_float(t.m << 16);
+  y -= __uint_as_float(t.m & 0xffff0000u);
+  t.l = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{x, y}), bf16x2));
+  return t;
+}
+// a . b, the small products first.
+__device__ __forceinline__ f32x4 dot3(const u32x4 (&a)[3], const u32x4 (&b)[3], f32x4 c) {
+  using M = Mfma16x16x32<BF16>;
+  c = M::run(a[0], b[2], c);
+  c = M::run(a[2], b[0], c);
+  c = M::run(a[1], b[1], c);
+  c = M::run(a[0], b[1], c);
+  c = M::run(a[1], b[0], c);
+  return M::run(a[0], b[0], c);
+}
+
+template <int D, int QT, int KT>
+__global__ __launch_bounds__(kNT, D == 256 ? 1 : 2) void window_f32_kernel(Win a) {
+  using L = TileLds<D, KT>;
+  constexpr int TQ = 64 * QT, NKS = D / 32, NDT = D / 16, NJ = KT / 16;
+  constexpr int PER = KT * D / 8 / kNT;  // 8-element chunks of a tile a thread, of K and of V
+  constexpr int LD = D + 4;              // fp32 rows of the careful pass
+  static_assert(PER >= 1 && 16 * LD * 4 <= 3 * L::BYTES);
+  __shared__ __align__(16) uint8_t kl[3 * L::BYTES], vl[3 * L::BYTES];
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int lane = lane_id(), g = lane >> 4, c16 = lane & 15;
   int t0, h;
   int64_t b;
   if (!place<TQ>(a, t0, b, h)) return;
   const Walk walk = walk_of<TQ, KT>(a, b, t0);
   const int T = a.T, n = walk.n, window = a.window, sinks = a.sinks;
-  const int tw = t0 + 16 * wave, wave_last = min(tw + 15, n - 1), tq = tw + c16;
-  const float* kb = static_cast<const float*>(a.K) + b * T * a.ldk + static_cast<int64_t>(h / a.G) * D;
-  const float* vb = static_cast<const float*>(a.V) + b * T * a.ldv + static_cast<int64_t>(h / a.G) * D;
-  f32x4 q[NKK];
-  {
-    const float* src = static_cast<const float*>(a.Q) + (b * T + min(tq, T - 1)) * a.ldq + static_cast<int64_t>(h) * D;
+  const int tw = t0 + 16 * QT * wave, wave_last = min(tw + 16 * QT - 1, n - 1);
+  const float* const kb = static_cast<const float*>(a.K) + b * T * a.ldk + static_cast<int64_t>(h / a.G) * D;
+  const float* const vb = static_cast<const float*>(a.V) + b * T * a.ldv + static_cast<int64_t>(h / a.G) * D;
+  const float* const qb = static_cast<const float*>(a.Q) + b * T * a.ldq + static_cast<int64_t>(h) * D;
+
+  f32x4 kx[PER][2], vx[PER][2];
+  auto fetch = [&](int kt) __attribute__((always_inline)) {  // rows past the sequence: zeros
+    const __amdgpu_buffer_rsrc_t kr = rows_rsrc(reinterpret_cast<const char*>(kb), kt * KT, n, static_cast<uint32_t>(a.ldk) * 4u);
+    const __amdgpu_buffer_rsrc_t vr = rows_rsrc(reinterpret_cast<const char*>(vb), kt * KT, n, static_cast<uint32_t>(a.ldv) * 4u);
 #pragma unroll
-    for (int kk = 0; kk < NKK; ++kk) q[kk] = *reinterpret_cast<const f32x4*>(src + 16 * kk + 4 * g);
+    for (int i = 0; i < PER; ++i) {
+      const int c = tid + i * kNT, r = c / L::NCH, d = c % L::NCH * 32;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        kx[i][e] = buffer_load_f32x4(kr, static_cast<int>(r * static_cast<uint32_t>(a.ldk) * 4u) + d + 16 * e, 0, 0);
+        vx[i][e] = buffer_load_f32x4(vr, static_cast<int>(r * static_cast<uint32_t>(a.ldv) * 4u) + d + 16 * e, 0, 0);
+      }
+    }
+  };
+  auto split = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int c = tid + i * kNT, r = c / L::NCH, ch = c % L::NCH;
+      u32x4 k3[3], v3[3];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const Three k = split3(kx[i][e >> 1][2 * (e & 1)], kx[i][e >> 1][2 * (e & 1) + 1]);
+        const Three v = split3(vx[i][e >> 1][2 * (e & 1)], vx[i][e >> 1][2 * (e & 1) + 1]);
+        k3[0][e] = k.h; k3[1][e] = k.m; k3[2][e] = k.l;
+        v3[0][e] = v.h; v3[1][e] = v.m; v3[2][e] = v.l;
+      }
+#pragma unroll
+      for (int p = 0; p < 3; ++p) {
+        *reinterpret_cast<u32x4*>(kl + p * L::BYTES + r * 2 * D + 16 * (ch ^ L::swz_k(r))) = k3[p];
+        *reinterpret_cast<u32x4*>(vl + p * L::BYTES + r * 2 * D + 16 * (ch ^ L::swz_v(r))) = v3[p];
+      }
+    }
+  };
+
+  u32x4 q[QT][NKS][3];
+  int tq[QT];
+#pragma unroll
+  for (int qt = 0; qt < QT; ++qt) {
+    tq[qt] = tw + 16 * qt + c16;
+    const float* src = qb + min(tq[qt], T - 1) * a.ldq + 8 * g;
+#pragma unroll
+    for (int ks = 0; ks < NKS; ++ks) {
+      float x[8];
+      load_f32<8>(src + 32 * ks, x);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const Three t = split3(__uint_as_float(__float_as_uint(x[2 * e]) ^ a.flip), __uint_as_float(__float_as_uint(x[2 * e + 1]) ^ a.flip));
+        q[qt][ks][0][e] = t.h; q[qt][ks][1][e] = t.m; q[qt][ks][2][e] = t.l;
+      }
+    }
   }
-  f32x4 o[NDT];
-  float m, l;
-  auto run = [&](auto careful) __attribute__((always_inline)) {
-    constexpr bool CAREFUL = decltype(careful)::value;
-    m = -INFINITY;
-    l = 0.0f;
+  f32x4 o[NDT][QT];
+  float m[QT], l[QT];
+  auto clear = [&]() {
 #pragma unroll
-    for (int d = 0; d < NDT; ++d) o[d] = f32x4{0, 0, 0, 0};
-    for (int v = 0; v < walk.total; ++v) {
-      const int s0 = walk.tile(v) * KT, s1 = s0 + KT - 1;
+    for (int qt = 0; qt < QT; ++qt) {
+      m[qt] = -INFINITY;
+      l[qt] = 0.0f;
+#pragma unroll
+      for (int d = 0; d < NDT; ++d) o[d][qt] = f32x4{0, 0, 0, 0};
+    }
+  };
+  // Logits of nj 16-key tiles from s0 on into exponentials (of one: the careful pass), the sums
+  // scaled by what the maximum moves.
+  auto weigh = [&](auto nj, auto& st, uint32_t& ok, bool inner, int qt, int s0) __attribute__((always_inline)) {
+    constexpr int E = 4 * decltype(nj)::value;
+    ok = 0xffffu;
+    if (!inner) {
+      ok = 0;
+      const int far = tq[qt] - s0 - 4 * g, near = far - window, sink = sinks - s0 - 4 * g;
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const int s = 16 * (e >> 2) + (e & 3);
+        ok |= s <= far && (s > near || s < sink) ? 1u << e : 0u;
+      }
+    }
+    float top = -INFINITY;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      if (!inner) st[e >> 2][e & 3] = ok >> e & 1u ? st[e >> 2][e & 3] : -INFINITY;
+      top = fmaxf(top, st[e >> 2][e & 3]);
+    }
+    top = mul(max_xor32(max_xor16(top)), a.scale_log2);
+    if (ballot(top > m[qt] + 8.f)) {
+      const float next = fmaxf(m[qt], top);
+      const float fall = m[qt] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[qt] - next);
+      m[qt] = next;
+      l[qt] *= fall;
+#pragma unroll
+      for (int d = 0; d < NDT; ++d) o[d][qt] *= fall;
+    }
+    const float ref = m[qt] == -INFINITY ? 0.0f : m[qt];
+#pragma unroll
+    for (int e = 0; e < E; ++e) st[e >> 2][e & 3] = weight<E == 4>(st[e >> 2][e & 3], a.scale_log2, ref);
+#pragma unroll
+    for (int e = 0; e < E; ++e) l[qt] += st[e >> 2][e & 3];
+  };
+  auto seen = [&](int s0, int s1) { return s0 <= wave_last && (s1 > tw - window || s0 < sinks); };
+  auto all_see = [&](int s0, int s1) { return s1 <= tw && (s0 > wave_last - window || s1 < sinks); };
+
+  clear();
+  if (walk.total > 0) fetch(walk.tile(0));
+  for (int v = 0; v < walk.total; ++v) {
+    const int s0 = walk.tile(v) * KT, s1 = s0 + KT - 1;
+    block_sync_lds();  // the last tile has been read
+    split();
+    if (v + 1 < walk.total) fetch(walk.tile(v + 1));
+    block_sync_lds();
+    if (!seen(s0, s1)) continue;
+    const bool inner = all_see(s0, s1);
+    f32x4 st[QT][NJ];
+    const DSA_LDS uint8_t* const kp = (const DSA_LDS uint8_t*)kl + c16 * 2 * D;
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+#pragma unroll
+      for (int qt = 0; qt < QT; ++qt) st[qt][j] = f32x4{0, 0, 0, 0};
+#pragma unroll
+      for (int ks = 0; ks < NKS; ++ks) {
+        u32x4 x[3];
+#pragma unroll
+        for (int p = 0; p < 3; ++p)
+          x[p] = *reinterpret_cast<const DSA_LDS u32x4*>(kp + p * L::BYTES + 16 * j * 2 * D + 16 * ((4 * ks + g) ^ L::swz_k(c16)));
+#pragma unroll
+        for (int qt = 0; qt < QT; ++qt) st[qt][j] = dot3(x, q[qt][ks], st[qt][j]);
+      }
+    }
+    u32x4 p3[QT][NJ / 2][3];
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) {
+      uint32_t ok;
+      weigh(std::integral_constant<int, NJ>{}, st[qt], ok, inner, qt, s0);
+#pragma unroll
+      for (int j = 0; j < NJ; ++j)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const Three t = split3(st[qt][j][2 * e], st[qt][j][2 * e + 1]);
+          const int w = 2 * (j & 1) + e;
+          p3[qt][j >> 1][0][w] = t.h; p3[qt][j >> 1][1][w] = t.m; p3[qt][j >> 1][2][w] = t.l;
+        }
+    }
+    const int vr = 4 * g + (c16 >> 2);
+    const DSA_LDS uint8_t* const vp = (const DSA_LDS uint8_t*)vl + vr * 2 * D + 8 * (c16 & 1);
+#pragma unroll
+    for (int d = 0; d < NDT; ++d)
+#pragma unroll
+      for (int jj = 0; jj < NJ / 2; ++jj) {
+        u32x4 x[3];
+#pragma unroll
+        for (int p = 0; p < 3; ++p) {
+          const DSA_LDS uint8_t* at = vp + p * L::BYTES + 32 * jj * 2 * D + 16 * ((2 * d + ((c16 & 3) >> 1)) ^ L::swz_v(vr));
+          const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((DSA_LDS s16x4*)at);
+          const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((DSA_LDS s16x4*)(at + 16 * 2 * D));
+          const uint2 l2 = __builtin_bit_cast(uint2, lo), h2 = __builtin_bit_cast(uint2, hi);
+          x[p] = u32x4{l2.x, l2.y, h2.x, h2.y};
+        }
+#pragma unroll
+        for (int qt = 0; qt < QT; ++qt) o[d][qt] = dot3(x, p3[qt][jj], o[d][qt]);
+      }
+  }
+
+  bool odd = false;
+#pragma unroll
+  for (int qt = 0; qt < QT; ++qt) {
+    const float all = sum_xor32(sum_xor16(l[qt]));
+    odd |= tq[qt] < n && !(all > 0.0f && finite_f32(all));
+#pragma unroll
+    for (int d = 0; d < NDT; ++d)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) odd |= tq[qt] < n && !finite_f32(o[d][qt][r]);
+  }
+  if (__syncthreads_or(odd)) {
+    // 16 keys at a time, fp32 rows as they are.  K-slots: element i of a lane's 16 bytes of K
+    // is step i (dims 16kk + 4g + i), token 4g + r is step r of P's.
+    float* const kf = reinterpret_cast<float*>(kl);
+    float* const vf = reinterpret_cast<float*>(vl);
+    clear();
+    for (int v = 0; v < walk.total * NJ; ++v) {
+      const int s0 = walk.tile(v / NJ) * KT + v % NJ * 16, s1 = s0 + 15;
       __syncthreads();
-      for (int i = tid; i < KT * D / 4; i += kNT) {
+      for (int i = tid; i < 16 * D / 4; i += kNT) {
         const int r = i / (D / 4), d = i % (D / 4) * 4;
         f32x4 x{0, 0, 0, 0}, y{0, 0, 0, 0};
         if (s0 + r < n) {
           x = *reinterpret_cast<const f32x4*>(kb + (s0 + r) * a.ldk + d);
           y = *reinterpret_cast<const f32x4*>(vb + (s0 + r) * a.ldv + d);
         }
-        *reinterpret_cast<f32x4*>(kt_ + r * LD + d) = x;
-        *reinterpret_cast<f32x4*>(vt_ + r * LD + d) = y;
+        *reinterpret_cast<f32x4*>(kf + r * LD + d) = x;
+        *reinterpret_cast<f32x4*>(vf + r * LD + d) = y;
       }
       __syncthreads();
-      if (s0 > wave_last || (s1 <= tw - window && s0 >= sinks)) continue;
-      f32x4 st[NJ];
+      if (!seen(s0, s1)) continue;
+      const bool inner = all_see(s0, s1);
 #pragma unroll
-      for (int j = 0; j < NJ; ++j) {
-        st[j] = f32x4{0, 0, 0, 0};
+      for (int qt = 0; qt < QT; ++qt) {
+        const float* src = qb + min(tq[qt], T - 1) * a.ldq + 4 * g;
+        f32x4 st[1] = {f32x4{0, 0, 0, 0}};
+        for (int kk = 0; kk < D / 16; ++kk) {
+          const f32x4 x = *reinterpret_cast<const f32x4*>(kf + c16 * LD + 16 * kk + 4 * g);
+          const f32x4 y = *reinterpret_cast<const f32x4*>(src + 16 * kk);
 #pragma unroll
-        for (int kk = 0; kk < NKK; ++kk) {
-          const f32x4 x = *reinterpret_cast<const f32x4*>(kt_ + (16 * j + c16) * LD + 16 * kk + 4 * g);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) st[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[i], q[kk][i], st[j], 0, 0, 0);
+          for (int i = 0; i < 4; ++i) st[0] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[i], __uint_as_float(__float_as_uint(y[i]) ^ a.flip), st[0], 0, 0, 0);
         }
-      }
-      const bool inner = s1 <= tw && (s0 > wave_last - window || s1 < sinks);
-      uint32_t ok = 0xffffu;
-      if (!inner) {
-        ok = 0;
-        const int far = tq - s0 - 4 * g, near = far - window, sink = sinks - s0 - 4 * g;
+        uint32_t ok;
+        weigh(std::integral_constant<int, 1>{}, st, ok, inner, qt, s0);
+        bool bad = false;
 #pragma unroll
-        for (int e = 0; e < 4 * NJ; ++e) {
-          const int s = 16 * (e >> 2) + (e & 3);
-          ok |= s <= far && (s > near || s < sink) ? 1u << e : 0u;
-        }
-      }
-      float top = -INFINITY;
-#pragma unroll
-      for (int e = 0; e < 4 * NJ; ++e) {
-        const float x = st[e >> 2][e & 3] * a.scale_log2;
-        st[e >> 2][e & 3] = ok >> e & 1u ? x : -INFINITY;
-        top = fmaxf(top, st[e >> 2][e & 3]);
-      }
-      top = max_xor32(max_xor16(top));
-      if (ballot(top > m + 8.f)) {
-        const float next = fmaxf(m, top);
-        const float fall = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - next);
-        m = next;
-        l *= fall;
-#pragma unroll
-        for (int d = 0; d < NDT; ++d) o[d] *= fall;
-      }
-      const float ref = m == -INFINITY ? 0.0f : m;
-#pragma unroll
-      for (int e = 0; e < 4 * NJ; ++e) {
-        st[e >> 2][e & 3] = __builtin_amdgcn_exp2f(st[e >> 2][e & 3] - ref);
-        l += st[e >> 2][e & 3];
-      }
-      bool odd = false;
-#pragma unroll
-      for (int j = 0; j < NJ; ++j)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const float* row = vt_ + (16 * j + 4 * g + r) * LD + c16;
+        for (int r = 0; r < 4; ++r)
 #pragma unroll
           for (int d = 0; d < NDT; ++d) {
-            float x = row[16 * d];
-            if constexpr (CAREFUL) {
-              odd |= !finite_f32(x);
-              x = finite_f32(x) ? x : 0.0f;
+            const float x = vf[(4 * g + r) * LD + 16 * d + c16];
+            bad |= !finite_f32(x);
+            o[d][qt] = __builtin_amdgcn_mfma_f32_16x16x4f32(finite_f32(x) ? x : 0.0f, st[0][r], o[d][qt], 0, 0, 0);
+          }
+        if (!ballot(bad)) continue;
+        for (int s = 0; s < min(16, n - s0); ++s) {
+          const int from = (s >> 2) * 16 + c16, e0 = s & 3;
+          const float mine = e0 == 0 ? st[0][0] : e0 == 1 ? st[0][1] : e0 == 2 ? st[0][2] : st[0][3];
+          const float p = __shfl(mine, from, kWave);
+          const bool yes = static_cast<uint32_t>(__shfl(static_cast<int>(ok), from, kWave)) >> e0 & 1u;
+#pragma unroll
+          for (int d = 0; d < NDT; ++d)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const float x = vf[s * LD + 16 * d + 4 * g + r];
+              if (yes && !finite_f32(x)) o[d][qt][r] += p * x;
             }
-            o[d] = __builtin_amdgcn_mfma_f32_16x16x4f32(x, st[j][r], o[d], 0, 0, 0);
-          }
-        }
-      if constexpr (CAREFUL) {
-        if (ballot(odd)) {
-          for (int s = 0; s < min(KT, n - s0); ++s) {
-            const int from = ((s >> 2) & 3) * 16 + c16, e0 = 4 * (s >> 4) + (s & 3);
-            float mine = 0.0f;
-#pragma unroll
-            for (int e = 0; e < 4 * NJ; ++e) mine = e == e0 ? st[e >> 2][e & 3] : mine;
-            const float p = __shfl(mine, from, kWave);
-            const bool yes = static_cast<uint32_t>(__shfl(static_cast<int>(ok), from, kWave)) >> e0 & 1u;
-#pragma unroll
-            for (int d = 0; d < NDT; ++d)
-#pragma unroll
-              for (int r = 0; r < 4; ++r) {
-                const float x = vt_[s * LD + 16 * d + 4 * g + r];
-                if (yes && !finite_f32(x)) o[d][r] += p * x;
-              }
-          }
         }
       }
     }
-  };
-  run(std::false_type{});
-  bool odd = false;
-  if (tq < n) {
-#pragma unroll
-    for (int d = 0; d < NDT; ++d)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) odd |= !finite_f32(o[d][r]);
   }
-  if (__syncthreads_or(odd)) run(std::true_type{});
-  l = sum_xor32(sum_xor16(l));
-  if (tq >= T) return;
-  const float inv = tq < n ? 1.0f / l : __builtin_nanf("");
-  float* to = static_cast<float*>(a.out) + ((b * T + tq) * a.HQ + h) * D;
+
 #pragma unroll
-  for (int d = 0; d < NDT; ++d) store4<F32>(to + 16 * d + 4 * g, o[d] * inv);
+  for (int qt = 0; qt < QT; ++qt) {
+    const float sum = sum_xor32(sum_xor16(l[qt]));
+    if (tq[qt] >= T) continue;
+    const float inv = tq[qt] < n ? 1.0f / sum : __builtin_nanf("");
+    float* to = static_cast<float*>(a.out) + ((b * T + tq[qt]) * a.HQ + h) * D;
+#pragma unroll
+    for (int d = 0; d < NDT; ++d) store4<F32>(to + 16 * d + 4 * g, o[d][qt] * inv);
+  }
 }
 
 template <typename Tag>
@@ -535,15 +700,16 @@ hipError_t launch_window_attn(const WindowArgs& a, int dtype, hipStream_t stream
   w.G = a.HQ / a.HKV;
   w.window = a.window;
   w.sinks = a.sinks;
-  w.scale_log2 = a.scale * 1.4426950408889634f;
+  w.scale_log2 = std::max(std::fabs(a.scale * 1.4426950408889634f), 0x1p-126f);
+  w.flip = a.scale < 0.0f ? dtype == 0 ? 0x80000000u : 0x80008000u : 0u;
   if (dtype == 1) return launch_16<BF16>(w, a.D, stream);
   if (dtype == 2) return launch_16<F16>(w, a.D, stream);
-  const dim3 grid(static_cast<uint32_t>(blocks_of<64>(w)));
-  switch (a.D) {
-    case 32: window_f32_kernel<32, 64><<<grid, kNT, 0, stream>>>(w); break;
-    case 64: window_f32_kernel<64, 64><<<grid, kNT, 0, stream>>>(w); break;
-    case 128: window_f32_kernel<128, 64><<<grid, kNT, 0, stream>>>(w); break;
-    default: window_f32_kernel<256, 32><<<grid, kNT, 0, stream>>>(w);
+  const dim3 grid(static_cast<uint32_t>(a.D <= 64 ? blocks_of<128>(w) : blocks_of<64>(w)));
+  switch (a.D) {  // registers and LDS
+    case 32: window_f32_kernel<32, 2, 64><<<grid, kNT, 0, stream>>>(w); break;
+    case 64: window_f32_kernel<64, 2, 64><<<grid, kNT, 0, stream>>>(w); break;
+    case 128: window_f32_kernel<128, 1, 32><<<grid, kNT, 0, stream>>>(w); break;
+    default: window_f32_kernel<256, 1, 32><<<grid, kNT, 0, stream>>>(w);
   }
   return hipGetLastError();
 }
