@@ -4,7 +4,7 @@
 //   O[b,t,h,:] = sum_s p_s V[b,s,h/G,:],  p = softmax_s(<Q[b,t,h], K[b,s,h/G]> scale)
 // over s <= t with s > t - window or s < sinks.
 //
-// A block takes 128 queries of one head (64 of 256 dimensions), a wave 32, and walks the tiles of 64 keys that
+// A block takes 128 queries of one head, a wave 32 (or 64, 16), and walks the tiles of 64 keys that
 // any of them sees: those of the first tokens, then those of the window.  K and V go to
 // LDS by DMA, two buffers each, the products run transposed,
 //   S^T = K . Q^T,  O^T = V^T . P^T,
@@ -14,6 +14,7 @@
 #include <cmath>
 #include <type_traits>
 
+#include "dsa_launch.h"
 #include "kv8.h"
 #include "tile_common.h"
 
@@ -118,7 +119,7 @@ __device__ __forceinline__ void store4(typename Tag::raw* to, f32x4 y) {
 // non-finite elements taken out of the product and added to the rows that see them.
 // ---------------------------------------------------------------------------
 template <typename Tag, int D, int QT>
-__global__ __launch_bounds__(kNT, D == 256 ? 1 : 2) void window_kernel(Win a) {
+__global__ __launch_bounds__(kNT, D == 256 ? 1 : D == 128 ? 2 : QT == 2 ? 3 : 4) void window_kernel(Win a) {
   using raw = typename Tag::raw;
   using M = Mfma16x16x32<Tag>;
   using L = TileLds<D>;
@@ -222,14 +223,27 @@ __global__ __launch_bounds__(kNT, D == 256 ? 1 : 2) void window_kernel(Win a) {
         float mx = -INFINITY;
         ok[qt] = 0xffffu;
         if constexpr (MASKED) {
-          ok[qt] = 0;
           const int far = tq[qt] - s0 - 4 * g, near = far - window, sink = sinks - s0 - 4 * g;
+          if constexpr (CAREFUL) {
+            ok[qt] = 0;
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const int s = 16 * (e >> 2) + (e & 3);
-            const bool yes = s <= far && (s > near || s < sink);
-            ok[qt] |= yes ? 1u << e : 0u;
-            st[e >> 2][qt][e & 3] = yes ? st[e >> 2][qt][e & 3] : -INFINITY;
+            for (int e = 0; e < 16; ++e) {
+              const int s = 16 * (e >> 2) + (e & 3);
+              ok[qt] |= s <= far && (s > near || s < sink) ? 1u << e : 0u;
+              st[e >> 2][qt][e & 3] = ok[qt] >> e & 1u ? st[e >> 2][qt][e & 3] : -INFINITY;
+            }
+          } else if (s0 >= sinks) {  // near < s <= far in one comparison
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              const int s = 16 * (e >> 2) + (e & 3);
+              st[e >> 2][qt][e & 3] = static_cast<uint32_t>(far - s) < static_cast<uint32_t>(window) ? st[e >> 2][qt][e & 3] : -INFINITY;
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              const int s = 16 * (e >> 2) + (e & 3);
+              st[e >> 2][qt][e & 3] = s <= far && (s > near || s < sink) ? st[e >> 2][qt][e & 3] : -INFINITY;
+            }
           }
         }
 #pragma unroll
@@ -327,20 +341,34 @@ __global__ __launch_bounds__(kNT, D == 256 ? 1 : 2) void window_kernel(Win a) {
     __builtin_amdgcn_sched_barrier(0);
     wait_dma_keep<0>();
     block_sync_lds();
-    auto step = [&](int v, DSA_LDS uint8_t* kc, DSA_LDS uint8_t* vc, DSA_LDS uint8_t* kn, DSA_LDS uint8_t* vn) __attribute__((always_inline)) {
+    auto step = [&](auto masked, int v, DSA_LDS uint8_t* kc, DSA_LDS uint8_t* vc, DSA_LDS uint8_t* kn, DSA_LDS uint8_t* vn) __attribute__((always_inline)) {
       if (v + 1 < walk.total) fetch(walk.tile(v + 1), kn, vn);
       __builtin_amdgcn_sched_barrier(0);
-      const int s0 = walk.tile(v) * kKT, s1 = s0 + kKT - 1;
-      if (s0 <= wave_last && (s1 > tw - window || s0 < sinks)) {
-        if (!CAREFUL && s1 <= tw && (s0 > wave_last - window || s1 < sinks)) compute(std::false_type{}, s0, kc, vc);
-        else compute(std::true_type{}, s0, kc, vc);
-      }
+      const int s0 = walk.tile(v) * kKT;
+      if constexpr (!decltype(masked)::value) compute(std::false_type{}, s0, kc, vc);
+      else if (s0 <= wave_last && (s0 + kKT > tw - window + 1 || s0 < sinks)) compute(std::true_type{}, s0, kc, vc);
       wait_dma_keep<0>();
       block_sync_lds();
     };
-    for (int v = 0; v < walk.total; v += 2) {
-      step(v, kl0, vl0, kl1, vl1);
-      if (v + 1 < walk.total) step(v + 1, kl1, vl1, kl0, vl0);
+    // Tiles that all queries of the block see whole are a loop of their own (in one with the
+    // others, the compiler copies O, 64 registers, once a tile).
+    const int last = min(t0 + TQ, n) - 1, whole = last >= window ? (last - window) / kKT + 1 : 0;
+    const int w0 = (walk.first + max(0, whole - walk.near) + 1) & ~1;
+    const int w1 = CAREFUL ? w0 : w0 + max(0, (walk.first + t0 / kKT - walk.near - w0) & ~1);
+    int v = 0;
+    auto edges = [&](int end) __attribute__((always_inline)) {
+      for (; v < end; v += 2) {
+        step(std::true_type{}, v, kl0, vl0, kl1, vl1);
+        if (v + 1 < end) step(std::true_type{}, v + 1, kl1, vl1, kl0, vl0);
+      }
+    };
+    for (int phase = 0; phase < 2; ++phase) {
+      edges(phase ? walk.total : min(w0, walk.total));
+      if (phase || w1 <= w0) continue;
+      for (; v < w1; v += 2) {
+        step(std::false_type{}, v, kl0, vl0, kl1, vl1);
+        step(std::false_type{}, v + 1, kl1, vl1, kl0, vl0);
+      }
     }
   };
 
@@ -394,20 +422,15 @@ __device__ __forceinline__ Three split3(float x, float y) {
   t.l = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{x, y}), bf16x2));
   return t;
 }
-// a . b, the small products first.
-__device__ __forceinline__ f32x4 dot3(const u32x4 (&a)[3], const u32x4 (&b)[3], f32x4 c) {
-  using M = Mfma16x16x32<BF16>;
-  c = M::run(a[0], b[2], c);
-  c = M::run(a[2], b[0], c);
-  c = M::run(a[1], b[1], c);
-  c = M::run(a[0], b[1], c);
-  c = M::run(a[1], b[0], c);
-  return M::run(a[0], b[0], c);
-}
+// The six products, the small ones first; a chain of them waits for each before it, so callers
+// take one of every chain in turn.
+constexpr int kProducts = 6;
+__device__ constexpr int kLeft[kProducts] = {0, 2, 1, 0, 1, 0}, kRight[kProducts] = {2, 0, 1, 1, 0, 0};
 
 template <int D, int QT, int KT>
-__global__ __launch_bounds__(kNT, D == 256 ? 1 : 2) void window_f32_kernel(Win a) {
+__global__ __launch_bounds__(kNT, D * QT >= 256 ? 1 : 2) void window_f32_kernel(Win a) {
   using L = TileLds<D, KT>;
+  using M = Mfma16x16x32<BF16>;
   constexpr int TQ = 64 * QT, NKS = D / 32, NDT = D / 16, NJ = KT / 16;
   constexpr int PER = KT * D / 8 / kNT;  // 8-element chunks of a tile a thread, of K and of V
   constexpr int LD = D + 4;              // fp32 rows of the careful pass
@@ -536,21 +559,31 @@ __global__ __launch_bounds__(kNT, D == 256 ? 1 : 2) void window_f32_kernel(Win a
     if (!seen(s0, s1)) continue;
     const bool inner = all_see(s0, s1);
     f32x4 st[QT][NJ];
+    __builtin_amdgcn_s_setprio(1);
     const DSA_LDS uint8_t* const kp = (const DSA_LDS uint8_t*)kl + c16 * 2 * D;
 #pragma unroll
-    for (int j = 0; j < NJ; ++j) {
+    for (int j = 0; j < NJ; ++j)
 #pragma unroll
       for (int qt = 0; qt < QT; ++qt) st[qt][j] = f32x4{0, 0, 0, 0};
 #pragma unroll
-      for (int ks = 0; ks < NKS; ++ks) {
-        u32x4 x[3];
+    for (int ks = 0; ks < NKS; ++ks)
 #pragma unroll
-        for (int p = 0; p < 3; ++p)
-          x[p] = *reinterpret_cast<const DSA_LDS u32x4*>(kp + p * L::BYTES + 16 * j * 2 * D + 16 * ((4 * ks + g) ^ L::swz_k(c16)));
+      for (int j0 = 0; j0 < NJ; j0 += 2) {
+        u32x4 x[2][3];
 #pragma unroll
-        for (int qt = 0; qt < QT; ++qt) st[qt][j] = dot3(x, q[qt][ks], st[qt][j]);
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int p = 0; p < 3; ++p)
+            x[j][p] = *reinterpret_cast<const DSA_LDS u32x4*>(kp + p * L::BYTES + 16 * (j0 + j) * 2 * D + 16 * ((4 * ks + g) ^ L::swz_k(c16)));
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int e = 0; e < kProducts; ++e)
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int qt = 0; qt < QT; ++qt) st[qt][j0 + j] = M::run(x[j][kLeft[e]], q[qt][ks][kRight[e]], st[qt][j0 + j]);
       }
-    }
+    __builtin_amdgcn_s_setprio(0);
     u32x4 p3[QT][NJ / 2][3];
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt) {
@@ -565,24 +598,37 @@ __global__ __launch_bounds__(kNT, D == 256 ? 1 : 2) void window_f32_kernel(Win a
           p3[qt][j >> 1][0][w] = t.h; p3[qt][j >> 1][1][w] = t.m; p3[qt][j >> 1][2][w] = t.l;
         }
     }
+    __builtin_amdgcn_s_setprio(1);
     const int vr = 4 * g + (c16 >> 2);
     const DSA_LDS uint8_t* const vp = (const DSA_LDS uint8_t*)vl + vr * 2 * D + 8 * (c16 & 1);
+    constexpr int DG = QT == 1 ? 4 : 2;  // 16-dim tiles in turn
+    static_assert(NDT % 2 == 0);
 #pragma unroll
-    for (int d = 0; d < NDT; ++d)
+    for (int d0 = 0; d0 < NDT; d0 += DG)
 #pragma unroll
       for (int jj = 0; jj < NJ / 2; ++jj) {
-        u32x4 x[3];
+        u32x4 x[DG][3];
 #pragma unroll
-        for (int p = 0; p < 3; ++p) {
-          const DSA_LDS uint8_t* at = vp + p * L::BYTES + 32 * jj * 2 * D + 16 * ((2 * d + ((c16 & 3) >> 1)) ^ L::swz_v(vr));
-          const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((DSA_LDS s16x4*)at);
-          const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((DSA_LDS s16x4*)(at + 16 * 2 * D));
-          const uint2 l2 = __builtin_bit_cast(uint2, lo), h2 = __builtin_bit_cast(uint2, hi);
-          x[p] = u32x4{l2.x, l2.y, h2.x, h2.y};
-        }
+        for (int d = 0; d < DG; ++d)
 #pragma unroll
-        for (int qt = 0; qt < QT; ++qt) o[d][qt] = dot3(x, p3[qt][jj], o[d][qt]);
+          for (int p = 0; p < 3; ++p) {
+            if (d0 + d >= NDT) continue;
+            const DSA_LDS uint8_t* at = vp + p * L::BYTES + 32 * jj * 2 * D + 16 * ((2 * (d0 + d) + ((c16 & 3) >> 1)) ^ L::swz_v(vr));
+            const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((DSA_LDS s16x4*)at);
+            const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((DSA_LDS s16x4*)(at + 16 * 2 * D));
+            const uint2 l2 = __builtin_bit_cast(uint2, lo), h2 = __builtin_bit_cast(uint2, hi);
+            x[d][p] = u32x4{l2.x, l2.y, h2.x, h2.y};
+          }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int e = 0; e < kProducts; ++e)
+#pragma unroll
+          for (int d = 0; d < DG; ++d)
+#pragma unroll
+            for (int qt = 0; qt < QT; ++qt)
+              if (d0 + d < NDT) o[d0 + d][qt] = M::run(x[d][kLeft[e]], p3[qt][jj][kRight[e]], o[d0 + d][qt]);
       }
+    __builtin_amdgcn_s_setprio(0);
   }
 
   bool odd = false;
@@ -667,15 +713,32 @@ __global__ __launch_bounds__(kNT, D == 256 ? 1 : 2) void window_f32_kernel(Win a
   }
 }
 
-template <typename Tag>
-hipError_t launch_16(const Win& w, int D, hipStream_t stream) {
-  const dim3 grid(static_cast<uint32_t>(D == 256 ? blocks_of<64>(w) : blocks_of<128>(w)));
-  switch (D) {
-    case 32: window_kernel<Tag, 32, 2><<<grid, kNT, 0, stream>>>(w); break;
-    case 64: window_kernel<Tag, 64, 2><<<grid, kNT, 0, stream>>>(w); break;
-    case 128: window_kernel<Tag, 128, 2><<<grid, kNT, 0, stream>>>(w); break;
-    default: window_kernel<Tag, 256, 1><<<grid, kNT, 0, stream>>>(w);  // registers
-  }
+// 128 queries a block where that leaves four blocks a compute unit, else 64 (us with 128 / 64,
+// bf16: 8 heads of 128, 2048 tokens, window 1024 33.6 / 22.3; 16 of 64, 4 x 1777, window 500
+// 32.8 / 31.0; 32 on 8 of 128, 4096 tokens, window 1024 84 / 93).
+// fp32, whose tiles take longer to make, needs two (8 heads of 64, 2 x 4096 tokens, window 1024:
+// 109 / 133).
+bool wide_tiles(const Win& w, int a_unit) {
+  return blocks_of<128>(w) >= a_unit * int64_t{device_cus() > 0 ? device_cus() : 256};
+}
+
+template <typename Tag, int D>
+void launch_16(const Win& w, hipStream_t stream) {
+  if constexpr (D <= 128)  // registers
+    if (wide_tiles(w, 4)) return (void)(window_kernel<Tag, D, 2><<<static_cast<uint32_t>(blocks_of<128>(w)), kNT, 0, stream>>>(w));
+  window_kernel<Tag, D, 1><<<static_cast<uint32_t>(blocks_of<64>(w)), kNT, 0, stream>>>(w);
+}
+template <int D, int KT>
+void launch_32(const Win& w, hipStream_t stream) {
+  if constexpr (D <= 64)  // registers
+    if (wide_tiles(w, 2)) return (void)(window_f32_kernel<D, 2, KT><<<static_cast<uint32_t>(blocks_of<128>(w)), kNT, 0, stream>>>(w));
+  window_f32_kernel<D, 1, KT><<<static_cast<uint32_t>(blocks_of<64>(w)), kNT, 0, stream>>>(w);
+}
+template <int D>
+hipError_t launch_dims(const Win& w, int dtype, hipStream_t stream) {
+  if (dtype == 1) launch_16<BF16, D>(w, stream);
+  else if (dtype == 2) launch_16<F16, D>(w, stream);
+  else launch_32<D, (D <= 64 ? 64 : 32)>(w, stream);
   return hipGetLastError();
 }
 
@@ -702,16 +765,12 @@ hipError_t launch_window_attn(const WindowArgs& a, int dtype, hipStream_t stream
   w.sinks = a.sinks;
   w.scale_log2 = std::max(std::fabs(a.scale * 1.4426950408889634f), 0x1p-126f);
   w.flip = a.scale < 0.0f ? dtype == 0 ? 0x80000000u : 0x80008000u : 0u;
-  if (dtype == 1) return launch_16<BF16>(w, a.D, stream);
-  if (dtype == 2) return launch_16<F16>(w, a.D, stream);
-  const dim3 grid(static_cast<uint32_t>(a.D <= 64 ? blocks_of<128>(w) : blocks_of<64>(w)));
-  switch (a.D) {  // registers and LDS
-    case 32: window_f32_kernel<32, 2, 64><<<grid, kNT, 0, stream>>>(w); break;
-    case 64: window_f32_kernel<64, 2, 64><<<grid, kNT, 0, stream>>>(w); break;
-    case 128: window_f32_kernel<128, 1, 32><<<grid, kNT, 0, stream>>>(w); break;
-    default: window_f32_kernel<256, 1, 32><<<grid, kNT, 0, stream>>>(w);
+  switch (a.D) {
+    case 32: return launch_dims<32>(w, dtype, stream);
+    case 64: return launch_dims<64>(w, dtype, stream);
+    case 128: return launch_dims<128>(w, dtype, stream);
+    default: return launch_dims<256>(w, dtype, stream);
   }
-  return hipGetLastError();
 }
 
 }  // namespace dsa
