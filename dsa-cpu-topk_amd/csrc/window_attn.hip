@@ -26,7 +26,7 @@ struct Win {
   void* out;
   const int32_t* count;
   int64_t B, ldq, ldk, ldv;
-  int T, HQ, G, window, sinks;
+  int T, HQ, HKV, G, window, sinks;
   float scale_log2;  // positive: times a masked -Inf it is one
   uint32_t flip;     // Q's sign bits, where the scale is negative
 };
@@ -54,27 +54,25 @@ __device__ __forceinline__ Walk walk_of(const Win& a, int64_t b, int t0) {
 
 // Block -> (tile of queries, batch, head): the tiles of one K/V head go to one XCD (block
 // i starts on XCD i % 8), the latest, which see most, first.
+// (32-bit throughout: a 64-bit division costs as much as a short prompt's tile.)
 template <int TQ>
-__device__ __forceinline__ bool place(const Win& a, int& t0, int64_t& b, int& h) {
-  const int ntile = (a.T + TQ - 1) / TQ, HKV = a.HQ / a.G;
-  const int64_t pairs = a.B * HKV;  // (b, K/V head)
-  const int64_t lanes = (pairs + 7) / 8;
-  int64_t i = blockIdx.x;
-  const int64_t x = i % 8;
-  i /= 8;
-  const int hh = static_cast<int>(i % a.G);
-  i /= a.G;
-  const int64_t pair = i % lanes * 8 + x;
-  t0 = (ntile - 1 - static_cast<int>(i / lanes)) * TQ;
+__device__ __forceinline__ bool place(const Win& a, int& t0, int64_t& b, int& h, int& hk) {
+  const uint32_t ntile = static_cast<uint32_t>(a.T + TQ - 1) / TQ, G = a.G, HKV = a.HKV;
+  const uint32_t pairs = static_cast<uint32_t>(a.B) * HKV, lanes = (pairs + 7) / 8;  // (b, K/V head)
+  const uint32_t i = blockIdx.x / 8, j = i / G, tile = j / lanes;
+  const uint32_t pair = (j - tile * lanes) * 8 + blockIdx.x % 8;
+  t0 = static_cast<int>((ntile - 1 - tile) * TQ);
   if (pair >= pairs) return false;
-  b = pair / HKV;
-  h = static_cast<int>(pair % HKV) * a.G + hh;
+  const uint32_t bb = pair / HKV;
+  b = bb;
+  hk = static_cast<int>(pair - bb * HKV);
+  h = static_cast<int>(hk * G + (i - j * G));
   return true;
 }
 template <int TQ>
 int64_t blocks_of(const Win& a) {
   const int64_t ntile = (a.T + TQ - 1) / TQ;
-  return (a.B * (a.HQ / a.G) + 7) / 8 * 8 * a.G * ntile;
+  return (a.B * a.HKV + 7) / 8 * 8 * a.G * ntile;
 }
 
 __device__ __forceinline__ float mul(float x, float y) {  // rounded by itself
@@ -130,17 +128,17 @@ __global__ __launch_bounds__(kNT, D == 256 ? 1 : D == 128 ? 2 : QT == 2 ? 3 : 4)
 
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lane = lane_id(), g = lane >> 4, c16 = lane & 15;
-  int t0, h;
+  int t0, h, hk;
   int64_t b;
-  if (!place<TQ>(a, t0, b, h)) return;
+  if (!place<TQ>(a, t0, b, h, hk)) return;
   const Walk walk = walk_of<TQ, kKT>(a, b, t0);
   const int T = a.T, n = walk.n, window = a.window, sinks = a.sinks;
   const int tw = t0 + 16 * QT * wave, wave_last = min(tw + 16 * QT - 1, n - 1);
   raw* const out = static_cast<raw*>(a.out) + (b * T * a.HQ + h) * D;
 
   const raw* Qb = static_cast<const raw*>(a.Q) + b * T * a.ldq + static_cast<int64_t>(h) * D;
-  const char* const kbase = reinterpret_cast<const char*>(static_cast<const raw*>(a.K) + b * T * a.ldk + static_cast<int64_t>(h / a.G) * D);
-  const char* const vbase = reinterpret_cast<const char*>(static_cast<const raw*>(a.V) + b * T * a.ldv + static_cast<int64_t>(h / a.G) * D);
+  const char* const kbase = reinterpret_cast<const char*>(static_cast<const raw*>(a.K) + b * T * a.ldk + static_cast<int64_t>(hk) * D);
+  const char* const vbase = reinterpret_cast<const char*>(static_cast<const raw*>(a.V) + b * T * a.ldv + static_cast<int64_t>(hk) * D);
   const uint32_t krow = static_cast<uint32_t>(a.ldk) * 2u, vrow = static_cast<uint32_t>(a.ldv) * 2u;
   uint32_t koff[PW], voff[PW];  // of this wave's 16-byte chunks within a tile
 #pragma unroll
@@ -438,14 +436,14 @@ __global__ __launch_bounds__(kNT, D * QT >= 256 ? 1 : 2) void window_f32_kernel(
   __shared__ __align__(16) uint8_t kl[3 * L::BYTES], vl[3 * L::BYTES];
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lane = lane_id(), g = lane >> 4, c16 = lane & 15;
-  int t0, h;
+  int t0, h, hk;
   int64_t b;
-  if (!place<TQ>(a, t0, b, h)) return;
+  if (!place<TQ>(a, t0, b, h, hk)) return;
   const Walk walk = walk_of<TQ, KT>(a, b, t0);
   const int T = a.T, n = walk.n, window = a.window, sinks = a.sinks;
   const int tw = t0 + 16 * QT * wave, wave_last = min(tw + 16 * QT - 1, n - 1);
-  const float* const kb = static_cast<const float*>(a.K) + b * T * a.ldk + static_cast<int64_t>(h / a.G) * D;
-  const float* const vb = static_cast<const float*>(a.V) + b * T * a.ldv + static_cast<int64_t>(h / a.G) * D;
+  const float* const kb = static_cast<const float*>(a.K) + b * T * a.ldk + static_cast<int64_t>(hk) * D;
+  const float* const vb = static_cast<const float*>(a.V) + b * T * a.ldv + static_cast<int64_t>(hk) * D;
   const float* const qb = static_cast<const float*>(a.Q) + b * T * a.ldq + static_cast<int64_t>(h) * D;
 
   f32x4 kx[PER][2], vx[PER][2];
@@ -482,6 +480,7 @@ __global__ __launch_bounds__(kNT, D * QT >= 256 ? 1 : 2) void window_f32_kernel(
     }
   };
 
+  if (walk.total > 0) fetch(walk.tile(0));
   u32x4 q[QT][NKS][3];
   int tq[QT];
 #pragma unroll
@@ -549,7 +548,6 @@ __global__ __launch_bounds__(kNT, D * QT >= 256 ? 1 : 2) void window_f32_kernel(
   auto all_see = [&](int s0, int s1) { return s1 <= tw && (s0 > wave_last - window || s1 < sinks); };
 
   clear();
-  if (walk.total > 0) fetch(walk.tile(0));
   for (int v = 0; v < walk.total; ++v) {
     const int s0 = walk.tile(v) * KT, s1 = s0 + KT - 1;
     block_sync_lds();  // the last tile has been read
@@ -760,6 +758,7 @@ hipError_t launch_window_attn(const WindowArgs& a, int dtype, hipStream_t stream
   w.ldv = a.ldv;
   w.T = a.T;
   w.HQ = a.HQ;
+  w.HKV = a.HKV;
   w.G = a.HQ / a.HKV;
   w.window = a.window;
   w.sinks = a.sinks;

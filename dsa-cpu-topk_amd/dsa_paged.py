@@ -39,33 +39,43 @@ def rope_tables(positions: int, R: int, base: float = 10000.0, device="cuda"):
     return angle.cos().float(), angle.sin().float()
 
 
+_TYPES = {torch.float32: L.DSA_F32, torch.bfloat16: L.DSA_BF16, torch.float16: L.DSA_F16}
+
+
 def _tokens(x: torch.Tensor, dtype: torch.dtype):
-    """(x, token stride): [B, T, H, D] in `dtype` as the kernels take it: a token's heads side by
-    side, tokens a stride of 16 bytes' multiple apart (the columns of one projection's
-    output), batch elements T of them; a contiguous copy of anything else."""
-    B, T, H, D = x.shape
-    if x.dtype is dtype and x.data_ptr() & 15 == 0 and x.numel():
+    """(x, its address, token stride): [B, T, H, D] in `dtype` as the kernels take it: a token's
+    heads side by side, tokens a stride of 16 bytes' multiple apart (the columns of one
+    projection's output), batch elements T of them; a contiguous copy of anything else."""
+    at = x.data_ptr()
+    if x.dtype is dtype and at & 15 == 0:
+        B, T, H, D = x.shape
         if x.is_contiguous():
-            return x, H * D
+            return x, at, H * D
         sb, st, sh, sd = x.stride()
-        if sd == 1 and (H == 1 or sh == D) and st >= H * D and st <= 1 << 24 and st * x.element_size() % 16 == 0 \
+        if x.numel() and sd == 1 and (H == 1 or sh == D) and H * D <= st <= 1 << 24 and st * x.element_size() % 16 == 0 \
                 and (B == 1 or sb == T * st):
-            return x, st
-    return L.prep(x, dtype), H * D
+            return x, at, st
+    x = L.prep(x, dtype)
+    return x, x.data_ptr(), x.shape[2] * x.shape[3]
 
 
 def _span_args(window: int | None, sinks: int):
-    assert window is None or int(window) >= 1, f"window={window} must be >= 1 (None: all)"
-    assert int(sinks) >= 0, f"sinks={sinks} must be >= 0"
-    return (0 if window is None else int(window)), int(sinks)
+    W = 0 if window is None else int(window)
+    n = int(sinks)
+    assert window is None or W >= 1, f"window={window} must be >= 1 (None: all)"
+    assert n >= 0, f"sinks={sinks} must be >= 0"
+    return W, n
 
 
-def _out(out, shape, dtype, device):
+def _out(out, shape, dtype, like):
+    """The caller's `out`, checked, or a new tensor of that shape (`like`: one on its GPU)."""
     if out is None:
-        return torch.empty(shape, device=device, dtype=dtype)
-    assert out.dtype is dtype and out.shape == shape and out.is_contiguous() and out.device == device \
+        if like.dtype is dtype and like.shape == shape and like.is_contiguous():
+            return torch.empty_like(like)
+        return like.new_empty(shape, dtype=dtype)
+    assert out.dtype is dtype and out.shape == shape and out.is_contiguous() and out.device == like.device \
         and out.data_ptr() % 16 == 0, \
-        f"out: contiguous 16-byte aligned {dtype} {tuple(shape)} on {device} (got {out.dtype} {tuple(out.shape)} on {out.device})"
+        f"out: contiguous 16-byte aligned {dtype} {tuple(shape)} on {like.device} (got {out.dtype} {tuple(out.shape)} on {out.device})"
     return out
 
 
@@ -82,29 +92,32 @@ def window_attention(Q: torch.Tensor, K: torch.Tensor, V: torch.Tensor, *, windo
     a sequence's T rows are tokens (a padded batch); the others get NaN.  scale: of the
     logits, default 1/sqrt(D).  What a token does not see does not reach its row, NaN
     and Inf included."""
-    L.require_gpu(Q, K, V)
-    assert Q.dim() == 4 and K.dim() == 4 and V.dim() == 4, "Q [B,T,HQ,D], K and V [B,T,HKV,D]"
-    B, T, HQ, D = Q.shape
-    HKV = K.shape[2]
-    assert K.shape == (B, T, HKV, D) and V.shape == (B, T, HKV, D), \
-        f"K {tuple(K.shape)} and V {tuple(V.shape)} must be {(B, T, HKV, D)}"
-    device = Q.device
-    assert K.device == device and V.device == device, "Q, K and V must be on one GPU"
+    if not (Q.is_cuda and K.is_cuda and V.is_cuda):
+        L.require_gpu(Q, K, V)
+    shape, kv = Q.shape, K.shape
+    assert len(shape) == 4 and len(kv) == 4, "Q [B,T,HQ,D], K and V [B,T,HKV,D]"
+    B, T, HQ, D = shape
+    HKV = kv[2]
+    assert kv[0] == B and kv[1] == T and kv[3] == D and V.shape == kv, \
+        f"K {tuple(kv)} and V {tuple(V.shape)} must be {(B, T, HKV, D)}"
+    index = Q.get_device()
+    assert K.get_device() == index and V.get_device() == index, "Q, K and V must be on one GPU"
     W, sinks = _span_args(window, sinks)
     dt = L.common_dtype(Q, K, V)
-    (q, ldq), (k, ldk), (v, ldv) = _tokens(Q, dt), _tokens(K, dt), _tokens(V, dt)
+    q, q_ptr, ldq = _tokens(Q, dt)
+    k, k_ptr, ldk = _tokens(K, dt)
+    v, v_ptr, ldv = _tokens(V, dt)
     count_ptr = None
     if count is not None:
-        assert count.dtype is torch.int32 and count.shape == (B,) and count.device == device, \
-            f"count: int32 {(B,)} on {device} (got {count.dtype} {tuple(count.shape)} on {count.device})"
+        assert count.dtype is torch.int32 and count.shape == (B,) and count.get_device() == index, \
+            f"count: int32 {(B,)} on {Q.device} (got {count.dtype} {tuple(count.shape)} on {count.device})"
         count = count.contiguous()
         count_ptr = count.data_ptr()
-    out = _out(out, (B, T, HQ, D), dt, device)
-    with L.on_device(device):
+    out = _out(out, shape, dt, Q)
+    with L.on_device(Q.device):
         rc = L.lib().dsa_window_attention(
-            q.data_ptr(), k.data_ptr(), v.data_ptr(), L.dtype_code(dt), count_ptr, B, T, HQ, HKV, D, ldq, ldk, ldv,
-            W or max(T, 1), sinks, 1.0 / math.sqrt(D) if scale is None else float(scale), out.data_ptr(),
-            L.stream_ptr(device))
+            q_ptr, k_ptr, v_ptr, _TYPES[dt], count_ptr, B, T, HQ, HKV, D, ldq, ldk, ldv, W or max(T, 1), sinks,
+            D ** -0.5 if scale is None else float(scale), out.data_ptr(), L.stream_ptr(Q.device))
     if rc != L.DSA_OK:
         L.check(rc, "window_attention")
     return out
@@ -158,6 +171,7 @@ class KV8Cache:
         self._c = L.Kv8Cache(codes.data_ptr(), scales.data_ptr(), pages.data_ptr(), length.data_ptr(),
                              lost.data_ptr(), B, NP, max_pages, HKV, DK, DV, 64 * per)
         self._ref = ctypes.addressof(self._c)
+        self._lib = L.lib()
         # sizes that no call takes are refused here
         _workspace_bytes(self, 0, HKV, 0, 0, 0)
 
@@ -221,7 +235,8 @@ def _workspace_bytes(cache: KV8Cache, Tq: int, HQ: int, n: int, window: int, sin
 
 
 def _call(cache: KV8Cache, what: str, fn, *args) -> None:
-    """fn(cache, *args, stream) on the cache's GPU; the usual case enters no context."""
+    """fn(cache, *args, stream) on the cache's GPU.  Single-token calls are bound by
+    the host, so the usual case enters no context."""
     if torch.cuda.current_device() == cache.index:
         rc = fn(cache._ref, *args, L.stream_ptr(cache.device))
     else:
@@ -248,27 +263,25 @@ def kv8_append(cache: KV8Cache, K: torch.Tensor, V: torch.Tensor, *, rope=None, 
     Q [B,T,HQ,DK]: rotated too; keys: K's rotated rows are returned as well, both in their
     type, of all T rows, NaN at positions past the last slot.  Without rope they come back as
     they are."""
-    assert K.dim() == 4 and V.dim() == 4, "K [B,T,HKV,DK], V [B,T,HKV,DV]"
-    B, T = K.shape[:2]
-    assert K.shape == (cache.B, T, cache.HKV, cache.DK), \
-        f"K shape {tuple(K.shape)} != {(cache.B, T, cache.HKV, cache.DK)}"
-    assert V.shape == (cache.B, T, cache.HKV, cache.DV), \
+    kv = K.shape
+    assert len(kv) == 4, "K [B,T,HKV,DK], V [B,T,HKV,DV]"
+    B, T = kv[0], kv[1]
+    assert B == cache.B and kv[2] == cache.HKV and kv[3] == cache.DK, \
+        f"K shape {tuple(kv)} != {(cache.B, T, cache.HKV, cache.DK)}"
+    assert V.shape == (B, T, cache.HKV, cache.DV), \
         f"V shape {tuple(V.shape)} != {(cache.B, T, cache.HKV, cache.DV)}"
     _here(cache, K, V)
-    xs = (K, V)
     HQ = 0
     if Q is not None:
         assert Q.dim() == 4 and (Q.shape[0], Q.shape[1], Q.shape[3]) == (B, T, cache.DK), \
             f"Q shape {tuple(Q.shape)}: B={B}, T={T}, DK={cache.DK}"
         _here(cache, Q)
         HQ = Q.shape[2]
-        if rope is not None:
-            xs = (K, V, Q)
-    dt = L.common_dtype(*xs)
-    k, ldk = _tokens(K, dt)
-    v, ldv = _tokens(V, dt)
+    dt = L.common_dtype(K, V) if Q is None or rope is None else L.common_dtype(K, V, Q)
+    k, k_ptr, ldk = _tokens(K, dt)
+    v, v_ptr, ldv = _tokens(V, dt)
     R = rows = ldq = 0
-    cos_ptr = sin_ptr = start_ptr = count_ptr = q_ptr = q_out = k_out = None
+    cos_ptr = sin_ptr = start_ptr = count_ptr = q_ptr = q_out = k_out = q_out_ptr = k_out_ptr = None
     if rope is not None:
         cos, sin = rope
         assert cos.dim() == 2 and cos.shape == sin.shape and cos.dtype is torch.float32 and sin.dtype is torch.float32, \
@@ -278,20 +291,20 @@ def kv8_append(cache: KV8Cache, K: torch.Tensor, V: torch.Tensor, *, rope=None, 
         cos, sin = L.prep(cos, torch.float32), L.prep(sin, torch.float32)
         cos_ptr, sin_ptr = cos.data_ptr(), sin.data_ptr()
         if Q is not None:
-            q, ldq = _tokens(Q, dt)
-            q_ptr = q.data_ptr()
-            q_out = torch.empty((B, T, HQ, cache.DK), device=cache.device, dtype=dt)
+            q, q_ptr, ldq = _tokens(Q, dt)
+            q_out = _out(None, Q.shape, dt, Q)
+            q_out_ptr = q_out.data_ptr()
         if keys:
-            k_out = torch.empty((B, T, cache.HKV, cache.DK), device=cache.device, dtype=dt)
+            k_out = _out(None, kv, dt, K)
+            k_out_ptr = k_out.data_ptr()
     if start is not None:
         start = _ints(start, (B,), "start", cache)
         start_ptr = start.data_ptr()
     if count is not None:
         count = _ints(count, (B,), "count", cache)
         count_ptr = count.data_ptr()
-    _call(cache, "kv8_append", L.lib().dsa_kv8_append, k.data_ptr(), v.data_ptr(), q_ptr, L.dtype_code(dt), T, HQ,
-          ldk, ldv, ldq, cos_ptr, sin_ptr, rows, R, 1 if pairs else 0, start_ptr, count_ptr,
-          k_out.data_ptr() if k_out is not None else None, q_out.data_ptr() if q_out is not None else None)
+    _call(cache, "kv8_append", cache._lib.dsa_kv8_append, k_ptr, v_ptr, q_ptr, _TYPES[dt], T, HQ, ldk, ldv, ldq,
+          cos_ptr, sin_ptr, rows, R, 1 if pairs else 0, start_ptr, count_ptr, k_out_ptr, q_out_ptr)
     if rope is None:
         return Q, (K if keys else None)
     return q_out, k_out
@@ -312,10 +325,11 @@ def kv8_rows(cache: KV8Cache, slots: torch.Tensor | None = None, *, span: int | 
         slots_ptr = slots.data_ptr()
     else:
         N = _span(cache, span)
-    assert dtype in (torch.float32, torch.bfloat16, torch.float16), f"unsupported dtype {dtype}"
-    K = torch.empty((cache.B, N, cache.HKV, cache.DK), device=cache.device, dtype=dtype)
-    V = torch.empty((cache.B, N, cache.HKV, cache.DV), device=cache.device, dtype=dtype)
-    _call(cache, "kv8_rows", L.lib().dsa_kv8_rows, slots_ptr, N, L.dtype_code(dtype), K.data_ptr(), V.data_ptr())
+    code = _TYPES.get(dtype)
+    assert code is not None, f"unsupported dtype {dtype}"
+    K = cache.codes.new_empty((cache.B, N, cache.HKV, cache.DK), dtype=dtype)
+    V = torch.empty_like(K) if cache.DV == cache.DK else cache.codes.new_empty((cache.B, N, cache.HKV, cache.DV), dtype=dtype)
+    _call(cache, "kv8_rows", cache._lib.dsa_kv8_rows, slots_ptr, N, code, K.data_ptr(), V.data_ptr())
     return K, V
 
 
@@ -339,22 +353,32 @@ def kv8_attention(cache: KV8Cache, Q: torch.Tensor, *, window: int | None = None
     more in use, fewer blocks join).  count int32 [B]: how many of the Tq are tokens, as
     kv8_append's; the others see nothing.  A token that sees nothing gets NaN; slots on no
     page count for nothing.  scale: of the logits, default 1/sqrt(DK)."""
-    assert Q.dim() == 4 and (Q.shape[0], Q.shape[3]) == (cache.B, cache.DK), \
-        f"Q shape {tuple(Q.shape)}: B={cache.B}, DK={cache.DK}"
-    B, Tq, HQ, _ = Q.shape
+    shape = Q.shape
+    assert len(shape) == 4 and shape[0] == cache.B and shape[3] == cache.DK, \
+        f"Q shape {tuple(shape)}: B={cache.B}, DK={cache.DK}"
+    B, Tq, HQ, _ = shape
     _here(cache, Q)
     W, sinks = _span_args(window, sinks)
     n = _span(cache, span)
-    dt = L.common_dtype(Q)
-    q = L.prep(Q, dt)
+    dt, q = Q.dtype, Q
+    if dt not in _TYPES:
+        dt = torch.float32
+    q_ptr = Q.data_ptr()
+    if q_ptr & 15 or Q.dtype is not dt or not Q.is_contiguous():
+        q = L.prep(Q, dt)
+        q_ptr = q.data_ptr()
     count_ptr = None
     if count is not None:
         count = _ints(count, (B,), "count", cache)
         count_ptr = count.data_ptr()
-    out = _out(out, (B, Tq, HQ, cache.DV), dt, cache.device)
+    if cache.DV != cache.DK:
+        shape = (B, Tq, HQ, cache.DV)
+    out = _out(out, shape, dt, q)
     nws = _workspace_bytes(cache, Tq, HQ, n, W, sinks)
-    ws = torch.empty(nws, device=cache.device, dtype=torch.uint8) if nws else None
-    _call(cache, "kv8_attention", L.lib().dsa_kv8_attention, q.data_ptr(), L.dtype_code(dt), count_ptr, Tq, HQ, n, W,
-          sinks, cache.scale if scale is None else float(scale), out.data_ptr(),
-          ws.data_ptr() if nws else None, nws)
+    ws_ptr = None
+    if nws:
+        ws = cache.codes.new_empty(nws)
+        ws_ptr = ws.data_ptr()
+    _call(cache, "kv8_attention", cache._lib.dsa_kv8_attention, q_ptr, _TYPES[dt], count_ptr, Tq, HQ, n, W, sinks,
+          cache.scale if scale is None else float(scale), out.data_ptr(), ws_ptr, nws)
     return out

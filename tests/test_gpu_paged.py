@@ -192,7 +192,7 @@ def test_columns_of_a_projection(dev):
     Q = y[..., :HQ * D].unflatten(-1, (HQ, D))
     K = y[..., HQ * D:(HQ + HKV) * D].unflatten(-1, (HKV, D))
     V = y[..., (HQ + HKV) * D:].unflatten(-1, (HKV, D))
-    assert P._tokens(K, BF16)[0].data_ptr() == K.data_ptr() and P._tokens(K, BF16)[1] == (HQ + 2 * HKV) * D
+    assert P._tokens(K, BF16)[1:] == (K.data_ptr(), (HQ + 2 * HKV) * D)
     rope = P.rope_tables(192, D, device=dev)
     out = []
     for copy in (False, True):
