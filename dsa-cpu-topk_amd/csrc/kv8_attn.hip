@@ -120,7 +120,7 @@ __device__ __forceinline__ int chunk_of(int r, int at) {
 }
 
 template <typename Tag, int DK, int DV, int RT, bool SHARED>
-__global__ __launch_bounds__(kNT, DK <= 128 ? 2 : 1) void attn_kernel(AttnArgs a) {
+__global__ __launch_bounds__(kNT, DK <= 128 || (SHARED && Tag::kBytes == 2) ? 2 : 1) void attn_kernel(AttnArgs a) {
   using raw = typename Tag::raw;
   constexpr int NP = Tag::kBytes == 4 ? 2 : 1;          // f16 pieces of Q and of p
   constexpr int NJ = DK / 64, HALF = DK % 64 != 0;      // 16-byte runs of a K row a lane, and 8-byte ones
@@ -673,7 +673,9 @@ Plan plan_of(const Kv8& c, int64_t Tq, int HQ, int64_t n, int64_t window, int64_
     const int64_t near = (window + Tq - 1 + kBlk - 1) / kBlk + 1 + (sinks < n ? (sinks + kBlk - 1) / kBlk : most);
     most = near < most ? near : most;
   }
-  const int64_t steps = most > waves ? (most + waves - 1) / waves : 1;
+  // few turns of a block's waves cost less than the launch that joins splits, and a split takes two at least
+  const int64_t turns = (most + waves - 1) / waves;
+  const int64_t steps = turns <= 5 ? 1 : turns / 2;
   // as many splits as all run at once: the chunks go over 8 XCDs in equal numbers, and
   // one that waits for a place doubles the time (2 x 33 blocks an XCD of 2 x 32 places:
   // 35 us for what takes 20 in 60)

@@ -1,5 +1,7 @@
 // kv8_cache.hip -- what goes into the paged 8-bit cache and comes back out of it
 // (gfx950).
+#include <algorithm>
+
 #include "dsa_launch.h"
 #include "kv8.h"
 
@@ -162,20 +164,23 @@ __device__ __forceinline__ void make_nan(float (&x)[8]) {
 // Of a dimension's 16 words of V, word w holds tokens t .. t + 3.
 __device__ __forceinline__ int word_token(int w) { return (w & 3) * 16 + (w >> 2) * 4; }
 
-// A block of threads takes the heads [h0, h1) of one block of 64 slots, one after
-// another, and then their share of the query heads, with the angles of its tokens in
-// registers.  Of K a thread has one unit of some tokens; of V 4 tokens by 8
+// A block of threads takes a group of heads of one block of 64 slots, with the angles of
+// its tokens in registers: K/V heads one after another (short ones two or four side by
+// side), or query heads.  Of K a thread has one unit of some tokens; of V 4 tokens by 8
 // dimensions, which it turns into words of 4 tokens (a word of the cache has one owner,
 // so bytes that stay are merged without a barrier, and a wave writes whole rows of 64).
 template <typename Tag, int DK, int DV>
-__global__ __launch_bounds__(kNT) void append_kernel(Kv8 c, Kv8Append a, int nblk, int groups, int update) {
+__global__ __launch_bounds__(kNT) void append_kernel(Kv8 c, Kv8Append a, int nblk, int kv_groups, int q_groups, int update) {
   using raw = typename Tag::raw;
-  constexpr int NU = DK / 16, kRows = kNT / NU, kPasses = (kBlk + kRows - 1) / kRows;
-  constexpr int kItems = 2 * DV, kTurns = (kItems + kNT - 1) / kNT;  // of V: 16 words by DV / 8 dimensions' eights
+  constexpr int kSide = DK >= 96 ? 1 : 128 / DK, kThreads = kNT / kSide, kWaves = kThreads / kWave;  // of one head
+  constexpr int NU = DK / 16, kRows = kThreads / NU, kPasses = (kBlk + kRows - 1) / kRows;
+  constexpr int kItems = 2 * DV, kTurns = (kItems + kThreads - 1) / kThreads;  // of V: 16 words by DV / 8 dimensions' eights
   __shared__ uint32_t tops[2][2][4];
   const int64_t S = c.slots();
-  const int grp = blockIdx.x % groups;
-  const uint32_t rest = blockIdx.x / groups;
+  const uint32_t blocks = static_cast<uint32_t>(c.B) * nblk;
+  const int grp = blockIdx.x / blocks;  // all of K and V first: they take longest
+  const uint32_t rest = blockIdx.x % blocks;
+  const int side = threadIdx.x / kThreads, tid = threadIdx.x % kThreads;
   const int64_t b = rest / nblk;
   const Span s = span_of(c, a, b);
   const int64_t blk = (s.have >> 6) + rest % nblk, first = blk * kBlk;
@@ -185,7 +190,7 @@ __global__ __launch_bounds__(kNT) void append_kernel(Kv8 c, Kv8Append a, int nbl
   const int64_t row0 = b * a.T - s.have + first;  // the call's row of the block's token 0
   const bool pairs = a.pairs != 0;
 
-  const int u = threadIdx.x % NU, r0 = threadIdx.x / NU;
+  const int u = tid % NU, r0 = tid / NU;
   const Unit un = unit_of(u, DK, a.R, pairs);
   Angles ang[kPasses];
 #pragma unroll
@@ -194,8 +199,10 @@ __global__ __launch_bounds__(kNT) void append_kernel(Kv8 c, Kv8Append a, int nbl
     if (r0 < kRows && t >= lo && t < all) load_angles(a, un, min(first + t, S - 1), ang[p]);
   }
 
-  const int h0 = c.HKV * grp / groups, h1 = c.HKV * (grp + 1) / groups;
-  for (int h = h0; h < h1; ++h) {
+  const int h0 = grp < kv_groups ? c.HKV * grp / kv_groups : 0, h1 = grp < kv_groups ? c.HKV * (grp + 1) / kv_groups : 0;
+  for (int hh = h0, turn_no = 0; hh < h1; hh += kSide, ++turn_no) {
+    const int h = min(hh + side, h1 - 1);
+    const bool mine = hh + side < h1;  // the last head's threads may have neighbours without one
     const int64_t at = first < s.end ? kv8_block(c, b, blk, h) : -1;
     const int hi = at >= 0 ? static_cast<int>(min(s.end - first, int64_t{kBlk})) : lo;
     uint8_t* const codes = c.codes + at * c.block_bytes();
@@ -207,18 +214,18 @@ __global__ __launch_bounds__(kNT) void append_kernel(Kv8 c, Kv8Append a, int nbl
 #pragma unroll
     for (int p = 0; p < kPasses; ++p) {
       const int t = r0 + p * kRows;
-      if (r0 >= kRows || t < lo || t >= (a.K_out ? all : hi)) continue;
+      if (!mine || r0 >= kRows || t < lo || t >= (a.K_out ? all : hi)) continue;
       load_cvt<Tag, 8>(ksrc + t * a.ldk + un.lo, k0[p]);
       load_cvt<Tag, 8>(ksrc + t * a.ldk + un.hi, k1[p]);
     }
 #pragma unroll
     for (int p = 0; p < kTurns; ++p) {
-      const int i = threadIdx.x + p * kNT, d = (i >> 6) * 32 + (i & 3) * 8, t = word_token((i >> 2) & 15);
+      const int i = tid + p * kThreads, d = (i >> 6) * 32 + (i & 3) * 8, t = word_token((i >> 2) & 15);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
 #pragma unroll
         for (int x = 0; x < 8; ++x) v[p][e][x] = 0.0f;
-        if (i < kItems && t + e >= lo && t + e < hi) load_cvt<Tag, 8>(vsrc + (t + e) * a.ldv + d, v[p][e]);
+        if (mine && i < kItems && t + e >= lo && t + e < hi) load_cvt<Tag, 8>(vsrc + (t + e) * a.ldv + d, v[p][e]);
       }
     }
     if (lo > 0 && lo < hi) {
@@ -228,7 +235,7 @@ __global__ __launch_bounds__(kNT) void append_kernel(Kv8 c, Kv8Append a, int nbl
 #pragma unroll
     for (int p = 0; p < kPasses; ++p) {
       const int t = r0 + p * kRows;
-      if (r0 >= kRows || t < lo || t >= (a.K_out ? all : hi)) continue;
+      if (!mine || r0 >= kRows || t < lo || t >= (a.K_out ? all : hi)) continue;
       turn(k0[p], k1[p], ang[p], un, pairs);
       if (t < hi) {
 #pragma unroll
@@ -253,19 +260,24 @@ __global__ __launch_bounds__(kNT) void append_kernel(Kv8 c, Kv8Append a, int nbl
         for (int i = 0; i < 8; ++i) top_v = max(top_v, finite_bits(v[p][e][i]));
     top_k = wave_max_bits(top_k);
     top_v = wave_max_bits(top_v);
-    uint32_t(&top)[2][4] = tops[h & 1];
+    uint32_t(&top)[2][4] = tops[turn_no & 1];
     if ((threadIdx.x & 63) == 0) {
       top[0][threadIdx.x >> 6] = top_k;
       top[1][threadIdx.x >> 6] = top_v;
     }
     __syncthreads();  // the old scales have been read; the next head writes the other tops
-    const uint32_t new_k = max(old_k, kv8_scale(max(max(top[0][0], top[0][1]), max(top[0][2], top[0][3]))));
-    const uint32_t new_v = max(old_v, kv8_scale(max(max(top[1][0], top[1][1]), max(top[1][2], top[1][3]))));
-    if (threadIdx.x == 0) *reinterpret_cast<uint16_t*>(scale_at) = static_cast<uint16_t>(new_k | new_v << 8);
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      top_k = max(top_k, top[0][side * kWaves + w]);
+      top_v = max(top_v, top[1][side * kWaves + w]);
+    }
+    if (!mine) continue;
+    const uint32_t new_k = max(old_k, kv8_scale(top_k)), new_v = max(old_v, kv8_scale(top_v));
+    if (tid == 0) *reinterpret_cast<uint16_t*>(scale_at) = static_cast<uint16_t>(new_k | new_v << 8);
     // Held tokens whose block's scale grows are rounded again, to the new one.
     if (lo > 0 && new_k > old_k) {
       const float f = fall_of(old_k, new_k);
-      for (int i = threadIdx.x; i < lo * DK / 4; i += kNT) {
+      for (int i = tid; i < lo * DK / 4; i += kThreads) {
         uint32_t* w = reinterpret_cast<uint32_t*>(codes) + i;
         *w = rescale4(*w, f);
       }
@@ -284,7 +296,7 @@ __global__ __launch_bounds__(kNT) void append_kernel(Kv8 c, Kv8Append a, int nbl
     const bool grows = lo > 0 && new_v > old_v;
 #pragma unroll
     for (int p = 0; p < kTurns; ++p) {
-      const int i = threadIdx.x + p * kNT, d = (i >> 6) * 32 + (i & 3) * 8, w = (i >> 2) & 15, t = word_token(w);
+      const int i = tid + p * kThreads, d = (i >> 6) * 32 + (i & 3) * 8, w = (i >> 2) & 15, t = word_token(w);
       if (i >= kItems || t >= hi || (t + 4 <= lo && !grows)) continue;
       uint2 q[4];
 #pragma unroll
@@ -320,8 +332,8 @@ __global__ __launch_bounds__(kNT) void append_kernel(Kv8 c, Kv8Append a, int nbl
     }
   }
 
-  if (a.Q_out) {
-    const int q0 = static_cast<int>(static_cast<int64_t>(a.HQ) * grp / groups), q1 = static_cast<int>(static_cast<int64_t>(a.HQ) * (grp + 1) / groups);
+  if (grp >= kv_groups) {
+    const int q0 = a.HQ * (grp - kv_groups) / q_groups, q1 = a.HQ * (grp - kv_groups + 1) / q_groups;
     const raw* __restrict__ const from = static_cast<const raw*>(a.Q);
     raw* __restrict__ const to = static_cast<raw*>(a.Q_out);
 #pragma unroll
@@ -331,7 +343,7 @@ __global__ __launch_bounds__(kNT) void append_kernel(Kv8 c, Kv8Append a, int nbl
       const raw* src = from + (row0 + t) * a.ldq;
       raw* dst = to + (row0 + t) * a.HQ * DK;
 #pragma unroll 4
-      for (int h = q0; h < q1; ++h) {
+      for (int h = q0 + side; h < q1; h += kSide) {
         float x[8], y[8];
         load_cvt<Tag, 8>(src + static_cast<int64_t>(h) * DK + un.lo, x);
         load_cvt<Tag, 8>(src + static_cast<int64_t>(h) * DK + un.hi, y);
@@ -596,10 +608,14 @@ hipError_t append_dims(const Kv8& c, const Kv8Append& a, hipStream_t stream) {
     return hipGetLastError();
   }
   const int nblk = static_cast<int>((a.T + kBlk - 2) / kBlk + 1);
-  // the angles are loaded once for the heads of a group: as many as leave four blocks a compute unit
-  const int64_t want = 16 * int64_t{device_cus() > 0 ? device_cus() : 256}, blocks = c.B * nblk;
-  const int groups = static_cast<int>(blocks * c.HKV <= want ? c.HKV : (want + blocks - 1) / blocks);
-  append_kernel<Tag, DK, DV><<<static_cast<uint32_t>(blocks * groups), kNT, 0, stream>>>(c, a, nblk, groups, a.start != nullptr);
+  // The angles are loaded once for the heads of a group, so a group is as large as leaves the
+  // blocks that run at once, two a compute unit, for K and V and as many for the queries: 190 us
+  // for 2 x 16384 tokens of 32 and 8 heads of 128; smaller groups took 196 (4) to 219 (8).
+  const int64_t want = 2 * int64_t{device_cus() > 0 ? device_cus() : 256}, blocks = c.B * nblk;
+  auto groups_of = [&](int64_t heads) { return static_cast<int>(std::min(heads, (want + blocks - 1) / blocks)); };
+  constexpr int kSide = DK >= 96 ? 1 : 128 / DK;
+  const int kv = groups_of((c.HKV + kSide - 1) / kSide), q = a.Q_out ? groups_of((a.HQ + kSide - 1) / kSide) : 0;
+  append_kernel<Tag, DK, DV><<<static_cast<uint32_t>(blocks * (kv + q)), kNT, 0, stream>>>(c, a, nblk, kv, q, a.start != nullptr);
   // where the blocks read the length to find their place, a launch of its own changes it
   if (!a.start) append_counts_kernel<<<static_cast<uint32_t>(c.B), kNT, 0, stream>>>(c, a);
   return hipGetLastError();
