@@ -117,12 +117,15 @@ __device__ __forceinline__ void store4(typename Tag::raw* to, f32x4 y) {
 // non-finite elements taken out of the product and added to the rows that see them.
 // ---------------------------------------------------------------------------
 template <typename Tag, int D, int QT>
-__global__ __launch_bounds__(kNT, D == 256 ? 1 : D == 128 ? 2 : QT == 2 ? 3 : 4) void window_kernel(Win a) {
+__global__ __launch_bounds__(kNT, D >= 128 ? 2 : QT == 2 ? 3 : 4) void window_kernel(Win a) {
   using raw = typename Tag::raw;
   using M = Mfma16x16x32<Tag>;
-  using L = TileLds<D>;
+  // Keys of a tile: at D = 256 half as many let two blocks share a compute unit (11 sequences of
+  // 543 tokens, 4 heads: 30 us with 64 keys, 23 with 32).  A lane has E logits of one query.
+  constexpr int KT = D == 256 ? 32 : 64, NJ = KT / 16, E = 4 * NJ;
+  using L = TileLds<D, KT>;
   constexpr int TQ = 64 * QT, NKS = D / 32, NDT = D / 16;
-  constexpr int KJ = D == 256 ? 1 : 4;           // 16-key tiles whose K fragments are read at once
+  constexpr int KJ = D == 256 ? 1 : NJ;          // 16-key tiles whose K fragments are read at once
   constexpr int PW = L::BYTES / 1024 / (kNT / kWave);
   __shared__ __align__(16) uint8_t k0[L::BYTES], k1[L::BYTES], v0[L::BYTES], v1[L::BYTES];
 
@@ -131,7 +134,7 @@ __global__ __launch_bounds__(kNT, D == 256 ? 1 : D == 128 ? 2 : QT == 2 ? 3 : 4)
   int t0, h, hk;
   int64_t b;
   if (!place<TQ>(a, t0, b, h, hk)) return;
-  const Walk walk = walk_of<TQ, kKT>(a, b, t0);
+  const Walk walk = walk_of<TQ, KT>(a, b, t0);
   const int T = a.T, n = walk.n, window = a.window, sinks = a.sinks;
   const int tw = t0 + 16 * QT * wave, wave_last = min(tw + 16 * QT - 1, n - 1);
   raw* const out = static_cast<raw*>(a.out) + (b * T * a.HQ + h) * D;
@@ -149,8 +152,8 @@ __global__ __launch_bounds__(kNT, D == 256 ? 1 : D == 128 ? 2 : QT == 2 ? 3 : 4)
   }
   // rows past the sequence read as zeros
   auto fetch = [&](int kt, DSA_LDS uint8_t* kd, DSA_LDS uint8_t* vd) __attribute__((always_inline)) {
-    dma_tile<PW>(rows_rsrc(kbase, kt * kKT, n, krow), koff, kd, wave);
-    dma_tile<PW>(rows_rsrc(vbase, kt * kKT, n, vrow), voff, vd, wave);
+    dma_tile<PW>(rows_rsrc(kbase, kt * KT, n, krow), koff, kd, wave);
+    dma_tile<PW>(rows_rsrc(vbase, kt * KT, n, vrow), voff, vd, wave);
   };
   DSA_LDS uint8_t* const kl0 = (DSA_LDS uint8_t*)k0;
   DSA_LDS uint8_t* const kl1 = (DSA_LDS uint8_t*)k1;
@@ -190,10 +193,10 @@ __global__ __launch_bounds__(kNT, D == 256 ? 1 : D == 128 ? 2 : QT == 2 ? 3 : 4)
     }
     auto compute = [&](auto masked, int s0, const DSA_LDS uint8_t* kl, const DSA_LDS uint8_t* vl) __attribute__((always_inline)) {
       constexpr bool MASKED = decltype(masked)::value;
-      f32x4 st[4][QT];
+      f32x4 st[NJ][QT];
       __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-      for (int jp = 0; jp < 4; jp += KJ) {
+      for (int jp = 0; jp < NJ; jp += KJ) {
         u32x4 ka[KJ][NKS];
 #pragma unroll
         for (int jj = 0; jj < KJ; ++jj)
@@ -212,7 +215,7 @@ __global__ __launch_bounds__(kNT, D == 256 ? 1 : D == 128 ? 2 : QT == 2 ? 3 : 4)
         }
       }
       __builtin_amdgcn_s_setprio(0);
-      u32x4 pf[QT][2];
+      u32x4 pf[QT][NJ / 2];
       bool grow = false;
       float alpha[QT];
       uint32_t ok[QT];  // bit 4j + r: key s0 + 16j + 4g + r is seen
@@ -225,27 +228,27 @@ __global__ __launch_bounds__(kNT, D == 256 ? 1 : D == 128 ? 2 : QT == 2 ? 3 : 4)
           if constexpr (CAREFUL) {
             ok[qt] = 0;
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
+            for (int e = 0; e < E; ++e) {
               const int s = 16 * (e >> 2) + (e & 3);
               ok[qt] |= s <= far && (s > near || s < sink) ? 1u << e : 0u;
               st[e >> 2][qt][e & 3] = ok[qt] >> e & 1u ? st[e >> 2][qt][e & 3] : -INFINITY;
             }
           } else if (s0 >= sinks) {  // near < s <= far in one comparison
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
+            for (int e = 0; e < E; ++e) {
               const int s = 16 * (e >> 2) + (e & 3);
               st[e >> 2][qt][e & 3] = static_cast<uint32_t>(far - s) < static_cast<uint32_t>(window) ? st[e >> 2][qt][e & 3] : -INFINITY;
             }
           } else {
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
+            for (int e = 0; e < E; ++e) {
               const int s = 16 * (e >> 2) + (e & 3);
               st[e >> 2][qt][e & 3] = s <= far && (s > near || s < sink) ? st[e >> 2][qt][e & 3] : -INFINITY;
             }
           }
         }
 #pragma unroll
-        for (int e = 0; e < 16; ++e) mx = fmaxf(mx, st[e >> 2][qt][e & 3]);
+        for (int e = 0; e < E; ++e) mx = fmaxf(mx, st[e >> 2][qt][e & 3]);
         mx = mul(max_xor32(max_xor16(mx)), a.scale_log2);
         // the maximum moves when a tile's passes it by 2^8: p then stays far below overflow
         const bool up = mx > m[qt] + 8.f;
@@ -255,9 +258,9 @@ __global__ __launch_bounds__(kNT, D == 256 ? 1 : D == 128 ? 2 : QT == 2 ? 3 : 4)
         m[qt] = m_new;
         const float ref = m_new == -INFINITY ? 0.f : m_new;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) st[e >> 2][qt][e & 3] = weight<CAREFUL>(st[e >> 2][qt][e & 3], a.scale_log2, ref);
+        for (int e = 0; e < E; ++e) st[e >> 2][qt][e & 3] = weight<CAREFUL>(st[e >> 2][qt][e & 3], a.scale_log2, ref);
 #pragma unroll
-        for (int jj = 0; jj < 2; ++jj)
+        for (int jj = 0; jj < NJ / 2; ++jj)
           pf[qt][jj] = u32x4{M::pack(st[2 * jj][qt][0], st[2 * jj][qt][1]), M::pack(st[2 * jj][qt][2], st[2 * jj][qt][3]),
                              M::pack(st[2 * jj + 1][qt][0], st[2 * jj + 1][qt][1]), M::pack(st[2 * jj + 1][qt][2], st[2 * jj + 1][qt][3])};
       }
@@ -270,7 +273,7 @@ __global__ __launch_bounds__(kNT, D == 256 ? 1 : D == 128 ? 2 : QT == 2 ? 3 : 4)
         }
       }
 #pragma unroll
-      for (int jj = 0; jj < 2; ++jj)
+      for (int jj = 0; jj < NJ / 2; ++jj)
 #pragma unroll
         for (int e = 0; e < 4; ++e)
 #pragma unroll
@@ -279,11 +282,11 @@ __global__ __launch_bounds__(kNT, D == 256 ? 1 : D == 128 ? 2 : QT == 2 ? 3 : 4)
       __builtin_amdgcn_s_setprio(1);
 #pragma unroll
       for (int dg = 0; dg < NDT; dg += VG) {
-        u32x4 vfrag[VG][2];
+        u32x4 vfrag[VG][NJ / 2];
 #pragma unroll
         for (int d = 0; d < VG; ++d)
 #pragma unroll
-          for (int jj = 0; jj < 2; ++jj) {
+          for (int jj = 0; jj < NJ / 2; ++jj) {
             const DSA_LDS uint8_t* va = vl + vofs[dg + d] + 32 * jj * (2 * D);
             const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((DSA_LDS s16x4*)va);
             const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((DSA_LDS s16x4*)(va + 16 * (2 * D)));
@@ -302,7 +305,7 @@ __global__ __launch_bounds__(kNT, D == 256 ? 1 : D == 128 ? 2 : QT == 2 ? 3 : 4)
 #pragma unroll
         for (int d = 0; d < VG; ++d)
 #pragma unroll
-          for (int jj = 0; jj < 2; ++jj)
+          for (int jj = 0; jj < NJ / 2; ++jj)
 #pragma unroll
             for (int qt = 0; qt < QT; ++qt) o[dg + d][qt] = M::run(vfrag[d][jj], pf[qt][jj], o[dg + d][qt]);
       }
@@ -310,13 +313,13 @@ __global__ __launch_bounds__(kNT, D == 256 ? 1 : D == 128 ? 2 : QT == 2 ? 3 : 4)
       if constexpr (CAREFUL) {
         if (ballot(odd != 0)) {
           const raw* v = reinterpret_cast<const raw*>(vbase) + static_cast<int64_t>(s0) * a.ldv;
-          for (int s = 0; s < min(kKT, n - s0); ++s) {  // key s0 + s: lane group s / 4 % 4, entry 4 (s / 16) + s % 4
+          for (int s = 0; s < min(KT, n - s0); ++s) {  // key s0 + s: lane group s / 4 % 4, entry 4 (s / 16) + s % 4
             const int from = ((s >> 2) & 3) * 16 + c16;
 #pragma unroll
             for (int qt = 0; qt < QT; ++qt) {
               float mine = 0.0f;  // this lane's p of entry 4 (s / 16) + s % 4, as the product took it
 #pragma unroll
-              for (int e = 0; e < 16; ++e) {
+              for (int e = 0; e < E; ++e) {
                 const uint32_t w = pf[qt][e >> 3][(e >> 1) & 3];
                 const float pe = to_f32(Tag{}, static_cast<uint16_t>(e & 1 ? w >> 16 : w & 0xffffu));
                 mine = e == 4 * (s >> 4) + (s & 3) ? pe : mine;
@@ -342,17 +345,17 @@ __global__ __launch_bounds__(kNT, D == 256 ? 1 : D == 128 ? 2 : QT == 2 ? 3 : 4)
     auto step = [&](auto masked, int v, DSA_LDS uint8_t* kc, DSA_LDS uint8_t* vc, DSA_LDS uint8_t* kn, DSA_LDS uint8_t* vn) __attribute__((always_inline)) {
       if (v + 1 < walk.total) fetch(walk.tile(v + 1), kn, vn);
       __builtin_amdgcn_sched_barrier(0);
-      const int s0 = walk.tile(v) * kKT;
+      const int s0 = walk.tile(v) * KT;
       if constexpr (!decltype(masked)::value) compute(std::false_type{}, s0, kc, vc);
-      else if (s0 <= wave_last && (s0 + kKT > tw - window + 1 || s0 < sinks)) compute(std::true_type{}, s0, kc, vc);
+      else if (s0 <= wave_last && (s0 + KT > tw - window + 1 || s0 < sinks)) compute(std::true_type{}, s0, kc, vc);
       wait_dma_keep<0>();
       block_sync_lds();
     };
     // Tiles that all queries of the block see whole are a loop of their own (in one with the
     // others, the compiler copies O, 64 registers, once a tile).
-    const int last = min(t0 + TQ, n) - 1, whole = last >= window ? (last - window) / kKT + 1 : 0;
+    const int last = min(t0 + TQ, n) - 1, whole = last >= window ? (last - window) / KT + 1 : 0;
     const int w0 = (walk.first + max(0, whole - walk.near) + 1) & ~1;
-    const int w1 = CAREFUL ? w0 : w0 + max(0, (walk.first + t0 / kKT - walk.near - w0) & ~1);
+    const int w1 = CAREFUL ? w0 : w0 + max(0, (walk.first + t0 / KT - walk.near - w0) & ~1);
     int v = 0;
     auto edges = [&](int end) __attribute__((always_inline)) {
       for (; v < end; v += 2) {
