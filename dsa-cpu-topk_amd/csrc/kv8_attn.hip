@@ -33,7 +33,6 @@
 namespace dsa {
 namespace {
 
-
 struct AttnArgs {
   Kv8 c;
   const void* Q;
@@ -677,9 +676,9 @@ Plan plan_of(const Kv8& c, int64_t Tq, int HQ, int64_t n, int64_t window, int64_
   const int64_t turns = (most + waves - 1) / waves;
   const int64_t steps = turns <= 5 ? 1 : turns / 2;
   // as many splits as all run at once: the chunks go over 8 XCDs in equal numbers, and
-  // one that waits for a place doubles the time (2 x 33 blocks an XCD of 2 x 32 places:
-  // 35 us for what takes 20 in 60)
-  const int64_t room = (c.DK <= 128 ? 2 : 1) * int64_t{device_cus() > 0 ? device_cus() : 256};
+  // one that waits for a place makes a second round (4 sequences, 48 rows of one head of 128
+  // over 8191 slots: 35 us with 2 x 33 blocks an XCD of 2 x 32 places, 29 with 2 x 32)
+  const int64_t room = (c.DK <= 128 || (p.shared && !fp32) ? 2 : 1) * int64_t{device_cus() > 0 ? device_cus() : 256};
   const int64_t chunks = rows < 1 ? 0 : room / p.row_tiles / 8 * 8, pairs = c.B * c.HKV;
   int64_t splits = pairs < 1 || pairs >= chunks ? 1 : chunks / pairs;
   splits = splits > steps ? steps : splits;

@@ -595,9 +595,9 @@ int dsa_window_attention(const void* Q, const void* K, const void* V, int dtype,
  * hold nothing.  Pages that no visible slot lies on (behind a window) need no id.  The
  * buffers are device memory of the caller's, in this struct on the host, which is read
  * before the call returns.  A call that writes pages and any other call on them need
- * the order of one stream or an event between them.  Two sequences may share pages that
- * are only read; blocks that a call writes belong to one sequence.  Values of length
- * outside [0, max_pages*page] count as the nearer end.
+ * the order of one stream or an event between them.  Two entries of the table may name
+ * one page that is only read (a shared prompt); a block that a call writes is named by one
+ * entry.  Values of length outside [0, max_pages*page] count as the nearer end.
  * No reference counterpart: it has no cache.
  * Constraints: B <= 65535; 1 <= NP, max_pages; page = 64 * 2^j <= 65536;
  *   max_pages*page <= 2^31 - 256; 1 <= HKV <= 1024; DK = DV in {32, 64, 96, 128, 192,
