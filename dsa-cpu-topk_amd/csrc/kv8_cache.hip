@@ -1,5 +1,10 @@
 // kv8_cache.hip -- what goes into the paged 8-bit cache and comes back out of it
 // (gfx950).
+//
+// A block of 64 slots of one head has one scale for K and one for V, the least 2^e with
+// max|x| <= 448 * 2^e, so its values' maximum has to be known before the first code is: who
+// encodes a block holds all its new tokens in registers meanwhile, and reads each once.  All
+// of it moves bytes; nothing is bound by arithmetic.
 #include <algorithm>
 
 #include "dsa_launch.h"
@@ -169,6 +174,12 @@ __device__ __forceinline__ int word_token(int w) { return (w & 3) * 16 + (w >> 2
 // side), or query heads.  Of K a thread has one unit of some tokens; of V 4 tokens by 8
 // dimensions, which it turns into words of 4 tokens (a word of the cache has one owner,
 // so bytes that stay are merged without a barrier, and a wave writes whole rows of 64).
+//
+// Bound by memory: 2 x 16384 tokens of 32 and 8 heads of 128 in bf16 with rotated keys, 805 MB
+// read and written, take 190 us, 4.2 TB/s where a large copy reaches 5.1.  (A block a head, which
+// loads the angles anew for each, took 251.)  8 prompts of 1001 tokens of 8 heads of 64 in fp32:
+// 17 us.  What a thread holds allows two blocks a compute unit,
+// whose waves wait in 78 of 100 cycles.
 template <typename Tag, int DK, int DV>
 __global__ __launch_bounds__(kNT) void append_kernel(Kv8 c, Kv8Append a, int nblk, int kv_groups, int q_groups, int update) {
   using raw = typename Tag::raw;
@@ -363,7 +374,8 @@ __global__ __launch_bounds__(kNT) void append_kernel(Kv8 c, Kv8Append a, int nbl
 // Few tokens (a decode step): a block of threads takes a sequence whole, so that one launch also
 // changes its length.  A wave takes the K or the V of one head, a unit of one token a
 // lane, then units of the queries; what does not depend on the position is loaded before the
-// position is known.
+// position is known.  Bound by latency, that of the chain length, page, scale, codes: 32 sequences
+// of 32 and 8 heads of 128 in bf16, 11 MB, take 8.1 us.
 constexpr int kFew = 4;  // tokens, by 16 units: a wave
 template <typename Tag, int DK, int DV>
 __global__ __launch_bounds__(1024) void append_few_kernel(Kv8 c, Kv8Append a) {
@@ -499,7 +511,8 @@ __global__ __launch_bounds__(kNT) void append_counts_kernel(Kv8 c, Kv8Append a) 
 // Slots back as values; zeros for a slot that holds nothing.  A block of threads takes 64
 // entries of a list, one head.  Where they are one block's slots in order (as
 // the first N slots are, and runs that begin with a block), a thread takes 4 tokens by 8
-// dimensions of V from words of 4 tokens; else it gathers bytes.
+// dimensions of V from words of 4 tokens; else it gathers bytes.  Bound by memory: 2 x 16384 slots
+// of 8 heads of 128 as bf16, 201 MB, take 46 us, 4.4 TB/s; gathered, 143.
 __device__ __forceinline__ void decode8(uint32_t w0, uint32_t w1, float f, float (&x)[8]) {
   const f32x2 a = __builtin_amdgcn_cvt_pk_f32_fp8(w0, false), b = __builtin_amdgcn_cvt_pk_f32_fp8(w0, true);
   const f32x2 c = __builtin_amdgcn_cvt_pk_f32_fp8(w1, false), d = __builtin_amdgcn_cvt_pk_f32_fp8(w1, true);
