@@ -15,19 +15,19 @@
 // So no value of the cache is rounded.  Rows of Q are scaled by a power of two into f16's
 // range and enter as one f16 piece (16-bit types) or two (fp32, 23 bits); p likewise.
 //
-// Few rows (!SHARED): each of a block's four waves takes blocks of its own in turn, its
+// Few rows or short rows of K (!SHARED): each of a block's four waves takes blocks of its own in turn, its
 // operands straight into registers; K of the next block is on its way while p and V are
 // multiplied, V while the logits are formed, the page id two turns ahead.  Bound by memory: 16
 // caches of up to 32768 slots, 32 heads on 8 of 128, 834 MB, take 149 us, 5.6 TB/s (a large
 // array is read at 6.35).  Operands by way of LDS, as below, or eight waves a block were slower.
 //
-// Many rows (SHARED): the waves take different rows of the same blocks.  Codes go to LDS by
+// Many long rows, or few slots (SHARED): the waves take different rows of the same blocks.  Codes go to LDS by
 // DMA, whole rows at a time and in two buffers (lanes next to each other fetch bytes next to
 // each other: a lane's own operand is 16 bytes of a row of its own, which costs the L1 64
 // accesses an instruction where this takes 16), rows' 16-byte chunks swizzled so that no two
 // lanes meet on a bank when they are read as operands.  Bound by the vector instructions that widen
-// the codes and weigh the logits, which 32 rows a wave share (16-bit types, DK <= 128: more have no
-// registers): 4 x 48 tokens of 16 heads on one of 128 over 8191 slots, 10.5 GFLOP, take 29 us;
+// the codes and weigh the logits, which 32 rows a wave share where there are enough (DK <= 128 of
+// 16-bit types: more have no registers): 4 x 48 tokens of 16 heads on one of 128 over 8191 slots, 10.5 GFLOP, take 29 us;
 // 60 with waves on slots of their own.
 #include <algorithm>
 
@@ -44,6 +44,7 @@ struct AttnArgs {
   const int32_t* count;
   int Tq, HQ, G;
   int row_tiles, splits;
+  uint32_t few_chunks;  // sequences, K/V heads and splits where they are below 8, else 0
   int64_t n;       // slots that count
   int64_t window;  // 0: all
   int64_t sinks;
@@ -140,8 +141,11 @@ __global__ __launch_bounds__(kNT, DK <= 128 || (SHARED && Tag::kBytes == 2) ? 2 
 
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = lane_id();
   const int g = lane >> 4, col = lane & 15, wr = SHARED ? wave : 0, wt = SHARED ? 0 : wave;
-  // Blocks of one chunk of slots and their row tiles go to one XCD (block i starts on XCD i % 8).
-  const uint32_t chunk = blockIdx.x % 8 + blockIdx.x / (8 * a.row_tiles) * 8, rt = blockIdx.x / 8 % a.row_tiles;
+  // Blocks of one chunk of slots and their row tiles go to one XCD (block i starts on XCD i % 8);
+  // where chunks are fewer than the XCDs, row tiles go over all of them.
+  const uint32_t few = a.few_chunks;
+  const uint32_t chunk = few ? blockIdx.x % few : blockIdx.x % 8 + blockIdx.x / (8 * a.row_tiles) * 8;
+  const uint32_t rt = few ? blockIdx.x / few : blockIdx.x / 8 % a.row_tiles;
   const int split = chunk % a.splits;
   const uint32_t bh = chunk / a.splits;
   const int h = bh % a.c.HKV;
@@ -587,7 +591,7 @@ __global__ __launch_bounds__(kNT, DK <= 128 || (SHARED && Tag::kBytes == 2) ? 2 
 
 constexpr int kMaxSplits = 512;
 
-// Few splits: a thread joins 4 columns of a row, all splits on their way at once.
+// Few splits of many rows: a thread joins 4 columns of a row, all splits on their way at once.
 constexpr int kFewSplits = 8;
 template <typename Tag>
 __global__ __launch_bounds__(kNT) void join_few_kernel(const float* __restrict__ part, const float2* __restrict__ ml,
@@ -667,25 +671,37 @@ struct Plan {
 
 Plan plan_of(const Kv8& c, int64_t Tq, int HQ, int64_t n, int64_t window, int64_t sinks, bool fp32) {
   Plan p;
-  const int64_t rows = Tq * (HQ / c.HKV);
-  // 32 rows a wave share the widening of K and V, where the registers hold them
-  p.shared = rows > 32;
-  p.rt = !fp32 && (p.shared ? rows > 64 && c.DK <= 128 : rows > 16 && c.DK <= 96) ? 2 : 1;
-  const int64_t tile = 16 * p.rt * (p.shared ? kWaves : 1), waves = p.shared ? 1 : kWaves;
-  p.row_tiles = static_cast<int>((rows + tile - 1) / tile);
+  const int64_t rows = Tq * (HQ / c.HKV), tiles = (rows + 15) / 16, pairs = c.B * c.HKV;
   int64_t most = (n + kBlk - 1) / kBlk;  // blocks that a row tile walks
   if (window > 0) {
     const int64_t near = (window + Tq - 1 + kBlk - 1) / kBlk + 1 + (sinks < n ? (sinks + kBlk - 1) / kBlk : most);
     most = near < most ? near : most;
   }
-  // few turns of a block's waves cost less than the launch that joins splits, and a split takes two at least
+  const int64_t work = pairs * tiles * most;
+  // Rows share blocks of slots by way of LDS where there are rows for it and, beyond the few
+  // slots that leave a wave nothing of its own, enough to do to pay for the barriers and the
+  // joins; the shorter K rows are, the fewer accesses that saves.  us, waves' own / shared (bf16):
+  //   D 128, 48 rows: 32 pairs of 1024 slots 10.6 / 13.7, of 8192 29.3 / 26.0; 128 of 16384 187 / 127
+  //   D 64: 128 pairs of 16384, 64 rows 79 / 84; D 192: 256 of 700, 48 rows 32.0 / 28.7
+  //   D 64, 464 rows over 58 slots: 96 pairs 15.1 / 8.4; 800 rows over 100: 2 pairs 5.4 / 6.1
+  p.shared = rows > 32 && (most <= 4 ? pairs * tiles >= 1024 : c.DK > 96 && work >= (c.DK > 128 ? 8192 : 12288));
+  // 32 rows a wave share the widening of K and V where the registers hold them, against half
+  // the blocks (16 / 32 rows):
+  //   own, D 64, 64 rows: 32 pairs of 8192 slots 17.9 / 19.5; 256 of 4096 42.1 / 36.1
+  //   shared, D 128: 256 pairs of 4096 and 64 rows 73 / 92; 4 of 32768 and 768 rows 98 / 84
+  p.rt = !fp32 && (p.shared ? c.DK == 128 && most > 4 && rows > 512 : c.DK <= 96 && rows > 16 && work >= 24576) ? 2 : 1;
+  const int64_t tile = 16 * p.rt * (p.shared ? kWaves : 1), waves = p.shared ? 1 : kWaves;
+  p.row_tiles = static_cast<int>((rows + tile - 1) / tile);
+  // A few turns of a block's waves cost less than the launch that joins splits (one head's 5
+  // turns: 10.6 whole, 10.4 split; 6: 11.9, 9.5; shared, 4: 13.7, 13.0), and a split takes two at least.
   const int64_t turns = (most + waves - 1) / waves;
-  const int64_t steps = turns <= 5 ? 1 : turns / 2;
+  const int64_t steps = turns <= (p.shared ? 3 : 5) ? 1 : turns / 2;
   // as many splits as all run at once: the chunks go over 8 XCDs in equal numbers, and
   // one that waits for a place makes a second round (4 sequences, 48 rows of one head of 128
   // over 8191 slots: 35 us with 2 x 33 blocks an XCD of 2 x 32 places, 29 with 2 x 32)
   const int64_t room = (c.DK <= 128 || (p.shared && !fp32) ? 2 : 1) * int64_t{device_cus() > 0 ? device_cus() : 256};
-  const int64_t chunks = rows < 1 ? 0 : room / p.row_tiles / 8 * 8, pairs = c.B * c.HKV;
+  int64_t chunks = rows < 1 ? 0 : room / p.row_tiles;
+  if (chunks >= 8) chunks = chunks / 8 * 8;
   int64_t splits = pairs < 1 || pairs >= chunks ? 1 : chunks / pairs;
   splits = splits > steps ? steps : splits;
   p.splits = static_cast<int>(splits > kMaxSplits ? kMaxSplits : splits);
@@ -702,17 +718,17 @@ int64_t workspace_of(const Kv8& c, int64_t Tq, int HQ, int64_t n, int64_t window
 
 template <typename Tag, int DK, int DV>
 void launch_dims(const AttnArgs& a, const Plan& p, uint32_t grid, hipStream_t stream) {
-  if constexpr (Tag::kBytes == 2 && DK <= 128)
+  if constexpr (Tag::kBytes == 2 && DK == 128)
     if (p.shared && p.rt == 2) return (void)(attn_kernel<Tag, DK, DV, 2, true><<<grid, kNT, 0, stream>>>(a));
   if constexpr (Tag::kBytes == 2 && DK <= 96)
-    if (p.rt == 2) return (void)(attn_kernel<Tag, DK, DV, 2, false><<<grid, kNT, 0, stream>>>(a));
+    if (!p.shared && p.rt == 2) return (void)(attn_kernel<Tag, DK, DV, 2, false><<<grid, kNT, 0, stream>>>(a));
   if (p.shared) attn_kernel<Tag, DK, DV, 1, true><<<grid, kNT, 0, stream>>>(a);
   else attn_kernel<Tag, DK, DV, 1, false><<<grid, kNT, 0, stream>>>(a);
 }
 
 template <typename Tag>
 hipError_t launch_type(const AttnArgs& a, const Plan& p, hipStream_t stream) {
-  const int64_t chunks = (a.c.B * a.c.HKV * p.splits + 7) / 8 * 8;
+  const int64_t chunks = a.few_chunks ? a.few_chunks : (a.c.B * a.c.HKV * p.splits + 7) / 8 * 8;
   const uint32_t grid = static_cast<uint32_t>(chunks * p.row_tiles);
   if (a.c.DK != a.c.DV) launch_dims<Tag, 192, 128>(a, p, grid, stream);
   else switch (a.c.DK) {
@@ -725,9 +741,12 @@ hipError_t launch_type(const AttnArgs& a, const Plan& p, hipStream_t stream) {
   }
   typename Tag::raw* const out = static_cast<typename Tag::raw*>(a.out);
   const int64_t rows = a.c.B * a.Tq * a.HQ;
-  if (p.splits > kFewSplits) {
+  if (p.splits == 1) return hipGetLastError();
+  // many rows: a few a block (with the attention, of 8496 rows 26 us, 34 with a block a row; of 128
+  // 12.9 and 11.1)
+  if (p.splits > kFewSplits || rows < 1024) {
     join_kernel<Tag><<<static_cast<uint32_t>(rows), kNT, 0, stream>>>(a.part, a.ml, p.splits, a.c.DV, out);
-  } else if (p.splits > 1) {
+  } else {
     const int64_t per = kNT / (a.c.DV / 4);
     join_few_kernel<Tag><<<static_cast<uint32_t>((rows + per - 1) / per), kNT, 0, stream>>>(a.part, a.ml, p.splits, a.c.DV, rows, out);
   }
@@ -760,6 +779,7 @@ hipError_t launch_kv8_attn(const Kv8& c, const void* Q, int dtype, const int32_t
   a.G = HQ / c.HKV;
   a.row_tiles = p.row_tiles;
   a.splits = p.splits;
+  a.few_chunks = c.B * c.HKV * p.splits < 8 ? static_cast<uint32_t>(c.B * c.HKV * p.splits) : 0u;
   a.n = n;
   a.window = window;
   a.sinks = sinks;

@@ -64,6 +64,33 @@ def test_attention_of_more_shapes(dev, B, lengths, HQ, HKV, DK, DV, Tq, window, 
     check_attention(dev, cache, Q, dtype, window, sinks, count, span, scale)
 
 
+@pytest.mark.parametrize("B, length, HQ, HKV, D, Tq, window, sinks, count, dtype", [
+    (1, 6200, 4, 1, 64, 1024, None, 0, None, BF16),     # 32 rows a wave, waves of their own slots, four splits
+    (1, 6200, 4, 1, 96, 1024, None, 0, [1000], F16),
+    (1, 3100, 4, 1, 128, 1024, None, 0, None, BF16),    # 32 rows a wave, shared, sixteen splits
+    (1, 3100, 4, 1, 128, 1024, None, 0, [1001], F32),
+    (1, 2500, 8, 1, 128, 1024, 700, 70, None, F16),
+    (1, 4200, 4, 1, 256, 512, 4000, 3, None, BF16),
+    (1, 4200, 4, 1, 192, 512, None, 0, None, F32),
+    (8, 200, 64, 8, 64, 32, None, 0, [32, 0, 1, 31, 32, 32, 17, 32], BF16),   # a few slots, shared
+    (8, 150, 64, 8, 32, 32, 40, 1, None, F32),
+    (8, 66, 64, 8, 96, 32, None, 0, None, F16),
+    (8, 200, 64, 8, 128, 32, 64, 0, None, F32),
+    (1, 300, 8, 1, 32, 600, None, 0, None, BF16),       # more tokens than slots, chunks fewer than XCDs
+])
+def test_pieces_of_many_rows(dev, B, length, HQ, HKV, D, Tq, window, sinks, count, dtype):
+    """Pieces of prompts behind a cache.  NaN of a late slot's V reaches the rows that see it alone."""
+    lengths = [length - 3 * b for b in range(B)]
+    S = -(-length // 64) * 64 + 64
+    cache = filled(dev, B, S, HKV, D, D, lengths, 64, seed=D + Tq)
+    for b, at in enumerate(n - 5 for n in lengths):
+        row = cache.codes[cache.pages[b, at // 64], 0, 0]
+        row[64 * D:].view(D, 64)[::7, O.PLACE[at % 64]] = 0x7F
+    Q = randn(gen(Tq + D), B, Tq, HQ, D, dtype=dtype)
+    out, _ = check_attention(dev, cache, Q, dtype, window, sinks, count)
+    assert bool(out[0, :2].isfinite().all()) or length < Tq
+
+
 def test_pages_past_32_bits(dev):
     """Pages beyond 4 GiB of codes hold and give what the same tokens do in a small pool."""
     HKV, D, page, S, T = 8, 128, 4096, 8192, 5000
