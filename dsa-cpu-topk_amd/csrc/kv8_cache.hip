@@ -628,9 +628,10 @@ hipError_t append_dims(const Kv8& c, const Kv8Append& a, hipStream_t stream) {
   auto groups_of = [&](int64_t heads) { return static_cast<int>(std::min(heads, (want + blocks - 1) / blocks)); };
   constexpr int kSide = DK >= 96 ? 1 : 128 / DK;
   const int kv = groups_of((c.HKV + kSide - 1) / kSide), q = a.Q_out ? groups_of((a.HQ + kSide - 1) / kSide) : 0;
-  append_kernel<Tag, DK, DV><<<static_cast<uint32_t>(blocks * (kv + q)), kNT, 0, stream>>>(c, a, nblk, kv, q, a.start != nullptr);
-  // where the blocks read the length to find their place, a launch of its own changes it
-  if (!a.start) append_counts_kernel<<<static_cast<uint32_t>(c.B), kNT, 0, stream>>>(c, a);
+  // where the blocks read the length (to find their place, or as the count), a launch of its own changes it
+  const bool update = a.start != nullptr && a.count != c.length;
+  append_kernel<Tag, DK, DV><<<static_cast<uint32_t>(blocks * (kv + q)), kNT, 0, stream>>>(c, a, nblk, kv, q, update);
+  if (!update) append_counts_kernel<<<static_cast<uint32_t>(c.B), kNT, 0, stream>>>(c, a);
   return hipGetLastError();
 }
 

@@ -622,7 +622,8 @@ typedef struct dsa_kv8_cache {
  *   (a cos - b sin, b cos + a sin),  cos, sin [table rows][R/2] fp32 at the position,
  * in fp32, each product and sum rounded once.  R = 0: nothing is rotated.  The first count[b]
  * (null: T) tokens go into the cache; then length[b] = start[b] + count[b], at most
- * the last slot's end, and lost[b] counts those that found no slot or no page.
+ * the last slot's end, and lost[b] counts those that found no slot or no page.  start and
+ * count may be length itself: they are read before it changes.
  *   A block's scale is the least 2^e (from 2^-117 on) with max|x| <= 448 * 2^e over its
  * new finite values, and not below the block's scale so far where it holds tokens of
  * before; x / 2^e rounds to the nearest e4m3, ties to even, Inf and NaN become NaN.

@@ -167,6 +167,21 @@ def test_start_is_the_length(dev):
     assert all(same(getattr(caches[0], n), getattr(caches[1], n)) for n in ("codes", "scales", "length", "lost"))
 
 
+def test_count_is_the_length(dev):
+    """count=cache.length: how much there is, written again."""
+    g = gen(16)
+    B, T, HKV, D = 40, 300, 8, 64
+    K, V = randn(g, B, T, HKV, D).to(dev), randn(g, B, T, HKV, D).to(dev)
+    many = ints(dev, [(17 * b) % (T + 1) for b in range(B)])
+    zero = torch.zeros_like(many)
+    caches = [P.KV8Cache.empty(B, 320, HKV, D, D, device=dev) for _ in range(2)]
+    caches[0].length.copy_(many)
+    P.kv8_append(caches[0], K, V, start=zero, count=caches[0].length)
+    P.kv8_append(caches[1], K, V, start=zero, count=many)
+    assert all(same(getattr(caches[0], n), getattr(caches[1], n)) for n in ("codes", "scales", "length", "lost"))
+    assert eq(caches[0].length, many)
+
+
 def test_work_on_another_stream(dev):
     """A chain of calls on a stream of its own, its temporaries freed meanwhile."""
     g = gen(8)
