@@ -624,7 +624,7 @@ __global__ __launch_bounds__(kNT) void join_few_kernel(const float* __restrict__
   store4<Tag>(out + row * DV + d, z * (1.0f / all));
 }
 
-// A block joins one row's splits: of 3072 rows of 128 in 20 splits, 31 MB, in 8 us.  (Threads that
+// A block joins one row's splits: 20 of rows of 128, 31 MB in all, in 8 us.  (Threads that
 // take 4 columns and every eighth split took 9, threads that hold all splits of 4 columns 28.)
 template <typename Tag>
 __global__ __launch_bounds__(kNT) void join_kernel(const float* __restrict__ part, const float2* __restrict__ ml,
