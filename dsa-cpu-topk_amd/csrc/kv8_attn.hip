@@ -44,7 +44,7 @@ struct AttnArgs {
   const int32_t* count;
   int Tq, HQ, G;
   int row_tiles, splits;
-  uint32_t few_chunks;  // sequences, K/V heads and splits where they are below 8, else 0
+  uint32_t few_chunks;  // sequences, K/V heads and splits where they are few, else 0
   int64_t n;       // slots that count
   int64_t window;  // 0: all
   int64_t sinks;
@@ -142,7 +142,7 @@ __global__ __launch_bounds__(kNT, DK <= 128 || (SHARED && Tag::kBytes == 2) ? 2 
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = lane_id();
   const int g = lane >> 4, col = lane & 15, wr = SHARED ? wave : 0, wt = SHARED ? 0 : wave;
   // Blocks of one chunk of slots and their row tiles go to one XCD (block i starts on XCD i % 8);
-  // where chunks are fewer than the XCDs, row tiles go over all of them.
+  // where a few chunks would not fill them alike, row tiles go round over all of them.
   const uint32_t few = a.few_chunks;
   const uint32_t chunk = few ? blockIdx.x % few : blockIdx.x % 8 + blockIdx.x / (8 * a.row_tiles) * 8;
   const uint32_t rt = few ? blockIdx.x / few : blockIdx.x / 8 % a.row_tiles;
@@ -779,7 +779,9 @@ hipError_t launch_kv8_attn(const Kv8& c, const void* Q, int dtype, const int32_t
   a.G = HQ / c.HKV;
   a.row_tiles = p.row_tiles;
   a.splits = p.splits;
-  a.few_chunks = c.B * c.HKV * p.splits < 8 ? static_cast<uint32_t>(c.B * c.HKV * p.splits) : 0u;
+  // (12 heads of 64, 512 tokens of 8 each over 1000 slots: 41 us with two heads on four of the XCDs, 31
+  // so; with many chunks the XCDs have much the same, and a chunk's row tiles one L2)
+  a.few_chunks = c.B * c.HKV * p.splits < 64 ? static_cast<uint32_t>(c.B * c.HKV * p.splits) : 0u;
   a.n = n;
   a.window = window;
   a.sinks = sinks;

@@ -52,27 +52,25 @@ __device__ __forceinline__ Walk walk_of(const Win& a, int64_t b, int t0) {
   return w;
 }
 
-// Block -> (tile of queries, batch, head): the tiles of one K/V head go to one XCD (block
-// i starts on XCD i % 8), the latest, which see most, first.
+// Block -> (tile of queries, batch, head), the latest tiles, which see most, first.  The
+// sequences' K/V heads lie innermost, so that the tiles of one go to one XCD where they are a
+// multiple of 8 (block i starts on XCD i % 8), and all XCDs have the same work where they are
+// not: one head of 128, 8 query heads, 8192 tokens, window 1000, 312 us on one XCD, 60 on all;
+// 9 K/V heads, 16384 tokens, window 2048, 977 with two on one of them, 695 so.
 // (32-bit throughout: a 64-bit division costs as much as a short prompt's tile.)
 template <int TQ>
-__device__ __forceinline__ bool place(const Win& a, int& t0, int64_t& b, int& h, int& hk) {
+__device__ __forceinline__ void place(const Win& a, int& t0, int64_t& b, int& h, int& hk) {
   const uint32_t ntile = static_cast<uint32_t>(a.T + TQ - 1) / TQ, G = a.G, HKV = a.HKV;
-  const uint32_t pairs = static_cast<uint32_t>(a.B) * HKV, lanes = (pairs + 7) / 8;  // (b, K/V head)
-  const uint32_t i = blockIdx.x / 8, j = i / G, tile = j / lanes;
-  const uint32_t pair = (j - tile * lanes) * 8 + blockIdx.x % 8;
+  const uint32_t pairs = static_cast<uint32_t>(a.B) * HKV;  // (b, K/V head)
+  const uint32_t i = blockIdx.x / pairs, pair = blockIdx.x - i * pairs, tile = i / G, bb = pair / HKV;
   t0 = static_cast<int>((ntile - 1 - tile) * TQ);
-  if (pair >= pairs) return false;
-  const uint32_t bb = pair / HKV;
   b = bb;
   hk = static_cast<int>(pair - bb * HKV);
-  h = static_cast<int>(hk * G + (i - j * G));
-  return true;
+  h = static_cast<int>(hk * G + (i - tile * G));
 }
 template <int TQ>
 int64_t blocks_of(const Win& a) {
-  const int64_t ntile = (a.T + TQ - 1) / TQ;
-  return (a.B * a.HKV + 7) / 8 * 8 * a.G * ntile;
+  return a.B * a.HQ * ((a.T + TQ - 1) / TQ);
 }
 
 __device__ __forceinline__ float mul(float x, float y) {  // rounded by itself
@@ -138,7 +136,7 @@ __global__ __launch_bounds__(kNT, D >= 128 ? 2 : QT == 2 ? 3 : 4) void window_ke
   const int lane = lane_id(), g = lane >> 4, c16 = lane & 15;
   int t0, h, hk;
   int64_t b;
-  if (!place<TQ>(a, t0, b, h, hk)) return;
+  place<TQ>(a, t0, b, h, hk);
   const Walk walk = walk_of<TQ, KT>(a, b, t0);
   const int T = a.T, n = walk.n, window = a.window, sinks = a.sinks;
   const int tw = t0 + 16 * QT * wave, wave_last = min(tw + 16 * QT - 1, n - 1);
@@ -437,20 +435,26 @@ __device__ __forceinline__ Three split3(float x, float y) {
 constexpr int kProducts = 6;
 __device__ constexpr int kLeft[kProducts] = {0, 2, 1, 0, 1, 0}, kRight[kProducts] = {2, 0, 1, 1, 0, 0};
 
-template <int D, int QT, int KT>
-__global__ __launch_bounds__(kNT, D * QT >= 256 ? 1 : 2) void window_f32_kernel(Win a) {
+//
+// TEAMS = 2, where blocks are so few that each has a compute unit to itself: two teams of four
+// waves take every other tile for the same queries and join their sums at the end.
+template <int D, int QT, int KT, int TEAMS>
+__global__ __launch_bounds__(kNT * TEAMS, TEAMS == 2 || D * QT >= 256 ? 1 : 2) void window_f32_kernel(Win a) {
   using L = TileLds<D, KT>;
   using M = Mfma16x16x32<BF16>;
   constexpr int TQ = 64 * QT, NKS = D / 32, NDT = D / 16, NJ = KT / 16;
   constexpr int PER = KT * D / 8 / kNT;  // 8-element chunks of a tile a thread, of K and of V
   constexpr int LD = D + 4;              // fp32 rows of the careful pass
   static_assert(PER >= 1 && 16 * LD * 4 <= 3 * L::BYTES);
-  __shared__ __align__(16) uint8_t kl[3 * L::BYTES], vl[3 * L::BYTES];
-  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  __shared__ __align__(16) uint8_t k_lds[TEAMS * 3 * L::BYTES], v_lds[TEAMS * 3 * L::BYTES];
+  const int team = TEAMS == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / kNT);
+  uint8_t* const kl = k_lds + team * 3 * L::BYTES;
+  uint8_t* const vl = v_lds + team * 3 * L::BYTES;
+  const int tid = TEAMS == 1 ? threadIdx.x : threadIdx.x % kNT, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lane = lane_id(), g = lane >> 4, c16 = lane & 15;
   int t0, h, hk;
   int64_t b;
-  if (!place<TQ>(a, t0, b, h, hk)) return;
+  place<TQ>(a, t0, b, h, hk);
   const Walk walk = walk_of<TQ, KT>(a, b, t0);
   const int T = a.T, n = walk.n, window = a.window, sinks = a.sinks;
   const int tw = t0 + 16 * QT * wave, wave_last = min(tw + 16 * QT - 1, n - 1);
@@ -492,7 +496,7 @@ __global__ __launch_bounds__(kNT, D * QT >= 256 ? 1 : 2) void window_f32_kernel(
     }
   };
 
-  if (walk.total > 0) fetch(walk.tile(0));
+  if (team < walk.total) fetch(walk.tile(team));
   u32x4 q[QT][NKS][3];
   int tq[QT];
 #pragma unroll
@@ -560,13 +564,13 @@ __global__ __launch_bounds__(kNT, D * QT >= 256 ? 1 : 2) void window_f32_kernel(
   auto all_see = [&](int s0, int s1) { return s1 <= tw && (s0 > wave_last - window || s1 < sinks); };
 
   clear();
-  for (int v = 0; v < walk.total; ++v) {
-    const int s0 = walk.tile(v) * KT, s1 = s0 + KT - 1;
+  for (int v0 = 0; v0 < walk.total; v0 += TEAMS) {
+    const int v = v0 + team, s0 = walk.tile(v) * KT, s1 = s0 + KT - 1;
     block_sync_lds();  // the last tile has been read
-    split();
-    if (v + 1 < walk.total) fetch(walk.tile(v + 1));
+    if (v < walk.total) split();
+    if (v + TEAMS < walk.total) fetch(walk.tile(v + TEAMS));
     block_sync_lds();
-    if (!seen(s0, s1)) continue;
+    if (v >= walk.total || !seen(s0, s1)) continue;
     const bool inner = all_see(s0, s1);
     f32x4 st[QT][NJ];
     __builtin_amdgcn_s_setprio(1);
@@ -641,9 +645,31 @@ __global__ __launch_bounds__(kNT, D * QT >= 256 ? 1 : 2) void window_f32_kernel(
     __builtin_amdgcn_s_setprio(0);
   }
 
+  if constexpr (TEAMS == 2) {
+    static_assert(QT == 1 && NDT * kNT * 16 <= TEAMS * 3 * L::BYTES);
+    f32x4* const other_o = reinterpret_cast<f32x4*>(k_lds);
+    float2* const other = reinterpret_cast<float2*>(v_lds);
+    __syncthreads();
+    if (team == 1) {
+#pragma unroll
+      for (int d = 0; d < NDT; ++d) other_o[d * kNT + tid] = o[d][0];
+      other[tid] = make_float2(m[0], l[0]);
+    }
+    __syncthreads();
+    if (team == 0) {
+      const float2 x = other[tid];
+      const float top = fmaxf(m[0], x.x), ref = top == -INFINITY ? 0.0f : top;
+      const float f = __builtin_amdgcn_exp2f(m[0] - ref), g = __builtin_amdgcn_exp2f(x.x - ref);
+      l[0] = l[0] * f + x.y * g;
+#pragma unroll
+      for (int d = 0; d < NDT; ++d) o[d][0] = o[d][0] * f + other_o[d * kNT + tid] * g;
+    }
+  }
+
   bool odd = false;
 #pragma unroll
   for (int qt = 0; qt < QT; ++qt) {
+    if (team) break;  // its sums are in the first team's
     const float all = sum_xor32(sum_xor16(l[qt]));
     odd |= tq[qt] < n && !(all > 0.0f && finite_f32(all));
 #pragma unroll
@@ -712,6 +738,7 @@ __global__ __launch_bounds__(kNT, D * QT >= 256 ? 1 : 2) void window_f32_kernel(
     }
   }
 
+  if (team) return;
 #pragma unroll
   for (int qt = 0; qt < QT; ++qt) {
     const float sum = sum_xor32(sum_xor16(l[qt]));
@@ -741,8 +768,13 @@ void launch_16(const Win& w, hipStream_t stream) {
 template <int D, int KT>
 void launch_32(const Win& w, hipStream_t stream) {
   if constexpr (D <= 64)  // registers
-    if (wide_tiles(w, 2)) return (void)(window_f32_kernel<D, 2, KT><<<static_cast<uint32_t>(blocks_of<128>(w)), kNT, 0, stream>>>(w));
-  window_f32_kernel<D, 1, KT><<<static_cast<uint32_t>(blocks_of<64>(w)), kNT, 0, stream>>>(w);
+    if (wide_tiles(w, 2)) return (void)(window_f32_kernel<D, 2, KT, 1><<<static_cast<uint32_t>(blocks_of<128>(w)), kNT, 0, stream>>>(w));
+  const uint32_t blocks = static_cast<uint32_t>(blocks_of<64>(w));
+  // one / two teams, us: 8 heads of 128, 2 x 1000 tokens 77 / 56, 4 heads of 64, 2 x 438 tokens 23 / 18;
+  // past a block a compute unit the other block is the better neighbour (512 blocks of 128: 58 / 65)
+  if constexpr (D <= 128)  // LDS
+    if (w.T > KT && blocks <= static_cast<uint32_t>(device_cus() > 0 ? device_cus() : 256)) return (void)(window_f32_kernel<D, 1, KT, 2><<<blocks, 2 * kNT, 0, stream>>>(w));
+  window_f32_kernel<D, 1, KT, 1><<<blocks, kNT, 0, stream>>>(w);
 }
 template <int D>
 hipError_t launch_dims(const Win& w, int dtype, hipStream_t stream) {

@@ -148,11 +148,30 @@ def test_strides_past_32_bits(dev, dtype):
     (40, 130, 16, 2, 32, 64, 1, None, F16),          # 128 queries a block
     (24, 300, 16, 4, 128, 130, 2, None, BF16),
     (40, 129, 8, 8, 64, None, 0, None, F32),
+    (11, 130, 10, 5, 64, None, 0, None, F32),        # 330 blocks, one team of waves each
+    (11, 130, 10, 5, 128, 65, 2, None, F32),
+    (12, 129, 9, 3, 32, 20, 0, None, F32),
+    (1, 700, 9, 3, 128, 300, 0, None, BF16),         # K/V heads that are no multiple of 8
+    (1, 64, 2, 1, 64, None, 0, None, F32),           # one tile of keys, two, three
+    (1, 128, 2, 1, 64, None, 0, [127], F32),
+    (1, 192, 2, 1, 64, None, 0, None, F32),
 ])
 def test_window_of_more_shapes(dev, B, T, HQ, HKV, D, window, sinks, count, dtype):
     g = gen(B + T)
     Q, K, V = (randn(g, B, T, h, D, dtype=dtype) for h in (HQ, HKV, HKV))
     check_window(dev, Q, K, V, dtype, window, sinks, count)
+
+
+@pytest.mark.parametrize("D, dtype", [(32, F32), (64, F32), (128, F32), (256, F32), (64, BF16), (128, F16)])
+def test_window_of_many_blocks_keeps_what_is_not_seen_out(dev, D, dtype):
+    """NaN and Inf in keys and values, in batches whose blocks fill the card."""
+    g = gen(D + 1)
+    B, T = 12, 150
+    Q, K, V = (randn(g, B, T, h, D, dtype=dtype) for h in (8, 4, 4))
+    for b in range(0, B, 2):
+        V[b, 30 + b, 0, 3], V[b, 100, 1, 7], V[b, 101, 1, 7], K[b, 70, 2, 5] = math.nan, math.inf, -math.inf, math.nan
+    out, _ = check_window(dev, Q, K, V, dtype, 40, 2)
+    assert bool(out[1::2].isfinite().all()) and bool(out[0, 30:70, :2, 3].isnan().all()) and bool(out[0, :, 6:].isfinite().all())
 
 
 def test_start_is_the_length(dev):
