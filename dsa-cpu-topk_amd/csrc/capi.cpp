@@ -719,8 +719,9 @@ int dsa_window_attention(const void* Q, const void* K, const void* V, int dtype,
   if (!stride_ok(ldq, static_cast<int64_t>(HQ) * D, dtype) || !stride_ok(ldk, static_cast<int64_t>(HKV) * D, dtype) ||
       !stride_ok(ldv, static_cast<int64_t>(HKV) * D, dtype))
     return fail(DSA_EINVAL, "window_attention: strides %lld %lld %lld must hold a token's heads, be multiples of 16 bytes and at most 2^24", (long long)ldq, (long long)ldk, (long long)ldv);
-  // a launch holds 2^32 threads of 256 a block, the batch's heads filled up to 8
-  if ((B + 7) * HQ * ((T + 63) / 64) >= (int64_t{1} << 24)) return fail(DSA_EINVAL, "window_attention: (B+7)*HQ*ceil(T/64) must be < 2^24");
+  // a launch holds 2^32 threads of 256 a block (by division: the product of the largest passes 64 bits)
+  const int64_t blocks = HQ * ((T + 63) / 64);
+  if (blocks > 0 && B > ((int64_t{1} << 24) - 1) / blocks) return fail(DSA_EINVAL, "window_attention: B*HQ*ceil(T/64) must be < 2^24");
   if (B * T == 0) return DSA_OK;
   if (!Q || !K || !V || !out) return fail(DSA_EINVAL, "window_attention: null pointer");
   if (!aligned16(Q) || !aligned16(K) || !aligned16(V) || !aligned16(out) || !aligned4(count))

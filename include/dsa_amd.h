@@ -572,8 +572,8 @@ int dsa_kv4_make_room(const dsa_kv4_cache* cache, const int32_t* count, int64_t 
  *   T of them), e.g. the columns of one projection's output.
  * No reference counterpart: its attention sees what the indexer selects.
  * Constraints: D in {32, 64, 128, 256}; HQ a multiple of HKV, at most 1024;
- *   window >= 1, sinks >= 0; T < 2^31 - 256; strides below 2^24 elements, in bytes
- *   multiples of 16; pointers 16-byte aligned, count 4; (B+7)*HQ*ceil(T/64) < 2^24.
+ *   window >= 1, sinks >= 0; T < 2^31 - 256; strides up to 2^24 elements, in bytes
+ *   multiples of 16; pointers 16-byte aligned, count 4; B*HQ*ceil(T/64) < 2^24.
  */
 int dsa_window_attention(const void* Q, const void* K, const void* V, int dtype, const int32_t* count,
                          int64_t B, int64_t T, int HQ, int HKV, int D, int64_t ldq, int64_t ldk,

@@ -139,6 +139,7 @@ WINDOW = (FAKE, FAKE, FAKE, L.DSA_BF16, None, 2, 64, 8, 4, 64, 512, 256, 256, 16
     (dict(_13=0), "window"), (dict(_13=-5), "window"), (dict(_14=-1), "sinks"), (dict(_15=float("inf")), "scale"),
     (dict(_0=FAKE + 8), "aligned"), (dict(_1=FAKE + 2), "aligned"), (dict(_2=FAKE + 8), "aligned"), (dict(_16=FAKE + 4), "aligned"),
     (dict(_5=1 << 30), "2^24"), (dict(_6=1 << 30), "2^24"),
+    (dict(_5=1 << 21), "2^24"), (dict(_5=1 << 30, _6=1 << 30, _7=1024, _8=1024, _10=1 << 17, _11=1 << 17, _12=1 << 17), "2^24"),  # 2^21 * 8; 2^64
 ])
 def test_window_refusals(changes, needle):
     rc = L.lib().dsa_window_attention(*put(WINDOW, **changes))
