@@ -361,20 +361,13 @@ def _plain_window(s):
 
 
 # --- the framework's calls -----------------------------------------------------------------------
-_module = None
-
-
 def _framework():
-    """The framework's module, imported once, as a program does."""
-    global _module
-    if _module is None:
-        pkg = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "dsa-cpu-topk_amd")
-        if pkg not in sys.path:
-            sys.path.insert(0, pkg)
-        import dsa_paged
+    pkg = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "dsa-cpu-topk_amd")
+    if pkg not in sys.path:
+        sys.path.insert(0, pkg)
+    import dsa_paged
 
-        _module = dsa_paged
-    return _module
+    return dsa_paged
 
 
 def _held(s):
