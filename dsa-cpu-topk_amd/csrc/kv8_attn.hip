@@ -246,8 +246,8 @@ __global__ __launch_bounds__(kNT, DK <= 128 || (SHARED && Tag::kBytes == 2) ? 2 
   const int32_t* const pages = a.c.pages + b * a.c.max_pages;
   auto block_of = [&](int32_t v) { return v < nsink ? v : near + v - nsink; };
   auto page_of = [&](int32_t v) { return pages[block_of(max(0, min(v, total - 1))) >> a.c.page_shift]; };  // of a block past the last: any
-  // A block's place in the pool; where its page is none, it holds nothing and the
-  // pool's first block stands in.
+  // A block's place in the pool; where its page is none, it holds nothing: the pool's first
+  // block stands in for the loads, and what it has there (its scale too) goes nowhere.
   auto place = [&](int32_t v, int32_t page, bool& held) __attribute__((always_inline)) {
     page = __builtin_amdgcn_readfirstlane(page);
     held = page >= 0 && page < a.c.NP;
@@ -282,7 +282,7 @@ __global__ __launch_bounds__(kNT, DK <= 128 || (SHARED && Tag::kBytes == 2) ? 2 
   };
   u32x4 p[RT][NP][2];
   uint32_t ok[RT];  // bit 4j + i: slot s0 + 16j + 4g + i is seen
-  auto weights = [&](uint32_t sc, int32_t s0, bool held, bool inner) __attribute__((always_inline)) {
+  auto weights = [&](uint32_t sc, int32_t s0, bool inner) __attribute__((always_inline)) {
     const float ks = __uint_as_float((sc & 255u) << 23);
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
@@ -293,7 +293,7 @@ __global__ __launch_bounds__(kNT, DK <= 128 || (SHARED && Tag::kBytes == 2) ? 2 
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
           const int32_t s = s0 + (e >> 2) * 16 + 4 * g + (e & 3);
-          if (held && s < mine[r].end && (s >= mine[r].low || s < sinks)) ok[r] |= 1u << e;
+          if (s < mine[r].end && (s >= mine[r].low || s < sinks)) ok[r] |= 1u << e;
           st[r][e >> 2][e & 3] = ok[r] >> e & 1u ? st[r][e >> 2][e & 3] : -INFINITY;
         }
       }
@@ -403,7 +403,7 @@ __global__ __launch_bounds__(kNT, DK <= 128 || (SHARED && Tag::kBytes == 2) ? 2 
       }
     }
   };
-  auto is_inner = [&](int32_t s0, bool held) { return held && s0 + kBlk <= lo.end && (s0 >= hi.low || s0 + kBlk <= sinks); };
+  auto is_inner = [&](int32_t s0) { return s0 + kBlk <= lo.end && (s0 >= hi.low || s0 + kBlk <= sinks); };
 
   if constexpr (!SHARED) {
     u32x4 kr[4][NJ > 0 ? NJ : 1], vr[NDT];
@@ -450,9 +450,10 @@ __global__ __launch_bounds__(kNT, DK <= 128 || (SHARED && Tag::kBytes == 2) ? 2 
       }
       page1 = page2;
       __builtin_amdgcn_sched_barrier(0);
+      if (!held_now) continue;
       const int32_t s0 = block_of(v) * kBlk;
-      const bool inner = is_inner(s0, held_now);
-      weights(sc_now, s0, held_now, inner);
+      const bool inner = is_inner(s0);
+      weights(sc_now, s0, inner);
       sums(sc_now, inner, [&](int d) { return vr[d]; });
     }
   } else {
@@ -511,13 +512,13 @@ __global__ __launch_bounds__(kNT, DK <= 128 || (SHARED && Tag::kBytes == 2) ? 2 
       page1 = page2;
       __builtin_amdgcn_sched_barrier(0);
       const int32_t s0 = block_of(v) * kBlk;
-      if (any_rows && s0 < hi.end && (s0 + kBlk > lo.low || s0 < sinks)) {
-        const bool inner = is_inner(s0, held_now);
+      if (held_now && any_rows && s0 < hi.end && (s0 + kBlk > lo.low || s0 < sinks)) {
+        const bool inner = is_inner(s0);
         const DSA_LDS uint8_t* const kp = kc + col * DK;
         const DSA_LDS uint8_t* const vp = vc + col * kBlk + 16 * chunk_at<4>(col, g);
         logits([&](int j, int i) { return *reinterpret_cast<const DSA_LDS u32x4*>(kp + 16 * j * DK + 16 * chunk_at<NCK>(col, 4 * i + g)); },
                [&](int j) { return *reinterpret_cast<const DSA_LDS u32x2*>(kp + 16 * j * DK + 16 * chunk_at<NCK>(col, 4 * NJ + (g >> 1)) + 8 * (g & 1)); });
-        weights(sc_now, s0, held_now, inner);
+        weights(sc_now, s0, inner);
         sums(sc_now, inner, [&](int d) { return *reinterpret_cast<const DSA_LDS u32x4*>(vp + 16 * d * kBlk); });
       }
       wait_dma_keep<0>();
