@@ -233,14 +233,17 @@ __global__ __launch_bounds__(kNT, DK <= 128 || (SHARED && Tag::kBytes == 2) ? 2 
 
   float m[RT], l[RT];
   f32x4 o[RT][NDT];
+  // V's scale byte in units of which a row's o is held, of a block in which the row weighs a
+  // slot; 0: o is nothing yet.
+  uint32_t unit[RT];
 #pragma unroll
   for (int r = 0; r < RT; ++r) {
     m[r] = -INFINITY;
     l[r] = 0.0f;
+    unit[r] = 0;
 #pragma unroll
     for (int d = 0; d < NDT; ++d) o[r][d] = f32x4{0, 0, 0, 0};
   }
-  uint32_t unit = 0;  // V's scale byte in units of which o is held; 0: o is nothing yet
 
   const int32_t step = a.splits * WT;
   const int32_t* const pages = a.c.pages + b * a.c.max_pages;
@@ -306,6 +309,8 @@ __global__ __launch_bounds__(kNT, DK <= 128 || (SHARED && Tag::kBytes == 2) ? 2 
         const float fall = m[r] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[r] - next);
         m[r] = next;
         l[r] *= fall;
+        // what has fallen to nothing has no unit either
+        if (max_xor32_u32(max_xor16_u32(__float_as_uint(l[r]))) == 0) unit[r] = 0;
 #pragma unroll
         for (int d = 0; d < NDT; ++d) o[r][d] *= fall;
       }
@@ -344,9 +349,30 @@ __global__ __launch_bounds__(kNT, DK <= 128 || (SHARED && Tag::kBytes == 2) ? 2 
       }
       fix = ballot(any != 0) != 0;
     }
+    // A row in which none of the block's slots weighs anything (it sees none, or its p are all 0)
+    // adds zeros whatever their unit, and keeps its own.
     const uint32_t vb = sc >> 8;
-    if (unit == 0) unit = vb;
-    if (vb == unit && !fix) {
+    uint32_t with[RT];
+    bool apart = false;
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+      with[r] = vb;
+      apart |= unit[r] != vb;
+    }
+    if (ballot(apart)) {
+      apart = false;
+#pragma unroll
+      for (int r = 0; r < RT; ++r) {
+        uint32_t any = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) any |= p[r][0][0][e] | p[r][0][1][e];
+        const bool weighs = max_xor32_u32(max_xor16_u32(any)) != 0;
+        if (weighs && unit[r] == 0) unit[r] = vb;
+        if (!weighs) with[r] = unit[r];
+        apart |= unit[r] != with[r];
+      }
+    }
+    if (!ballot(apart) && !fix) {
 #pragma unroll
       for (int d = 0; d < NDT; ++d) {
         const u32x4 w = read(d), x = widen8(w[0], w[1]), y = widen8(w[2], w[3]);
@@ -361,9 +387,14 @@ __global__ __launch_bounds__(kNT, DK <= 128 || (SHARED && Tag::kBytes == 2) ? 2 
       return;
     }
     // the larger scale becomes the unit: what is beyond fp32 below it weighs nothing
-    const float down = vb > unit ? ldexpf(1.0f, static_cast<int>(unit) - static_cast<int>(vb)) : 1.0f;
-    const float add = vb > unit ? 1.0f : ldexpf(1.0f, static_cast<int>(vb) - static_cast<int>(unit));
-    unit = max(unit, vb);
+    float down[RT], add[RT];
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+      const int up = static_cast<int>(with[r]) - static_cast<int>(unit[r]);
+      down[r] = ldexpf(1.0f, -max(up, 0));
+      add[r] = ldexpf(1.0f, min(up, 0));
+      unit[r] = max(unit[r], with[r]);
+    }
 #pragma unroll
     for (int d = 0; d < NDT; ++d) {
       u32x4 w = read(d), is;  // is: e4m3's 1 where a NaN is, 0 elsewhere
@@ -385,7 +416,7 @@ __global__ __launch_bounds__(kNT, DK <= 128 || (SHARED && Tag::kBytes == 2) ? 2 
           acc = mfma(y, p[r][k][1], acc);
         }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[r][d][e] = fmaf(acc[e], add, o[r][d][e] * down);
+        for (int e = 0; e < 4; ++e) o[r][d][e] = fmaf(acc[e], add[r], o[r][d][e] * down[r]);
         if (fix) {
           u32x4 see[2];  // 1 where seen, as p lies
 #pragma unroll
@@ -531,7 +562,6 @@ __global__ __launch_bounds__(kNT, DK <= 128 || (SHARED && Tag::kBytes == 2) ? 2 
     }
   }
 
-  const float us = __uint_as_float(unit << 23);
 #pragma unroll
   for (int r = 0; r < RT; ++r) {
     l[r] = sum_xor32(sum_xor16(l[r]));
@@ -541,7 +571,7 @@ __global__ __launch_bounds__(kNT, DK <= 128 || (SHARED && Tag::kBytes == 2) ? 2 
       l[r] = 0.0f;
     }
 #pragma unroll
-    for (int d = 0; d < NDT; ++d) o[r][d] = token[r] ? o[r][d] * us : f32x4{0, 0, 0, 0};
+    for (int d = 0; d < NDT; ++d) o[r][d] = token[r] ? o[r][d] * __uint_as_float(unit[r] << 23) : f32x4{0, 0, 0, 0};
   }
   auto finish = [&](int row, int d, f32x4 x, float top, float all) __attribute__((always_inline)) {
     const int64_t hr = (b * a.Tq + row / a.G) * a.HQ + h * a.G + row % a.G;

@@ -3,11 +3,14 @@ formats: scales far apart or of pages of nobody, values near the largest, shares
 prompts that fill the card.  Against 64 bits, under paged_oracle's bounds."""
 from __future__ import annotations
 
+import math
+
 import pytest
 import torch
 
 import dsa_paged as P
-from test_gpu_paged import BF16, F32, check_attention, filled, gen, randn
+import paged_oracle as O
+from test_gpu_paged import BF16, F32, check_attention, filled, gen, randn, state
 
 pytestmark = pytest.mark.gpu
 
@@ -50,3 +53,39 @@ def test_pages_of_nobody_have_no_scale(dev, dtype, shape):
     out, _ = check_attention(dev, cache, Q, dtype, None, 0)
     assert bool(out.isfinite().all())
     check_attention(dev, cache, Q, dtype, 150, 3)
+
+
+def check_rows(dev, cache, Q, dtype, window):
+    """check_attention, with a row's own largest |V|: among the slots that weigh more than 2^-60 in it
+    (the tests' other ones weigh 2^-1000 and less, 0 in any p)."""
+    B, Tq, HQ, D = Q.shape
+    out = P.kv8_attention(cache, Q.to(dev), window=window).double().cpu()
+    K, V = state(cache).values()
+    G = HQ // cache.HKV
+    for b, n in enumerate(cache.length.tolist()):
+        ok = O.sees(n, n - Tq + torch.arange(Tq), torch.arange(cache.S), window, 0)
+        ref, mass, big = O.attention(Q[b], K[b], V[b], ok, D ** -0.5)
+        vmax = torch.zeros(Tq, HQ, 1, dtype=torch.float64)
+        for h in range(HQ):
+            p = torch.softmax((Q[b, :, h].double() @ K[b, :, h // G].nan_to_num().T * D ** -0.5).masked_fill(~ok, -math.inf), -1)
+            vmax[:, h, 0] = torch.where(p > 2.0 ** -60, V[b, :, h // G].nan_to_num().abs().amax(-1), 0.0).amax(-1)
+        lim = O.bound(dtype, n, D, mass, big, ref, False, vmax)
+        err = (out[b] - ref).abs()
+        assert bool((err <= lim).all()), (b, float((err / lim).max()))
+
+
+@pytest.mark.parametrize("shape, window", [((2, [400, 400], 4, 1, 64, 2), 336), ((8, [200] * 8, 64, 8, 128, 32), 120)])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_scales_that_weigh_nothing(dev, dtype, shape, window):
+    """A block of very large values that some rows of a tile do not see, or in which no slot
+    weighs anything for them, takes nothing from their small ones."""
+    B, lengths, HQ, HKV, D, Tq = shape
+    cache = filled(dev, B, 448, HKV, D, D, lengths, seed=D)
+    first = cache.pages[:, 0].long()
+    cache.scales[..., 1] -= 60
+    cache.scales[first, :, 0, 1] += 160
+    check_rows(dev, cache, randn(gen(Tq), B, Tq, HQ, D, dtype=dtype), dtype, window)
+    # the block's keys all against the queries: logits of -14336 and less
+    cache.codes[first, :, 0, :64 * D], cache.scales[first, :, 0, 0] = 0xFE, 127
+    Q = 4.0 + 0.1 * randn(gen(Tq), B, Tq, HQ, D)
+    check_rows(dev, cache, Q.to(dtype), dtype, None)
