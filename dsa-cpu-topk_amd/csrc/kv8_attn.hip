@@ -50,7 +50,7 @@ struct AttnArgs {
   int64_t sinks;
   float scale_log2;
   void* out;
-  float* part;  // [B*Tq*HQ][splits][DV]
+  float* part;  // [B*Tq*HQ][splits][DV], each split's own result
   float2* ml;   // [B*Tq*HQ][splits]: maximum (log2) and sum
 };
 
@@ -570,16 +570,19 @@ __global__ __launch_bounds__(kNT, DK <= 128 || (SHARED && Tag::kBytes == 2) ? 2 
       m[r] = -INFINITY;
       l[r] = 0.0f;
     }
+    // Divided by the sum of weights before V's unit comes in: the mean of values that fp32 holds
+    // is one too, where p times them, 2^10 and more, may not be.  (v_rcp_f32 is within 2^-23.)
+    const float inv = l[r] == 0.0f ? 0.0f : __builtin_amdgcn_rcpf(l[r]), us = __uint_as_float(unit[r] << 23);
 #pragma unroll
-    for (int d = 0; d < NDT; ++d) o[r][d] = token[r] ? o[r][d] * __uint_as_float(unit[r] << 23) : f32x4{0, 0, 0, 0};
+    for (int d = 0; d < NDT; ++d) o[r][d] = token[r] ? o[r][d] * inv * us : f32x4{0, 0, 0, 0};
   }
   auto finish = [&](int row, int d, f32x4 x, float top, float all) __attribute__((always_inline)) {
     const int64_t hr = (b * a.Tq + row / a.G) * a.HQ + h * a.G + row % a.G;
     if (a.splits > 1) {
       *reinterpret_cast<f32x4*>(a.part + (hr * a.splits + split) * DV + d) = x;
       if (d == 0) a.ml[hr * a.splits + split] = make_float2(top, all);
-    } else {  // 0 / 0 where nothing is seen
-      store4<Tag>(static_cast<raw*>(a.out) + hr * DV + d, x * (1.0f / all));
+    } else {
+      store4<Tag>(static_cast<raw*>(a.out) + hr * DV + d, all == 0.0f ? x * __builtin_nanf("") : x);  // nothing is seen
     }
   };
   if constexpr (SHARED) {
@@ -607,14 +610,13 @@ __global__ __launch_bounds__(kNT, DK <= 128 || (SHARED && Tag::kBytes == 2) ? 2 
 #pragma unroll
       for (int w = 1; w < WT; ++w) top = fmaxf(top, sum_m[w][r]);
       const float ref = top == -INFINITY ? 0.0f : top;
-      float all = 0.0f;
+      float share[WT], all = 0.0f;
       f32x4 x{0, 0, 0, 0};
 #pragma unroll
-      for (int w = 0; w < WT; ++w) {
-        const float f = __builtin_amdgcn_exp2f(sum_m[w][r] - ref);
-        all += f * sum_l[w][r];
-        x += *reinterpret_cast<const f32x4*>(sum_o + (w * kTile + r) * DV + d) * f;
-      }
+      for (int w = 0; w < WT; ++w) all += share[w] = __builtin_amdgcn_exp2f(sum_m[w][r] - ref) * sum_l[w][r];
+      const float inv = all == 0.0f ? 0.0f : 1.0f / all;
+#pragma unroll
+      for (int w = 0; w < WT; ++w) x += *reinterpret_cast<const f32x4*>(sum_o + (w * kTile + r) * DV + d) * (share[w] * inv);
       finish(block_row + r, d, x, top, all);
     }
   }
@@ -648,11 +650,15 @@ __global__ __launch_bounds__(kNT) void join_few_kernel(const float* __restrict__
 #pragma unroll
   for (int s = 0; s < kFewSplits; ++s) {
     if (s >= splits) break;
-    const float f = __builtin_amdgcn_exp2f(x[s].x - ref);
-    all += f * x[s].y;
-    z += f32x4{y[s].x, y[s].y, y[s].z, y[s].w} * f;
+    all += x[s].y *= __builtin_amdgcn_exp2f(x[s].x - ref);
   }
-  store4<Tag>(out + row * DV + d, z * (1.0f / all));
+  const float inv = 1.0f / all;  // nothing is seen: 0 * Inf
+#pragma unroll
+  for (int s = 0; s < kFewSplits; ++s) {
+    if (s >= splits) break;
+    z += f32x4{y[s].x, y[s].y, y[s].z, y[s].w} * (x[s].y * inv);
+  }
+  store4<Tag>(out + row * DV + d, z);
 }
 
 // A block joins one row's splits: 20 of rows of 128, 31 MB in all, in 8 us.  (Threads that
@@ -674,19 +680,19 @@ __global__ __launch_bounds__(kNT) void join_kernel(const float* __restrict__ par
   float all = 0.0f;
   for (int s = threadIdx.x; s < splits; s += kNT) {
     const float2 x = mine[s];
-    const float f = __builtin_amdgcn_exp2f(x.x - ref);
+    const float f = __builtin_amdgcn_exp2f(x.x - ref) * x.y;
     factor[s] = f;
-    all += f * x.y;
+    all += f;
   }
   all = wave_sum(all);
   if ((threadIdx.x & 63) == 0) both[threadIdx.x >> 6].y = all;
   __syncthreads();
   all = both[0].y + both[1].y + both[2].y + both[3].y;
   if (threadIdx.x >= DV) return;
+  const float inv = 1.0f / all;  // nothing is seen: 0 * Inf
   float x = 0.0f;
 #pragma unroll 8
-  for (int s = 0; s < splits; ++s) x += factor[s] * part[(row * splits + s) * DV + threadIdx.x];
-  x /= all;
+  for (int s = 0; s < splits; ++s) x += factor[s] * inv * part[(row * splits + s) * DV + threadIdx.x];
   if constexpr (Tag::kBytes == 4) out[row * DV + threadIdx.x] = x;
   else if constexpr (__is_same(Tag, BF16)) out[row * DV + threadIdx.x] = __builtin_bit_cast(uint16_t, static_cast<__bf16>(x));
   else out[row * DV + threadIdx.x] = __builtin_bit_cast(uint16_t, static_cast<_Float16>(x));

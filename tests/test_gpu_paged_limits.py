@@ -10,7 +10,7 @@ import torch
 
 import dsa_paged as P
 import paged_oracle as O
-from test_gpu_paged import BF16, F32, check_attention, filled, gen, randn, state
+from test_gpu_paged import BF16, F32, check_attention, filled, gen, ints, randn, state
 
 pytestmark = pytest.mark.gpu
 
@@ -36,6 +36,7 @@ FEW = (2, [400, 390], 4, 1, 64, 4)      # own: B, lengths, HQ, HKV, D, Tq
 SPLIT = (1, [9000], 4, 1, 64, 1)        # own, joined by a second launch
 MANY = (8, [250 - b for b in range(8)], 64, 8, 128, 32)   # shared
 PIECE = (1, [3100], 4, 1, 128, 1024)    # shared, joined; 16-bit types 32 rows a wave
+LONG = (1, [6200], 4, 1, 64, 1024)      # own, 32 rows a wave, few splits joined by threads
 
 
 @pytest.mark.parametrize("shape", [FEW, SPLIT, MANY, PIECE])
@@ -89,3 +90,20 @@ def test_scales_that_weigh_nothing(dev, dtype, shape, window):
     cache.codes[first, :, 0, :64 * D], cache.scales[first, :, 0, 0] = 0xFE, 127
     Q = 4.0 + 0.1 * randn(gen(Tq), B, Tq, HQ, D)
     check_rows(dev, cache, Q.to(dtype), dtype, None)
+
+
+@pytest.mark.parametrize("shape", [FEW, SPLIT, MANY, PIECE, LONG])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_values_near_the_largest(dev, dtype, shape):
+    """V up to 1.75 * 2^127, the largest that reads back as a number: a mean of them is one."""
+    B, lengths, HQ, HKV, D, Tq = shape
+    g = gen(D + Tq)
+    S = -(-max(lengths) // 64) * 64
+    cache = P.KV8Cache.empty(B, S, HKV, D, D, device=dev)
+    K, V = randn(g, B, max(lengths), HKV, D), randn(g, B, max(lengths), HKV, D).clamp(-3.5, 3.5) * 2.0 ** 126
+    V[:, :, :, 3] = 1.75 * 2.0 ** 127
+    V[:, 5:, 0, 4] = -1.75 * 2.0 ** 127
+    P.kv8_append(cache, K.to(dev), V.to(dev), count=ints(dev, lengths))
+    Q = randn(gen(Tq), B, Tq, HQ, D, dtype=dtype)
+    out, _ = check_attention(dev, cache, Q, dtype, None, 0)
+    assert bool(out.isfinite().all()) and bool((out[..., 3].double() / (1.75 * 2.0 ** 127) - 1).abs().max() < 2.0 ** -8)
