@@ -17,6 +17,7 @@
 #include "dsa_launch.h"
 #include "kv8.h"
 #include "tile_common.h"
+#include "window_walk.h"
 
 namespace dsa {
 namespace {
@@ -31,25 +32,9 @@ struct Win {
   uint32_t flip;     // Q's sign bits, where the scale is negative
 };
 
-// What of the tiles of KT keys a block of TQ queries from t0 on walks.
-struct Walk {
-  int n;            // tokens of the sequence
-  int first, near;  // tiles of the first tokens: 0 .. first - 1, then near, near + 1, ...
-  int total;
-  __device__ __forceinline__ int tile(int v) const { return v < first ? v : near + v - first; }
-};
 template <int TQ, int KT>
-__device__ __forceinline__ Walk walk_of(const Win& a, int64_t b, int t0) {
-  Walk w;
-  w.n = a.count ? max(0, min(a.count[b], a.T)) : a.T;
-  if (t0 >= w.n) {
-    w.first = w.near = w.total = 0;
-    return w;
-  }
-  w.near = max(0, t0 - a.window + 1) / KT;
-  w.first = min((a.sinks + KT - 1) / KT, w.near);
-  w.total = w.first + (min(t0 + TQ, w.n) - 1) / KT - w.near + 1;
-  return w;
+__device__ __forceinline__ Walk walk_in(const Win& a, int64_t b, int t0) {
+  return walk_of<TQ, KT>(a.count ? max(0, min(a.count[b], a.T)) : a.T, a.window, a.sinks, t0);
 }
 
 // Block -> (tile of queries, batch, head), the latest tiles, which see most, first.  The
@@ -137,7 +122,7 @@ __global__ __launch_bounds__(kNT, D >= 128 ? 2 : QT == 2 ? 3 : 4) void window_ke
   int t0, h, hk;
   int64_t b;
   place<TQ>(a, t0, b, h, hk);
-  const Walk walk = walk_of<TQ, KT>(a, b, t0);
+  const Walk walk = walk_in<TQ, KT>(a, b, t0);
   const int T = a.T, n = walk.n, window = a.window, sinks = a.sinks;
   const int tw = t0 + 16 * QT * wave, wave_last = min(tw + 16 * QT - 1, n - 1);
   raw* const out = static_cast<raw*>(a.out) + (b * T * a.HQ + h) * D;
@@ -356,9 +341,7 @@ __global__ __launch_bounds__(kNT, D >= 128 ? 2 : QT == 2 ? 3 : 4) void window_ke
     };
     // Tiles that all queries of the block see whole are a loop of their own (in one with the
     // others, the compiler copies O, 64 registers, once a tile).
-    const int last = min(t0 + TQ, n) - 1, whole = last >= window ? (last - window) / KT + 1 : 0;
-    const int w0 = (walk.first + max(0, whole - walk.near) + 1) & ~1;
-    const int w1 = CAREFUL ? w0 : w0 + max(0, (walk.first + t0 / KT - walk.near - w0) & ~1);
+    const int w0 = walk.whole0, w1 = CAREFUL ? w0 : walk.whole1;
     int v = 0;
     auto edges = [&](int end) __attribute__((always_inline)) {
       for (; v < end; v += 2) {
@@ -455,7 +438,7 @@ __global__ __launch_bounds__(kNT * TEAMS, TEAMS == 2 || D * QT >= 256 ? 1 : 2) v
   int t0, h, hk;
   int64_t b;
   place<TQ>(a, t0, b, h, hk);
-  const Walk walk = walk_of<TQ, KT>(a, b, t0);
+  const Walk walk = walk_in<TQ, KT>(a, b, t0);
   const int T = a.T, n = walk.n, window = a.window, sinks = a.sinks;
   const int tw = t0 + 16 * QT * wave, wave_last = min(tw + 16 * QT - 1, n - 1);
   const float* const kb = static_cast<const float*>(a.K) + b * T * a.ldk + static_cast<int64_t>(hk) * D;
