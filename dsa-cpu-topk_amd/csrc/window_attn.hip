@@ -63,13 +63,20 @@ __device__ __forceinline__ float mul(float x, float y) {  // rounded by itself
   return x * y;
 }
 // 2^(x scale - ref).  An fma keeps x scale whole, where ref, the maximum's product, was
-// rounded: at logits of 2^28 and more all p of a row are then beyond or below a 16-bit
+// rounded: at logits of 2^28 (f16: 2^25) and more all p of a row may be beyond or below a 16-bit
 // type, which leaves no finite result, and the careful pass rounds each as ref was.
 template <bool CAREFUL>
 __device__ __forceinline__ float weight(float x, float scale, float ref) {
   return __builtin_amdgcn_exp2f(CAREFUL ? mul(x, scale) - ref : fmaf(x, scale, -ref));
 }
 __device__ __forceinline__ bool finite_f32(float x) { return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u; }
+// p is held as 2^(kUp + logit - maximum), the maximum moves when a tile's passes it by kSlack.
+// bf16 has fp32's range; in f16 what is small beside the largest then stays normal down to 2^-24
+// of it, and p below 2^15.
+template <typename Tag>
+constexpr float kUp = __is_same(Tag, F16) ? 10.0f : 0.0f;
+template <typename Tag>
+constexpr float kSlack = __is_same(Tag, F16) ? 5.0f : 8.0f;
 // Bit 15 of each half that is Inf or NaN.
 template <typename Tag>
 __device__ __forceinline__ uint32_t odd_halves(uint32_t w) {
@@ -238,13 +245,12 @@ __global__ __launch_bounds__(kNT, D >= 128 ? 2 : QT == 2 ? 3 : 4) void window_ke
 #pragma unroll
         for (int e = 0; e < E; ++e) mx = fmaxf(mx, st[e >> 2][qt][e & 3]);
         mx = mul(max_xor32(max_xor16(mx)), a.scale_log2);
-        // the maximum moves when a tile's passes it by 2^8: p then stays far below overflow
-        const bool up = mx > m[qt] + 8.f;
+        const bool up = mx > m[qt] + kSlack<Tag>;
         const float m_new = up ? mx : m[qt];
         alpha[qt] = up ? __builtin_amdgcn_exp2f(m[qt] - m_new) : 1.f;
         grow |= up && m[qt] != -INFINITY;
         m[qt] = m_new;
-        const float ref = m_new == -INFINITY ? 0.f : m_new;
+        const float ref = m_new == -INFINITY ? 0.f : m_new - kUp<Tag>;
 #pragma unroll
         for (int e = 0; e < E; ++e) st[e >> 2][qt][e & 3] = weight<CAREFUL>(st[e >> 2][qt][e & 3], a.scale_log2, ref);
 #pragma unroll

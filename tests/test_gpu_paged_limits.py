@@ -10,7 +10,7 @@ import torch
 
 import dsa_paged as P
 import paged_oracle as O
-from test_gpu_paged import BF16, F32, check_attention, filled, gen, ints, randn, state
+from test_gpu_paged import BF16, F16, F32, check_attention, filled, gen, ints, randn, state
 
 pytestmark = pytest.mark.gpu
 
@@ -107,3 +107,26 @@ def test_values_near_the_largest(dev, dtype, shape):
     Q = randn(gen(Tq), B, Tq, HQ, D, dtype=dtype)
     out, _ = check_attention(dev, cache, Q, dtype, None, 0)
     assert bool(out.isfinite().all()) and bool((out[..., 3].double() / (1.75 * 2.0 ** 127) - 1).abs().max() < 2.0 ** -8)
+
+
+@pytest.mark.parametrize("B, HQ, D", [(1, 2, 32), (1, 2, 64), (1, 2, 128), (1, 2, 256), (16, 16, 64), (16, 16, 128)])
+def test_small_shares_of_fp16_prompts(dev, B, HQ, D):
+    """A first token 15 nats above all others, with a value of 0: what the others add, 2^-21.6 of
+    their values each, keeps f16's precision.  Their logits are alike, so roundings of p add up.
+
+    p is held as 2^10 and more times its share of the largest, so a share from 2^-24 on is a normal
+    f16 and smaller ones are off by 2^-25 of the 2^10: n 2^-35 vmax in place of n 2^-24 vmax."""
+    T = 500
+    g = gen(D)
+    Q = torch.ones(1, T, HQ, D)
+    K = torch.zeros(1, T, 1, D)
+    K[:, 0] = 15.0 / math.sqrt(D)
+    V = 1.0 + 0.2 * randn(g, 1, T, 1, D)
+    V[:, 0] = 0.0
+    Q, K, V = Q.half(), K.half(), V.half()
+    out = P.window_attention(*(x.to(dev).expand(B, -1, -1, -1) for x in (Q, K, V)))
+    ref, mass, big = O.attention(Q[0], K[0], V[0], O.sees(T, torch.arange(T), torch.arange(T), None, 0), D ** -0.5)
+    vmax = float(V.double().abs().max())
+    lim = O.bound(F16, T, D, mass, big, ref, True, vmax * 2.0 ** -11)
+    err = (out.double().cpu() - ref).abs() / lim
+    assert float(err.max()) <= 1.0, float(err.max())
