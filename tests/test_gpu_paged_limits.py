@@ -10,7 +10,7 @@ import torch
 
 import dsa_paged as P
 import paged_oracle as O
-from test_gpu_paged import BF16, F16, F32, check_attention, filled, gen, ints, randn, state
+from test_gpu_paged import BF16, F16, F32, check_attention, check_window, filled, gen, ints, randn, state
 
 pytestmark = pytest.mark.gpu
 
@@ -130,3 +130,40 @@ def test_small_shares_of_fp16_prompts(dev, B, HQ, D):
     lim = O.bound(F16, T, D, mass, big, ref, True, vmax * 2.0 ** -11)
     err = (out.double().cpu() - ref).abs() / lim
     assert float(err.max()) <= 1.0, float(err.max())
+
+
+# Batches whose blocks fill the card, so that a block takes 128 queries (1024 blocks of 128 and more in 16
+# bits, 512 in fp32), at windows that leave tiles which all queries of a block see whole.
+@pytest.mark.parametrize("B, T, HQ, HKV, D, window, sinks, count, dtype", [
+    (13, 520, 16, 2, 64, 400, 3, None, F16),
+    (13, 520, 16, 2, 128, 391, 70, None, BF16),
+    (13, 520, 16, 1, 128, None, 0, [520, 519, 1, 0, 64, 65, 128, 129, 200, 320, 400, 512, 513], F16),
+    (13, 520, 16, 1, 64, None, 0, [513, 64, 520, 0, 449, 448, 447, 2, 257, 256, 255, 100, 384], BF16),
+    (13, 520, 16, 1, 32, 330, 130, None, BF16),
+    (13, 520, 8, 2, 64, 400, 3, None, F32),
+    (13, 520, 8, 1, 32, None, 0, [520, 519, 1, 0, 64, 65, 128, 129, 200, 320, 400, 512, 513], F32),
+])
+def test_window_of_128_queries_a_block(dev, B, T, HQ, HKV, D, window, sinks, count, dtype):
+    g = gen(B + T + D)
+    Q, K, V = (randn(g, B, T, h, D, dtype=dtype) for h in (HQ, HKV, HKV))
+    if count is not None:
+        for b in range(B):
+            Q[b, count[b]:], K[b, count[b]:], V[b, count[b]:] = math.nan, math.inf, math.nan
+    check_window(dev, Q, K, V, dtype, window, sinks, count)
+
+
+@pytest.mark.parametrize("D, dtype", [(32, BF16), (64, BF16), (64, F16), (128, BF16), (128, F16), (32, F32), (64, F32)])
+def test_window_of_128_queries_keeps_what_is_not_seen_out(dev, D, dtype):
+    """NaN and Inf in keys and values where a block takes 128 queries."""
+    g = gen(D + 1)
+    B, T, HQ, window = 13, 520, 8 if dtype == F32 else 16, 300
+    Q, K, V = (randn(g, B, T, h, D, dtype=dtype) for h in (HQ, 2, 2))
+    for b in range(0, B, 2):
+        V[b, 30 + b, 0, 3], V[b, 100, 0, 7], V[b, 101, 0, 7], K[b, 170, 1, 5] = math.nan, math.inf, -math.inf, math.nan
+        V[b, 1, 1, 2] = -math.inf
+    out, _ = check_window(dev, Q, K, V, dtype, window, 2)
+    half = HQ // 2
+    assert bool(out[1::2].isfinite().all()) and bool(out[0, 30:330, :half, 3].isnan().all())
+    assert bool(out[0, 100, :half, 7].isposinf().all()) and bool(out[0, 101:400, :half, 7].isnan().all()) and bool(out[0, 401:, :half].isfinite().all())
+    assert bool((out[0, 1:170, half:, 2] == -math.inf).all()) and bool(out[0, 170:470, half:].isnan().all())
+    assert bool((out[0, 470:, half:, 2] == -math.inf).all())
