@@ -64,7 +64,7 @@ def _span_args(window: int | None, sinks: int):
     n = int(sinks)
     assert window is None or W >= 1, f"window={window} must be >= 1 (None: all)"
     assert n >= 0, f"sinks={sinks} must be >= 0"
-    return W, n
+    return min(W, 1 << 62), min(n, 1 << 62)  # (ctypes keeps an integer's low 64 bits)
 
 
 def _out(out, shape, dtype, like):

@@ -167,3 +167,18 @@ def test_window_of_128_queries_keeps_what_is_not_seen_out(dev, D, dtype):
     assert bool(out[0, 100, :half, 7].isposinf().all()) and bool(out[0, 101:400, :half, 7].isnan().all()) and bool(out[0, 401:, :half].isfinite().all())
     assert bool((out[0, 1:170, half:, 2] == -math.inf).all()) and bool(out[0, 170:470, half:].isnan().all())
     assert bool((out[0, 470:, half:, 2] == -math.inf).all())
+
+
+def test_windows_past_64_bits(dev):
+    """A window or a number of first tokens that no 64-bit integer holds is all of them."""
+    g = gen(5)
+    Q, K, V = (randn(g, 1, 100, 2, 64, dtype=BF16).to(dev) for _ in range(3))
+    every = P.window_attention(Q, K, V)
+    for kw in (dict(window=2 ** 64 + 5), dict(window=2 ** 63), dict(window=3, sinks=2 ** 64), dict(window=3, sinks=2 ** 63 + 1)):
+        assert torch.equal(P.window_attention(Q, K, V, **kw), every), kw
+    cache = P.KV8Cache.empty(1, 128, 2, 64, 64, device=dev)
+    P.kv8_append(cache, K, V)
+    q = Q[:, -3:].contiguous()
+    every = P.kv8_attention(cache, q)
+    for kw in (dict(window=2 ** 64 + 5), dict(window=2 ** 63), dict(window=3, sinks=2 ** 64), dict(window=3, sinks=2 ** 63 + 1)):
+        assert torch.equal(P.kv8_attention(cache, q, **kw), every), kw
