@@ -91,7 +91,8 @@ def window_attention(Q: torch.Tensor, K: torch.Tensor, V: torch.Tensor, *, windo
     are.  window None: every earlier token.  count int32 [B]: how many of
     a sequence's T rows are tokens (a padded batch); the others get NaN.  scale: of the
     logits, default 1/sqrt(D).  What a token does not see does not reach its row, NaN
-    and Inf included."""
+    and Inf included.  (Prompts of the cache's other head sizes, 96 and 192, go over the pages,
+    by kv8_attention after their append.)"""
     if not (Q.is_cuda and K.is_cuda and V.is_cuda):
         L.require_gpu(Q, K, V)
     shape, kv = Q.shape, K.shape
@@ -255,14 +256,14 @@ def kv8_append(cache: KV8Cache, K: torch.Tensor, V: torch.Tensor, *, rope=None, 
     K [B,T,HKV,DK], V [B,T,HKV,DV] (one type of fp32, bf16 or fp16; mixed ones go as fp32),
     the columns of one projection's output as they are.  The tokens' positions, and slots, are
     start[b] + i, start int32 [B] (default: the cache's length, which then grows; 0 for new
-    prompts, less than the length to take drafted tokens back).  count int32 [B]: how many of
+    prompts, less than the length to take drafted tokens back; outside [0, S] the nearer end).  count int32 [B]: how many of
     the T are tokens (a padded batch; default all).  Tokens past the last slot or on no page
     are not stored but counted in cache.lost.
     rope: (cos, sin) fp32 [>= S, R/2] (rope_tables), R a multiple of 16 up to DK: the first R
     dimensions turn, as two halves, or with pairs neighbour by neighbour; None: nothing turns.
-    Q [B,T,HQ,DK]: rotated too; keys: K's rotated rows are returned as well, both in their
-    type, of all T rows, NaN at positions past the last slot.  Without rope they come back as
-    they are."""
+    Q [B,T,HQ,DK]: rotated too; keys: K's rotated rows are returned as well.  Both are of all T
+    rows, NaN at positions past the last slot, in the one type that K, V and Q have (fp32 where
+    their types differ).  Without rope they come back as they are."""
     kv = K.shape
     assert len(kv) == 4, "K [B,T,HKV,DK], V [B,T,HKV,DV]"
     B, T = kv[0], kv[1]

@@ -566,7 +566,10 @@ int dsa_kv4_make_room(const dsa_kv4_cache* cache, const int32_t* count, int64_t 
  * get NaN, as empty rows do everywhere here.  What a query does not see does not
  * reach its result, NaN and Inf included.
  *   out [B,T,HQ,D] of dtype: fp32 arithmetic throughout for fp32; 16-bit types round
- * p to their type for its product with V and for the sum it is divided by.
+ * p to their type for its product with V and for the sum it is divided by (f16 as 2^10 and
+ * more times its share of the largest, normal down to 2^-24 of that).  The sums are divided
+ * last: in fp32 and bf16 p goes up to 2^8, so that 2^8 n max|V| over the n tokens that a row
+ * sees must stay below fp32's range (f16's values always do).
  *   Q [B,T,HQ,D], K, V [B,T,HKV,D] of dtype (fp32, bf16, fp16), consecutive tokens
  *   ldq / ldk / ldv elements apart (at least HQ*D, HKV*D, HKV*D; a batch element spans
  *   T of them), e.g. the columns of one projection's output.
@@ -597,7 +600,8 @@ int dsa_window_attention(const void* Q, const void* K, const void* V, int dtype,
  * before the call returns.  A call that writes pages and any other call on them need
  * the order of one stream or an event between them.  Two entries of the table may name
  * one page that is only read (a shared prompt); a block that a call writes is named by one
- * entry.  Values of length outside [0, max_pages*page] count as the nearer end.
+ * entry.  Values of length (and of an append's start) outside [0, max_pages*page] count as the
+ * nearer end.
  * No reference counterpart: it has no cache.
  * Constraints: B <= 65535; 1 <= NP, max_pages; page = 64 * 2^j <= 65536;
  *   max_pages*page <= 2^31 - 256; 1 <= HKV <= 1024; DK = DV in {32, 64, 96, 128, 192,
@@ -657,7 +661,9 @@ int dsa_kv8_rows(const dsa_kv8_cache* cache, const int32_t* slots, int64_t N, in
  * others see nothing: NaN), over the slots among the first n.  window 0: all of them.
  *   fp32 logits, softmax and sums; the cache's values enter the products unrounded; Q
  * and p as f16 with a power of two for each row of Q (16-bit types) or as two such
- * pieces (fp32: 22 bits and more).
+ * pieces (fp32: 22 bits and more).  A row's sums are held in units of the largest V scale of the
+ * blocks in which it weighs a slot, and divided before that scale comes in: values up to
+ * fp32's largest give finite results; what lies 2^-126 of that unit and less is lost.
  *   Q [B,Tq,HQ,DK], out [B,Tq,HQ,DV] of dtype (fp32, bf16, fp16), 16-byte aligned; HQ a
  *   multiple of HKV, at most 1024; n <= max_pages*page; B*Tq*HQ < 2^23.
  *   workspace: device memory of dsa_kv8_attention_workspace_bytes, 16-byte aligned, used
