@@ -10,15 +10,17 @@
 //   S^T = K . Q^T    A = K's codes, which f16 holds exactly; B = Q
 //   O^T = V^T . P^T  A = V's codes as they lie in the cache; B = P straight from S^T's
 //                    registers (lane group g holds tokens 16j + 4g + i of each row)
-// The block's scales are powers of two: K's goes into the factor of the logits, V's is
-// the unit in which the sums are held (a block of another unit is added apart, exactly).
+// The block's scales are powers of two: K's goes into the factor of the logits, V's is the
+// unit in which a row's sums are held (a block of another unit is added apart, exactly).
+// Sums are divided by those of p before the unit comes in, for each wave and each split, and
+// joined as shares that add up to 1: a mean of numbers that fp32 holds stays one.
 // So no value of the cache is rounded.  Rows of Q are scaled by a power of two into f16's
 // range and enter as one f16 piece (16-bit types) or two (fp32, 23 bits); p likewise.
 //
 // Few rows or short rows of K (!SHARED): each of a block's four waves takes blocks of its own in turn, its
 // operands straight into registers; K of the next block is on its way while p and V are
 // multiplied, V while the logits are formed, the page id two turns ahead.  Bound by memory: 16
-// caches of up to 32768 slots, 32 heads on 8 of 128, 834 MB, take 149 us, 5.6 TB/s (a large
+// caches of up to 32768 slots, 32 heads on 8 of 128, 834 MB, take 152 us, 5.5 TB/s (a large
 // array is read at 6.35).  Operands by way of LDS, as below, or eight waves a block were slower.
 //
 // Many long rows, or few slots (SHARED): the waves take different rows of the same blocks.  Codes go to LDS by
@@ -26,9 +28,9 @@
 // each other: a lane's own operand is 16 bytes of a row of its own, which costs the L1 64
 // accesses an instruction where this takes 16), rows' 16-byte chunks swizzled so that no two
 // lanes meet on a bank when they are read as operands.  Bound by the vector instructions that widen
-// the codes and weigh the logits, which 32 rows a wave share where there are enough (DK <= 128 of
-// 16-bit types: more have no registers): 4 x 48 tokens of 16 heads on one of 128 over 8191 slots, 10.5 GFLOP, take 29 us;
-// 60 with waves on slots of their own.
+// the codes and weigh the logits, which 32 rows a wave share where there are enough (DK = 128 of
+// 16-bit types: more have no registers): 4 x 48 tokens of 16 heads on one of 128 over 8191 slots,
+// 10.5 GFLOP, take 30 us; 60 with waves on slots of their own.
 #include <algorithm>
 
 #include "dsa_launch.h"
@@ -725,7 +727,12 @@ Plan plan_of(const Kv8& c, int64_t Tq, int HQ, int64_t n, int64_t window, int64_
   // 32 rows a wave share the widening of K and V where the registers hold them, against half
   // the blocks (16 / 32 rows):
   //   own, D 64, 64 rows: 32 pairs of 8192 slots 17.9 / 19.5; 256 of 4096 42.1 / 36.1
-  //   shared, D 128: 256 pairs of 4096 and 64 rows 73 / 92; 4 of 32768 and 768 rows 98 / 84
+  //   shared, D 128, 4 pairs of 8192 slots: 512 rows 32.8 / 35.1, 640 38.3 / 38.1, 768 40.7 / 42.1,
+  //     2048 70.3 / 62.0; 8 pairs: 256 29.6 / 31.9, 512 41.8 / 41.5, 768 58.4 / 56.3, 2048 123 / 103
+  //   256 pairs of 4096: 64 78 / 96, 128 122 / 113, 192 163 / 171, 256 215 / 179, 512 384 / 334
+  //   4 pairs of 32768: 192 37.0 / 39.4, 256 42.0 / 41.5, 384 59.1 / 53.7, 512 68.6 / 61.4, 768 101 / 87
+  // (From 640 rows on 32 cost a few in 100 at most and win a tenth or more where there is much to do;
+  // the latter would from 256 on.)
   p.rt = !fp32 && (p.shared ? c.DK == 128 && most > 4 && rows > 512 : c.DK <= 96 && rows > 16 && work >= 24576) ? 2 : 1;
   const int64_t tile = 16 * p.rt * (p.shared ? kWaves : 1), waves = p.shared ? 1 : kWaves;
   p.row_tiles = static_cast<int>((rows + tile - 1) / tile);

@@ -375,7 +375,10 @@ __global__ __launch_bounds__(kNT) void append_kernel(Kv8 c, Kv8Append a, int nbl
 // changes its length.  A wave takes the K or the V of one head, a unit of one token a
 // lane, then units of the queries; what does not depend on the position is loaded before the
 // position is known.  Bound by latency, that of the chain length, page, scale, codes: 32 sequences
-// of 32 and 8 heads of 128 in bf16, 11 MB, take 8.1 us.
+// of 32 and 8 heads of 128 in bf16, 11 MB, take 6.7 us in a graph (8.1 each alone) where no block's
+// scale grows.  Where one does, its held codes move a word a lane a trip, each waited for: with
+// random tokens from a block's slot 8 to 55 some head's scale grows in nearly every step, which
+// then takes 15.8 on average, and 26.6 where all heads' do (one sequence: 6.0, 7.0, 15.1).
 constexpr int kFew = 4;  // tokens, by 16 units: a wave
 template <typename Tag, int DK, int DV>
 __global__ __launch_bounds__(1024) void append_few_kernel(Kv8 c, Kv8Append a) {
@@ -511,8 +514,9 @@ __global__ __launch_bounds__(kNT) void append_counts_kernel(Kv8 c, Kv8Append a) 
 // Slots back as values; zeros for a slot that holds nothing.  A block of threads takes 64
 // entries of a list, one head.  Where they are one block's slots in order (as
 // the first N slots are, and runs that begin with a block), a thread takes 4 tokens by 8
-// dimensions of V from words of 4 tokens; else it gathers bytes.  Bound by memory: 2 x 16384 slots
-// of 8 heads of 128 as bf16, 201 MB, take 46 us, 4.4 TB/s; gathered, 143.
+// dimensions of V from words of 4 tokens; else it gathers bytes, which lie 64 apart in V, as the
+// attention wants them.  Bound by memory: 2 x 16384 slots of 8 heads of 128 as bf16, 201 MB, take
+// 46 us, 4.4 TB/s; gathered, 143.
 __device__ __forceinline__ void decode8(uint32_t w0, uint32_t w1, float f, float (&x)[8]) {
   const f32x2 a = __builtin_amdgcn_cvt_pk_f32_fp8(w0, false), b = __builtin_amdgcn_cvt_pk_f32_fp8(w0, true);
   const f32x2 c = __builtin_amdgcn_cvt_pk_f32_fp8(w1, false), d = __builtin_amdgcn_cvt_pk_f32_fp8(w1, true);
@@ -621,9 +625,15 @@ hipError_t append_dims(const Kv8& c, const Kv8Append& a, hipStream_t stream) {
     return hipGetLastError();
   }
   const int nblk = static_cast<int>((a.T + kBlk - 2) / kBlk + 1);
-  // The angles are loaded once for the heads of a group, so a group is as large as leaves the
-  // blocks that run at once, two a compute unit, for K and V and as many for the queries: 190 us
-  // for 2 x 16384 tokens of 32 and 8 heads of 128; smaller groups took 196 (4) to 219 (8).
+  // The angles are loaded once for the heads of a group, so a group is as large as leaves two blocks a
+  // compute unit for K and V and as many for the queries: 190 us for 2 x 16384 tokens of 32 and 8
+  // heads of 128; smaller groups took 196 (4) to 219 (8).  Two run at once of up to 128 dimensions and of
+  // 192 with V of 128, past that one.  us for one block / two / four a unit:
+  //   32 and 8 heads of 128: 2000 tokens 12.9 / 13.8 / 14.4, 8192 36 / 42 / 48, 16384 91 / 105 / 104
+  //   8 and 8: 4096 of 128 18.7 / 17.1 / 17.1, 8 x 1001 of 64 in fp32 22.0 / 20.1 / 20.1
+  //   no queries, 8 heads, 3000 tokens: of 128 14.6 / 10.1 / 10.1, of 256 34.6 / 25.8 / 25.6
+  //   16 and 4 heads: 2 x 8192 of 192 126 / 130 / 141, 16384 of 256 133 / 138 / 155
+  // One is better by up to a seventh where queries outnumber keys, two by up to a third where not.
   const int64_t want = 2 * int64_t{device_cus() > 0 ? device_cus() : 256}, blocks = c.B * nblk;
   auto groups_of = [&](int64_t heads) { return static_cast<int>(std::min(heads, (want + blocks - 1) / blocks)); };
   constexpr int kSide = DK >= 96 ? 1 : 128 / DK;

@@ -41,7 +41,8 @@ __device__ __forceinline__ Walk walk_in(const Win& a, int64_t b, int t0) {
 // sequences' K/V heads lie innermost, so that the tiles of one go to one XCD where they are a
 // multiple of 8 (block i starts on XCD i % 8), and all XCDs have the same work where they are
 // not: one head of 128, 8 query heads, 8192 tokens, window 1000, 312 us on one XCD, 60 on all;
-// 9 K/V heads, 16384 tokens, window 2048, 977 with two on one of them, 695 so.
+// 9 K/V heads, 16384 tokens, window 2048, 977 with two on one of them, 695 so.  (At D = 256 the
+// same loses: 36 heads on 9, 2121 us with a head's tiles on one XCD, 2497 so.)
 // (32-bit throughout: a 64-bit division costs as much as a short prompt's tile.)
 template <int TQ>
 __device__ __forceinline__ void place(const Win& a, int& t0, int64_t& b, int& h, int& hk) {
@@ -107,9 +108,9 @@ __device__ __forceinline__ void store4(typename Tag::raw* to, f32x4 y) {
 // non-finite elements taken out of the product and added to the rows that see them.
 //
 // Bound by the products and, in turn with them, the softmax: 32768 tokens, 32 heads on 8 of 128,
-// window 2048, 1073 GFLOP of pairs that are seen, take 1.07-1.11 ms, 0.97-1.0 PFLOP/s where a
-// large product reaches 1.2; the matrix units are busy in 44 of 100 cycles.  (1.20 with whole
-// tiles in one loop with the others, 1.10 with a loop of their own.)
+// window 2048, 1073 GFLOP of pairs that are seen, take 1.11-1.14 ms, 0.94-0.97 PFLOP/s where a
+// large product reaches 1.2; the matrix units are busy in 45 of 100 cycles.  (A tenth more with
+// whole tiles in one loop with the others than with a loop of their own.)
 // ---------------------------------------------------------------------------
 template <typename Tag, int D, int QT>
 __global__ __launch_bounds__(kNT, D >= 128 ? 2 : QT == 2 ? 3 : 4) void window_kernel(Win a) {
@@ -401,8 +402,9 @@ __global__ __launch_bounds__(kNT, D >= 128 ? 2 : QT == 2 ? 3 : 4) void window_ke
 // taken out of the product and added to the rows that see them.
 //
 // Bound by the products: 2 x 4096 tokens, 8 heads of 64, window 1024, 15.0 GFLOP of pairs that are
-// seen, take 106 us, 142 TFLOP/s where a large fp32 product reaches 154 (211 us on the fp32 instructions); the matrix units are busy in 35 of 100 cycles, the rest goes to pieces of K and V
-// (each block makes its own), of p, and the softmax.
+// seen, take 107 us one after another, 140 TFLOP/s where a large fp32 product reaches 154 (125 in the
+// first launches after a pause; 211 on the fp32 instructions); the matrix units are busy in 35 of
+// 100 cycles, the rest goes to pieces of K and V (each block makes its own), of p, and the softmax.
 // ---------------------------------------------------------------------------
 struct Three {
   uint32_t h, m, l;  // two elements' pieces

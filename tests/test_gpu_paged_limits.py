@@ -182,3 +182,17 @@ def test_windows_past_64_bits(dev):
     every = P.kv8_attention(cache, q)
     for kw in (dict(window=2 ** 64 + 5), dict(window=2 ** 63), dict(window=3, sinks=2 ** 64), dict(window=3, sinks=2 ** 63 + 1)):
         assert torch.equal(P.kv8_attention(cache, q, **kw), every), kw
+
+
+@pytest.mark.parametrize("DK, DV, window, dtype", [(96, 96, None, BF16), (192, 192, 100, F32), (192, 128, None, F16)])
+def test_prompts_over_the_pages(dev, DK, DV, window, dtype):
+    """Whole prompts of a padded batch over the cache that they were appended to, at the head sizes
+    that window_attention does not take."""
+    g = gen(DK + DV)
+    B, T, HQ, HKV, lengths = 3, 200, 4, 2, [200, 1, 130]
+    rope = P.rope_tables(256, DK, device=dev)
+    cache = P.KV8Cache.empty(B, 256, HKV, DK, DV, page=128, device=dev)
+    Q, K, V = randn(g, B, T, HQ, DK, dtype=dtype), randn(g, B, T, HKV, DK, dtype=dtype), randn(g, B, T, HKV, DV, dtype=dtype)
+    many = ints(dev, lengths)
+    q, _ = P.kv8_append(cache, K.to(dev), V.to(dev), rope=rope, Q=Q.to(dev), count=many)
+    check_attention(dev, cache, q.cpu(), dtype, window, 2, lengths)
